@@ -59,8 +59,10 @@ enum {
   PKV_VEC_NONFINITE_RESIDUAL = 24,/* turbo-quant/src/qjl.rs:210 */
   PKV_VEC_NORM_RANGE = 25,        /* fib-quant/src/codec.rs:1003 (second pass of encode_batch) */
   PKV_VEC_DEVICE_WAIT = 26,       /* no counterpart: a bounded wait inside a kernel ran out (the payload is not valid) */
-  PKV_VEC_MISALIGNED_DST = 27     /* no counterpart: a per-tensor cache offset of a *_multi call is negative or not
+  PKV_VEC_MISALIGNED_DST = 27,    /* no counterpart: a per-tensor cache offset of a *_multi call is negative or not
                                      a multiple of 16 bytes (that batch is skipped) */
+  PKV_VEC_BAD_SEQUENCE = 28       /* no counterpart: a length or page number of a sequence of a 4-bit cache is out of
+                                     range (the index is the sequence's; see the pkv_kv4_* calls) */
 };
 
 const char* pkv_status_string(int status);
@@ -418,6 +420,96 @@ int pkv_turbo_decode_batches_compact(const pkv_turbo_profile* p, const uint8_t* 
 int pkv_tqb1_header_write(const pkv_turbo_profile* p, uint32_t n_vectors, uint8_t* out38);
 int pkv_tqb1_header_parse(const pkv_turbo_profile* p, const uint8_t* bytes, int64_t len,
                           uint32_t* n_vectors);
+
+/* ---- a KV cache that stays in 4 bits ------------------------------------- */
+/* No counterpart in the reference.  The codecs above store a cache; this is the cache a model decodes from: one
+ * layer's keys and values in pages, 4 bits a value, read by the attention kernel as they are.
+ *
+ * Format.  Channels come in blocks of 16; a value is (n - 8) * s with a 4-bit n and the block's 8-bit scale s, bits
+ * 14..7 of a binary16 (5 exponent and 3 fraction bits, at most 7168).  s = amax / 7 rounded to nearest even,
+ * n = 8 + clamp(x / s rounded to nearest even, -8, 7).  Every value is exact in binary16 and bfloat16; 4.5 bits a value.
+ * Sixteen tokens of one kv head form an atom of 18 * dim bytes: K codes [16][dim/2] (channel 2i in the low half of
+ * byte i), V codes [16][dim/2], K scales [16][dim/16], V scales [16][dim/16]; for dim = 128 the two 32-byte halves of
+ * the V code row of token t are swapped where t & 2.  A page is [n_kv_heads][page_tokens / 16] atoms, the pool
+ * [n_pages] pages.  A row of zero bytes is a row of zeros.
+ *
+ * Slot j of sequence s lies in page page_table[s][j / page_tokens]; the entries up to the sequence's length are read.
+ * Attention may share pages between sequences (a common prefix); a page that a call writes belongs to one.
+ * lens[s] is the number of slots in use, those that the call appends included: a step raises the lengths once, for
+ * all layers, before its first call.  ends[s] is the number of tokens the sequence has had (a query's position is
+ * counted from it); null = lens.  positions[s][h][j] is the position of the token in a slot, below ends[s]; null = the slot's
+ * own number, as long as nothing was evicted.  mass[s][h][j] is the attention weight a token has received.  Both are
+ * [n_seqs][n_kv_heads][max_pages * page_tokens].
+ *
+ * A sequence whose length is negative or above max_pages * page_tokens, or that has a page number outside [0, n_pages) among the
+ * entries a call reads, is reported as PKV_VEC_BAD_SEQUENCE with its index.  A sequence with a bad length counts as empty,
+ * the tokens of a bad page as absent; nothing is read or written through either.
+ * All of these calls return PKV_ERR_UNSUPPORTED for a dim other than 64 and 128 or page_tokens that is not a multiple of 16,
+ * only enqueue work on the caller's stream, and allocate nothing. */
+typedef struct pkv_kv4_cache {
+  uint8_t* pages;             /* [n_pages][n_kv_heads][page_tokens / 16][18 * dim], 16-byte aligned */
+  const int32_t* page_table;  /* [n_seqs][max_pages] */
+  const int32_t* lens;        /* [n_seqs] */
+  const int32_t* ends;        /* [n_seqs] or null */
+  int32_t* positions;         /* or null */
+  float* mass;                /* or null */
+  int64_t n_pages;
+  int32_t dim, n_kv_heads, page_tokens, n_seqs, max_pages;
+  int32_t reserved;           /* 0 */
+} pkv_kv4_cache;
+
+/* Vectors of [n_seqs][n_tokens][heads][dim], strides in elements (multiples of 4 for f32, of 8 for the 16-bit types;
+ * the base 16-byte aligned), the dim values of a vector contiguous. */
+typedef struct pkv_kv4_rows {
+  int64_t seq_stride, token_stride, head_stride;
+  int32_t n_tokens;
+  int32_t dtype;  /* PKV_DST_* */
+} pkv_kv4_rows;
+
+/* Writes the keys and values of each sequence's newest tokens: row i of sequence s goes to slot
+ * lens[s] - new_lens[s] + i (new_lens null: n_tokens for every sequence); rows from new_lens[s] on are ignored.  Their
+ * positions become ends[s] - new_lens[s] + i and their mass 0.  A row with a value that is not finite
+ * (PKV_VEC_NONFINITE_INPUT), or one too large for the scale (PKV_VEC_NORM_RANGE), is stored as zeros and reported with
+ * the index ((s * n_tokens + i) * n_kv_heads + h) * 2 + (0 for K, 1 for V). */
+int pkv_kv4_append_dev(const pkv_kv4_cache* cache, const void* k_dev, const pkv_kv4_rows* k_rows, const void* v_dev,
+                       const pkv_kv4_rows* v_rows, const int32_t* new_lens_dev, uint64_t* err_dev, void* stream);
+/* The inverse: the values the newest tokens of each sequence stand for, at the rows an append would take them from;
+ * new_lens = lens reads everything.  Rows from new_lens[s] on stay as they were. */
+int pkv_kv4_read_dev(const pkv_kv4_cache* cache, void* k_dev, const pkv_kv4_rows* k_rows, void* v_dev,
+                     const pkv_kv4_rows* v_rows, const int32_t* new_lens_dev, uint64_t* err_dev, void* stream);
+
+typedef struct pkv_kv4_attend_args {
+  float scale;         /* of the products q . k */
+  int32_t n_q_heads;   /* a multiple of n_kv_heads: head h reads kv head h / (n_q_heads / n_kv_heads) */
+  int32_t window;      /* > 0: a token sees the `window` newest positions up to its own; 0: all up to its own */
+  int32_t sinks;       /* with a window: positions below `sinks` stay visible too */
+  int32_t accumulate;  /* 1: mass += the weights of this call's queries */
+  int32_t max_len;     /* no length is above it (a hint for the split of the work); 0: the table's capacity */
+} pkv_kv4_attend_args;
+/* out = softmax(scale * q K^T) V over the visible tokens of each sequence, read from the pages.  The queries are the
+ * newest tokens: row i of sequence s has position ends[s] - q_lens[s] + i (q_lens null: n_tokens for every sequence)
+ * and sees the cached tokens of positions up to it.  Rows from q_lens[s] on are neither read nor written.  A query that
+ * sees nothing gets zeros.  lse_dev (may be null unless accumulating): [n_seqs][n_tokens][n_q_heads] f32, the natural logarithm of
+ * the sum of exponentials, -inf where nothing is visible.  q and out have the same type.
+ * Products, softmax statistics and sums are f32; weights enter the second product in binary16 (f32 queries: as two
+ * binary16 terms).  The result does not depend on the order in which blocks run.
+ * workspace_dev: pkv_kv4_attend_workspace_bytes bytes (may be 0), 16-byte aligned, not shared with a call that can
+ * overlap. */
+int64_t pkv_kv4_attend_workspace_bytes(const pkv_kv4_cache* cache, const pkv_kv4_rows* q_rows,
+                                       const pkv_kv4_attend_args* args);
+int pkv_kv4_attend_dev(const pkv_kv4_cache* cache, const void* q_dev, const pkv_kv4_rows* q_rows, void* out_dev,
+                       const pkv_kv4_rows* out_rows, float* lse_dev, const int32_t* q_lens_dev,
+                       const pkv_kv4_attend_args* args, void* workspace_dev, int64_t workspace_bytes, uint64_t* err_dev,
+                       void* stream);
+
+/* Cuts every sequence longer than `budget` down to `budget` slots, per kv head: tokens of positions below `sinks` and
+ * from ends[s] - recent on stay (sinks + recent <= budget), then those with the largest mass (ties: the lowest slot; a
+ * mass that is negative or NaN counts as 0).  Kept tokens in slots below `budget` stay where they are; the j-th kept slot from `budget` on moves, with its
+ * position and mass, to the j-th slot freed below.  Slots from `budget` on keep their bytes; lens is not changed (the
+ * caller lowers it to min(lens, budget) once all layers are done).  Needs mass and positions. */
+int64_t pkv_kv4_evict_workspace_bytes(const pkv_kv4_cache* cache, int32_t budget);
+int pkv_kv4_evict_dev(const pkv_kv4_cache* cache, int32_t budget, int32_t sinks, int32_t recent, void* workspace_dev,
+                      int64_t workspace_bytes, uint64_t* err_dev, void* stream);
 
 /* The binary32 arguments (bit patterns, ascending) on which this host's logf (function 0, positive
  * normal arguments) or expf (function 1, |x| <= 89) differs from the portable function; host-only,

@@ -34,6 +34,7 @@ VEC_NONFINITE_RESIDUAL = 24
 VEC_NORM_RANGE = 25
 VEC_DEVICE_WAIT = 26
 VEC_MISALIGNED_DST = 27
+VEC_BAD_SEQUENCE = 28
 
 NORM_FP16, NORM_F32 = 0, 1
 ARGMIN_PAIRWISE, ARGMIN_SEQUENTIAL = 0, 1
@@ -85,6 +86,26 @@ class Layout(C.Structure):
     @property
     def batch_count(self) -> int:
         return self.n_batches[0] * self.n_batches[1] * self.n_batches[2]
+
+
+class Kv4CacheC(C.Structure):
+    """pkv_kv4_cache"""
+    _fields_ = [("pages", C.c_void_p), ("page_table", C.c_void_p), ("lens", C.c_void_p), ("ends", C.c_void_p),
+                ("positions", C.c_void_p), ("mass", C.c_void_p), ("n_pages", C.c_int64), ("dim", C.c_int32),
+                ("n_kv_heads", C.c_int32), ("page_tokens", C.c_int32), ("n_seqs", C.c_int32),
+                ("max_pages", C.c_int32), ("reserved", C.c_int32)]
+
+
+class Kv4RowsC(C.Structure):
+    """pkv_kv4_rows"""
+    _fields_ = [("seq_stride", C.c_int64), ("token_stride", C.c_int64), ("head_stride", C.c_int64),
+                ("n_tokens", C.c_int32), ("dtype", C.c_int32)]
+
+
+class Kv4AttendC(C.Structure):
+    """pkv_kv4_attend_args"""
+    _fields_ = [("scale", C.c_float), ("n_q_heads", C.c_int32), ("window", C.c_int32), ("sinks", C.c_int32),
+                ("accumulate", C.c_int32), ("max_len", C.c_int32)]
 
 
 class PkvError(RuntimeError):
@@ -165,6 +186,13 @@ _SIGS = {
                                                  C.POINTER(C.c_int32), C.POINTER(C.c_int64)]),
     "pkv_tqb1_header_write": (C.c_int, [_V, C.c_uint32, _V]),
     "pkv_tqb1_header_parse": (C.c_int, [_V, _V, C.c_int64, C.POINTER(C.c_uint32)]),
+    "pkv_kv4_append_dev": (C.c_int, [C.POINTER(Kv4CacheC), _V, C.POINTER(Kv4RowsC), _V, C.POINTER(Kv4RowsC), _V, _V, _V]),
+    "pkv_kv4_read_dev": (C.c_int, [C.POINTER(Kv4CacheC), _V, C.POINTER(Kv4RowsC), _V, C.POINTER(Kv4RowsC), _V, _V, _V]),
+    "pkv_kv4_attend_workspace_bytes": (C.c_int64, [C.POINTER(Kv4CacheC), C.POINTER(Kv4RowsC), C.POINTER(Kv4AttendC)]),
+    "pkv_kv4_attend_dev": (C.c_int, [C.POINTER(Kv4CacheC), _V, C.POINTER(Kv4RowsC), _V, C.POINTER(Kv4RowsC), _V, _V,
+                                     C.POINTER(Kv4AttendC), _V, C.c_int64, _V, _V]),
+    "pkv_kv4_evict_workspace_bytes": (C.c_int64, [C.POINTER(Kv4CacheC), C.c_int32]),
+    "pkv_kv4_evict_dev": (C.c_int, [C.POINTER(Kv4CacheC), C.c_int32, C.c_int32, C.c_int32, _V, C.c_int64, _V, _V]),
     "pkv_host_libm_exceptions": (C.c_int, [C.c_int32, _V, C.c_int64, C.POINTER(C.c_int64), C.POINTER(C.c_int32)]),
     "pkv_launch_count": (C.c_int64, []),
     "pkv_test_skip_tensor_issue": (C.c_int, [C.c_int]),

@@ -257,6 +257,7 @@ const char* pkv_status_string(int s) {
     case PKV_VEC_NONFINITE_RESIDUAL: return "non-finite residual";
     case PKV_VEC_NORM_RANGE: return "norm not representable in the wire norm format";
     case PKV_VEC_DEVICE_WAIT: return "a wait inside a kernel ran out; the output is not valid";
+    case PKV_VEC_BAD_SEQUENCE: return "length or page number of a sequence out of range";
     default: return "unknown status";
   }
 }

@@ -1,0 +1,218 @@
+// Writing vectors into the 4-bit KV cache and reading them back.
+//
+// A thread owns one block of 16 channels of a token's key and of its value: the block's largest magnitude needs
+// no other thread, and both loads are in flight together.  A CTA covers 128 / (D / 16) tokens of one kv head, so that
+// its code and scale bytes form contiguous runs.  Both kernels are bound by HBM: a vector is read once and written
+// once.
+#include "pkv_kv4.cuh"
+
+using namespace pkv_kv4;
+
+namespace {
+
+constexpr int kThreads = 128;
+
+// The nearest scale to amax / 7 (ties to the even code), as its byte; 256 if it is beyond kMaxScaleByte.  Decided
+// on exact products: the candidate below an approximate quotient, then amax against 7 x the midpoint above it.
+__device__ __forceinline__ uint32_t scale_byte(float amax) {
+  const float s = __fmul_rn(amax, 0.142857149f);
+  if (s > 8192.0f) return 256u;
+  float lo, step;
+  if (s >= 6.103515625e-05f) {  // 2^-14 and up: 3 fraction bits
+    lo = __uint_as_float(__float_as_uint(s) & 0xfff00000u);
+    step = __uint_as_float((__float_as_uint(s) & 0x7f800000u) - (3u << 23));
+  } else {
+    step = 7.62939453125e-06f;  // 2^-17
+    lo = __fmul_rn(floorf(__fmul_rn(s, 131072.0f)), step);
+  }
+  // the code of lo: multiples of 2^-17 below 2^-14, then exponent and fraction bits
+  uint32_t code = lo < 6.103515625e-05f ? (uint32_t)__fmul_rn(lo, 131072.0f) : (__float_as_uint(lo) >> 20) - (112u << 3);
+  const float mid7 = __fmul_rn(7.0f, __fadd_rn(lo, __fmul_rn(0.5f, step)));  // exact: 5 bits x 3 bits
+  if (amax > mid7 || (amax == mid7 && (code & 1u))) code++;
+  return code > (uint32_t)kMaxScaleByte ? 256u : code;
+}
+
+__device__ __forceinline__ float scale_value(uint32_t byte) {
+  return __half2float(__ushort_as_half((unsigned short)(byte << 7)));
+}
+
+// 16 channels -> 8 code bytes and the scale byte; false if they cannot be stored.
+template <int T>
+__device__ __forceinline__ bool quantise(const float (&x)[16], uint2& codes, uint32_t& byte, int& why) {
+  float amax = 0.0f;
+  bool finite = true;
+#pragma unroll
+  for (int i = 0; i < 16; i++) {
+    finite = finite && pkv_finite(x[i]);
+    amax = fmaxf(amax, fabsf(x[i]));
+  }
+  if (!finite) {
+    why = PKV_VEC_NONFINITE_INPUT;
+    return false;
+  }
+  byte = scale_byte(amax);
+  if (byte > 255u) {
+    why = PKV_VEC_NORM_RANGE;
+    return false;
+  }
+  if (byte == 0u) {  // every value below half the smallest scale: zeros (code 8)
+    codes = make_uint2(0x88888888u, 0x88888888u);
+    return true;
+  }
+  const float s = scale_value(byte), r = __frcp_rn(s);
+  uint32_t w[2] = {0u, 0u};
+#pragma unroll
+  for (int i = 0; i < 16; i++) {
+    uint32_t n;
+    if constexpr (T == PKV_DST_F32) {
+      // x / s to the nearest integer, decided on the exact remainder (an f32 quotient can round onto a tie)
+      const float q = rintf(fminf(fmaxf(__fmul_rn(x[i], r), -8.0f), 7.0f));
+      const float rest = __fmaf_rn(-q, s, x[i]), half = __fmul_rn(0.5f, s);
+      const int qi = (int)q, odd = qi & 1;
+      int up = rest > half || (rest == half && odd) ? 1 : 0;
+      int down = rest < -half || (rest == -half && odd) ? 1 : 0;
+      n = (uint32_t)(min(7, max(-8, qi + up - down)) + 8);
+    } else {
+      // At most 11 significant bits over 4: a quotient that is no tie is at least 2^-13 away from one, so rounding it to
+      // a multiple of 2^-15 first (the sum with 384) restores exact ties and moves nothing across one.
+      const float q = fminf(fmaxf(__fmul_rn(x[i], r), -8.0f), 7.0f);
+      const float near = __fadd_rn(q, 384.0f);
+      n = __float_as_uint(__fadd_rn(near, 12582912.0f + 8.0f - 384.0f)) & 15u;
+    }
+    w[i >> 3] |= n << (4 * (i & 7));
+  }
+  codes = make_uint2(w[0], w[1]);
+  return true;
+}
+
+// Where row i of a call goes; false if it is not one of the sequence's.
+__device__ __forceinline__ bool row_slot(const Cache& c, int s, int i, int n_tokens, const int32_t* new_lens, uint64_t* err,
+                                         int* slot, int* position) {
+  const int n = c.length(s, err);
+  const int fresh = new_lens ? new_lens[s] : n_tokens;
+  if (fresh < 0 || fresh > n_tokens || fresh > n) {
+    pkv_report(err, 0, s, PKV_VEC_BAD_SEQUENCE);
+    return false;
+  }
+  *slot = n - fresh + i;
+  *position = c.end(s, n) - fresh + i;
+  return i < fresh;
+}
+
+template <int D, int T>
+__global__ void __launch_bounds__(kThreads)
+kv4_append_kernel(Cache c, const typename PkvDst<T>::type* __restrict__ k, Rows kr,
+                  const typename PkvDst<T>::type* __restrict__ v, Rows vr, const int32_t* __restrict__ new_lens, uint64_t* err) {
+  using A = Atom<D>;
+  constexpr int TOK = kThreads / A::SROW;
+  const int b = threadIdx.x % A::SROW;  // block of 16 channels
+  const int s = blockIdx.z, h = blockIdx.y;
+  const int i = blockIdx.x * TOK + threadIdx.x / A::SROW;
+  if (i >= kr.n) return;
+  float x[2][16];
+  load_f32<T, 16>(k + s * kr.seq + i * kr.token + h * kr.head + 16 * b, x[0]);
+  load_f32<T, 16>(v + s * vr.seq + i * vr.token + h * vr.head + 16 * b, x[1]);
+  int slot, position;
+  if (!row_slot(c, s, i, kr.n, new_lens, err, &slot, &position)) return;
+  uint8_t* atom = c.atom(s, h, slot / kAtomTokens, A::BYTES, err);
+  if (!atom) return;
+  const int t = slot % kAtomTokens;
+  const unsigned row_lanes = ((1u << A::SROW) - 1u) << ((threadIdx.x & 31) / A::SROW * A::SROW);
+#pragma unroll
+  for (int side = 0; side < 2; side++) {
+    uint2 codes = make_uint2(0u, 0u);
+    uint32_t byte = 0u;
+    int why = 0;
+    const bool ok = quantise<T>(x[side], codes, byte, why);
+    // one block that cannot be stored empties the whole row; the row's threads are neighbours in a warp
+    if (!__all_sync(row_lanes, ok)) {
+      codes = make_uint2(0u, 0u);
+      byte = 0u;
+      if (!ok) pkv_report(err, 0, (((int64_t)s * kr.n + i) * c.heads + h) * 2 + side, why);
+    }
+    const int at = side ? A::VC + t * A::ROW + ((8 * b) ^ A::vswap(t)) : A::KC + t * A::ROW + 8 * b;
+    *reinterpret_cast<uint2*>(atom + at) = codes;
+    atom[(side ? A::VS : A::KS) + t * A::SROW + b] = (uint8_t)byte;
+  }
+  if (b == 0) {
+    if (c.positions) c.positions[c.stat(s, h) + slot] = position;
+    if (c.mass) c.mass[c.stat(s, h) + slot] = 0.0f;
+  }
+}
+
+template <int D, int T>
+__global__ void __launch_bounds__(kThreads)
+kv4_read_kernel(Cache c, typename PkvDst<T>::type* __restrict__ k, Rows kr, typename PkvDst<T>::type* __restrict__ v,
+                Rows vr, const int32_t* __restrict__ new_lens, uint64_t* err) {
+  using A = Atom<D>;
+  constexpr int TOK = kThreads / A::SROW;
+  const int b = threadIdx.x % A::SROW;
+  const int s = blockIdx.z, h = blockIdx.y;
+  const int i = blockIdx.x * TOK + threadIdx.x / A::SROW;
+  if (i >= kr.n) return;
+  int slot, position;
+  if (!row_slot(c, s, i, kr.n, new_lens, err, &slot, &position)) return;
+  const uint8_t* atom = c.atom(s, h, slot / kAtomTokens, A::BYTES, err);
+  if (!atom) return;
+  const int t = slot % kAtomTokens;
+#pragma unroll
+  for (int side = 0; side < 2; side++) {
+    const int at = side ? A::VC + t * A::ROW + ((8 * b) ^ A::vswap(t)) : A::KC + t * A::ROW + 8 * b;
+    const uint2 codes = *reinterpret_cast<const uint2*>(atom + at);
+    const float scale = scale_value(atom[(side ? A::VS : A::KS) + t * A::SROW + b]);
+    float x[16];
+#pragma unroll
+    for (int j = 0; j < 16; j++)
+      x[j] = __fmul_rn((float)((int)(((j < 8 ? codes.x : codes.y) >> (4 * (j & 7))) & 15u) - 8), scale);
+    if (side == 0) store_f32<T, 16>(k + s * kr.seq + i * kr.token + h * kr.head + 16 * b, x);
+    else store_f32<T, 16>(v + s * vr.seq + i * vr.token + h * vr.head + 16 * b, x);
+  }
+}
+
+template <int D, int T>
+void launch_rows(bool append, const Cache& c, const void* k, const Rows& kr, const void* v, const Rows& vr,
+                 const int32_t* new_lens, uint64_t* err, cudaStream_t s) {
+  using E = typename PkvDst<T>::type;
+  constexpr int TOK = kThreads / Atom<D>::SROW;
+  const dim3 grid((unsigned)((kr.n + TOK - 1) / TOK), (unsigned)c.heads, (unsigned)c.n_seqs);
+  if (append)
+    kv4_append_kernel<D, T><<<grid, kThreads, 0, s>>>(c, (const E*)k, kr, (const E*)v, vr, new_lens, err);
+  else
+    kv4_read_kernel<D, T><<<grid, kThreads, 0, s>>>(c, (E*)const_cast<void*>(k), kr, (E*)const_cast<void*>(v), vr, new_lens, err);
+}
+
+int rows_call(bool append, const pkv_kv4_cache* cache, const void* k, const pkv_kv4_rows* k_rows, const void* v,
+              const pkv_kv4_rows* v_rows, const int32_t* new_lens, uint64_t* err, void* stream) {
+  Cache c;
+  Rows kr, vr;
+  if (int st = make_cache(cache, &c)) return st;
+  if (int st = make_rows(k, k_rows, &kr)) return st;
+  if (int st = make_rows(v, v_rows, &vr)) return st;
+  if (!err || kr.n != vr.n || k_rows->dtype != v_rows->dtype) return PKV_ERR_INVALID_ARGUMENT;
+  if (kr.n > c.capacity && !new_lens) return PKV_ERR_INVALID_ARGUMENT;
+  if (kr.n == 0 || c.n_seqs == 0) return PKV_OK;
+  cudaStream_t s = (cudaStream_t)stream;
+#define PKV_KV4_ROWS(D)                                                                                                    \
+  switch (k_rows->dtype) {                                                                                                 \
+    case PKV_DST_F32: launch_rows<D, PKV_DST_F32>(append, c, k, kr, v, vr, new_lens, err, s); break;                       \
+    case PKV_DST_F16: launch_rows<D, PKV_DST_F16>(append, c, k, kr, v, vr, new_lens, err, s); break;                       \
+    default: launch_rows<D, PKV_DST_BF16>(append, c, k, kr, v, vr, new_lens, err, s); break;                               \
+  }
+  if (cache->dim == 64) PKV_KV4_ROWS(64) else PKV_KV4_ROWS(128)
+#undef PKV_KV4_ROWS
+  pkv_count_launch();
+  return pkv_cuda_status(cudaGetLastError());
+}
+
+}  // namespace
+
+extern "C" int pkv_kv4_append_dev(const pkv_kv4_cache* cache, const void* k_dev, const pkv_kv4_rows* k_rows,
+                                  const void* v_dev, const pkv_kv4_rows* v_rows, const int32_t* new_lens_dev,
+                                  uint64_t* err_dev, void* stream) {
+  return rows_call(true, cache, k_dev, k_rows, v_dev, v_rows, new_lens_dev, err_dev, stream);
+}
+
+extern "C" int pkv_kv4_read_dev(const pkv_kv4_cache* cache, void* k_dev, const pkv_kv4_rows* k_rows, void* v_dev,
+                                const pkv_kv4_rows* v_rows, const int32_t* new_lens_dev, uint64_t* err_dev, void* stream) {
+  return rows_call(false, cache, k_dev, k_rows, v_dev, v_rows, new_lens_dev, err_dev, stream);
+}

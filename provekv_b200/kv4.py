@@ -1,0 +1,226 @@
+"""A KV cache that stays in 4 bits while a model decodes from it.
+
+The codecs of this package store a cache and give it back in f32 or 16 bits; between the two, a server that keeps many
+contexts resident wants the cache small while it is read at every step.  `Kv4Cache` is one layer's keys and values
+in pages of 4-bit codes (4.5 bits a value with the scales): `append` writes a step's vectors (or vectors the
+codecs decoded), `attend` is attention straight from the pages (shared kv heads, one query token or many, a sliding
+window with sinks), `evict` cuts a cache down to a budget by the attention weight its tokens received, and `read` gives
+values back.  The format and the exact meaning of each call are in include/provekv_b200.h (``pkv_kv4_*``).
+
+The lengths belong to the step, not to the layer: raise ``lens`` (and ``ends``) once, then call the layers::
+
+    lens += 1                                   # int32 [n_seqs], on the device, shared by all layers
+    for layer, cache in enumerate(caches):
+        cache.append(k, v)                      # [n_seqs, 1, n_kv_heads, dim]
+        out, lse = cache.attend(q)              # [n_seqs, 1, n_q_heads, dim]
+
+Calls only enqueue work on the current torch stream of the cache's device and allocate through torch, so they can be captured into a
+CUDA graph.  What a kernel finds wrong (a page number out of range, a value that is not finite) goes to the
+cache's error word: `check` reads it.
+"""
+from __future__ import annotations
+
+import ctypes as C
+
+from . import _lib as L
+from .patch import dst_dtype_of
+
+__all__ = ["Kv4Cache", "atom_bytes", "ATOM_TOKENS"]
+
+ATOM_TOKENS = 16
+
+
+def atom_bytes(dim: int) -> int:
+    """Bytes of 16 tokens of one kv head, keys and values."""
+    return 18 * dim
+
+
+def _rows(t, name: str, cache: "Kv4Cache", heads: int | None = None) -> L.Kv4RowsC:
+    if t.dim() != 4 or t.shape[0] != cache.n_seqs or t.shape[3] != cache.dim:
+        raise ValueError(f"{name} must be [{cache.n_seqs}][tokens][heads][{cache.dim}], not {tuple(t.shape)}")
+    if heads is not None and t.shape[2] != heads:
+        raise ValueError(f"{name} has {t.shape[2]} heads, the cache {heads}")
+    if t.device != cache.device:
+        raise ValueError(f"{name} is on {t.device}, the cache on {cache.device}")
+    if t.stride(3) != 1 and t.numel():
+        raise ValueError(f"the values of a vector of {name} must be contiguous")
+    return L.Kv4RowsC(t.stride(0), t.stride(1), t.stride(2), t.shape[1], dst_dtype_of(t))
+
+
+class Kv4Cache:
+    """One layer's cache over tensors the caller owns.
+
+    pages       uint8 [n_pages][n_kv_heads][page_tokens / 16][18 * dim], contiguous
+    page_table  int32 [n_seqs][max_pages]: the pages of each sequence
+    lens        int32 [n_seqs]: slots in use, a step's new tokens included
+    ends        int32 [n_seqs]: tokens the sequence has had (None: as many as it holds)
+    positions   int32 [n_seqs][n_kv_heads][max_pages * page_tokens]: position of the token in a slot (None: the slot's number)
+    mass        f32, the same shape: attention weight received
+    """
+
+    def __init__(self, pages, page_table, lens, *, ends=None, positions=None, mass=None):
+        import torch
+        if pages.dim() != 4 or pages.dtype != torch.uint8:
+            raise ValueError("pages must be uint8 [n_pages][n_kv_heads][page_tokens / 16][18 * dim]")
+        n_pages, self.n_kv_heads, atoms, width = pages.shape
+        self.dim, self.page_tokens, self.device = width // 18, atoms * ATOM_TOKENS, pages.device
+        if width not in (atom_bytes(64), atom_bytes(128)):
+            raise ValueError(f"an atom has 18 * 64 or 18 * 128 bytes, not {width}")
+        if page_table.dim() != 2:
+            raise ValueError("page_table must be [n_seqs][max_pages]")
+        self.n_seqs, max_pages = page_table.shape
+        self.capacity = max_pages * self.page_tokens
+        stats = (self.n_seqs, self.n_kv_heads, self.capacity)
+        for name, t, dtype, shape in (("pages", pages, torch.uint8, pages.shape), ("page_table", page_table, torch.int32, page_table.shape),
+                                      ("lens", lens, torch.int32, (self.n_seqs,)), ("ends", ends, torch.int32, (self.n_seqs,)),
+                                      ("positions", positions, torch.int32, stats), ("mass", mass, torch.float32, stats)):
+            if t is None:
+                continue
+            if t.dtype != dtype or tuple(t.shape) != tuple(shape):
+                raise ValueError(f"{name} must be {dtype} of shape {tuple(shape)}, not {t.dtype} of {tuple(t.shape)}")
+            if not t.is_contiguous():
+                raise ValueError(f"{name} must be contiguous")
+            if t.device != self.device:
+                raise ValueError(f"{name} is on {t.device}, the pages on {self.device}")
+        if self.device.type != "cuda":
+            raise ValueError("a Kv4Cache lives on a CUDA device")
+        self.pages, self.page_table, self.lens, self.ends, self.positions, self.mass = (
+            pages, page_table, lens, ends, positions, mass)
+        ptr = lambda t: None if t is None else t.data_ptr()  # noqa: E731
+        self._c = L.Kv4CacheC(ptr(pages), ptr(page_table), ptr(lens), ptr(ends), ptr(positions), ptr(mass), n_pages,
+                              self.dim, self.n_kv_heads, self.page_tokens, self.n_seqs, max_pages, 0)
+        self.error = torch.full((1,), -1, dtype=torch.int64, device=self.device)
+
+    @classmethod
+    def allocate(cls, n_layers: int, n_seqs: int, n_kv_heads: int, dim: int, max_tokens: int, *, page_tokens: int = 64,
+                 evictable: bool = False, device="cuda") -> list["Kv4Cache"]:
+        """Empty caches for `n_layers` layers that share page table, `lens` and `ends`; each sequence owns the pages of
+        `max_tokens` tokens.  `evictable`: with positions and mass."""
+        import torch
+        max_pages = -(-max_tokens // page_tokens)
+        table = torch.arange(n_seqs * max_pages, dtype=torch.int32, device=device).view(n_seqs, max_pages)
+        lens, ends = (torch.zeros(n_seqs, dtype=torch.int32, device=device) for _ in range(2))
+        out = []
+        for _ in range(n_layers):
+            pages = torch.zeros((n_seqs * max_pages, n_kv_heads, page_tokens // ATOM_TOKENS, atom_bytes(dim)), dtype=torch.uint8,
+                                device=device)
+            stats = (n_seqs, n_kv_heads, max_pages * page_tokens)
+            out.append(cls(pages, table, lens, ends=ends,
+                           positions=torch.zeros(stats, dtype=torch.int32, device=device) if evictable else None,
+                           mass=torch.zeros(stats, dtype=torch.float32, device=device) if evictable else None))
+        return out
+
+    # -- calls -----------------------------------------------------------------------------------------------------------
+    def _stream(self):
+        import torch
+        return torch.cuda.current_stream(self.device).cuda_stream
+
+    def _guard(self):
+        import torch
+        return torch.cuda.device(self.device)
+
+    def _per_seq(self, t, name: str):
+        import torch
+        if t is None:
+            return None
+        if t.dtype != torch.int32 or tuple(t.shape) != (self.n_seqs,) or not t.is_contiguous() or t.device != self.device:
+            raise ValueError(f"{name} must be a contiguous int32 [{self.n_seqs}] tensor on {self.device}")
+        return t.data_ptr()
+
+    def append(self, k, v, new_lens=None) -> None:
+        """Writes the newest tokens of each sequence: row i of ``k`` and ``v`` [n_seqs][n][n_kv_heads][dim] goes to slot
+        lens - n + i (with ``new_lens`` int32 [n_seqs]: the first new_lens[s] rows to lens - new_lens + i)."""
+        kr, vr = _rows(k, "k", self, self.n_kv_heads), _rows(v, "v", self, self.n_kv_heads)
+        if k.shape != v.shape:
+            raise ValueError("k and v must have the same shape")
+        if k.numel() == 0:
+            return
+        with self._guard():
+            L.check(L.lib().pkv_kv4_append_dev(C.byref(self._c), k.data_ptr(), C.byref(kr), v.data_ptr(), C.byref(vr),
+                                               self._per_seq(new_lens, "new_lens"), self.error.data_ptr(), self._stream()))
+
+    def read(self, n: int, dtype=None, new_lens=None, out=None):
+        """(k, v) [n_seqs][n][n_kv_heads][dim]: the values the newest tokens stand for, at the rows `append` would take
+        them from.  Rows from new_lens[s] on are zeros, or as they were in ``out`` = (k, v)."""
+        import torch
+        if out is None:
+            shape = (2, self.n_seqs, n, self.n_kv_heads, self.dim)
+            make = torch.empty if new_lens is None else torch.zeros
+            out = make(shape, dtype=dtype or torch.float32, device=self.device).unbind(0)
+        k, v = out
+        if k.shape[1] != n or (dtype is not None and k.dtype != dtype):
+            raise ValueError("out does not have the rows or the type asked for")
+        kr, vr = _rows(k, "k", self, self.n_kv_heads), _rows(v, "v", self, self.n_kv_heads)
+        if k.shape != v.shape:
+            raise ValueError("k and v must have the same shape")
+        if k.numel() == 0:
+            return k, v
+        with self._guard():
+            L.check(L.lib().pkv_kv4_read_dev(C.byref(self._c), k.data_ptr(), C.byref(kr), v.data_ptr(), C.byref(vr),
+                                             self._per_seq(new_lens, "new_lens"), self.error.data_ptr(), self._stream()))
+        return k, v
+
+    def attend(self, q, *, scale: float | None = None, window: int = 0, sinks: int = 0, q_lens=None, accumulate: bool = False,
+               max_len: int = 0, out=None, lse=None):
+        """(out, lse): attention of the newest tokens' queries ``q`` [n_seqs][n][n_q_heads][dim] over what their
+        sequences hold, each up to its own position.
+
+        scale       of the products; None: dim ** -0.5
+        window      > 0: only the `window` newest positions, and those below `sinks`
+        q_lens      int32 [n_seqs]: the first q_lens[s] rows are sequence s's newest tokens, the others padding (zeros in a new
+                    ``out``, untouched in a given one; the same for ``lse``)
+        accumulate  adds the weights of these queries to ``mass``
+        max_len     a bound on the lengths that the host knows (sizes the split of the work; any value is correct)
+        lse         f32 [n_seqs][n][n_q_heads], natural logarithm; -inf where a query sees nothing (its out is zeros)
+        """
+        import torch
+        if accumulate and self.mass is None:
+            raise ValueError("accumulate needs a cache with mass")
+        qr = _rows(q, "q", self)
+        make = torch.empty if q_lens is None else torch.zeros
+        if out is None:
+            out = make(q.shape, dtype=q.dtype, device=self.device)
+        elif out.shape != q.shape or out.dtype != q.dtype:
+            raise ValueError("out must have the shape and type of q")
+        outr = _rows(out, "out", self)
+        if lse is None:
+            lse = make(q.shape[:3], dtype=torch.float32, device=self.device)
+        elif lse.shape != q.shape[:3] or lse.dtype != torch.float32 or not lse.is_contiguous() or lse.device != self.device:
+            raise ValueError("lse must be contiguous f32 [n_seqs][tokens][heads] on the cache's device")
+        if q.numel() == 0:
+            return out, lse
+        args = L.Kv4AttendC(self.dim ** -0.5 if scale is None else scale, q.shape[2], window, sinks, int(accumulate), max_len)
+        lib = L.lib()
+        with self._guard():
+            need = lib.pkv_kv4_attend_workspace_bytes(C.byref(self._c), C.byref(qr), C.byref(args))
+            work = torch.empty(need, dtype=torch.uint8, device=self.device) if need else None
+            L.check(lib.pkv_kv4_attend_dev(C.byref(self._c), q.data_ptr(), C.byref(qr), out.data_ptr(), C.byref(outr), lse.data_ptr(),
+                                           self._per_seq(q_lens, "q_lens"), C.byref(args), work.data_ptr() if need else None, need,
+                                           self.error.data_ptr(), self._stream()))
+        return out, lse
+
+    def evict(self, budget: int, *, sinks: int = 0, recent: int = 0) -> None:
+        """Cuts every sequence longer than `budget` down to it, per kv head: positions below `sinks`, the `recent` newest
+        positions, and the heaviest of the others stay (ties: the lowest slot).  Then ``lens.clamp_(max=budget)``, once
+        all layers are done."""
+        import torch
+        if self.positions is None or self.mass is None:
+            raise ValueError("evict needs a cache with positions and mass")
+        if self.n_seqs == 0:
+            return
+        lib = L.lib()
+        with self._guard():
+            need = lib.pkv_kv4_evict_workspace_bytes(C.byref(self._c), budget)
+            work = torch.empty(need, dtype=torch.uint8, device=self.device) if need else None
+            L.check(lib.pkv_kv4_evict_dev(C.byref(self._c), budget, sinks, recent, work.data_ptr() if need else None, need,
+                                          self.error.data_ptr(), self._stream()))
+
+    def check(self) -> None:
+        """Waits for the stream, raises PkvError for the first thing a kernel reported since the last check, and clears it."""
+        code, index = C.c_int32(0), C.c_int64(-1)
+        with self._guard():
+            s = self._stream()
+            st = L.lib().pkv_error_word_read(self.error.data_ptr(), s, C.byref(code), C.byref(index))
+            if st != L.OK:
+                L.check(L.lib().pkv_error_word_reset(self.error.data_ptr(), s))
+                raise L.PkvError(st, L.status_string(st), index.value)

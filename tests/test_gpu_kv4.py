@@ -1,0 +1,608 @@
+"""The 4-bit KV cache on the GPU against plain 64-bit arithmetic (kv4ref): codes bit for bit, attention within bounds
+derived below, evictions row for row."""
+import numpy as np
+import pytest
+
+import kv4ref
+import provekv_b200 as pk
+from provekv_b200 import _lib as L
+from provekv_b200 import kv4
+
+pytestmark = pytest.mark.gpu
+
+
+def _dt(name):
+    import torch
+    return getattr(torch, name)
+
+
+def _dev(a, dtype=None):
+    import torch
+    t = torch.from_numpy(np.ascontiguousarray(a))
+    return (t if dtype is None else t.to(dtype)).cuda()
+
+
+def _ints(a):
+    import torch
+    return _dev(np.asarray(a, np.int32), torch.int32)
+
+
+def _empty_cache(n_seqs, heads, dim, page_tokens, max_pages, rng, lens, **kw):
+    import torch
+    pages = torch.from_numpy(rng.integers(0, 256, (n_seqs * max_pages + 1, heads, page_tokens // 16, 18 * dim)).astype(np.uint8)).cuda()
+    table = torch.randperm(n_seqs * max_pages + 1)[:n_seqs * max_pages].view(n_seqs, max_pages).int().cuda()
+    return kv4.Kv4Cache(pages, table, _ints(lens), **kw)
+
+
+# -- append and read --------------------------------------------------------------------------------------------------
+def _hard_rows(rng, n, dim, dtype):
+    """Rows whose quotients sit on and beside ties, zero blocks, blocks below the smallest scale, large ones."""
+    import torch
+    x = rng.standard_normal((n, dim)) * np.exp(rng.uniform(-9, 6, (n, 1)))
+    b = x.reshape(n, -1, 16)
+    s = kv4ref.SCALES[rng.integers(24, 0xA0, b.shape[:2])]
+    ties = (rng.integers(-8, 8, b.shape) + 0.5) * s[..., None]
+    ties[..., 0] = 7 * s                                   # the block's scale is s itself
+    b[:n // 2] = np.where(np.abs(ties) <= 7 * s[..., None], ties, 0.0)[:n // 2]
+    b[n // 8] *= 1 + 2.0 ** -12
+    b[n // 4] *= 1 - 2.0 ** -23
+    b[-1] = 0.0
+    b[-2] *= 1e-7
+    b[-3] = rng.standard_normal(b[-3].shape) * 2.0 ** -16  # scales below 2^-14
+    b[-4] *= 7e4 / max(1.0, np.abs(b[-4]).max()) * 0.7     # close to the largest scale
+    b[-5, :, :] = 7 * 2.0 ** -14 * rng.choice([-1, 1, 0.5], b[-5].shape)
+    amax = 3.5 * (kv4ref.SCALES[0x40] + kv4ref.SCALES[0x41])
+    b[-6] = amax * rng.choice([1, -0.3, 0.7], b[-6].shape)  # amax / 7 half way between two scales
+    return torch.from_numpy(x).to(dtype)
+
+
+@pytest.mark.parametrize("dtype", ["float32", "float16", "bfloat16"])
+@pytest.mark.parametrize("dim,heads,page", [(64, 3, 16), (128, 2, 64), (128, 1, 48)])
+def test_append_writes_the_definition_and_read_gives_it_back(dtype, dim, heads, page):
+    import torch
+    rng = np.random.default_rng(dim + page)
+    n, seqs = 37, 3
+    lens, new = [37, 60, 45], [37, 20, 1]
+    cache = _empty_cache(seqs, heads, dim, page, -(-64 // page) + 1, rng, lens)
+    before = cache.pages.cpu().numpy().copy()
+    k, v = (_hard_rows(rng, seqs * n * heads, dim, _dt(dtype)).view(seqs, n, heads, dim) for _ in range(2))
+    cache.append(k.cuda(), v.cuda(), _ints(new))
+    cache.check()
+    want, table = before.copy(), cache.page_table.cpu().numpy()
+    values = np.zeros((2, seqs, n, heads, dim))
+    for s in range(seqs):
+        for i in range(new[s]):
+            slot = lens[s] - new[s] + i
+            for h in range(heads):
+                for side, x in enumerate((k, v)):
+                    codes, sc = kv4ref.quantise(x[s, i, h].double().numpy())
+                    kv4ref.put_row(want[table[s, slot // page]], h, slot % page, side, codes, sc, dim)
+                    values[side, s, i, h] = kv4ref.dequantise(codes, sc)
+    got = cache.pages.cpu().numpy()
+    assert np.array_equal(got, want), np.argwhere(got != want)[:5]
+    for t in (torch.float32, torch.float16, torch.bfloat16):
+        for side, r in enumerate(cache.read(n, t, _ints(new))):
+            assert r.dtype == t and np.array_equal(r.double().cpu().numpy(), values[side])
+    # rows behind a sequence's last stay as they were in a given output
+    out = torch.full((2, seqs, n, heads, dim), 5.0, device="cuda").unbind(0)
+    cache.read(n, None, _ints(new), out)
+    for side in range(2):
+        for s in range(seqs):
+            assert (out[side][s, new[s]:] == 5.0).all() and np.array_equal(out[side][s, :new[s]].double().cpu().numpy(), values[side, s, :new[s]])
+    cache.check()
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+def test_append_takes_strided_rows_and_keeps_statistics(dtype):
+    import torch
+    rng = np.random.default_rng(5)
+    seqs, heads, dim, page, n = 2, 4, 64, 32, 9
+    lens, ends = [9, 40], [9, 100]
+    pos = torch.full((seqs, heads, 64), -7, dtype=torch.int32, device="cuda")
+    mass = torch.full((seqs, heads, 64), 3.0, device="cuda")
+    cache = _empty_cache(seqs, heads, dim, page, 2, rng, lens, ends=_ints(ends), positions=pos, mass=mass)
+    packed = _dev(rng.standard_normal((n, seqs, 3 * heads, dim)), _dt(dtype))  # token first, K, V and something else side by side
+    k, v = packed[:, :, :heads].transpose(0, 1), packed[:, :, heads:2 * heads].transpose(0, 1)
+    cache.append(k, v)
+    cache.check()
+    for side, got in enumerate(cache.read(n, _dt(dtype))):
+        x = (k, v)[side].double().cpu().numpy()
+        assert np.array_equal(got.double().cpu().numpy(), kv4ref.dequantise(*kv4ref.quantise(x)))
+    for s in range(seqs):
+        first = lens[s] - n
+        assert (pos[s, :, first:lens[s]].cpu() == torch.arange(ends[s] - n, ends[s])).all()
+        assert (mass[s, :, first:lens[s]] == 0).all()
+        assert (pos[s, :, :first] == -7).all() and (pos[s, :, lens[s]:] == -7).all()
+        assert (mass[s, :, :first] == 3).all() and (mass[s, :, lens[s]:] == 3).all()
+
+
+def test_rows_that_cannot_be_stored_are_reported_and_become_zeros():
+    import torch
+    rng = np.random.default_rng(6)
+    cache = _empty_cache(2, 3, 64, 16, 2, rng, [5, 7])
+    k, v = (_dev(rng.standard_normal((2, 5, 3, 64)), torch.float32) for _ in range(2))
+    v[1, 2, 1, 40] = float("inf")
+    k[1, 4, 0, 3] = 7.0 * 7500
+    v[0, 3, 2, 63] = float("nan")
+    cache.append(k, v)
+    with pytest.raises(pk.PkvError) as e:
+        cache.check()
+    assert (e.value.status, e.value.vector_index) == (L.VEC_NONFINITE_INPUT, ((0 * 5 + 3) * 3 + 2) * 2 + 1)
+    cache.check()  # read and cleared
+    gk, gv = cache.read(5)
+    assert (gv[1, 2, 1] == 0).all() and (gk[1, 4, 0] == 0).all() and (gv[0, 3, 2] == 0).all()
+    assert (gk[1, 2, 1] != 0).any() and (gv[1, 4, 0] != 0).any()
+    k2, v2 = k.clone(), v.clone().nan_to_num(0, 0, 0)
+    cache.append(k2, v2)
+    with pytest.raises(pk.PkvError) as e:
+        cache.check()
+    assert (e.value.status, e.value.vector_index) == (L.VEC_NORM_RANGE, ((1 * 5 + 4) * 3 + 0) * 2)
+
+
+def test_bad_lengths_and_pages_are_reported_and_skipped():
+    import torch
+    rng = np.random.default_rng(7)
+    cache = _empty_cache(4, 2, 128, 16, 4, rng, [20, 65, -1, 30])
+    cache.page_table[3, 1] = cache.pages.shape[0]
+    cache.page_table[0, 0] = -5
+    before = cache.pages.clone()
+    x = _dev(rng.standard_normal((4, 20, 2, 128)), torch.bfloat16)
+    cache.append(x, x)
+    with pytest.raises(pk.PkvError) as e:
+        cache.check()
+    assert (e.value.status, e.value.vector_index) == (L.VEC_BAD_SEQUENCE, 0)
+    changed = set((cache.pages != before).flatten(1).any(1).nonzero().flatten().tolist())
+    assert changed == {int(cache.page_table[0, 1]), int(cache.page_table[3, 0])}
+    q = _dev(rng.standard_normal((4, 1, 4, 128)), torch.bfloat16)
+    out, lse = cache.attend(q)
+    with pytest.raises(pk.PkvError) as e:
+        cache.check()
+    assert (e.value.status, e.value.vector_index) == (L.VEC_BAD_SEQUENCE, 0)
+    assert (out[1] == 0).all() and (out[2] == 0).all() and torch.isinf(lse[1:3]).all()
+    # the tokens of the good pages alone
+    table, pages = cache.page_table.cpu().numpy(), cache.pages.cpu().numpy()
+    val = kv4ref.decode_all(pages, table[:, 1:], [4, 0, 0, 0], 128)
+    want, wlse, _, A, D, V = kv4ref.attend(q.double().cpu().numpy(), val, [4, 0, 0, 0], [4, 1, 1, 4], None, 2, 128 ** -0.5, 0, 0, [1, 1, 1, 1])
+    _close(out[:1], lse[:1], want[:1], wlse[:1], A[:1], D[:1], V[:1])
+    bad = _ints([1, 2, 0, -1])
+    cache.lens.copy_(_ints([20, 20, 20, 20]))
+    cache.page_table[0, 0], cache.page_table[3, 1] = 0, 0
+    out, lse = torch.full_like(q, 9.0), torch.full((4, 1, 4), 9.0, device="cuda")
+    cache.attend(q, q_lens=bad, out=out, lse=lse)
+    with pytest.raises(pk.PkvError) as e:
+        cache.check()
+    assert (e.value.status, e.value.vector_index) == (L.VEC_BAD_SEQUENCE, 1)
+    assert (out[0] != 9).any() and (out[1:] == 9).all() and (lse[1:] == 9).all()
+
+
+# -- attention ------------------------------------------------------------------------------------------------------------
+def _within(got, want, tol, what):
+    off = np.abs(got - want) - tol
+    if not (off <= 0).all():
+        at = np.unravel_index(np.nanargmax(np.where(np.isnan(off), np.inf, off)), off.shape)
+        raise AssertionError(f"{what} at {at}: {got[at]} is not {want[at]} within {np.broadcast_to(tol, off.shape)[at]}")
+
+
+def _close(out, lse, want, wlse, A, D, V):
+    """Scores are f32 sums of dim exact products in at most 2 dim / 16 steps of the tensor cores, each within 2^-22 of the
+    largest partial sum, and three f32 roundings after: off by at most eps = 2^-18 D.  A weight is then within a
+    factor exp(2 eps) (its own error and its sum's) of the true one, and enters the second product in binary16 (2^-11; f32
+    queries: two terms, 2^-21).  So out is off by (w + 2 eps + 2^-18) A plus its own rounding.
+    Binary16 ends at 2^-25 (half its last subnormal): weights are kept 2^7 and more times too large, so a key of whatever weight
+    is also off by up to 2^-32 of the row's largest weight, which is below 1 after the division by the sum: 2^-32 sum |v|."""
+    import torch
+    w, unit = {torch.float32: (2.0 ** -21, 2.0 ** -24), torch.float16: (2.0 ** -11, 2.0 ** -11),
+               torch.bfloat16: (2.0 ** -11, 2.0 ** -8)}[out.dtype]
+    got, glse = out.double().cpu().numpy(), lse.double().cpu().numpy()
+    eps = 2.0 ** -18 * D[..., None]
+    tol = (w + 2 * eps + 2.0 ** -18) * A + 2.0 ** -32 * V + unit * np.abs(want) + (2.0 ** -25 if out.dtype == torch.float16 else 0.0)
+    _within(got, want, tol, "out")
+    none = np.isinf(wlse)
+    assert np.array_equal(none, np.isneginf(glse)) and not np.isnan(glse).any()
+    _within(glse[~none], wlse[~none], (eps[..., 0] + 2.0 ** -22 * np.abs(wlse) + 2.0 ** -20)[~none], "lse")
+
+
+def _attend_case(seed, dtype, dim, heads, group, page, lens, q_len, window, sinks, moved, accumulate, q_lens=None, max_len=0,
+                 scale=None):
+    import torch
+    rng = np.random.default_rng(seed)
+    S = len(lens)
+    pages, table, values = kv4ref.fill(rng, S, heads, dim, page, lens)
+    cap = table.shape[1] * page
+    ends, pos = np.asarray(lens), None
+    if moved:
+        ends = np.asarray(lens) + rng.integers(0, 50, S)
+        pos = np.zeros((S, heads, cap), np.int32)
+        for s, n in enumerate(lens):
+            for h in range(heads):
+                pos[s, h, :n] = rng.permutation(int(ends[s]))[:n]
+    mass = _dev(np.abs(rng.standard_normal((S, heads, cap))), torch.float32) if accumulate else None
+    mass0 = mass.double().cpu().numpy() if accumulate else None
+    cache = kv4.Kv4Cache(_dev(pages), _ints(table), _ints(lens), ends=_ints(ends) if moved else None,
+                         positions=_ints(pos) if moved else None, mass=mass)
+    q = _dev(rng.standard_normal((S, q_len, heads * group, dim)) * 2, _dt(dtype))
+    ql = q_lens if q_lens is not None else [q_len] * S
+    before = cache.pages.clone()
+    out, lse = cache.attend(q, scale=scale, window=window, sinks=sinks, accumulate=accumulate, max_len=max_len,
+                            q_lens=None if q_lens is None else _ints(q_lens))
+    cache.check()
+    assert torch.equal(before, cache.pages)
+    want = kv4ref.attend(q.double().cpu().numpy(), values, lens, ends, pos, group, dim ** -0.5 if scale is None else scale, window, sinks, ql)
+    for s in range(S):  # padding rows of a fresh output are zeros
+        assert (out[s, ql[s]:] == 0).all() and (lse[s, ql[s]:] == 0).all()
+        want[1][s, ql[s]:] = 0.0
+    _close(out, lse, want[0], want[1], *want[3:])
+    if accumulate:
+        got = mass.double().cpu().numpy()
+        full = mass0.copy()
+        full[:, :, :values.shape[3]] += want[2]
+        eps = 2.0 ** -18 * want[4].max() + 2.0 ** -22 * np.abs(want[1][~np.isinf(want[1])]).max(initial=0.0) + 2.0 ** -19
+        _within(got, full, 2 * eps * (full - mass0) + 2.0 ** -23 * full, "mass")
+        assert np.array_equal(got[full == mass0], mass0[full == mass0])  # what no query saw is untouched
+    return cache, q, out, lse
+
+
+@pytest.mark.parametrize("dtype", ["float32", "float16", "bfloat16"])
+@pytest.mark.parametrize("dim,heads,group,page", [(64, 2, 7, 16), (128, 2, 4, 64), (64, 3, 1, 48), (128, 1, 12, 32)])
+@pytest.mark.parametrize("lens", [[1], [0, 16, 17, 33], [31, 32, 200]])
+def test_single_tokens(dtype, dim, heads, group, page, lens):
+    _attend_case(dim + len(lens), dtype, dim, heads, group, page, lens, 1, 0, 0, False, False)
+
+
+@pytest.mark.parametrize("dtype", ["float32", "float16", "bfloat16"])
+@pytest.mark.parametrize("window,sinks", [(1, 0), (16, 0), (40, 4), (33, 40), (500, 3), (5, 1000)])
+@pytest.mark.parametrize("moved", [False, True])
+def test_windows_and_sinks(dtype, window, sinks, moved):
+    _attend_case(window + sinks, dtype, 128, 2, 3, 32, [0, 5, 77, 210], 1, window, sinks, moved, True)
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("q_len,group", [(2, 1), (3, 4), (5, 7), (33, 2), (40, 1)])
+@pytest.mark.parametrize("window,sinks,moved", [(0, 0, False), (20, 3, False), (0, 0, True), (30, 2, True)])
+def test_several_tokens_are_causal(dtype, dim, q_len, group, window, sinks, moved):
+    _attend_case(q_len * group, dtype, dim, 2, group, 16, [40, 41, 131], q_len, window, sinks, moved, True)
+
+
+def test_padded_queries_and_more_queries_than_tokens():
+    # 3 of 6 rows are padding in the first sequence, none in the second, all in the third; the fourth has fewer tokens than queries
+    _attend_case(3, "float16", 128, 2, 2, 16, [30, 6, 12, 4], 6, 0, 0, False, True, q_lens=[3, 6, 0, 5])
+    _attend_case(4, "float32", 64, 2, 2, 16, [30, 6, 12, 4], 6, 3, 1, True, True, q_lens=[3, 6, 0, 4])
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+def test_long_rows_are_split_and_joined(dtype):
+    _attend_case(11, dtype, 64, 1, 2, 128, [3001], 1, 0, 0, False, True)
+    _attend_case(12, dtype, 128, 1, 9, 64, [700, 1500], 1, 0, 0, False, False)
+    _attend_case(13, dtype, 128, 1, 2, 64, [1700], 4, 900, 70, False, True)
+    # a bound that is too small only makes the last part longer
+    _attend_case(14, dtype, 64, 1, 2, 64, [1700, 3], 1, 0, 0, False, True, max_len=600)
+
+
+def test_a_longer_query_chunk():
+    _attend_case(21, "bfloat16", 128, 1, 4, 64, [300], 200, 0, 0, False, True)
+    _attend_case(22, "float16", 64, 2, 2, 48, [150, 260], 130, 50, 5, False, False, q_lens=[130, 77])
+
+
+def test_large_and_small_scales_of_queries():
+    """Rows of q far from 1 in either direction keep their bits (a power of two per row)."""
+    for dtype, f in (("float32", 1e20), ("float32", 1e-20), ("bfloat16", 1e-30), ("bfloat16", 1e15), ("float16", 1e-4)):
+        import torch
+        rng = np.random.default_rng(31)
+        pages, table, values = kv4ref.fill(rng, 1, 1, 64, 16, [50])
+        cache = kv4.Kv4Cache(_dev(pages), _ints(table), _ints([50]))
+        q = _dev(rng.standard_normal((1, 1, 2, 64)) * f, _dt(dtype))
+        scale = 0.125 / f
+        out, lse = cache.attend(q, scale=scale)
+        s32 = float(np.float32(scale))
+        want = kv4ref.attend(q.double().cpu().numpy(), values, [50], [50], None, 2, s32, 0, 0, [1])
+        _close(out, lse, want[0], want[1], *want[3:])
+
+
+def test_queries_that_are_not_finite_spoil_their_own_rows_only():
+    import torch
+    rng = np.random.default_rng(32)
+    pages, table, _ = kv4ref.fill(rng, 2, 2, 128, 16, [50, 3000])
+    cache = kv4.Kv4Cache(_dev(pages), _ints(table), _ints([50, 3000]))
+    q = _dev(rng.standard_normal((2, 1, 8, 128)), torch.bfloat16)
+    clean, _ = cache.attend(q)
+    q2 = q.clone()
+    q2[0, 0, 3, 5] = float("nan")
+    q2[1, 0, 6, 100] = float("inf")
+    out, lse = cache.attend(q2)
+    spoilt = torch.zeros((2, 1, 8), dtype=torch.bool, device="cuda")
+    spoilt[0, 0, 3] = spoilt[1, 0, 6] = True
+    assert torch.isnan(out[spoilt]).all() and torch.isnan(lse[spoilt]).all()
+    assert torch.equal(out[~spoilt], clean[~spoilt])
+
+
+def test_sequences_may_share_a_prefix_and_repeat_a_page():
+    import torch
+    rng = np.random.default_rng(33)
+    pages, table, values = kv4ref.fill(rng, 2, 2, 64, 16, [64, 64])
+    table[1, :2] = table[0, :2]
+    table[1, 2] = table[0, 1]
+    values[1, :, :, :32] = values[0, :, :, :32]
+    values[1, :, :, 32:48] = values[0, :, :, 16:32]
+    cache = kv4.Kv4Cache(_dev(pages), _ints(table), _ints([64, 64]))
+    q = _dev(rng.standard_normal((2, 1, 4, 64)), torch.float16)
+    out, lse = cache.attend(q)
+    want = kv4ref.attend(q.double().cpu().numpy(), values, [64, 64], [64, 64], None, 2, 0.125, 0, 0, [1, 1])
+    _close(out, lse, want[0], want[1], *want[3:])
+
+
+def test_strided_queries_and_outputs():
+    import torch
+    rng = np.random.default_rng(34)
+    pages, table, values = kv4ref.fill(rng, 2, 2, 64, 16, [30, 55])
+    cache = kv4.Kv4Cache(_dev(pages), _ints(table), _ints([30, 55]))
+    packed = _dev(rng.standard_normal((3, 2, 12, 64)), torch.float32)
+    q = packed[:, :, 4:10].transpose(0, 1)
+    room = torch.full((2, 6, 4, 72), 7.0, device="cuda")
+    out = room[..., 4:68].transpose(1, 2)[:, :3]
+    got, lse = cache.attend(q, out=out)
+    assert got.data_ptr() == out.data_ptr()
+    want = kv4ref.attend(q.double().cpu().numpy(), values, [30, 55], [30, 55], None, 3, 0.125, 0, 0, [3, 3])
+    _close(out, lse, want[0], want[1], *want[3:])
+    assert (room[..., :4] == 7).all() and (room[..., 68:] == 7).all() and (room[:, :, 3] == 7).all()
+
+
+def test_the_class_refuses():
+    import torch
+    rng = np.random.default_rng(35)
+    cache = _empty_cache(2, 2, 64, 16, 4, rng, [5, 7])
+    q = torch.zeros((2, 1, 4, 64), device="cuda")
+    for bad in (dict(accumulate=True), dict(out=torch.zeros((2, 1, 4, 64), device="cuda", dtype=torch.float16)),
+                dict(lse=torch.zeros((2, 1, 3), device="cuda")), dict(q_lens=torch.zeros(2, device="cuda"))):
+        with pytest.raises(ValueError):
+            cache.attend(q, **bad)
+    with pytest.raises(ValueError):
+        cache.attend(q[:1])
+    with pytest.raises(ValueError):
+        cache.attend(q.cpu())
+    with pytest.raises(TypeError):
+        cache.attend(q.double())
+    with pytest.raises(pk.PkvError) as e:
+        cache.attend(torch.zeros((2, 1, 3, 64), device="cuda"))
+    assert e.value.status == L.ERR_INVALID_ARGUMENT
+    with pytest.raises(ValueError):
+        cache.evict(4)
+    with pytest.raises(ValueError):
+        cache.append(q[:, :, :2], q[:, :, :3])
+    with pytest.raises(ValueError):
+        cache.read(3, torch.float16, out=(q[:, :, :2], q[:, :, :2]))
+    cache.check()
+
+
+# -- eviction ---------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dim,heads,page", [(64, 2, 16), (128, 3, 64)])
+@pytest.mark.parametrize("lens,budget,sinks,recent", [([100, 64, 65, 0], 64, 4, 16), ([1500, 1100], 1030, 0, 0), ([90, 128], 20, 10, 10),
+                                                      ([300, 77], 1, 0, 1), ([200], 199, 3, 60)])
+def test_evictions(dim, heads, page, lens, budget, sinks, recent):
+    import torch
+    rng = np.random.default_rng(len(lens) + budget)
+    S = len(lens)
+    pages, table, _ = kv4ref.fill(rng, S, heads, dim, page, [min(n, 130) for n in lens])
+    max_pages = -(-max(lens) // page)
+    if table.shape[1] < max_pages:  # the rows are random bytes there
+        pages = rng.integers(0, 256, (S * max_pages, heads, page // 16, 18 * dim)).astype(np.uint8)
+        table = rng.permutation(S * max_pages).reshape(S, max_pages).astype(np.int32)
+    else:
+        table = np.maximum(table, 0)
+    cap = table.shape[1] * page
+    ends = np.asarray(lens) + rng.integers(0, 40, S)
+    pos, mass = np.full((S, heads, cap), -1, np.int32), np.zeros((S, heads, cap), np.float32)
+    for s, n in enumerate(lens):
+        for h in range(heads):
+            pos[s, h, :n] = rng.permutation(int(ends[s]))[:n]
+            mass[s, h, :n] = np.exp(3 * rng.standard_normal(n))
+            mass[s, h, :n][rng.random(n) < 0.3] = rng.choice([0.0, 0.5, 0.25, np.inf, 1e-42])  # many equal
+            if n > 20:
+                mass[s, h, 3], mass[s, h, 11] = np.nan, -1.0
+    cache = kv4.Kv4Cache(_dev(pages), _ints(table), _ints(lens), ends=_ints(ends), positions=_ints(pos), mass=_dev(mass))
+    want_pages, want_pos, want_mass = pages.copy(), pos.copy(), mass.copy()
+    for s, n in enumerate(lens):
+        for h in range(heads):
+            for to, fro in kv4ref.evict(pos[s, h], mass[s, h].astype(np.float64), n, int(ends[s]), budget, sinks, recent):
+                for side in range(2):
+                    codes, sc = kv4ref.get_row(pages[table[s, fro // page]], h, fro % page, side, dim)
+                    kv4ref.put_row(want_pages[table[s, to // page]], h, to % page, side, codes, sc, dim)
+                want_pos[s, h, to], want_mass[s, h, to] = pos[s, h, fro], mass[s, h, fro]
+    cache.evict(budget, sinks=sinks, recent=recent)
+    cache.check()
+    assert np.array_equal(cache.positions.cpu().numpy(), want_pos)
+    assert np.array_equal(cache.mass.cpu().numpy().view(np.uint32), want_mass.view(np.uint32))
+    got = cache.pages.cpu().numpy()
+    assert np.array_equal(got, want_pages), np.argwhere(got != want_pages)[:5]
+    assert cache.lens.tolist() == lens
+
+
+def test_eviction_of_a_sequence_longer_than_shared_memory_holds():
+    import torch
+    rng = np.random.default_rng(41)
+    n, budget, heads, page = 60000, 20000, 1, 64
+    cap = -(-n // page) * page
+    pages = torch.from_numpy(rng.integers(0, 256, (cap // page, heads, page // 16, 18 * 64)).astype(np.uint8))
+    table = np.arange(cap // page, dtype=np.int32)[None]
+    pos, mass = np.arange(cap, dtype=np.int32).reshape(1, 1, cap), rng.random((1, 1, cap)).astype(np.float32)
+    mass[..., ::7] = 0.5
+    cache = kv4.Kv4Cache(pages.cuda(), _ints(table), _ints([n]), positions=_ints(pos), mass=_dev(mass))
+    moves = kv4ref.evict(pos[0, 0], mass[0, 0].astype(np.float64), n, n, budget, 4, 100)
+    cache.evict(budget, sinks=4, recent=100)
+    cache.check()
+    to, fro = np.array(moves).T
+    want = pos[0, 0].copy()
+    want[to] = fro
+    assert np.array_equal(cache.positions.cpu().numpy()[0, 0], want)
+    k = cache.read(n)[0][0, :, 0].cpu().numpy()
+    cache2 = kv4.Kv4Cache(pages.cuda(), _ints(table), _ints([n]))
+    k2 = cache2.read(n)[0][0, :, 0].cpu().numpy()
+    assert np.array_equal(k[to].view(np.uint32), k2[fro].view(np.uint32))
+
+
+# -- together --------------------------------------------------------------------------------------------------------------
+def _steps(caches, steps, budget, gen, dtype, collect):
+    import torch
+    lens, ends = caches[0].lens, caches[0].ends
+    for n in steps:
+        lens += n
+        ends += n
+        for c in caches:
+            k, v = (torch.randn((c.n_seqs, n, c.n_kv_heads, c.dim), generator=gen, device="cuda", dtype=torch.float32).to(dtype) for _ in range(2))
+            q = torch.randn((c.n_seqs, n, 2 * c.n_kv_heads, c.dim), generator=gen, device="cuda", dtype=torch.float32).to(dtype)
+            c.append(k, v)
+            out, lse = c.attend(q, accumulate=True, window=40, sinks=2)
+            c.evict(budget, sinks=2, recent=10)
+            collect.append((c, k, v, q, out, lse))
+        lens.clamp_(max=budget)
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+def test_append_attend_evict_over_many_steps(dtype):
+    """A prompt, then tokens one by one and in drafts, two layers: at every step the attention equals that of a plain model
+    of the cache (a list of (position, key, value, mass) per head)."""
+    import torch
+    gen = torch.Generator(device="cuda").manual_seed(1)
+    S, H, d, budget = 2, 2, 64, 48
+    caches = kv4.Kv4Cache.allocate(2, S, H, d, 96, page_tokens=16, evictable=True)
+    log = []
+    steps = [40, 1, 1, 3, 1, 8, 1, 1, 20, 1]
+    _steps(caches, steps, budget, gen, _dt(dtype), log)
+    for c in caches:
+        c.check()
+    model = {id(c): [[[] for _ in range(H)] for _ in range(S)] for c in caches}
+    end, at = 0, 0
+    for n in steps:
+        end += n
+        for c in caches:
+            _, k, v, q, out, lse = log[at]
+            at += 1
+            kq, vq = (kv4ref.dequantise(*kv4ref.quantise(t.double().cpu().numpy())) for t in (k, v))
+            q = q.double().cpu().numpy()
+            for s in range(S):
+                for h in range(H):
+                    held = model[id(c)][s][h]
+                    held += [[end - n + i, kq[s, i, h], vq[s, i, h], 0.0] for i in range(n)]
+                    val = np.stack([np.stack([e[1] for e in held]), np.stack([e[2] for e in held])])[None, :, None]
+                    pos = np.array([e[0] for e in held])[None, None]
+                    w = kv4ref.attend(q[s:s + 1, :, 2 * h:2 * h + 2], val, [len(held)], [end], pos, 2, d ** -0.5, 40, 2, [n])
+                    _close(out[s:s + 1, :, 2 * h:2 * h + 2], lse[s:s + 1, :, 2 * h:2 * h + 2], w[0], w[1], *w[3:])
+                    for e, m in zip(held, w[2][0, 0]):
+                        e[3] += m
+                    # the gaps between weights are far above their error for these inputs, so the choice is the same
+                    for to, fro in kv4ref.evict(pos[0, 0], np.array([e[3] for e in held]), len(held), end, budget, 2, 10):
+                        held[to] = held[fro]
+                    del held[budget:]
+    for c in caches:
+        pos = c.positions.cpu().numpy()
+        for s in range(S):
+            for h in range(H):
+                assert [e[0] for e in model[id(c)][s][h]] == pos[s, h, :budget].tolist()
+
+
+def test_a_decoded_pool_becomes_resident():
+    """Vectors of a compressed shell, decoded to f32, go into the 4-bit cache and are attended to."""
+    import torch
+    from provekv_b200 import pool
+    d, H, T = 64, 2, 50
+    prof = pk.TurboProfile.from_seed(d, 4, 32, 42)
+    x = torch.randn((T * H, d), device="cuda")
+    stride = pool.payload_batch_stride(T * H, prof.record_bytes)
+    payload = torch.zeros(stride, dtype=torch.uint8, device="cuda")
+    err = torch.full((1,), -1, dtype=torch.int64, device="cuda")
+    lay = L.Layout.make(n_tokens=T, n_heads=H, token_stride=H * d, head_stride=d)
+    prof.encode_dev(x.data_ptr(), lay, payload.data_ptr(), stride, err.data_ptr())
+    dec = torch.empty((1, T, H, d), device="cuda")
+    prof.decode_patch_dev(payload.data_ptr(), stride, lay, dec.data_ptr(), err.data_ptr())
+    pk.read_error_word(err.data_ptr())
+    (cache,) = kv4.Kv4Cache.allocate(1, 1, H, d, T)
+    cache.lens += T
+    cache.append(dec, dec)
+    k, _ = cache.read(T)
+    cache.check()
+    want = kv4ref.dequantise(*kv4ref.quantise(dec.double().cpu().numpy()))
+    assert np.array_equal(k.double().cpu().numpy(), want)
+    rel = np.linalg.norm(want - dec.double().cpu().numpy()) / np.linalg.norm(want)
+    assert rel < 0.2
+
+
+def test_captured_steps_replay_with_new_lengths():
+    """One decode step in a CUDA graph: lengths, keys and queries change between replays, two graphs have workspaces of
+    their own, and the results are those of the calls made one by one."""
+    import torch
+    S, H, d, G = 2, 2, 128, 2
+    rng = np.random.default_rng(51)
+    make = lambda: kv4.Kv4Cache.allocate(1, S, H, d, 4000, evictable=True)[0]  # noqa: E731
+    live, plain = make(), make()
+    pre = _dev(rng.standard_normal((S, 2100, H, d)), torch.bfloat16)
+    for c in (live, plain):
+        c.lens += 2100
+        c.ends += 2100
+        c.append(pre, pre)
+    k, q = (torch.zeros((S, 1, n, d), dtype=torch.bfloat16, device="cuda") for n in (H, H * G))
+
+    def step(c):
+        c.lens += 1
+        c.ends += 1
+        c.append(k, k)
+        return c.attend(q, accumulate=True)
+
+    side = torch.cuda.Stream()
+    graphs, outs = [], []
+    with torch.cuda.stream(side):
+        for _ in range(2):
+            g = torch.cuda.CUDAGraph()
+            torch.cuda.synchronize()
+            with torch.cuda.graph(g, stream=side):
+                outs.append(step(live))
+            graphs.append(g)
+    for i in range(6):
+        k.copy_(_dev(rng.standard_normal((S, 1, H, d)), torch.bfloat16))
+        q.copy_(_dev(rng.standard_normal((S, 1, H * G, d)), torch.bfloat16))
+        torch.cuda.synchronize()
+        graphs[i % 2].replay()
+        torch.cuda.synchronize()
+        want = step(plain)
+        assert torch.equal(outs[i % 2][0], want[0]) and torch.equal(outs[i % 2][1], want[1])
+    assert torch.equal(live.mass, plain.mass) and torch.equal(live.pages, plain.pages) and torch.equal(live.positions, plain.positions)
+    live.check()
+
+
+def test_two_calls_at_once_on_two_streams():
+    import torch
+    rng = np.random.default_rng(52)
+    pages, table, _ = kv4ref.fill(rng, 1, 1, 64, 64, [2500])
+    cache = kv4.Kv4Cache(_dev(pages), _ints(table), _ints([2500]))
+    qs = [_dev(rng.standard_normal((1, 1, 4, 64)), torch.bfloat16) for _ in range(2)]
+    want = [cache.attend(q) for q in qs]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for _ in range(20):
+        got = []
+        for s, q in zip(streams, qs):
+            with torch.cuda.stream(s):
+                got.append(cache.attend(q))
+        torch.cuda.synchronize()
+        for a, b in zip(got, want):
+            assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+
+
+def test_far_pages_and_sums_do_not_wrap():
+    """Pages beyond 4 GiB, and a sequence in them."""
+    import torch
+    n_pages, page, H, d = 40000, 64, 16, 128
+    pages = torch.zeros((n_pages, H, page // 16, 18 * d), dtype=torch.uint8, device="cuda")  # 5.9 GB
+    assert pages.numel() > 1 << 32
+    table = torch.arange(n_pages - 3, n_pages, dtype=torch.int32, device="cuda").view(1, 3)
+    cache = kv4.Kv4Cache(pages, table, _ints([150]))
+    x = torch.randn((1, 150, H, d), device="cuda")
+    cache.append(x, x)
+    k, v = cache.read(150)
+    cache.check()
+    want = kv4ref.dequantise(*kv4ref.quantise(x.double().cpu().numpy()))
+    assert np.array_equal(k.double().cpu().numpy(), want) and torch.equal(k, v)
+    assert int(pages[:n_pages - 3].max()) == 0
+    q = torch.randn((1, 1, H, d), device="cuda")
+    out, lse = cache.attend(q)
+    w = kv4ref.attend(q.double().cpu().numpy(), np.stack([want.transpose(0, 2, 1, 3)] * 2, 1), [150], [150], None, 1, d ** -0.5, 0, 0, [1])
+    _close(out, lse, w[0], w[1], *w[3:])
