@@ -149,12 +149,16 @@ constexpr float kScaleShift = 128.0f;
 
 struct Scale {
   __half2 s, lo, hi;  // s', -1032 s', -1152 s'
+  // one of the two for both halves (the instructions select halves of their operands themselves)
+  __device__ __forceinline__ Scale low() const { return {__low2half2(s), __low2half2(lo), __low2half2(hi)}; }
+  __device__ __forceinline__ Scale high() const { return {__high2half2(s), __high2half2(lo), __high2half2(hi)}; }
 };
 __device__ __forceinline__ Scale scale_of(uint32_t two_halves) {  // two scales as binary16, s not yet divided
   Scale r;
-  r.s = __hmul2(*reinterpret_cast<const __half2*>(&two_halves), __float2half2_rn(1.0f / kScaleShift));
-  r.lo = __hmul2(r.s, __float2half2_rn(-1032.0f));
-  r.hi = __hmul2(r.s, __float2half2_rn(-1152.0f));
+  const __half2 s = *reinterpret_cast<const __half2*>(&two_halves);
+  r.s = __hmul2(s, __float2half2_rn(1.0f / kScaleShift));
+  r.lo = __hmul2(s, __float2half2_rn(-1032.0f / kScaleShift));
+  r.hi = __hmul2(s, __float2half2_rn(-1152.0f / kScaleShift));
   return r;
 }
 __device__ __forceinline__ uint32_t and_or(uint32_t a, uint32_t mask, uint32_t bits) {

@@ -1,8 +1,8 @@
 // Attention over the 4-bit KV cache.
 //
-// One kernel for a few query rows per kv head (a decode step, short drafts).  A warp works on its own: it streams
-// stages of 32 tokens (two atoms: keys and values with their scales in one contiguous run each) through a ring of
-// bulk copies and keeps running softmax statistics, so warps never wait for each other before the end.
+// One kernel for a few query rows per kv head (a decode step, short drafts).  Work is counted in units of 64 tokens (four
+// atoms, keys and values with their scales in one contiguous run).  A warp works on its own: it streams its units
+// through a ring of bulk copies and keeps running softmax statistics, so warps never wait for each other.
 //
 //   S^T = K Q^T     mma m16n8k16: 16 keys x 8 query rows; the A operand is dequantised straight into registers
 //   O^T = V^T P^T   16 channels x 8 query rows, contraction over the 16 keys of an atom
@@ -12,8 +12,12 @@
 // Key row m of a tile is token tau(m) = m/2 (even m) or 7 - m/2 (odd m) of its half atom, the same in both products:
 // the order in which the 16-byte pieces of K rows and the 8-byte pieces of V rows fall on distinct banks.
 //
-// The kernel is bound by HBM (9/8 dim bytes a token) and, close behind, by instruction issue: about 9 instructions
-// dequantise 8 values (pkv_kv4.cuh).
+// How the units are dealt out (make_plan):
+//   short rows   a CTA per (sequence, kv head, row tile); its warps take every fourth unit and join their sums in
+//                shared memory: one launch
+//   long rows    as many warps as the GPU holds; all units of all rows, laid end to end, are cut into equal runs, one a warp,
+//                whatever the lengths.  A row that was cut is joined by a second launch from the warps' sums.
+//
 #include <math.h>
 
 #include "pkv_kv4.cuh"
@@ -23,8 +27,10 @@ using namespace pkv_kv4;
 namespace {
 
 constexpr int kWarps = 4;
-constexpr int kStageTokens = 32;
-constexpr int kStages = 3;
+constexpr int kUnitTokens = 64, kUnitAtoms = 4;
+constexpr int kStages = 2;
+constexpr int kJoinWarps = 8;
+constexpr int kMassTokens = 32;  // keys a warp of the mass kernel holds
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 // Weights are kept times 2^7 and the running reference may lag the true maximum by 2^8: a weight in binary16 is at most
 // 2^15, and one 2^21 below the largest still has all its bits.
@@ -37,13 +43,14 @@ struct AttendParams {
   void* o_ptr;
   float* lse;
   const int32_t* q_lens;
-  float scale;
+  float scale;        // its magnitude
+  int negate;         // its sign
   int group, q_heads, window, sinks;
   int row_tiles;      // tiles of 8 NT query rows per (sequence, kv head)
-  int chunk;          // stages per CTA
-  int splits;         // CTAs per (sequence, kv head, row tile)
-  float* part_o;      // [tile][split][8 NT][D] unnormalised sums, splits > 1
-  float* part_ml;     // [tile][split][8 NT][2] reference and sum
+  int runs;           // warps that share the units of all rows; 0: a CTA per row tile
+  int whole_units;    // 1: a unit never crosses a page, one copy brings it
+  float* part_o;      // [run][2][8 NT][D] unnormalised sums of a run's first and last row, where it has only a part of it
+  float* part_ml;     // [run][2][8 NT][2] reference and sum
   uint64_t* err;
 };
 
@@ -53,10 +60,15 @@ __device__ __forceinline__ float exp2_fast(float x) {
   return r;
 }
 __device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// the first product of a chain: no accumulator to clear
+__device__ __forceinline__ void mma_first(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
+      : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));
 }
 __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
   uint32_t r;
@@ -80,9 +92,10 @@ __device__ __forceinline__ float row_power(float amax) {
 }
 
 // The B operand of S^T for query row `lane / 4`: this lane's D / 4 channels, in the order nibbles() delivers
-// the keys', odd channels divided by 16.  hi (and for f32 queries lo) [2 D / 32][2]; returns the inverse power.
+// the keys', odd channels divided by 16; negated for a negative softmax scale, so that scores are
+// scaled by something positive.  hi (and for f32 queries lo) [2 D / 32][2]; returns the inverse power.
 template <int D, int T>
-__device__ __forceinline__ float load_query(const typename PkvDst<T>::type* p, int q4, bool live, uint32_t (&hi)[D / 16][2],
+__device__ __forceinline__ float load_query(const typename PkvDst<T>::type* p, int q4, bool live, bool negate, uint32_t (&hi)[D / 16][2],
                                             uint32_t (&lo)[D / 16][2]) {
   constexpr int CH = D / 4;
   float x[CH];
@@ -97,7 +110,7 @@ __device__ __forceinline__ float load_query(const typename PkvDst<T>::type* p, i
   for (int i = 0; i < CH; i++) amax = fmaxf(amax, fabsf(x[i]));
   amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
   amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
-  const float pw = row_power(amax);
+  const float inv = 1.0f / row_power(amax), pw = negate ? -row_power(amax) : row_power(amax);
 #pragma unroll
   for (int j = 0; j < CH / 8; j++) {
 #pragma unroll
@@ -112,7 +125,7 @@ __device__ __forceinline__ float load_query(const typename PkvDst<T>::type* p, i
       }
     }
   }
-  return 1.0f / pw;
+  return inv;
 }
 
 // One atom's scores: S^T[16 keys][8 NT rows] from its K codes and scales in shared memory.
@@ -130,10 +143,11 @@ __device__ __forceinline__ void scores_of(const uint8_t* atom, int lane, const u
     w1[0] = b.x; w1[1] = b.y; w1[2] = b.z; w1[3] = b.w;
     const uint32_t u0 = *reinterpret_cast<const uint16_t*>(atom + A::KS + t0 * A::SROW + 2 * q4);
     const uint32_t u1 = *reinterpret_cast<const uint16_t*>(atom + A::KS + t1 * A::SROW + 2 * q4);
-    sc0[0] = scale_of((u0 & 0xffu) * 0x00800080u);
-    sc0[1] = scale_of((u0 >> 8) * 0x00800080u);
-    sc1[0] = scale_of((u1 & 0xffu) * 0x00800080u);
-    sc1[1] = scale_of((u1 >> 8) * 0x00800080u);
+    const Scale p0 = scale_of(__byte_perm(u0, 0u, 0x4140) << 7), p1 = scale_of(__byte_perm(u1, 0u, 0x4140) << 7);
+    sc0[0] = p0.low();
+    sc0[1] = p0.high();
+    sc1[0] = p1.low();
+    sc1[1] = p1.high();
   } else {
     const uint2 a = *reinterpret_cast<const uint2*>(atom + A::KC + t0 * A::ROW + 8 * q4);
     const uint2 b = *reinterpret_cast<const uint2*>(atom + A::KC + t1 * A::ROW + 8 * q4);
@@ -142,10 +156,9 @@ __device__ __forceinline__ void scores_of(const uint8_t* atom, int lane, const u
     sc0[0] = scale_of((uint32_t)atom[A::KS + t0 * A::SROW + q4] * 0x00800080u);
     sc1[0] = scale_of((uint32_t)atom[A::KS + t1 * A::SROW + q4] * 0x00800080u);
   }
-#pragma unroll
-  for (int n = 0; n < NT; n++)
-#pragma unroll
-    for (int i = 0; i < 4; i++) s[n][i] = 0.0f;
+  // F32: the tensor cores cut their sums off instead of rounding them; chains of at most D / 32 products of the queries' first
+  // terms, the second terms apart, keep that below the f32 error of the sum
+  float part[F32 ? NT : 1][2][4];
 #pragma unroll
   for (int j = 0; j < D / 32; j++) {
     uint32_t a[4], b[4];
@@ -155,15 +168,30 @@ __device__ __forceinline__ void scores_of(const uint8_t* atom, int lane, const u
     for (int u = 0; u < 2; u++)
 #pragma unroll
       for (int n = 0; n < NT; n++) {
-        mma(s[n], a[2 * u], b[2 * u], a[2 * u + 1], b[2 * u + 1], qhi[n][2 * j + u][0], qhi[n][2 * j + u][1]);
-        if constexpr (F32)
-          mma(s[n], a[2 * u], b[2 * u], a[2 * u + 1], b[2 * u + 1], qlo[n][2 * j + u][0], qlo[n][2 * j + u][1]);
+        const uint32_t h0 = qhi[n][2 * j + u][0], h1 = qhi[n][2 * j + u][1];
+        if constexpr (F32) {
+          float(&hi)[4] = 2 * j < D / 32 ? s[n] : part[n][0];
+          const uint32_t l0 = qlo[n][2 * j + u][0], l1 = qlo[n][2 * j + u][1];
+          if (2 * j % (D / 32) == 0 && u == 0) mma_first(hi, a[2 * u], b[2 * u], a[2 * u + 1], b[2 * u + 1], h0, h1);
+          else mma(hi, a[2 * u], b[2 * u], a[2 * u + 1], b[2 * u + 1], h0, h1);
+          if (j == 0 && u == 0) mma_first(part[n][1], a[2 * u], b[2 * u], a[2 * u + 1], b[2 * u + 1], l0, l1);
+          else mma(part[n][1], a[2 * u], b[2 * u], a[2 * u + 1], b[2 * u + 1], l0, l1);
+        } else {
+          if (j == 0 && u == 0) mma_first(s[n], a[2 * u], b[2 * u], a[2 * u + 1], b[2 * u + 1], h0, h1);
+          else mma(s[n], a[2 * u], b[2 * u], a[2 * u + 1], b[2 * u + 1], h0, h1);
+        }
       }
+  }
+  if constexpr (F32) {
+#pragma unroll
+    for (int n = 0; n < NT; n++)
+#pragma unroll
+      for (int i = 0; i < 4; i++) s[n][i] = __fadd_rn(__fadd_rn(s[n][i], part[n][0][i]), part[n][1][i]);
   }
 }
 
 // O^T += V^T P^T for one atom; p[n][0..1] is the B operand (f32 queries: p[n][2..3] its remainder).
-template <int D, int NT, bool F32>
+template <int D, int NT, bool F32, bool FIRST>
 __device__ __forceinline__ void weigh(const uint8_t* atom, int lane, const uint32_t (&p)[NT][F32 ? 4 : 2], float (&o)[D / 16][NT][4]) {
   using A = Atom<D>;
   const int q4 = lane & 3, g = lane >> 2;
@@ -203,230 +231,288 @@ __device__ __forceinline__ void weigh(const uint8_t* atom, int lane, const uint3
   for (int j = 0; j < D / 16; j++)
 #pragma unroll
     for (int n = 0; n < NT; n++) {
-      mma(o[j][n], m[0][2 * j], m[0][2 * j + 1], m[1][2 * j], m[1][2 * j + 1], p[n][0], p[n][1]);
+      if constexpr (FIRST) mma_first(o[j][n], m[0][2 * j], m[0][2 * j + 1], m[1][2 * j], m[1][2 * j + 1], p[n][0], p[n][1]);
+      else mma(o[j][n], m[0][2 * j], m[0][2 * j + 1], m[1][2 * j], m[1][2 * j + 1], p[n][0], p[n][1]);
       if constexpr (F32) mma(o[j][n], m[0][2 * j], m[0][2 * j + 1], m[1][2 * j], m[1][2 * j + 1], p[n][2], p[n][3]);
     }
 }
 
-// Which tokens a tile of query rows can see, in stages: `head` stages from slot 0 (the sinks), then those from
-// stage `from` on, `count` in all.
+// Which tokens a tile of query rows can see, in units: `head` units from slot 0 (the sinks), then those from unit
+// `from` on, `count` in all.
 struct Span {
   int head, from, count;
-  __device__ __forceinline__ int stage(int v) const { return v < head ? v : v - head + from; }
+  __device__ __forceinline__ int unit(int v) const { return v < head ? v : v - head + from; }
 };
-__device__ __forceinline__ Span visible_span(const AttendParams& p, int len, int end, int pos_first, int pos_last) {
+__device__ __forceinline__ Span visible_span(const AttendParams& p, int len, int pos_first, int pos_last) {
   Span r;
   int stop = len, lo = 0, sink = 0;
   if (!p.c.positions) {  // slots are positions
-    stop = min(len, pos_last + 1);
+    stop = max(0, min(len, pos_last + 1));
     if (p.window > 0) {
       lo = max(0, pos_first - p.window + 1);
-      sink = min(p.sinks, max(stop, 0));
+      sink = min(p.sinks, stop);
     }
   }
-  const int last = (max(stop, 0) + kStageTokens - 1) / kStageTokens;
-  r.head = (sink + kStageTokens - 1) / kStageTokens;
-  r.from = lo / kStageTokens;
+  const int last = (stop + kUnitTokens - 1) / kUnitTokens;
+  r.head = (sink + kUnitTokens - 1) / kUnitTokens;
+  r.from = lo / kUnitTokens;
   if (r.from <= r.head) r.from = r.head;
-  r.count = r.head + max(0, last - r.from);
-  if (r.from == r.head) r.count = last;
+  r.count = r.from == r.head ? last : r.head + max(0, last - r.from);
   return r;
 }
 
+// A sequence as the kernels see it: bad lengths are reported and count as empty.
+struct Sequence {
+  int len, end, qn;
+};
+__device__ __forceinline__ Sequence sequence_of(const AttendParams& p, int s) {
+  Sequence r;
+  r.len = p.c.length(s, p.err);
+  r.end = p.c.end(s, r.len);
+  r.qn = p.q_lens ? p.q_lens[s] : p.q.n;
+  if (r.qn < 0 || r.qn > p.q.n) {
+    pkv_report(p.err, 0, s, PKV_VEC_BAD_SEQUENCE);
+    r.qn = 0;
+  }
+  return r;
+}
+// Units of one (kv head, row tile) of a sequence: what its first to last query token see, at least one (a row that sees
+// nothing is written too), none without queries.
+__device__ __forceinline__ int units_of(const AttendParams& p, const Sequence& q) {
+  if (q.qn == 0) return 0;
+  return max(1, visible_span(p, q.len, q.end - q.qn, q.end - 1).count);
+}
+
+// Total units, and those before sequence `s`; whole CTA of W warps.
+template <int W>
+__device__ __forceinline__ void count_units(const AttendParams& p, int s, int64_t* total, int64_t* before, int64_t (&scratch)[2][W]) {
+  int64_t all = 0, pre = 0;
+  for (int i = threadIdx.x; i < p.c.n_seqs; i += 32 * W) {
+    const int u = units_of(p, sequence_of(p, i));
+    all += u;
+    if (i < s) pre += u;
+  }
+#pragma unroll
+  for (int o = 16; o; o >>= 1) {
+    all += __shfl_xor_sync(0xffffffffu, all, o);
+    pre += __shfl_xor_sync(0xffffffffu, pre, o);
+  }
+  if ((threadIdx.x & 31) == 0) {
+    scratch[0][threadIdx.x >> 5] = all;
+    scratch[1][threadIdx.x >> 5] = pre;
+  }
+  __syncthreads();
+  *total = *before = 0;
+#pragma unroll
+  for (int w = 0; w < W; w++) {
+    *total += scratch[0][w];
+    *before += scratch[1][w];
+  }
+}
+__device__ __forceinline__ int64_t units_per_run(int64_t total, int runs) { return total <= runs ? 1 : (total + runs - 1) / runs; }
+
 template <int D, int NT>
 struct Shared {
-  static constexpr int STAGE = 2 * Atom<D>::BYTES;
-  static constexpr int RING = kStages * STAGE;
+  static constexpr int UNIT = kUnitAtoms * Atom<D>::BYTES;
+  static constexpr int RING = kStages * UNIT;
   static constexpr int O_BYTES = 8 * NT * (D + 4) * 4;  // a warp's sums, in the space of its ring
   static constexpr int WARP = RING > O_BYTES ? RING : O_BYTES;
   static constexpr int BYTES = kWarps * WARP;
 };
 
+// A warp's ring: the slot that the next unit goes to or comes from, and the parity of the barrier there.
+struct Ring {
+  uint8_t* base;
+  uint64_t* bars;
+  int slot;
+  uint32_t phase;
+};
+
+template <int D, int NT>
+struct Sums {
+  float o[D / 16][NT][4];            // channels (lane / 4) D/8 + 2 j + i / 2, row 2 (lane % 4) + i % 2
+  float m[NT][2], l[NT][2];          // reference (log2) and sum of rows 2 (lane % 4) + e; l is this lane's part
+};
+
+// The units first, first + stride, .. (count of them) of row tile `tile`; whole warp.  False if a copy never came.
 template <int D, int NT, int T>
-__global__ void __launch_bounds__(kWarps * 32, (NT == 1 ? 4 : 2))
-kv4_attend_kernel(const __grid_constant__ AttendParams p) {
+__device__ __forceinline__ bool stream_units(const AttendParams& p, int s, int h, int tile, const Sequence& seq, int first, int stride,
+                                             int count, Ring& ring, Sums<D, NT>& r) {
   constexpr bool F32 = T == PKV_DST_F32;
   using A = Atom<D>;
   using S = Shared<D, NT>;
   using E = typename PkvDst<T>::type;
-  extern __shared__ __align__(128) uint8_t smem[];
-  __shared__ __align__(8) uint64_t bars[kWarps][kStages];
-  __shared__ float s_ml[kWarps][8 * NT][2];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int g = lane >> 2, q4 = lane & 3;
-  uint8_t* ring = smem + warp * S::WARP;
+  const int lane = threadIdx.x & 31, g = lane >> 2, q4 = lane & 3;
+  const int row0 = tile * 8 * NT, rows = seq.qn * p.group - row0;
+  const int len = seq.len, pos0 = seq.end - seq.qn;  // position of query token 0
+  const int first_token = row0 / p.group, last_token = min(seq.qn - 1, (row0 + 8 * NT - 1) / p.group);
+  const Span span = visible_span(p, len, pos0 + first_token, pos0 + last_token);
+  // a tile may see fewer units than its sequence counts
+  if (first >= span.count) count = 0;
+  else if (first + (int64_t)(count - 1) * stride >= span.count) count = (span.count - 1 - first) / stride + 1;
 
-  const int split = blockIdx.x, s = blockIdx.z;
-  const int h = blockIdx.y / p.row_tiles, tile = blockIdx.y - h * p.row_tiles;
-  const int len = p.c.length(s, p.err);
-  const int end = p.c.end(s, len);
-  int qn = p.q_lens ? p.q_lens[s] : p.q.n;
-  if (qn < 0 || qn > p.q.n) {
-    if (threadIdx.x == 0) pkv_report(p.err, 0, s, PKV_VEC_BAD_SEQUENCE);
-    qn = 0;
-  }
-  const int row0 = tile * 8 * NT, rows = qn * p.group - row0;  // rows of this tile that exist (may be more than it holds)
-  if (rows <= 0) return;
-  const int pos0 = end - qn;  // position of query token 0
-  const int first_token = row0 / p.group, last_token = min(qn - 1, (row0 + 8 * NT - 1) / p.group);
-  const Span span = visible_span(p, len, end, pos0 + first_token, pos0 + last_token);
-  // the last split takes what is left, should a length be above the caller's hint
-  const int v_begin = split * p.chunk, v_end = split == p.splits - 1 ? span.count : min(span.count, v_begin + p.chunk);
-  // a later split without work leaves nothing to combine; the first one writes the rows that see nothing
-  if (v_begin >= v_end && split > 0) return;
-
-  if (lane == 0)
-#pragma unroll
-    for (int i = 0; i < kStages; i++) pkv_mbar_init(&bars[warp][i], 1);
-  __syncwarp();
-
-  // ---- the stream of stages: this warp takes v_begin + warp, + 4, ...; page numbers are fetched for 16 stages at once,
-  // one atom per lane
-  const int n_mine = v_end - v_begin > warp ? (v_end - v_begin - warp + kWarps - 1) / kWarps : 0;
-  auto stage_of = [&](int i) { return span.stage(v_begin + warp + i * kWarps); };
-  auto page_of = [&](int i0) -> const uint8_t* {  // lane l: atom l & 1 of stage i0 + l / 2; null = nothing to load
-    const int i = i0 + (lane >> 1);
-    if (i >= n_mine) return nullptr;
-    const int a = stage_of(i) * 2 + (lane & 1);
-    if (a * kAtomTokens >= len) return nullptr;
-    return p.c.atom(s, h, a, A::BYTES, p.err);
+  // ---- the stream: page numbers are fetched for 8 units at once, one atom per lane, a batch ahead of their use
+  auto unit_of = [&](int i) { return span.unit(first + i * stride); };
+  auto atom_of = [&](int i0) -> int {  // lane l: atom l & 3 of unit i0 + l / 4; -1 = nothing to load
+    const int i = i0 + (lane >> 2);
+    if (i >= count) return -1;
+    const int a = unit_of(i) * kUnitAtoms + (lane & 3);
+    return a * kAtomTokens < len ? a : -1;
   };
-  const uint8_t* src = page_of(0);       // atoms of the batch being issued
-  unsigned live_issue = 0;               // bit l: src of lane l is there (for the batch being issued)
-  unsigned live_use = 0;                 // the same for the batch being consumed
-  live_issue = __ballot_sync(0xffffffffu, src != nullptr);
-  live_use = live_issue;
-  auto issue = [&](int i) {  // whole warp; i < n_mine
-    if (i && (i & 15) == 0) {
-      src = page_of(i);
-      live_issue = __ballot_sync(0xffffffffu, src != nullptr);
+  auto page_of = [&](int a) -> int { return a < 0 ? -1 : __ldg(p.c.table + (int64_t)s * p.c.max_pages + a / p.c.page_atoms); };
+  int atom = atom_of(0), page = page_of(atom);
+  const uint8_t* src = nullptr;
+  unsigned live_issue = 0, live_use = 0;  // bit l: the atom of lane l is there (batch being issued / consumed)
+  auto next_batch = [&](int i0) {         // the batch that starts at unit i0; its page numbers are on their way
+    src = nullptr;
+    if (atom >= 0) {
+      if (page < 0 || page >= p.c.n_pages) pkv_report(p.err, 0, s, PKV_VEC_BAD_SEQUENCE);
+      else src = p.c.pages + (((int64_t)page * p.c.heads + h) * p.c.page_atoms + atom % p.c.page_atoms) * (int64_t)A::BYTES;
     }
-    const int slot = i % kStages;
-    const int l = 2 * (i & 15);
-    uint8_t* dst = ring + slot * S::STAGE;
-    const unsigned pair = (live_issue >> l) & 3u;
-    if ((lane & ~1) == l) {
-      if (lane == l) pkv_mbar_expect_tx(&bars[warp][slot], (uint32_t)__popc(pair) * A::BYTES);
+    live_issue = __ballot_sync(0xffffffffu, src != nullptr);
+    atom = atom_of(i0 + 8);
+    page = page_of(atom);
+  };
+  int slot_in = ring.slot;
+  auto issue = [&](int i) {  // whole warp; i < count
+    if ((i & 7) == 0) next_batch(i);
+    const int l = 4 * (i & 7);
+    const uint32_t bytes = (uint32_t)__popc((live_issue >> l) & 15u) * A::BYTES;
+    uint8_t* dst = ring.base + slot_in * S::UNIT;
+    uint64_t* bar = ring.bars + slot_in;
+    if (lane == l) {
+      pkv_mbar_expect_tx(bar, bytes);
+      if (p.whole_units && bytes) pkv_bulk_load(dst, src, bytes, bar);
     }
-    __syncwarp();
-    if ((lane & ~1) == l && src) pkv_bulk_load(dst + (lane & 1) * A::BYTES, src, A::BYTES, &bars[warp][slot]);
+    if (!p.whole_units) {
+      __syncwarp();
+      if ((lane & ~3) == l && src) pkv_bulk_load(dst + (lane & 3) * A::BYTES, src, A::BYTES, bar);
+    }
+    if (++slot_in == kStages) slot_in = 0;
   };
   int issued = 0;
-  for (; issued < min(kStages, n_mine); issued++) issue(issued);
+  for (; issued < min(kStages, count); issued++) {
+    issue(issued);
+    if (issued == 0) live_use = live_issue;
+  }
 
   // ---- queries
   uint32_t qhi[NT][D / 16][2], qlo[NT][D / 16][2];
   float factor[NT][2];  // of the scores of rows 2 q4 and 2 q4 + 1: softmax scale, log2 e, powers of two
 #pragma unroll
   for (int n = 0; n < NT; n++) {
-    const int r = row0 + 8 * n + g, token = r / p.group, hq = h * p.group + (r - token * p.group);
-    const bool live = 8 * n + g < rows;
+    const int rr = row0 + 8 * n + g, token = rr / p.group, hq = h * p.group + (rr - token * p.group);
     const E* qp = reinterpret_cast<const E*>(p.q_ptr) + s * p.q.seq + (int64_t)token * p.q.token + hq * p.q.head;
-    const float inv = load_query<D, T>(qp, q4, live, qhi[n], qlo[n]);
+    const float inv = load_query<D, T>(qp, q4, 8 * n + g < rows, p.negate, qhi[n], qlo[n]);
     const float f = __fmul_rn(__fmul_rn(p.scale, kLog2e), kScaleShift);
 #pragma unroll
     for (int e = 0; e < 2; e++) factor[n][e] = __fmul_rn(f, __shfl_sync(0xffffffffu, inv, 4 * (2 * q4 + e)));
   }
-  int qpos[NT][2];
-#pragma unroll
-  for (int n = 0; n < NT; n++)
-#pragma unroll
-    for (int e = 0; e < 2; e++) qpos[n][e] = pos0 + (row0 + 8 * n + 2 * q4 + e) / p.group;
   const int qpos_min = pos0 + first_token, qpos_max = pos0 + last_token;
   // positions matter only where a row can see less than everything that is held
-  const bool by_position = p.c.positions != nullptr && (p.window > 0 || qn > 1);
+  const bool by_position = p.c.positions != nullptr && (p.window > 0 || seq.qn > 1);
   const int32_t* positions = by_position ? p.c.positions + p.c.stat(s, h) : nullptr;
 
-  float o[D / 16][NT][4];
-  float m_ref[NT][2], l_sum[NT][2];
 #pragma unroll
   for (int j = 0; j < D / 16; j++)
 #pragma unroll
     for (int n = 0; n < NT; n++)
 #pragma unroll
-      for (int i = 0; i < 4; i++) o[j][n][i] = 0.0f;
+      for (int i = 0; i < 4; i++) r.o[j][n][i] = 0.0f;
 #pragma unroll
   for (int n = 0; n < NT; n++)
 #pragma unroll
     for (int e = 0; e < 2; e++) {
-      m_ref[n][e] = -INFINITY;
-      l_sum[n][e] = 0.0f;
+      r.m[n][e] = -INFINITY;
+      r.l[n][e] = 0.0f;
     }
 
-  bool fine = true;
-  int done = 0;
-  for (; done < n_mine; done++) {
-    const int slot = done % kStages;
-    if (done && (done & 15) == 0) live_use = live_issue;  // issue() of this batch's first stage has run
-    const int token0 = stage_of(done) * kStageTokens;
-    int kpos = 0;
-    if (by_position && token0 + lane < len) kpos = __ldg(positions + token0 + lane);
-    const unsigned pair = (live_use >> (2 * (done & 15))) & 3u;
-    if (!__all_sync(0xffffffffu, pkv_mbar_wait(&bars[warp][slot], (uint32_t)(done / kStages) & 1u))) {
-      fine = false;
-      break;
-    }
-    uint8_t* stage = ring + slot * S::STAGE;
-    // tokens that are there, one bit each
-    unsigned there = token0 + kStageTokens <= len ? 0xffffffffu : (1u << (len - token0)) - 1u;
-    if (!(pair & 1u)) there &= 0xffff0000u;
-    if (!(pair & 2u)) there &= 0x0000ffffu;
-    if (there != 0xffffffffu) {
-      // values of absent tokens become zeros (any bytes may lie there; 0 x inf would spoil the sums)
-      if (!((there >> lane) & 1u)) {
-        uint8_t* sc = stage + (lane >> 4) * A::BYTES + A::VS + (lane & 15) * A::SROW;
+#pragma unroll 1
+  for (int done = 0; done < count; done++) {
+    if (done && (done & 7) == 0) live_use = live_issue;  // issue() of this batch's first unit has run
+    const int token0 = unit_of(done) * kUnitTokens;
+    int kpos[2] = {0, 0};
+    if (by_position) {
 #pragma unroll
-        for (int i = 0; i < A::SROW; i += 4) *reinterpret_cast<uint32_t*>(sc + i) = 0u;
+      for (int i = 0; i < 2; i++)
+        if (token0 + 32 * i + lane < len) kpos[i] = __ldg(positions + token0 + 32 * i + lane);
+    }
+    if (!__all_sync(0xffffffffu, pkv_mbar_wait(ring.bars + ring.slot, ring.phase))) {
+      // a copy never arrived: give the others their time, report, and leave nothing behind
+      for (int i = done + 1; i < issued; i++) {
+        if (++ring.slot == kStages) ring.slot = 0, ring.phase ^= 1u;
+        pkv_mbar_wait(ring.bars + ring.slot, ring.phase);
+      }
+      if (lane == 0) pkv_report(p.err, 0, s, PKV_VEC_DEVICE_WAIT);
+      return false;
+    }
+    uint8_t* unit = ring.base + ring.slot * S::UNIT;
+    const unsigned quad = (live_use >> (4 * (done & 7))) & 15u;
+    const bool whole = quad == 15u && token0 + kUnitTokens <= len;
+    unsigned there[2] = {0xffffffffu, 0xffffffffu};  // tokens that are there, one bit each
+    if (!whole) {
+#pragma unroll
+      for (int i = 0; i < 2; i++) {
+        const int left = len - token0 - 32 * i;
+        there[i] = left >= 32 ? 0xffffffffu : left <= 0 ? 0u : (1u << left) - 1u;
+        if (!((quad >> (2 * i)) & 1u)) there[i] &= 0xffff0000u;
+        if (!((quad >> (2 * i)) & 2u)) there[i] &= 0x0000ffffu;
+        // values of absent tokens become zeros (any bytes may lie there; 0 x inf would spoil the sums)
+        if (!((there[i] >> lane) & 1u)) {
+          uint8_t* sc = unit + (2 * i + (lane >> 4)) * A::BYTES + A::VS + (lane & 15) * A::SROW;
+#pragma unroll
+          for (int b = 0; b < A::SROW; b += 4) *reinterpret_cast<uint32_t*>(sc + b) = 0u;
+        }
       }
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       __syncwarp();
     }
-    const bool masked = there != 0xffffffffu || by_position || token0 + kStageTokens - 1 > qpos_min ||
-                        (p.window > 0 && qpos_max - token0 >= p.window && token0 + kStageTokens > p.sinks);
+    const bool masked = !whole || by_position || token0 + kUnitTokens - 1 > qpos_min ||
+                        (p.window > 0 && qpos_max - token0 >= p.window && token0 + kUnitTokens > p.sinks);
 
-    float sc[2][NT][4];
+    float sc[kUnitAtoms][NT][4];
 #pragma unroll
-    for (int a = 0; a < 2; a++) scores_of<D, NT, F32>(stage + a * A::BYTES, lane, qhi, qlo, sc[a]);
-    float top[NT][2];
+    for (int a = 0; a < kUnitAtoms; a++) scores_of<D, NT, F32>(unit + a * A::BYTES, lane, qhi, qlo, sc[a]);
+    float fac[NT][2];  // what the scores are still to be multiplied by
 #pragma unroll
     for (int n = 0; n < NT; n++)
 #pragma unroll
-      for (int e = 0; e < 2; e++) top[n][e] = -INFINITY;
+      for (int e = 0; e < 2; e++) fac[n][e] = factor[n][e];
     if (masked) {
 #pragma unroll
-      for (int a = 0; a < 2; a++)
+      for (int n = 0; n < NT; n++)
+#pragma unroll
+        for (int e = 0; e < 2; e++) fac[n][e] = 1.0f;
+#pragma unroll
+      for (int a = 0; a < kUnitAtoms; a++)
 #pragma unroll
         for (int hh = 0; hh < 2; hh++) {
-          const int t = 16 * a + 8 * hh + tau(g);
-          const int kp = by_position ? __shfl_sync(0xffffffffu, kpos, t) : token0 + t;
-          const bool held = (there >> t) & 1u;
+          const int t = 16 * (a & 1) + 8 * hh + tau(g);
+          const int kp = by_position ? __shfl_sync(0xffffffffu, kpos[a >> 1], t) : token0 + 32 * (a >> 1) + t;
+          const bool held = (there[a >> 1] >> t) & 1u;
 #pragma unroll
           for (int n = 0; n < NT; n++)
 #pragma unroll
             for (int e = 0; e < 2; e++) {
-              const int d = qpos[n][e] - kp;
+              const int d = pos0 + (row0 + 8 * n + 2 * q4 + e) / p.group - kp;
               const bool see = held && d >= 0 && (p.window == 0 || d < p.window || kp < p.sinks);
               float& x = sc[a][n][2 * hh + e];
               x = see ? __fmul_rn(x, factor[n][e]) : -INFINITY;
-              top[n][e] = fmaxf(top[n][e], x);
             }
         }
-    } else {
-#pragma unroll
-      for (int a = 0; a < 2; a++)
-#pragma unroll
-        for (int n = 0; n < NT; n++)
-#pragma unroll
-          for (int i = 0; i < 4; i++) {
-            sc[a][n][i] = __fmul_rn(sc[a][n][i], factor[n][i & 1]);
-            top[n][i & 1] = fmaxf(top[n][i & 1], sc[a][n][i]);
-          }
     }
+    float top[NT][2];
     bool raise = false;
 #pragma unroll
     for (int n = 0; n < NT; n++)
 #pragma unroll
-      for (int e = 0; e < 2; e++) raise = raise || top[n][e] > __fadd_rn(m_ref[n][e], kLag);
+      for (int e = 0; e < 2; e++) {
+        float t = fmaxf(sc[0][n][e], sc[0][n][2 + e]);
+#pragma unroll
+        for (int a = 1; a < kUnitAtoms; a++) t = fmaxf(t, fmaxf(sc[a][n][e], sc[a][n][2 + e]));
+        top[n][e] = __fmul_rn(t, fac[n][e]);
+        raise = raise || top[n][e] > __fadd_rn(r.m[n][e], kLag);
+      }
     if (__any_sync(0xffffffffu, raise)) {
 #pragma unroll
       for (int n = 0; n < NT; n++)
@@ -436,176 +522,321 @@ kv4_attend_kernel(const __grid_constant__ AttendParams p) {
           t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 4));
           t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 8));
           t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 16));
-          const float m = fmaxf(m_ref[n][e], t);
-          const float f = m_ref[n][e] == -INFINITY ? 0.0f : exp2_fast(__fsub_rn(m_ref[n][e], m));
-          m_ref[n][e] = m;
-          l_sum[n][e] = __fmul_rn(l_sum[n][e], f);
+          const float m = fmaxf(r.m[n][e], t);
+          const float f = r.m[n][e] == -INFINITY ? 0.0f : exp2_fast(__fsub_rn(r.m[n][e], m));
+          r.m[n][e] = m;
+          r.l[n][e] = __fmul_rn(r.l[n][e], f);
 #pragma unroll
           for (int j = 0; j < D / 16; j++) {
-            o[j][n][e] = __fmul_rn(o[j][n][e], f);
-            o[j][n][2 + e] = __fmul_rn(o[j][n][2 + e], f);
+            r.o[j][n][e] = __fmul_rn(r.o[j][n][e], f);
+            r.o[j][n][2 + e] = __fmul_rn(r.o[j][n][2 + e], f);
           }
         }
     }
-    uint32_t pb[2][NT][F32 ? 4 : 2];
+    uint32_t pb[kUnitAtoms][NT][F32 ? 4 : 2];
 #pragma unroll
     for (int n = 0; n < NT; n++) {
       float base[2];
 #pragma unroll
-      for (int e = 0; e < 2; e++) base[e] = m_ref[n][e] == -INFINITY ? 0.0f : __fsub_rn(m_ref[n][e], kWeightShift);
+      for (int e = 0; e < 2; e++) base[e] = r.m[n][e] == -INFINITY ? 0.0f : __fsub_rn(kWeightShift, r.m[n][e]);
 #pragma unroll
-      for (int a = 0; a < 2; a++)
+      for (int a = 0; a < kUnitAtoms; a++)
 #pragma unroll
         for (int hh = 0; hh < 2; hh++) {
-          const float w0 = exp2_fast(__fsub_rn(sc[a][n][2 * hh], base[0]));
-          const float w1 = exp2_fast(__fsub_rn(sc[a][n][2 * hh + 1], base[1]));
-          l_sum[n][0] = __fadd_rn(l_sum[n][0], w0);
-          l_sum[n][1] = __fadd_rn(l_sum[n][1], w1);
+          const float w0 = exp2_fast(__fmaf_rn(sc[a][n][2 * hh], fac[n][0], base[0]));
+          const float w1 = exp2_fast(__fmaf_rn(sc[a][n][2 * hh + 1], fac[n][1], base[1]));
+          r.l[n][0] = __fadd_rn(r.l[n][0], w0);
+          r.l[n][1] = __fadd_rn(r.l[n][1], w1);
           const uint32_t hw = half2_of(w0, w1);
           pb[a][n][hh] = transpose8(hw);
           if constexpr (F32) {
-            const float2 r = __half22float2(*reinterpret_cast<const __half2*>(&hw));
-            pb[a][n][2 + hh] = transpose8(half2_of(__fsub_rn(w0, r.x), __fsub_rn(w1, r.y)));
+            const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&hw));
+            pb[a][n][2 + hh] = transpose8(half2_of(__fsub_rn(w0, f.x), __fsub_rn(w1, f.y)));
           }
         }
     }
+    if constexpr (F32) {  // two atoms' sum on its own, then one rounded addition: a long chain would drift by its cut-off bits
 #pragma unroll
-    for (int a = 0; a < 2; a++) weigh<D, NT, F32>(stage + a * A::BYTES, lane, pb[a], o);
+      for (int a = 0; a < kUnitAtoms; a += 2) {
+        float t[D / 16][NT][4];
+        weigh<D, NT, F32, true>(unit + a * A::BYTES, lane, pb[a], t);
+        weigh<D, NT, F32, false>(unit + (a + 1) * A::BYTES, lane, pb[a + 1], t);
+#pragma unroll
+        for (int j = 0; j < D / 16; j++)
+#pragma unroll
+          for (int n = 0; n < NT; n++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) r.o[j][n][i] = __fadd_rn(r.o[j][n][i], t[j][n][i]);
+      }
+    } else {
+#pragma unroll
+      for (int a = 0; a < kUnitAtoms; a++) weigh<D, NT, F32, false>(unit + a * A::BYTES, lane, pb[a], r.o);
+    }
     __syncwarp();
-    if (issued < n_mine) issue(issued++);
+    if (issued < count) issue(issued++);  // into the slot that was just read
+    if (++ring.slot == kStages) ring.slot = 0, ring.phase ^= 1u;
   }
-  if (!fine) {  // a copy never arrived: give the others their time, report, and leave nothing behind
-    for (int i = done + 1; i < issued; i++) pkv_mbar_wait(&bars[warp][i % kStages], (uint32_t)(i / kStages) & 1u);
-    if (lane == 0) pkv_report(p.err, 0, s, PKV_VEC_DEVICE_WAIT);
-  }
-
-  // ---- the four warps' sums become one
 #pragma unroll
   for (int n = 0; n < NT; n++)
 #pragma unroll
-    for (int e = 0; e < 2; e++) {
-      float t = l_sum[n][e];
+    for (int e = 0; e < 2; e++) {  // the lanes' parts of the sums
+      float t = r.l[n][e];
       t = __fadd_rn(t, __shfl_xor_sync(0xffffffffu, t, 4));
       t = __fadd_rn(t, __shfl_xor_sync(0xffffffffu, t, 8));
-      t = __fadd_rn(t, __shfl_xor_sync(0xffffffffu, t, 16));
-      if (g == 0) {
-        s_ml[warp][8 * n + 2 * q4 + e][0] = m_ref[n][e];
-        s_ml[warp][8 * n + 2 * q4 + e][1] = t;
+      r.l[n][e] = __fadd_rn(t, __shfl_xor_sync(0xffffffffu, t, 16));
+    }
+  return true;
+}
+
+// Writes N channels of a row, sums x (scale and the 16 of odd channels already undone) over l.
+template <int T, int N>
+__device__ __forceinline__ void write_row(const AttendParams& p, int s, int h, int row, int channel, const float (&x)[N], float m, float l,
+                                          bool first) {
+  using E = typename PkvDst<T>::type;
+  const int token = row / p.group, hq = h * p.group + (row - token * p.group);
+  const float inv = l > 0.0f ? __fdiv_rn(1.0f, l) : (l == 0.0f ? 0.0f : l);
+  E* dst = reinterpret_cast<E*>(p.o_ptr) + s * p.o.seq + (int64_t)token * p.o.token + hq * p.o.head + channel;
+  float y[N];
+#pragma unroll
+  for (int i = 0; i < N; i++) y[i] = __fmul_rn(x[i], inv);
+  if constexpr (T == PKV_DST_F32 ? N % 4 == 0 : N % 8 == 0) {
+    store_f32<T, N>(dst, y);
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; i += 2) {
+      if constexpr (T == PKV_DST_F32) *reinterpret_cast<float2*>(dst + i) = make_float2(y[i], y[i + 1]);
+      else *reinterpret_cast<uint32_t*>(dst + i) = pkv_pack2<T>(y[i], y[i + 1]);
+    }
+  }
+  if (p.lse && first)
+    p.lse[((int64_t)s * p.q.n + token) * p.q_heads + hq] =
+        l == 0.0f ? -INFINITY : __fmul_rn(kLn2, __fadd_rn(m, __fsub_rn(log2f(l), kWeightShift)));
+}
+
+template <int D, int NT, int T>
+__global__ void __launch_bounds__(kWarps * 32, (NT == 1 ? 3 : 2))
+kv4_attend_kernel(const __grid_constant__ AttendParams p) {
+  using S = Shared<D, NT>;
+  extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ __align__(8) uint64_t bars[kWarps][kStages];
+  __shared__ float s_ml[kWarps][8 * NT][2];
+  __shared__ int64_t s_count[2][kWarps];
+  const int lane = threadIdx.x & 31, warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0);
+  const int g = lane >> 2, q4 = lane & 3;
+  Ring ring = {smem + warp * S::WARP, bars[warp], 0, 0u};
+  if (lane == 0)
+#pragma unroll
+    for (int i = 0; i < kStages; i++) pkv_mbar_init(&bars[warp][i], 1);
+  __syncwarp();
+  Sums<D, NT> r;
+
+  if (p.runs == 0) {
+    // ---- a CTA per row tile
+    const int s = blockIdx.z, h = blockIdx.y, tile = blockIdx.x;
+    const Sequence seq = sequence_of(p, s);
+    const int row0 = tile * 8 * NT, rows = seq.qn * p.group - row0;  // rows of this tile that exist (may be more than it holds)
+    if (rows <= 0) return;
+    const int units = units_of(p, seq);
+    stream_units<D, NT, T>(p, s, h, tile, seq, warp, kWarps, units > warp ? (units - warp + kWarps - 1) / kWarps : 0, ring, r);
+    if (g == 0)
+#pragma unroll
+      for (int n = 0; n < NT; n++)
+#pragma unroll
+        for (int e = 0; e < 2; e++) {
+          s_ml[warp][8 * n + 2 * q4 + e][0] = r.m[n][e];
+          s_ml[warp][8 * n + 2 * q4 + e][1] = r.l[n][e];
+        }
+    __syncwarp();  // every lane has read the ring's last unit
+    float* so = reinterpret_cast<float*>(ring.base);  // [8 NT][D + 4]
+#pragma unroll
+    for (int j = 0; j < D / 16; j++)
+#pragma unroll
+      for (int n = 0; n < NT; n++)
+#pragma unroll
+        for (int e = 0; e < 2; e++)
+          *reinterpret_cast<float2*>(so + (8 * n + 2 * q4 + e) * (D + 4) + g * (D / 8) + 2 * j) = make_float2(r.o[j][n][e], r.o[j][n][2 + e]);
+    __syncthreads();
+    for (int row = warp; row < min(8 * NT, rows); row += kWarps) {
+      float m = -INFINITY, l = 0.0f, f[kWarps], x[D / 32];
+#pragma unroll
+      for (int w = 0; w < kWarps; w++) m = fmaxf(m, s_ml[w][row][0]);
+#pragma unroll
+      for (int w = 0; w < kWarps; w++) {
+        f[w] = s_ml[w][row][0] == -INFINITY ? 0.0f : exp2_fast(__fsub_rn(s_ml[w][row][0], m));
+        l = __fmaf_rn(f[w], s_ml[w][row][1], l);
+      }
+#pragma unroll
+      for (int i = 0; i < D / 32; i++) {
+        float t = 0.0f;
+#pragma unroll
+        for (int w = 0; w < kWarps; w++)
+          t = __fmaf_rn(f[w], reinterpret_cast<const float*>(smem + w * S::WARP)[row * (D + 4) + lane * (D / 32) + i], t);
+        x[i] = __fmul_rn(t, (i & 1) ? kScaleShift / 16.0f : kScaleShift);
+      }
+      write_row<T, D / 32>(p, s, h, row0 + row, lane * (D / 32), x, m, l, lane == 0);
+    }
+    return;
+  }
+
+  // ---- equal runs of all units
+  int64_t total, unused;
+  count_units<kWarps>(p, 0, &total, &unused, s_count);
+  const int tiles = p.c.heads * p.row_tiles;  // row tiles of a sequence
+  total *= tiles;
+  const int64_t per = units_per_run(total, p.runs);
+  const int64_t run = (int64_t)blockIdx.x * kWarps + warp;
+  int64_t at = run * per;
+  const int64_t stop = min(total, at + per);
+  // the sequence that unit `at` lies in: 32 at a time
+  int s = 0;
+  int64_t base = 0;  // units before sequence s
+  while (at < stop) {
+    {
+      // move s and base to the sequence of unit `at`
+      for (;;) {
+        const int i = s + lane;
+        const int64_t mine = i < p.c.n_seqs ? (int64_t)units_of(p, sequence_of(p, i)) * tiles : 0;
+        int64_t upto = mine;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const int64_t t = __shfl_up_sync(0xffffffffu, upto, o);
+          if (lane >= o) upto += t;
+        }
+        const unsigned past = __ballot_sync(0xffffffffu, base + upto > at);
+        if (past) {
+          const int k = __ffs(past) - 1;
+          base += __shfl_sync(0xffffffffu, upto - mine, k);
+          s += k;
+          break;
+        }
+        base += __shfl_sync(0xffffffffu, upto, 31);
+        s += 32;
       }
     }
-  float* so = reinterpret_cast<float*>(ring);  // [8 NT][D + 4]
+    const Sequence seq = sequence_of(p, s);
+    const int units = units_of(p, seq);
+    // the row tiles of this sequence that the run reaches
+    while (at < stop && at < base + (int64_t)units * tiles) {
+      const int64_t off = at - base;
+      const int ht = (int)(off / units), v = (int)(off - (int64_t)ht * units);
+      const int n = (int)min((int64_t)(units - v), stop - at);
+      const int h = ht / p.row_tiles, tile = ht - h * p.row_tiles;
+      const int row0 = tile * 8 * NT, rows = min(8 * NT, seq.qn * p.group - row0);
+      at += n;
+      if (rows <= 0) continue;
+      const bool fine = stream_units<D, NT, T>(p, s, h, tile, seq, v, 1, n, ring, r);
+      const bool part = n < units;
+      const int64_t slot = (run * 2 + (v == 0)) * (8 * NT);
 #pragma unroll
-  for (int j = 0; j < D / 16; j++)
+      for (int nn = 0; nn < NT; nn++)
 #pragma unroll
-    for (int n = 0; n < NT; n++)
+        for (int e = 0; e < 2; e++) {
+          const int row = 8 * nn + 2 * q4 + e;
+          float x[D / 8];
 #pragma unroll
-      for (int i = 0; i < 4; i++) so[(8 * n + 2 * q4 + (i & 1)) * (D + 4) + g * (D / 8) + 2 * j + (i >> 1)] = o[j][n][i];
-  __syncthreads();
-  const int held_rows = min(8 * NT, rows);
-  for (int r = warp; r < held_rows; r += kWarps) {
-    float m = -INFINITY;
-#pragma unroll
-    for (int w = 0; w < kWarps; w++) m = fmaxf(m, s_ml[w][r][0]);
-    float l = 0.0f, f[kWarps];
-#pragma unroll
-    for (int w = 0; w < kWarps; w++) {
-      f[w] = s_ml[w][r][0] == -INFINITY ? 0.0f : exp2_fast(__fsub_rn(s_ml[w][r][0], m));
-      l = __fmaf_rn(f[w], s_ml[w][r][1], l);
-    }
-    float x[D / 32];
-#pragma unroll
-    for (int i = 0; i < D / 32; i++) {
-      float t = 0.0f;
-#pragma unroll
-      for (int w = 0; w < kWarps; w++)
-        t = __fmaf_rn(f[w], reinterpret_cast<const float*>(smem + w * S::WARP)[r * (D + 4) + lane * (D / 32) + i], t);
-      // undo the scale shift and the 16 of odd channels
-      x[i] = __fmul_rn(t, (i & 1) ? kScaleShift / 16.0f : kScaleShift);
-    }
-    if (p.splits > 1) {
-      const int64_t at = (((int64_t)s * gridDim.y + blockIdx.y) * p.splits + split) * (8 * NT) + r;
-      float* dst = p.part_o + at * D + lane * (D / 32);
-      if constexpr (D == 128) *reinterpret_cast<float4*>(dst) = make_float4(x[0], x[1], x[2], x[3]);
-      else *reinterpret_cast<float2*>(dst) = make_float2(x[0], x[1]);
-      if (lane == 0) *reinterpret_cast<float2*>(p.part_ml + at * 2) = make_float2(m, l);
-    } else {
-      const int rr = row0 + r, token = rr / p.group, hq = h * p.group + (rr - token * p.group);
-      const float inv = l > 0.0f ? __fdiv_rn(1.0f, l) : (l == 0.0f ? 0.0f : l);
-      E* dst = reinterpret_cast<E*>(p.o_ptr) + s * p.o.seq + (int64_t)token * p.o.token + hq * p.o.head + lane * (D / 32);
-#pragma unroll
-      for (int i = 0; i < D / 32; i += 2) {
-        const float a = __fmul_rn(x[i], inv), b = __fmul_rn(x[i + 1], inv);
-        if constexpr (F32) *reinterpret_cast<float2*>(dst + i) = make_float2(a, b);
-        else *reinterpret_cast<uint32_t*>(dst + i) = pkv_pack2<T>(a, b);
-      }
-      if (p.lse && lane == 0)
-        p.lse[((int64_t)s * p.q.n + token) * p.q_heads + hq] =
-            l == 0.0f ? -INFINITY : __fmul_rn(kLn2, __fadd_rn(m, __fsub_rn(log2f(l), kWeightShift)));
+          for (int j = 0; j < D / 16; j++) {
+            x[2 * j] = __fmul_rn(r.o[j][nn][e], kScaleShift);
+            x[2 * j + 1] = __fmul_rn(r.o[j][nn][2 + e], kScaleShift / 16.0f);
+          }
+          if (row < rows) {
+            if (part) {
+              store_f32<PKV_DST_F32, D / 8>(p.part_o + (slot + row) * D + g * (D / 8), x);
+              if (g == 0) *reinterpret_cast<float2*>(p.part_ml + (slot + row) * 2) = make_float2(r.m[nn][e], r.l[nn][e]);
+            } else {
+              write_row<T, D / 8>(p, s, h, row0 + row, g * (D / 8), x, r.m[nn][e], r.l[nn][e], g == 0);
+            }
+          }
+        }
+      if (!fine) return;
     }
   }
 }
 
-// Joins the splits of a row: one CTA per query row, a warp takes every fourth split.
+// Joins the parts of a query row that was cut: a CTA per row, a warp takes every eighth part.
 template <int D, int NT, int T>
-__global__ void __launch_bounds__(128)
+__global__ void __launch_bounds__(kJoinWarps * 32)
 kv4_combine_kernel(const __grid_constant__ AttendParams p) {
-  using E = typename PkvDst<T>::type;
-  __shared__ float s_o[4][D];
-  __shared__ float s_ml[4][2];
+  __shared__ int64_t s_count[2][kJoinWarps];
+  __shared__ float s_x[kJoinWarps][D], s_ml[kJoinWarps][2];
+  constexpr int N = D / 32;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int s = blockIdx.z, r = blockIdx.x % (8 * NT), tile = blockIdx.x / (8 * NT), h = blockIdx.y;
-  const int len = p.c.length(s, p.err), end = p.c.end(s, len);
-  int qn = p.q_lens ? p.q_lens[s] : p.q.n;
-  if (qn < 0 || qn > p.q.n) qn = 0;
-  const int row0 = tile * 8 * NT;
-  if (row0 + r >= qn * p.group) return;
-  const int first_token = row0 / p.group, last_token = min(qn - 1, (row0 + 8 * NT - 1) / p.group);
-  const Span span = visible_span(p, len, end, end - qn + first_token, end - qn + last_token);
-  const int n = min(p.splits, max(1, (span.count + p.chunk - 1) / p.chunk));  // splits that had work (the first always writes)
-  const int64_t base = (((int64_t)s * p.c.heads + h) * p.row_tiles + tile) * p.splits * (8 * NT) + r;
-  float m = -INFINITY, l = 0.0f, x[D / 32];
+  const int s = blockIdx.z, h = blockIdx.y, tile = blockIdx.x / (8 * NT), row = blockIdx.x % (8 * NT);
+  int64_t total, before;
+  count_units<kJoinWarps>(p, s, &total, &before, s_count);
+  const Sequence seq = sequence_of(p, s);
+  const int units = units_of(p, seq);
+  const int tiles = p.c.heads * p.row_tiles;
+  const int64_t per = units_per_run(total * tiles, p.runs);
+  const int64_t at = before * tiles + (int64_t)(h * p.row_tiles + tile) * units;
+  const int64_t first = at / per;
+  const int parts = (int)((at + units - 1) / per - first) + 1;
+  // every block waits, so that this launch never ends before the one it follows
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  if (tile * 8 * NT + row >= seq.qn * p.group || parts == 1) return;
+  auto slot_of = [&](int k) { return ((first + k) * 2 + (k == 0)) * (8 * NT) + row; };
+  float m = -INFINITY, l = 0.0f, x[N];
 #pragma unroll
-  for (int i = 0; i < D / 32; i++) x[i] = 0.0f;
-  for (int w = warp; w < n; w += 4) {
-    const int64_t at = base + (int64_t)w * (8 * NT);
-    const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + at * 2);
-    float y[D / 32];
+  for (int i = 0; i < N; i++) x[i] = 0.0f;
+  // a warp's parts: k = warp + 8 j; references of 32 of them at a time, then the sums, eight loads in flight
+  for (int k0 = warp; k0 < parts; k0 += 32 * kJoinWarps) {
+    const int n = min(32, (parts - k0 + kJoinWarps - 1) / kJoinWarps);
+    float2 ml = make_float2(-INFINITY, 0.0f);
+    if (lane < n) ml = *reinterpret_cast<const float2*>(p.part_ml + slot_of(k0 + lane * kJoinWarps) * 2);
+    float top = ml.x;
 #pragma unroll
-    for (int i = 0; i < D / 32; i++) y[i] = p.part_o[at * D + lane * (D / 32) + i];
-    if (ml.x == -INFINITY && ml.y == 0.0f) continue;
-    const float top = fmaxf(m, ml.x);
-    const float fa = m == -INFINITY ? 0.0f : exp2_fast(__fsub_rn(m, top)), fb = exp2_fast(__fsub_rn(ml.x, top));
+    for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    top = fmaxf(top, m);
+    const float fold = m == -INFINITY ? 0.0f : exp2_fast(__fsub_rn(m, top));
+    // (a part without a visible key, or with nothing but NaN, has no reference)
+    const float f = ml.x == -INFINITY ? (ml.y == 0.0f ? 0.0f : ml.y) : exp2_fast(__fsub_rn(ml.x, top));
+    float sum = __fmul_rn(f, ml.y);
+#pragma unroll
+    for (int o = 16; o; o >>= 1) sum = __fadd_rn(sum, __shfl_xor_sync(0xffffffffu, sum, o));
+    l = __fmaf_rn(l, fold, sum);
     m = top;
-    l = __fmaf_rn(l, fa, __fmul_rn(ml.y, fb));
 #pragma unroll
-    for (int i = 0; i < D / 32; i++) x[i] = __fmaf_rn(x[i], fa, __fmul_rn(y[i], fb));
+    for (int i = 0; i < N; i++) x[i] = __fmul_rn(x[i], fold);
+#pragma unroll 8
+    for (int j = 0; j < n; j++) {
+      const float fj = __shfl_sync(0xffffffffu, f, j);
+      const float* src = p.part_o + slot_of(k0 + j * kJoinWarps) * D + lane * N;
+      float y[N];
+      if constexpr (N == 4) {
+        const float4 v = *reinterpret_cast<const float4*>(src);
+        y[0] = v.x; y[1] = v.y; y[2] = v.z; y[3] = v.w;
+      } else {
+        const float2 v = *reinterpret_cast<const float2*>(src);
+        y[0] = v.x; y[1] = v.y;
+      }
+#pragma unroll
+      for (int i = 0; i < N; i++) x[i] = __fmaf_rn(fj, y[i], x[i]);
+    }
   }
 #pragma unroll
-  for (int i = 0; i < D / 32; i++) s_o[warp][lane * (D / 32) + i] = x[i];
+  for (int i = 0; i < N; i++) s_x[warp][lane * N + i] = x[i];
   if (lane == 0) {
     s_ml[warp][0] = m;
     s_ml[warp][1] = l;
   }
   __syncthreads();
-  if (threadIdx.x * 2 >= D) return;
-  float top = -INFINITY, sum = 0.0f, a = 0.0f, b = 0.0f;
+  if (warp) return;
+  const int w = lane & (kJoinWarps - 1);
+  float top = s_ml[w][0];
 #pragma unroll
-  for (int w = 0; w < 4; w++) top = fmaxf(top, s_ml[w][0]);
+  for (int o = kJoinWarps / 2; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  const float f = s_ml[w][0] == -INFINITY ? (s_ml[w][1] == 0.0f ? 0.0f : s_ml[w][1]) : exp2_fast(__fsub_rn(s_ml[w][0], top));
+  float sum = __fmul_rn(f, s_ml[w][1]);
 #pragma unroll
-  for (int w = 0; w < 4; w++) {
-    const float f = s_ml[w][0] == -INFINITY ? 0.0f : exp2_fast(__fsub_rn(s_ml[w][0], top));
-    sum = __fmaf_rn(f, s_ml[w][1], sum);
-    a = __fmaf_rn(f, s_o[w][2 * threadIdx.x], a);
-    b = __fmaf_rn(f, s_o[w][2 * threadIdx.x + 1], b);
+  for (int o = kJoinWarps / 2; o; o >>= 1) sum = __fadd_rn(sum, __shfl_xor_sync(0xffffffffu, sum, o));
+#pragma unroll
+  for (int i = 0; i < N; i++) x[i] = 0.0f;
+#pragma unroll
+  for (int k = 0; k < kJoinWarps; k++) {
+    const float fk = __shfl_sync(0xffffffffu, f, k);
+#pragma unroll
+    for (int i = 0; i < N; i++) x[i] = __fmaf_rn(fk, s_x[k][lane * N + i], x[i]);
   }
-  const int rr = row0 + r, token = rr / p.group, hq = h * p.group + (rr - token * p.group);
-  const float inv = sum > 0.0f ? __fdiv_rn(1.0f, sum) : (sum == 0.0f ? 0.0f : sum);
-  E* dst = reinterpret_cast<E*>(p.o_ptr) + s * p.o.seq + (int64_t)token * p.o.token + hq * p.o.head + 2 * threadIdx.x;
-  if constexpr (T == PKV_DST_F32) *reinterpret_cast<float2*>(dst) = make_float2(__fmul_rn(a, inv), __fmul_rn(b, inv));
-  else *reinterpret_cast<uint32_t*>(dst) = pkv_pack2<T>(__fmul_rn(a, inv), __fmul_rn(b, inv));
-  if (p.lse && threadIdx.x == 0)
-    p.lse[((int64_t)s * p.q.n + token) * p.q_heads + hq] =
-        sum == 0.0f ? -INFINITY : __fmul_rn(kLn2, __fadd_rn(top, __fsub_rn(log2f(sum), kWeightShift)));
+  write_row<T, N>(p, s, h, tile * 8 * NT + row, lane * N, x, top, sum, lane == 0);
 }
 
 // mass[key] += sum over the query rows of exp(score - lse).  A warp keeps the dequantised keys of 32 tokens in
@@ -624,9 +855,9 @@ kv4_mass_kernel(const __grid_constant__ AttendParams p) {
   if (qn < 0 || qn > p.q.n) qn = 0;
   if (qn == 0) return;
   const int pos0 = end - qn, rows = qn * p.group;
-  for (int token0 = (blockIdx.x * kWarps + warp) * kStageTokens; token0 < len; token0 += gridDim.x * kWarps * kStageTokens) {
+  for (int token0 = (blockIdx.x * kWarps + warp) * kMassTokens; token0 < len; token0 += gridDim.x * kWarps * kMassTokens) {
   const uint8_t* atom[2];
-  unsigned there = token0 + kStageTokens <= len ? 0xffffffffu : (1u << (len - token0)) - 1u;
+  unsigned there = token0 + kMassTokens <= len ? 0xffffffffu : (1u << (len - token0)) - 1u;
 #pragma unroll
   for (int a = 0; a < 2; a++) {
     atom[a] = token0 + 16 * a < len ? p.c.atom(s, h, token0 / 16 + a, A::BYTES, p.err) : nullptr;
@@ -649,11 +880,11 @@ kv4_mass_kernel(const __grid_constant__ AttendParams p) {
   int r_first = 0;
   if (!by_position && qn > 1) r_first = max(0, token0 - pos0) * p.group / 8 * 8;
   for (int r0 = r_first; r0 < rows; r0 += 8) {
-    if (!by_position && p.window > 0 && token0 >= p.sinks && pos0 + r0 / p.group - (token0 + kStageTokens - 1) >= p.window) break;
+    if (!by_position && p.window > 0 && token0 >= p.sinks && pos0 + r0 / p.group - (token0 + kMassTokens - 1) >= p.window) break;
     uint32_t qhi[1][D / 16][2], qlo[1][D / 16][2];
     const int r = r0 + g, token = r / p.group, hq = h * p.group + (r - token * p.group);
     const E* qp = reinterpret_cast<const E*>(p.q_ptr) + s * p.q.seq + (int64_t)token * p.q.token + hq * p.q.head;
-    const float inv = load_query<D, T>(qp, q4, r < rows, qhi[0], qlo[0]);
+    const float inv = load_query<D, T>(qp, q4, r < rows, p.negate, qhi[0], qlo[0]);
     const float lse = r < rows ? p.lse[((int64_t)s * p.q.n + token) * p.q_heads + hq] : -INFINITY;
     const float f = __fmul_rn(__fmul_rn(__fmul_rn(p.scale, kLog2e), kScaleShift), inv);
     float factor[2], base[2];
@@ -698,8 +929,8 @@ kv4_mass_kernel(const __grid_constant__ AttendParams p) {
 
 // ---- host ---------------------------------------------------------------------------------------------------------------
 struct Plan {
-  int nt, row_tiles, chunk, splits;
-  int64_t part_rows;  // rows of partial sums, 0 without a split
+  int nt, row_tiles, runs;
+  int64_t part_rows;  // rows of partial sums
 };
 
 int sm_count() {
@@ -714,21 +945,19 @@ Plan make_plan(const Cache& c, const pkv_kv4_rows* q, const pkv_kv4_attend_args*
   r.nt = rows > 8 ? 2 : 1;
   r.row_tiles = (int)((rows + 8 * r.nt - 1) / (8 * r.nt));
   int64_t longest = a->max_len > 0 && a->max_len < c.capacity ? a->max_len : c.capacity;
-  if (a->window > 0 && !c.positions) {  // slots outside the sinks and the window of a tile's tokens are never visited
-    const int64_t seen = (int64_t)a->window + a->sinks + q->n_tokens + 4 * kStageTokens;
+  if (a->window > 0 && !c.positions) {  // slots outside the sinks and the window of the query tokens are never visited
+    const int64_t seen = (int64_t)a->window + a->sinks + q->n_tokens + 3 * kUnitTokens;
     if (seen < longest) longest = seen;
   }
-  const int64_t stages = (longest + kStageTokens - 1) / kStageTokens;
-  const int64_t tiles = (int64_t)c.n_seqs * c.heads * r.row_tiles;
-  // enough CTAs for every SM to hold its four, and at least four stages for each of a CTA's warps
-  const int64_t want = (int64_t)sm_count() * (r.nt == 1 ? 4 : 2);
-  int64_t chunk = (stages * tiles + want - 1) / want;
-  if (chunk < 4 * kWarps) chunk = 4 * kWarps;
-  if (chunk > stages) chunk = stages > 0 ? stages : 1;
-  r.chunk = (int)((chunk + kWarps - 1) / kWarps * kWarps);
-  r.splits = (int)((stages + r.chunk - 1) / r.chunk);
-  if (r.splits < 1) r.splits = 1;
-  r.part_rows = r.splits > 1 ? tiles * r.splits * 8 * r.nt : 0;
+  const int64_t units = (longest + kUnitTokens - 1) / kUnitTokens;
+  // Rows of up to four units a warp are not worth a second launch.
+  r.runs = 0;
+  if (units > 4 * kWarps) {
+    const int64_t all = (units * c.n_seqs * c.heads * r.row_tiles + kWarps - 1) / kWarps * kWarps;
+    const int64_t resident = sm_count() * kWarps * (r.nt == 1 ? 3 : 2);
+    r.runs = (int)(all < resident ? all : resident);
+  }
+  r.part_rows = (int64_t)r.runs * 2 * 8 * r.nt;
   return r;
 }
 
@@ -738,11 +967,22 @@ int launch_attend(const AttendParams& p, cudaStream_t s) {
   constexpr int bytes = Shared<D, NT>::BYTES;
   if (bytes > 48 * 1024)
     if (cudaError_t ce = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes)) return pkv_cuda_status(ce);
-  kernel<<<dim3(p.splits, p.c.heads * p.row_tiles, p.c.n_seqs), kWarps * 32, bytes, s>>>(p);
+  const dim3 rows(p.row_tiles, p.c.heads, p.c.n_seqs);
+  kernel<<<p.runs ? dim3(p.runs / kWarps) : rows, kWarps * 32, bytes, s>>>(p);
   pkv_count_launch();
   if (cudaError_t ce = cudaGetLastError()) return pkv_cuda_status(ce);
-  if (p.splits > 1) {
-    kv4_combine_kernel<D, NT, T><<<dim3(p.row_tiles * 8 * NT, p.c.heads, p.c.n_seqs), 128, 0, s>>>(p);
+  if (p.runs) {
+    // its launch overlaps the end of the first kernel; it waits (griddepcontrol) before it reads the parts
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr = {};
+    cfg.gridDim = dim3(p.row_tiles * 8 * NT, p.c.heads, p.c.n_seqs);
+    cfg.blockDim = dim3(kJoinWarps * 32);
+    cfg.stream = s;
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    if (cudaError_t ce = cudaLaunchKernelEx(&cfg, kv4_combine_kernel<D, NT, T>, p)) return pkv_cuda_status(ce);
     pkv_count_launch();
   }
   return pkv_cuda_status(cudaGetLastError());
@@ -752,7 +992,7 @@ template <int D, int T>
 int launch_all(const AttendParams& p, int nt, bool accumulate, int longest, cudaStream_t s) {
   if (int st = nt == 1 ? launch_attend<D, 1, T>(p, s) : launch_attend<D, 2, T>(p, s)) return st;
   if (accumulate && longest > 0) {
-    const int per = kWarps * kStageTokens;
+    const int per = kWarps * kMassTokens;
     kv4_mass_kernel<D, T><<<dim3((longest + per - 1) / per, p.c.heads, p.c.n_seqs), kWarps * 32, 0, s>>>(p);
     pkv_count_launch();
   }
@@ -763,9 +1003,9 @@ int check_args(const Cache& c, const pkv_kv4_rows* q, const pkv_kv4_attend_args*
   if (!a || a->n_q_heads < 1 || a->n_q_heads % c.heads || a->window < 0 || a->sinks < 0 || a->max_len < 0 ||
       (a->accumulate != 0 && a->accumulate != 1) || !isfinite(a->scale))
     return PKV_ERR_INVALID_ARGUMENT;
-  // row numbers are 32-bit, and heads x row tiles is a grid dimension
+  // row numbers are 32-bit
   const int64_t rows = (int64_t)q->n_tokens * (a->n_q_heads / c.heads);
-  if (rows > 0x3fffffff || (rows / 8 + 1) * c.heads > 65535) return PKV_ERR_UNSUPPORTED;
+  if (rows > 0x3fffffff) return PKV_ERR_UNSUPPORTED;
   return PKV_OK;
 }
 
@@ -797,14 +1037,15 @@ extern "C" int pkv_kv4_attend_dev(const pkv_kv4_cache* cache, const void* q_dev,
   p.o_ptr = out_dev;
   p.lse = lse_dev;
   p.q_lens = q_lens_dev;
-  p.scale = args->scale;
+  p.scale = fabsf(args->scale);
+  p.negate = args->scale < 0.0f;
   p.q_heads = args->n_q_heads;
   p.group = args->n_q_heads / p.c.heads;
   p.window = args->window;
   p.sinks = args->sinks;
   p.row_tiles = plan.row_tiles;
-  p.chunk = plan.chunk;
-  p.splits = plan.splits;
+  p.runs = plan.runs;
+  p.whole_units = p.c.page_atoms % kUnitAtoms == 0;
   p.part_o = (float*)workspace_dev;
   p.part_ml = p.part_o + plan.part_rows * cache->dim;
   p.err = err_dev;
