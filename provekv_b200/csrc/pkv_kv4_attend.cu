@@ -16,7 +16,8 @@
 //   short rows   a CTA per (sequence, kv head, row tile); its warps take every fourth unit and join their sums in
 //                shared memory: one launch
 //   long rows    as many warps as the GPU holds; all units of all rows, laid end to end, are cut into equal runs, one a warp,
-//                whatever the lengths.  A row that was cut is joined by a second launch from the warps' sums.
+//                whatever the lengths.  The stream of units runs on from one row into the next.  A row that was cut is joined
+//                by a second launch from the warps' sums.
 //
 #include <math.h>
 
@@ -27,8 +28,10 @@ using namespace pkv_kv4;
 namespace {
 
 constexpr int kWarps = 4;
-constexpr int kUnitTokens = 64, kUnitAtoms = 4;
+constexpr int kUnitAtoms = 4, kUnitTokens = kUnitAtoms * kAtomTokens;
+constexpr int kBatch = 32 / kUnitAtoms;  // units whose page numbers a warp fetches at once
 constexpr int kStages = 2;
+constexpr int kMaxRows = 2048;           // (sequence, kv head, row tile)s that share runs
 constexpr int kJoinWarps = 8;
 constexpr int kMassTokens = 32;  // keys a warp of the mass kernel holds
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
@@ -48,9 +51,11 @@ struct AttendParams {
   int group, q_heads, window, sinks;
   int row_tiles;      // tiles of 8 NT query rows per (sequence, kv head)
   int runs;           // warps that share the units of all rows; 0: a CTA per row tile
+  int tile_rows;      // query rows of a tile, 8 NT
   int whole_units;    // 1: a unit never crosses a page, one copy brings it
   float* part_o;      // [run][2][8 NT][D] unnormalised sums of a run's first and last row, where it has only a part of it
   float* part_ml;     // [run][2][8 NT][2] reference and sum
+  int2* part_of;      // [sequence][kv head][row tile] first run and number of runs that have a part of it
   uint64_t* err;
 };
 
@@ -91,20 +96,13 @@ __device__ __forceinline__ float row_power(float amax) {
   return __uint_as_float((uint32_t)(x + 127) << 23);
 }
 
-// The B operand of S^T for query row `lane / 4`: this lane's D / 4 channels, in the order nibbles() delivers
-// the keys', odd channels divided by 16; negated for a negative softmax scale, so that scores are
-// scaled by something positive.  hi (and for f32 queries lo) [2 D / 32][2]; returns the inverse power.
+// The B operand of S^T for query row `lane / 4` from its values of channels (lane % 4) D/4 .. (this lane's), in the
+// order nibbles() delivers the keys', odd channels divided by 16; negated for a negative softmax scale, so that scores
+// are scaled by something positive.  hi (and for f32 queries lo) [D / 16][2]; returns the inverse power.
 template <int D, int T>
-__device__ __forceinline__ float load_query(const typename PkvDst<T>::type* p, int q4, bool live, bool negate, uint32_t (&hi)[D / 16][2],
-                                            uint32_t (&lo)[D / 16][2]) {
+__device__ __forceinline__ float query_operand(const float (&x)[D / 4], bool negate, uint32_t (&hi)[D / 16][2],
+                                               uint32_t (&lo)[D / 16][2]) {
   constexpr int CH = D / 4;
-  float x[CH];
-  if (live) {
-    load_f32<T, CH>(p + q4 * CH, x);
-  } else {
-#pragma unroll
-    for (int i = 0; i < CH; i++) x[i] = 0.0f;
-  }
   float amax = 0.0f;
 #pragma unroll
   for (int i = 0; i < CH; i++) amax = fmaxf(amax, fabsf(x[i]));
@@ -126,6 +124,20 @@ __device__ __forceinline__ float load_query(const typename PkvDst<T>::type* p, i
     }
   }
   return inv;
+}
+// Those values of query row `row` (of its kv head's, token by token).
+template <int D, int T>
+__device__ __forceinline__ void query_values(const AttendParams& p, int s, int h, int row, int rows, float (&x)[D / 4]) {
+  using E = typename PkvDst<T>::type;
+  const int token = row / p.group, hq = h * p.group + (row - token * p.group);
+  if (row < rows) {
+    load_f32<T, D / 4>(reinterpret_cast<const E*>(p.q_ptr) + s * p.q.seq + (int64_t)token * p.q.token + hq * p.q.head +
+                           (threadIdx.x & 3) * (D / 4),
+                       x);
+  } else {
+#pragma unroll
+    for (int i = 0; i < D / 4; i++) x[i] = 0.0f;
+  }
 }
 
 // One atom's scores: S^T[16 keys][8 NT rows] from its K codes and scales in shared memory.
@@ -282,34 +294,67 @@ __device__ __forceinline__ int units_of(const AttendParams& p, const Sequence& q
   if (q.qn == 0) return 0;
   return max(1, visible_span(p, q.len, q.end - q.qn, q.end - 1).count);
 }
-
-// Total units, and those before sequence `s`; whole CTA of W warps.
-template <int W>
-__device__ __forceinline__ void count_units(const AttendParams& p, int s, int64_t* total, int64_t* before, int64_t (&scratch)[2][W]) {
-  int64_t all = 0, pre = 0;
-  for (int i = threadIdx.x; i < p.c.n_seqs; i += 32 * W) {
-    const int u = units_of(p, sequence_of(p, i));
-    all += u;
-    if (i < s) pre += u;
-  }
-#pragma unroll
-  for (int o = 16; o; o >>= 1) {
-    all += __shfl_xor_sync(0xffffffffu, all, o);
-    pre += __shfl_xor_sync(0xffffffffu, pre, o);
-  }
-  if ((threadIdx.x & 31) == 0) {
-    scratch[0][threadIdx.x >> 5] = all;
-    scratch[1][threadIdx.x >> 5] = pre;
-  }
-  __syncthreads();
-  *total = *before = 0;
-#pragma unroll
-  for (int w = 0; w < W; w++) {
-    *total += scratch[0][w];
-    *before += scratch[1][w];
-  }
+// Row tiles of a kv head that the sequence's queries fill (row_tiles is the number for a full batch row).
+__device__ __forceinline__ int row_tiles_of(const AttendParams& p, const Sequence& q) {
+  return (q.qn * p.group + p.tile_rows - 1) / p.tile_rows;
 }
-__device__ __forceinline__ int64_t units_per_run(int64_t total, int runs) { return total <= runs ? 1 : (total + runs - 1) / runs; }
+// (below 2^31 for all sequences together, which make_plan sees to)
+__device__ __forceinline__ unsigned all_units_of(const AttendParams& p, const Sequence& q) {
+  return (unsigned)(units_of(p, q) * p.c.heads * row_tiles_of(p, q));
+}
+__device__ __forceinline__ unsigned all_units_of(const AttendParams& p, int s) {
+  return s < p.c.n_seqs ? all_units_of(p, sequence_of(p, s)) : 0u;
+}
+
+// The units of all rows, cut into runs as even as they can be; no run is empty before one that is not.
+struct Runs {
+  unsigned total, each, more;  // the first `more` runs have each + 1 units, the others `each`
+  __device__ __forceinline__ unsigned start(unsigned i) const { return min(total, i * each + min(i, more)); }
+  __device__ __forceinline__ unsigned of(unsigned unit) const {
+    const unsigned cut = more * (each + 1);
+    return unit < cut ? unit / (each + 1) : more + (unit - cut) / each;
+  }
+};
+// Whole warp; `mine` is all_units_of(p, lane).
+__device__ __forceinline__ Runs cut_runs(const AttendParams& p, unsigned mine) {
+  unsigned sum = mine;
+  for (int i = 32 + (threadIdx.x & 31); i < p.c.n_seqs; i += 32) sum += all_units_of(p, i);
+  Runs r;
+  r.total = __reduce_add_sync(0xffffffffu, sum);
+  const unsigned n = max(1u, min((unsigned)p.runs, r.total));
+  r.each = r.total / n;
+  r.more = r.total - r.each * n;
+  return r;
+}
+
+// A row tile on the way through all rows' units: sequence, kv head, tile; the last ones' index runs fastest.
+struct Cursor {
+  int s, h, tile, tiles, units;  // tiles of the sequence's kv heads; units of the tile, counted as the sequence's
+  Sequence seq;
+  Span span;
+  __device__ __forceinline__ void place(const AttendParams& p) {
+    const int pos0 = seq.end - seq.qn, row0 = tile * p.tile_rows;
+    span = visible_span(p, seq.len, pos0 + row0 / p.group, pos0 + min(seq.qn - 1, (row0 + p.tile_rows - 1) / p.group));
+  }
+  __device__ __forceinline__ void enter(const AttendParams& p, int s_) {
+    s = s_;
+    seq = sequence_of(p, s);
+    units = units_of(p, seq);
+    tiles = row_tiles_of(p, seq);
+  }
+  __device__ __forceinline__ void next(const AttendParams& p) {  // only called while there is one
+    if (++tile == tiles) {
+      tile = 0;
+      if (++h == p.c.heads) {
+        h = 0;
+        do enter(p, s + 1);
+        while (seq.qn == 0);
+      }
+    }
+    place(p);
+  }
+  __device__ __forceinline__ int rows(const AttendParams& p) const { return seq.qn * p.group; }
+};
 
 template <int D, int NT>
 struct Shared {
@@ -333,260 +378,6 @@ struct Sums {
   float o[D / 16][NT][4];            // channels (lane / 4) D/8 + 2 j + i / 2, row 2 (lane % 4) + i % 2
   float m[NT][2], l[NT][2];          // reference (log2) and sum of rows 2 (lane % 4) + e; l is this lane's part
 };
-
-// The units first, first + stride, .. (count of them) of row tile `tile`; whole warp.  False if a copy never came.
-template <int D, int NT, int T>
-__device__ __forceinline__ bool stream_units(const AttendParams& p, int s, int h, int tile, const Sequence& seq, int first, int stride,
-                                             int count, Ring& ring, Sums<D, NT>& r) {
-  constexpr bool F32 = T == PKV_DST_F32;
-  using A = Atom<D>;
-  using S = Shared<D, NT>;
-  using E = typename PkvDst<T>::type;
-  const int lane = threadIdx.x & 31, g = lane >> 2, q4 = lane & 3;
-  const int row0 = tile * 8 * NT, rows = seq.qn * p.group - row0;
-  const int len = seq.len, pos0 = seq.end - seq.qn;  // position of query token 0
-  const int first_token = row0 / p.group, last_token = min(seq.qn - 1, (row0 + 8 * NT - 1) / p.group);
-  const Span span = visible_span(p, len, pos0 + first_token, pos0 + last_token);
-  // a tile may see fewer units than its sequence counts
-  if (first >= span.count) count = 0;
-  else if (first + (int64_t)(count - 1) * stride >= span.count) count = (span.count - 1 - first) / stride + 1;
-
-  // ---- the stream: page numbers are fetched for 8 units at once, one atom per lane, a batch ahead of their use
-  auto unit_of = [&](int i) { return span.unit(first + i * stride); };
-  auto atom_of = [&](int i0) -> int {  // lane l: atom l & 3 of unit i0 + l / 4; -1 = nothing to load
-    const int i = i0 + (lane >> 2);
-    if (i >= count) return -1;
-    const int a = unit_of(i) * kUnitAtoms + (lane & 3);
-    return a * kAtomTokens < len ? a : -1;
-  };
-  auto page_of = [&](int a) -> int { return a < 0 ? -1 : __ldg(p.c.table + (int64_t)s * p.c.max_pages + a / p.c.page_atoms); };
-  int atom = atom_of(0), page = page_of(atom);
-  const uint8_t* src = nullptr;
-  unsigned live_issue = 0, live_use = 0;  // bit l: the atom of lane l is there (batch being issued / consumed)
-  auto next_batch = [&](int i0) {         // the batch that starts at unit i0; its page numbers are on their way
-    src = nullptr;
-    if (atom >= 0) {
-      if (page < 0 || page >= p.c.n_pages) pkv_report(p.err, 0, s, PKV_VEC_BAD_SEQUENCE);
-      else src = p.c.pages + (((int64_t)page * p.c.heads + h) * p.c.page_atoms + atom % p.c.page_atoms) * (int64_t)A::BYTES;
-    }
-    live_issue = __ballot_sync(0xffffffffu, src != nullptr);
-    atom = atom_of(i0 + 8);
-    page = page_of(atom);
-  };
-  int slot_in = ring.slot;
-  auto issue = [&](int i) {  // whole warp; i < count
-    if ((i & 7) == 0) next_batch(i);
-    const int l = 4 * (i & 7);
-    const uint32_t bytes = (uint32_t)__popc((live_issue >> l) & 15u) * A::BYTES;
-    uint8_t* dst = ring.base + slot_in * S::UNIT;
-    uint64_t* bar = ring.bars + slot_in;
-    if (lane == l) {
-      pkv_mbar_expect_tx(bar, bytes);
-      if (p.whole_units && bytes) pkv_bulk_load(dst, src, bytes, bar);
-    }
-    if (!p.whole_units) {
-      __syncwarp();
-      if ((lane & ~3) == l && src) pkv_bulk_load(dst + (lane & 3) * A::BYTES, src, A::BYTES, bar);
-    }
-    if (++slot_in == kStages) slot_in = 0;
-  };
-  int issued = 0;
-  for (; issued < min(kStages, count); issued++) {
-    issue(issued);
-    if (issued == 0) live_use = live_issue;
-  }
-
-  // ---- queries
-  uint32_t qhi[NT][D / 16][2], qlo[NT][D / 16][2];
-  float factor[NT][2];  // of the scores of rows 2 q4 and 2 q4 + 1: softmax scale, log2 e, powers of two
-#pragma unroll
-  for (int n = 0; n < NT; n++) {
-    const int rr = row0 + 8 * n + g, token = rr / p.group, hq = h * p.group + (rr - token * p.group);
-    const E* qp = reinterpret_cast<const E*>(p.q_ptr) + s * p.q.seq + (int64_t)token * p.q.token + hq * p.q.head;
-    const float inv = load_query<D, T>(qp, q4, 8 * n + g < rows, p.negate, qhi[n], qlo[n]);
-    const float f = __fmul_rn(__fmul_rn(p.scale, kLog2e), kScaleShift);
-#pragma unroll
-    for (int e = 0; e < 2; e++) factor[n][e] = __fmul_rn(f, __shfl_sync(0xffffffffu, inv, 4 * (2 * q4 + e)));
-  }
-  const int qpos_min = pos0 + first_token, qpos_max = pos0 + last_token;
-  // positions matter only where a row can see less than everything that is held
-  const bool by_position = p.c.positions != nullptr && (p.window > 0 || seq.qn > 1);
-  const int32_t* positions = by_position ? p.c.positions + p.c.stat(s, h) : nullptr;
-
-#pragma unroll
-  for (int j = 0; j < D / 16; j++)
-#pragma unroll
-    for (int n = 0; n < NT; n++)
-#pragma unroll
-      for (int i = 0; i < 4; i++) r.o[j][n][i] = 0.0f;
-#pragma unroll
-  for (int n = 0; n < NT; n++)
-#pragma unroll
-    for (int e = 0; e < 2; e++) {
-      r.m[n][e] = -INFINITY;
-      r.l[n][e] = 0.0f;
-    }
-
-#pragma unroll 1
-  for (int done = 0; done < count; done++) {
-    if (done && (done & 7) == 0) live_use = live_issue;  // issue() of this batch's first unit has run
-    const int token0 = unit_of(done) * kUnitTokens;
-    int kpos[2] = {0, 0};
-    if (by_position) {
-#pragma unroll
-      for (int i = 0; i < 2; i++)
-        if (token0 + 32 * i + lane < len) kpos[i] = __ldg(positions + token0 + 32 * i + lane);
-    }
-    if (!__all_sync(0xffffffffu, pkv_mbar_wait(ring.bars + ring.slot, ring.phase))) {
-      // a copy never arrived: give the others their time, report, and leave nothing behind
-      for (int i = done + 1; i < issued; i++) {
-        if (++ring.slot == kStages) ring.slot = 0, ring.phase ^= 1u;
-        pkv_mbar_wait(ring.bars + ring.slot, ring.phase);
-      }
-      if (lane == 0) pkv_report(p.err, 0, s, PKV_VEC_DEVICE_WAIT);
-      return false;
-    }
-    uint8_t* unit = ring.base + ring.slot * S::UNIT;
-    const unsigned quad = (live_use >> (4 * (done & 7))) & 15u;
-    const bool whole = quad == 15u && token0 + kUnitTokens <= len;
-    unsigned there[2] = {0xffffffffu, 0xffffffffu};  // tokens that are there, one bit each
-    if (!whole) {
-#pragma unroll
-      for (int i = 0; i < 2; i++) {
-        const int left = len - token0 - 32 * i;
-        there[i] = left >= 32 ? 0xffffffffu : left <= 0 ? 0u : (1u << left) - 1u;
-        if (!((quad >> (2 * i)) & 1u)) there[i] &= 0xffff0000u;
-        if (!((quad >> (2 * i)) & 2u)) there[i] &= 0x0000ffffu;
-        // values of absent tokens become zeros (any bytes may lie there; 0 x inf would spoil the sums)
-        if (!((there[i] >> lane) & 1u)) {
-          uint8_t* sc = unit + (2 * i + (lane >> 4)) * A::BYTES + A::VS + (lane & 15) * A::SROW;
-#pragma unroll
-          for (int b = 0; b < A::SROW; b += 4) *reinterpret_cast<uint32_t*>(sc + b) = 0u;
-        }
-      }
-      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-      __syncwarp();
-    }
-    const bool masked = !whole || by_position || token0 + kUnitTokens - 1 > qpos_min ||
-                        (p.window > 0 && qpos_max - token0 >= p.window && token0 + kUnitTokens > p.sinks);
-
-    float sc[kUnitAtoms][NT][4];
-#pragma unroll
-    for (int a = 0; a < kUnitAtoms; a++) scores_of<D, NT, F32>(unit + a * A::BYTES, lane, qhi, qlo, sc[a]);
-    float fac[NT][2];  // what the scores are still to be multiplied by
-#pragma unroll
-    for (int n = 0; n < NT; n++)
-#pragma unroll
-      for (int e = 0; e < 2; e++) fac[n][e] = factor[n][e];
-    if (masked) {
-#pragma unroll
-      for (int n = 0; n < NT; n++)
-#pragma unroll
-        for (int e = 0; e < 2; e++) fac[n][e] = 1.0f;
-#pragma unroll
-      for (int a = 0; a < kUnitAtoms; a++)
-#pragma unroll
-        for (int hh = 0; hh < 2; hh++) {
-          const int t = 16 * (a & 1) + 8 * hh + tau(g);
-          const int kp = by_position ? __shfl_sync(0xffffffffu, kpos[a >> 1], t) : token0 + 32 * (a >> 1) + t;
-          const bool held = (there[a >> 1] >> t) & 1u;
-#pragma unroll
-          for (int n = 0; n < NT; n++)
-#pragma unroll
-            for (int e = 0; e < 2; e++) {
-              const int d = pos0 + (row0 + 8 * n + 2 * q4 + e) / p.group - kp;
-              const bool see = held && d >= 0 && (p.window == 0 || d < p.window || kp < p.sinks);
-              float& x = sc[a][n][2 * hh + e];
-              x = see ? __fmul_rn(x, factor[n][e]) : -INFINITY;
-            }
-        }
-    }
-    float top[NT][2];
-    bool raise = false;
-#pragma unroll
-    for (int n = 0; n < NT; n++)
-#pragma unroll
-      for (int e = 0; e < 2; e++) {
-        float t = fmaxf(sc[0][n][e], sc[0][n][2 + e]);
-#pragma unroll
-        for (int a = 1; a < kUnitAtoms; a++) t = fmaxf(t, fmaxf(sc[a][n][e], sc[a][n][2 + e]));
-        top[n][e] = __fmul_rn(t, fac[n][e]);
-        raise = raise || top[n][e] > __fadd_rn(r.m[n][e], kLag);
-      }
-    if (__any_sync(0xffffffffu, raise)) {
-#pragma unroll
-      for (int n = 0; n < NT; n++)
-#pragma unroll
-        for (int e = 0; e < 2; e++) {
-          float t = top[n][e];
-          t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 4));
-          t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 8));
-          t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 16));
-          const float m = fmaxf(r.m[n][e], t);
-          const float f = r.m[n][e] == -INFINITY ? 0.0f : exp2_fast(__fsub_rn(r.m[n][e], m));
-          r.m[n][e] = m;
-          r.l[n][e] = __fmul_rn(r.l[n][e], f);
-#pragma unroll
-          for (int j = 0; j < D / 16; j++) {
-            r.o[j][n][e] = __fmul_rn(r.o[j][n][e], f);
-            r.o[j][n][2 + e] = __fmul_rn(r.o[j][n][2 + e], f);
-          }
-        }
-    }
-    uint32_t pb[kUnitAtoms][NT][F32 ? 4 : 2];
-#pragma unroll
-    for (int n = 0; n < NT; n++) {
-      float base[2];
-#pragma unroll
-      for (int e = 0; e < 2; e++) base[e] = r.m[n][e] == -INFINITY ? 0.0f : __fsub_rn(kWeightShift, r.m[n][e]);
-#pragma unroll
-      for (int a = 0; a < kUnitAtoms; a++)
-#pragma unroll
-        for (int hh = 0; hh < 2; hh++) {
-          const float w0 = exp2_fast(__fmaf_rn(sc[a][n][2 * hh], fac[n][0], base[0]));
-          const float w1 = exp2_fast(__fmaf_rn(sc[a][n][2 * hh + 1], fac[n][1], base[1]));
-          r.l[n][0] = __fadd_rn(r.l[n][0], w0);
-          r.l[n][1] = __fadd_rn(r.l[n][1], w1);
-          const uint32_t hw = half2_of(w0, w1);
-          pb[a][n][hh] = transpose8(hw);
-          if constexpr (F32) {
-            const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&hw));
-            pb[a][n][2 + hh] = transpose8(half2_of(__fsub_rn(w0, f.x), __fsub_rn(w1, f.y)));
-          }
-        }
-    }
-    if constexpr (F32) {  // two atoms' sum on its own, then one rounded addition: a long chain would drift by its cut-off bits
-#pragma unroll
-      for (int a = 0; a < kUnitAtoms; a += 2) {
-        float t[D / 16][NT][4];
-        weigh<D, NT, F32, true>(unit + a * A::BYTES, lane, pb[a], t);
-        weigh<D, NT, F32, false>(unit + (a + 1) * A::BYTES, lane, pb[a + 1], t);
-#pragma unroll
-        for (int j = 0; j < D / 16; j++)
-#pragma unroll
-          for (int n = 0; n < NT; n++)
-#pragma unroll
-            for (int i = 0; i < 4; i++) r.o[j][n][i] = __fadd_rn(r.o[j][n][i], t[j][n][i]);
-      }
-    } else {
-#pragma unroll
-      for (int a = 0; a < kUnitAtoms; a++) weigh<D, NT, F32, false>(unit + a * A::BYTES, lane, pb[a], r.o);
-    }
-    __syncwarp();
-    if (issued < count) issue(issued++);  // into the slot that was just read
-    if (++ring.slot == kStages) ring.slot = 0, ring.phase ^= 1u;
-  }
-#pragma unroll
-  for (int n = 0; n < NT; n++)
-#pragma unroll
-    for (int e = 0; e < 2; e++) {  // the lanes' parts of the sums
-      float t = r.l[n][e];
-      t = __fadd_rn(t, __shfl_xor_sync(0xffffffffu, t, 4));
-      t = __fadd_rn(t, __shfl_xor_sync(0xffffffffu, t, 8));
-      r.l[n][e] = __fadd_rn(t, __shfl_xor_sync(0xffffffffu, t, 16));
-    }
-  return true;
-}
 
 // Writes N channels of a row, sums x (scale and the 16 of odd channels already undone) over l.
 template <int T, int N>
@@ -613,14 +404,337 @@ __device__ __forceinline__ void write_row(const AttendParams& p, int s, int h, i
         l == 0.0f ? -INFINITY : __fmul_rn(kLn2, __fadd_rn(m, __fsub_rn(log2f(l), kWeightShift)));
 }
 
-template <int D, int NT, int T>
+// Streams a warp's units; whole warp.  DIRECT: units v, v + kWarps, .. of row tile `t`; the sums stay in `r`.
+// Otherwise: `count` units from unit v of row tile `t` on (number `at` of all rows' units), into the next row tiles; every row tile's sums are written
+// when it ends, into out if the run has all of it, else into the run's parts.
+template <int D, int NT, int T, bool DIRECT>
+__device__ __forceinline__ void stream_units(const AttendParams& p, Cursor t, int v, int count, Ring& ring, Sums<D, NT>& r,
+                                             Runs runs = Runs(), unsigned at = 0) {
+  constexpr bool F32 = T == PKV_DST_F32;
+  constexpr int STEP = DIRECT ? kWarps : 1;
+  using A = Atom<D>;
+  using S = Shared<D, NT>;
+  const int lane = threadIdx.x & 31, g = lane >> 2, q4 = lane & 3;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0);
+  float qx[NT][D / 4];  // the queries' values are on their way while the first page numbers and units are
+#pragma unroll
+  for (int n = 0; n < NT; n++) query_values<D, T>(p, t.s, t.h, t.tile * 8 * NT + 8 * n + g, t.rows(p), qx[n]);
+
+  // ---- the stream.  Page numbers are fetched for up to kBatch units of a row tile at once, one atom per lane, a batch ahead
+  // of their use.
+  Cursor ahead = t;        // row tile of the next batch to fetch
+  int ahead_v = v, left = count;  // its first unit, and the units not yet fetched
+  int next_n = 0, next_page = -1, next_s = 0;
+  int64_t next_at = -1;    // place of the lane's atom in its page, -1 = nothing to load
+  auto fetch = [&]() {
+    if (!DIRECT && ahead_v == ahead.units && left > 0) {
+      ahead.next(p);
+      ahead_v = 0;
+    }
+    next_n = min(kBatch, DIRECT ? left : min(left, ahead.units - ahead_v));
+    const int uv = ahead_v + (lane / kUnitAtoms) * STEP, a = ahead.span.unit(uv) * kUnitAtoms + lane % kUnitAtoms;
+    next_at = -1;
+    next_s = ahead.s;
+    if (lane / kUnitAtoms < next_n && uv < ahead.span.count && a * kAtomTokens < ahead.seq.len) {
+      const int page = a / p.c.page_atoms;
+      next_page = __ldg(p.c.table + (int64_t)ahead.s * p.c.max_pages + page);
+      next_at = (int64_t)ahead.h * p.c.page_atoms + (a - page * p.c.page_atoms);
+    }
+    left -= next_n;
+    ahead_v += next_n * STEP;
+  };
+  fetch();
+  const uint8_t* src = nullptr;
+  unsigned live = 0;       // bit l: the atom of lane l is there (batch being issued)
+  int batch_n = 0, batch_i = 0;
+  unsigned quads = 0;      // of each slot of the ring: which of the unit's atoms are there, 4 bits
+  int slot_in = ring.slot;
+  auto issue = [&]() {     // whole warp
+    if (__builtin_expect(batch_i == batch_n, 0)) {
+      src = nullptr;
+      if (next_at >= 0) {
+        if (next_page < 0 || next_page >= p.c.n_pages) pkv_report(p.err, 0, next_s, PKV_VEC_BAD_SEQUENCE);
+        else src = p.c.pages + ((int64_t)next_page * p.c.heads * p.c.page_atoms + next_at) * (int64_t)A::BYTES;
+      }
+      live = __ballot_sync(0xffffffffu, src != nullptr);
+      batch_n = next_n;
+      batch_i = 0;
+      fetch();
+    }
+    const int l = kUnitAtoms * batch_i;
+    const unsigned quad = (live >> l) & 15u;
+    const uint32_t bytes = (uint32_t)__popc(quad) * A::BYTES;
+    quads = (quads & ~(15u << (4 * slot_in))) | (quad << (4 * slot_in));
+    uint8_t* dst = ring.base + slot_in * S::UNIT;
+    uint64_t* bar = ring.bars + slot_in;
+    if (lane == l) {
+      pkv_mbar_expect_tx(bar, bytes);
+      if (p.whole_units && bytes) pkv_bulk_load(dst, src, bytes, bar);
+    }
+    if (!p.whole_units) {
+      __syncwarp();
+      if (lane / kUnitAtoms == batch_i && src) pkv_bulk_load(dst + lane % kUnitAtoms * A::BYTES, src, A::BYTES, bar);
+    }
+    batch_i++;
+    if (++slot_in == kStages) slot_in = 0;
+  };
+  int issued = 0;
+#pragma unroll 1
+  for (; issued < min(kStages, count); issued++) issue();
+
+  uint32_t qhi[NT][D / 16][2], qlo[NT][D / 16][2];
+  float factor[NT][2];  // of the scores of rows 2 q4 and 2 q4 + 1: softmax scale, log2 e, powers of two
+  int len, pos0, row0, qpos_min, qpos_max;
+  bool by_position;
+  const int32_t* positions;
+  auto begin_tile = [&]() {
+#pragma unroll
+    for (int n = 0; n < NT; n++) {
+      const float inv = query_operand<D, T>(qx[n], p.negate, qhi[n], qlo[n]);
+      const float f = __fmul_rn(__fmul_rn(p.scale, kLog2e), kScaleShift);
+#pragma unroll
+      for (int e = 0; e < 2; e++) factor[n][e] = __fmul_rn(f, __shfl_sync(0xffffffffu, inv, 4 * (2 * q4 + e)));
+    }
+    len = t.seq.len;
+    pos0 = t.seq.end - t.seq.qn;  // position of query token 0
+    row0 = t.tile * 8 * NT;
+    qpos_min = pos0 + row0 / p.group;
+    qpos_max = pos0 + min(t.seq.qn - 1, (row0 + 8 * NT - 1) / p.group);
+    // positions matter only where a row can see less than everything that is held
+    by_position = p.c.positions != nullptr && (p.window > 0 || t.seq.qn > 1);
+    positions = by_position ? p.c.positions + p.c.stat(t.s, t.h) : nullptr;
+#pragma unroll
+    for (int j = 0; j < D / 16; j++)
+#pragma unroll
+      for (int n = 0; n < NT; n++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) r.o[j][n][i] = 0.0f;
+#pragma unroll
+    for (int n = 0; n < NT; n++)
+#pragma unroll
+      for (int e = 0; e < 2; e++) {
+        r.m[n][e] = -INFINITY;
+        r.l[n][e] = 0.0f;
+      }
+  };
+  auto join_lanes = [&]() {
+#pragma unroll
+    for (int n = 0; n < NT; n++)
+#pragma unroll
+      for (int e = 0; e < 2; e++) {
+        float x = r.l[n][e];
+        x = __fadd_rn(x, __shfl_xor_sync(0xffffffffu, x, 4));
+        x = __fadd_rn(x, __shfl_xor_sync(0xffffffffu, x, 8));
+        r.l[n][e] = __fadd_rn(x, __shfl_xor_sync(0xffffffffu, x, 16));
+      }
+  };
+  auto end_tile = [&](int v0, int n_units) {  // units v0 .. v0 + n_units - 1 of tile t are in r; `at` is the first one's number
+    join_lanes();
+    const int run = blockIdx.x * kWarps + warp;
+    if (v0 == 0 && lane == 0)
+      p.part_of[((int64_t)t.s * p.c.heads + t.h) * p.row_tiles + t.tile] =
+          make_int2(run, n_units == t.units ? 1 : (int)runs.of(at + t.units - 1) - run + 1);
+#pragma unroll
+    for (int n = 0; n < NT; n++)
+#pragma unroll
+      for (int e = 0; e < 2; e++) {
+        const int row = 8 * n + 2 * q4 + e;
+        float x[D / 8];
+#pragma unroll
+        for (int j = 0; j < D / 16; j++) {
+          x[2 * j] = __fmul_rn(r.o[j][n][e], kScaleShift);
+          x[2 * j + 1] = __fmul_rn(r.o[j][n][2 + e], kScaleShift / 16.0f);
+        }
+        if (row0 + row < t.rows(p)) {
+          if (n_units < t.units) {  // a row that starts here and goes on has the run's second place
+            const int64_t slot = ((int64_t)run * 2 + (v0 == 0)) * (8 * NT) + row;
+            store_f32<PKV_DST_F32, D / 8>(p.part_o + slot * D + g * (D / 8), x);
+            if (g == 0) *reinterpret_cast<float2*>(p.part_ml + slot * 2) = make_float2(r.m[n][e], r.l[n][e]);
+          } else {
+            write_row<T, D / 8>(p, t.s, t.h, row0 + row, g * (D / 8), x, r.m[n][e], r.l[n][e], g == 0);
+          }
+        }
+      }
+  };
+  int left_here = count;
+#pragma unroll 1
+  for (;;) {
+    begin_tile();
+    const int v0 = v, n_here = DIRECT ? count : min(left_here, t.units - v);
+#pragma unroll 1
+    for (int i = 0; i < n_here; i++, v += STEP) {
+      const int token0 = t.span.unit(v) * kUnitTokens;
+      int kpos[2] = {0, 0};
+      if (__builtin_expect(by_position, 0)) {
+#pragma unroll
+        for (int k = 0; k < 2; k++)
+          if (token0 + 32 * k + lane < len) kpos[k] = __ldg(positions + token0 + 32 * k + lane);
+      }
+      if (__builtin_expect(!__all_sync(0xffffffffu, pkv_mbar_wait(ring.bars + ring.slot, ring.phase)), 0)) {
+        // a copy never arrived: give the others their time, report, and leave nothing behind
+        for (int k = 1; k < kStages; k++) {
+          if (++ring.slot == kStages) ring.slot = 0, ring.phase ^= 1u;
+          if (ring.slot != slot_in) pkv_mbar_wait(ring.bars + ring.slot, ring.phase);
+        }
+        if (lane == 0) pkv_report(p.err, 0, t.s, PKV_VEC_DEVICE_WAIT);
+        return;
+      }
+      uint8_t* unit = ring.base + ring.slot * S::UNIT;
+      const unsigned quad = (quads >> (4 * ring.slot)) & 15u;
+      const bool whole = quad == 15u && token0 + kUnitTokens <= len;
+      unsigned there[2] = {0xffffffffu, 0xffffffffu};  // tokens that are there, one bit each
+      if (__builtin_expect(!whole, 0)) {
+#pragma unroll
+        for (int k = 0; k < 2; k++) {
+          const int left = len - token0 - 32 * k;
+          there[k] = left >= 32 ? 0xffffffffu : left <= 0 ? 0u : (1u << left) - 1u;
+          if (!((quad >> (2 * k)) & 1u)) there[k] &= 0xffff0000u;
+          if (!((quad >> (2 * k)) & 2u)) there[k] &= 0x0000ffffu;
+          // values of absent tokens become zeros (any bytes may lie there; 0 x inf would spoil the sums)
+          if (!((there[k] >> lane) & 1u)) {
+            uint8_t* sc = unit + (2 * k + (lane >> 4)) * A::BYTES + A::VS + (lane & 15) * A::SROW;
+#pragma unroll
+            for (int b = 0; b < A::SROW; b += 4) *reinterpret_cast<uint32_t*>(sc + b) = 0u;
+          }
+        }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncwarp();
+      }
+      const bool masked = !whole || by_position || token0 + kUnitTokens - 1 > qpos_min ||
+                          (p.window > 0 && qpos_max - token0 >= p.window && token0 + kUnitTokens > p.sinks);
+
+      // two atoms at a time, not unrolled: the loop has to stay in the instruction cache
+#pragma unroll 1
+      for (int k = 0; k < 2; k++, unit += 2 * A::BYTES) {
+        float sc[2][NT][4];
+#pragma unroll
+        for (int a = 0; a < 2; a++) scores_of<D, NT, F32>(unit + a * A::BYTES, lane, qhi, qlo, sc[a]);
+        float fac[NT][2];  // what the scores are still to be multiplied by
+#pragma unroll
+        for (int n = 0; n < NT; n++)
+#pragma unroll
+          for (int e = 0; e < 2; e++) fac[n][e] = factor[n][e];
+        if (__builtin_expect(masked, 0)) {
+#pragma unroll
+          for (int n = 0; n < NT; n++)
+#pragma unroll
+            for (int e = 0; e < 2; e++) fac[n][e] = 1.0f;
+          const unsigned here = k ? there[1] : there[0];
+          const int kp0 = k ? kpos[1] : kpos[0];
+#pragma unroll
+          for (int a = 0; a < 2; a++)
+#pragma unroll
+            for (int hh = 0; hh < 2; hh++) {
+              const int at = 16 * a + 8 * hh + tau(g);
+              const int kp = by_position ? __shfl_sync(0xffffffffu, kp0, at) : token0 + 32 * k + at;
+              const bool held = (here >> at) & 1u;
+#pragma unroll
+              for (int n = 0; n < NT; n++)
+#pragma unroll
+                for (int e = 0; e < 2; e++) {
+                  const int d = pos0 + (row0 + 8 * n + 2 * q4 + e) / p.group - kp;
+                  const bool see = held && d >= 0 && (p.window == 0 || d < p.window || kp < p.sinks);
+                  float& x = sc[a][n][2 * hh + e];
+                  x = see ? __fmul_rn(x, factor[n][e]) : -INFINITY;
+                }
+            }
+        }
+        float top[NT][2];
+        bool raise = false;
+#pragma unroll
+        for (int n = 0; n < NT; n++)
+#pragma unroll
+          for (int e = 0; e < 2; e++) {
+            top[n][e] = __fmul_rn(fmaxf(fmaxf(sc[0][n][e], sc[0][n][2 + e]), fmaxf(sc[1][n][e], sc[1][n][2 + e])), fac[n][e]);
+            raise = raise || top[n][e] > __fadd_rn(r.m[n][e], kLag);
+          }
+        if (__builtin_expect(__any_sync(0xffffffffu, raise), 0)) {
+#pragma unroll
+          for (int n = 0; n < NT; n++)
+#pragma unroll
+            for (int e = 0; e < 2; e++) {
+              float x = top[n][e];
+              x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
+              x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
+              x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
+              const float m = fmaxf(r.m[n][e], x);
+              const float f = r.m[n][e] == -INFINITY ? 0.0f : exp2_fast(__fsub_rn(r.m[n][e], m));
+              r.m[n][e] = m;
+              r.l[n][e] = __fmul_rn(r.l[n][e], f);
+#pragma unroll
+              for (int j = 0; j < D / 16; j++) {
+                r.o[j][n][e] = __fmul_rn(r.o[j][n][e], f);
+                r.o[j][n][2 + e] = __fmul_rn(r.o[j][n][2 + e], f);
+              }
+            }
+        }
+        uint32_t pb[2][NT][F32 ? 4 : 2];
+#pragma unroll
+        for (int n = 0; n < NT; n++) {
+          float base[2];
+#pragma unroll
+          for (int e = 0; e < 2; e++) base[e] = r.m[n][e] == -INFINITY ? 0.0f : __fsub_rn(kWeightShift, r.m[n][e]);
+#pragma unroll
+          for (int a = 0; a < 2; a++)
+#pragma unroll
+            for (int hh = 0; hh < 2; hh++) {
+              const float w0 = exp2_fast(__fmaf_rn(sc[a][n][2 * hh], fac[n][0], base[0]));
+              const float w1 = exp2_fast(__fmaf_rn(sc[a][n][2 * hh + 1], fac[n][1], base[1]));
+              r.l[n][0] = __fadd_rn(r.l[n][0], w0);
+              r.l[n][1] = __fadd_rn(r.l[n][1], w1);
+              const uint32_t hw = half2_of(w0, w1);
+              pb[a][n][hh] = transpose8(hw);
+              if constexpr (F32) {
+                const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&hw));
+                pb[a][n][2 + hh] = transpose8(half2_of(__fsub_rn(w0, f.x), __fsub_rn(w1, f.y)));
+              }
+            }
+        }
+        if constexpr (F32) {  // two atoms' sum on its own, then one rounded addition: a long chain would drift by its cut-off bits
+          float two[D / 16][NT][4];
+          weigh<D, NT, F32, true>(unit, lane, pb[0], two);
+          weigh<D, NT, F32, false>(unit + A::BYTES, lane, pb[1], two);
+#pragma unroll
+          for (int j = 0; j < D / 16; j++)
+#pragma unroll
+            for (int n = 0; n < NT; n++)
+#pragma unroll
+              for (int e = 0; e < 4; e++) r.o[j][n][e] = __fadd_rn(r.o[j][n][e], two[j][n][e]);
+        } else {
+          weigh<D, NT, F32, false>(unit, lane, pb[0], r.o);
+          weigh<D, NT, F32, false>(unit + A::BYTES, lane, pb[1], r.o);
+        }
+      }
+      __syncwarp();
+      if (issued < count) {  // into the slot that was just read
+        issue();
+        issued++;
+      }
+      if (++ring.slot == kStages) ring.slot = 0, ring.phase ^= 1u;
+    }
+    if constexpr (DIRECT) {
+      join_lanes();
+      return;
+    } else {
+      end_tile(v0, n_here);
+      at += n_here;
+      left_here -= n_here;
+      if (left_here == 0) return;
+      t.next(p);
+      v = 0;
+#pragma unroll
+      for (int n = 0; n < NT; n++) query_values<D, T>(p, t.s, t.h, t.tile * 8 * NT + 8 * n + g, t.rows(p), qx[n]);
+    }
+  }
+}
+
+template <int D, int NT, int T, bool DIRECT>
 __global__ void __launch_bounds__(kWarps * 32, (NT == 1 ? 3 : 2))
 kv4_attend_kernel(const __grid_constant__ AttendParams p) {
   using S = Shared<D, NT>;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ __align__(8) uint64_t bars[kWarps][kStages];
-  __shared__ float s_ml[kWarps][8 * NT][2];
-  __shared__ int64_t s_count[2][kWarps];
+  __shared__ float s_ml[DIRECT ? kWarps : 1][8 * NT][2];
   const int lane = threadIdx.x & 31, warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0);
   const int g = lane >> 2, q4 = lane & 3;
   Ring ring = {smem + warp * S::WARP, bars[warp], 0, 0u};
@@ -630,14 +744,17 @@ kv4_attend_kernel(const __grid_constant__ AttendParams p) {
   __syncwarp();
   Sums<D, NT> r;
 
-  if (p.runs == 0) {
+  if constexpr (DIRECT) {
     // ---- a CTA per row tile
     const int s = blockIdx.z, h = blockIdx.y, tile = blockIdx.x;
-    const Sequence seq = sequence_of(p, s);
-    const int row0 = tile * 8 * NT, rows = seq.qn * p.group - row0;  // rows of this tile that exist (may be more than it holds)
+    Cursor t;
+    t.enter(p, s);
+    t.h = h;
+    t.tile = tile;
+    t.place(p);
+    const int row0 = tile * 8 * NT, rows = t.rows(p) - row0;  // rows of this tile that exist (may be more than it holds)
     if (rows <= 0) return;
-    const int units = units_of(p, seq);
-    stream_units<D, NT, T>(p, s, h, tile, seq, warp, kWarps, units > warp ? (units - warp + kWarps - 1) / kWarps : 0, ring, r);
+    stream_units<D, NT, T, true>(p, t, warp, t.span.count > warp ? (t.span.count - warp + kWarps - 1) / kWarps : 0, ring, r);
     if (g == 0)
 #pragma unroll
       for (int n = 0; n < NT; n++)
@@ -675,113 +792,72 @@ kv4_attend_kernel(const __grid_constant__ AttendParams p) {
       }
       write_row<T, D / 32>(p, s, h, row0 + row, lane * (D / 32), x, m, l, lane == 0);
     }
-    return;
-  }
-
+  } else {
   // ---- equal runs of all units
-  int64_t total, unused;
-  count_units<kWarps>(p, 0, &total, &unused, s_count);
-  const int tiles = p.c.heads * p.row_tiles;  // row tiles of a sequence
-  total *= tiles;
-  const int64_t per = units_per_run(total, p.runs);
-  const int64_t run = (int64_t)blockIdx.x * kWarps + warp;
-  int64_t at = run * per;
-  const int64_t stop = min(total, at + per);
-  // the sequence that unit `at` lies in: 32 at a time
+  const unsigned run = blockIdx.x * kWarps + warp;
+  unsigned units = all_units_of(p, lane);
+  const Runs runs = cut_runs(p, units);
+  const unsigned at = runs.start(run);
+  const int count = (int)(runs.start(run + 1) - at);
+  if (count == 0) return;
+  // the sequence that unit `at` lies in, 32 at a time
   int s = 0;
-  int64_t base = 0;  // units before sequence s
-  while (at < stop) {
-    {
-      // move s and base to the sequence of unit `at`
-      for (;;) {
-        const int i = s + lane;
-        const int64_t mine = i < p.c.n_seqs ? (int64_t)units_of(p, sequence_of(p, i)) * tiles : 0;
-        int64_t upto = mine;
+  unsigned base = 0;  // units before sequence s
+  for (;;) {
+    unsigned upto = units;
 #pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-          const int64_t t = __shfl_up_sync(0xffffffffu, upto, o);
-          if (lane >= o) upto += t;
-        }
-        const unsigned past = __ballot_sync(0xffffffffu, base + upto > at);
-        if (past) {
-          const int k = __ffs(past) - 1;
-          base += __shfl_sync(0xffffffffu, upto - mine, k);
-          s += k;
-          break;
-        }
-        base += __shfl_sync(0xffffffffu, upto, 31);
-        s += 32;
-      }
+    for (int o = 1; o < 32; o <<= 1) {
+      const unsigned x = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += x;
     }
-    const Sequence seq = sequence_of(p, s);
-    const int units = units_of(p, seq);
-    // the row tiles of this sequence that the run reaches
-    while (at < stop && at < base + (int64_t)units * tiles) {
-      const int64_t off = at - base;
-      const int ht = (int)(off / units), v = (int)(off - (int64_t)ht * units);
-      const int n = (int)min((int64_t)(units - v), stop - at);
-      const int h = ht / p.row_tiles, tile = ht - h * p.row_tiles;
-      const int row0 = tile * 8 * NT, rows = min(8 * NT, seq.qn * p.group - row0);
-      at += n;
-      if (rows <= 0) continue;
-      const bool fine = stream_units<D, NT, T>(p, s, h, tile, seq, v, 1, n, ring, r);
-      const bool part = n < units;
-      const int64_t slot = (run * 2 + (v == 0)) * (8 * NT);
-#pragma unroll
-      for (int nn = 0; nn < NT; nn++)
-#pragma unroll
-        for (int e = 0; e < 2; e++) {
-          const int row = 8 * nn + 2 * q4 + e;
-          float x[D / 8];
-#pragma unroll
-          for (int j = 0; j < D / 16; j++) {
-            x[2 * j] = __fmul_rn(r.o[j][nn][e], kScaleShift);
-            x[2 * j + 1] = __fmul_rn(r.o[j][nn][2 + e], kScaleShift / 16.0f);
-          }
-          if (row < rows) {
-            if (part) {
-              store_f32<PKV_DST_F32, D / 8>(p.part_o + (slot + row) * D + g * (D / 8), x);
-              if (g == 0) *reinterpret_cast<float2*>(p.part_ml + (slot + row) * 2) = make_float2(r.m[nn][e], r.l[nn][e]);
-            } else {
-              write_row<T, D / 8>(p, s, h, row0 + row, g * (D / 8), x, r.m[nn][e], r.l[nn][e], g == 0);
-            }
-          }
-        }
-      if (!fine) return;
+    const unsigned past = __ballot_sync(0xffffffffu, base + upto > at);
+    if (past) {
+      const int k = __ffs(past) - 1;
+      base += __shfl_sync(0xffffffffu, upto - units, k);
+      s += k;
+      break;
     }
+    base += __shfl_sync(0xffffffffu, upto, 31);
+    s += 32;
+    units = all_units_of(p, s + lane);
+  }
+  Cursor t;
+  t.enter(p, s);
+  const unsigned off = at - base, ht = off / (unsigned)t.units;
+  t.h = ht / (unsigned)t.tiles;
+  t.tile = ht - t.h * t.tiles;
+  t.place(p);
+  stream_units<D, NT, T, false>(p, t, (int)(off - ht * t.units), count, ring, r, runs, at);
   }
 }
 
-// Joins the parts of a query row that was cut: a CTA per row, a warp takes every eighth part.
-template <int D, int NT, int T>
+// Joins the parts of query rows that were cut: W warps a row (8 for a few long rows, 1 where there are many), each taking
+// every W-th part.
+template <int D, int NT, int T, int W>
 __global__ void __launch_bounds__(kJoinWarps * 32)
 kv4_combine_kernel(const __grid_constant__ AttendParams p) {
-  __shared__ int64_t s_count[2][kJoinWarps];
-  __shared__ float s_x[kJoinWarps][D], s_ml[kJoinWarps][2];
-  constexpr int N = D / 32;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int s = blockIdx.z, h = blockIdx.y, tile = blockIdx.x / (8 * NT), row = blockIdx.x % (8 * NT);
-  int64_t total, before;
-  count_units<kJoinWarps>(p, s, &total, &before, s_count);
-  const Sequence seq = sequence_of(p, s);
-  const int units = units_of(p, seq);
-  const int tiles = p.c.heads * p.row_tiles;
-  const int64_t per = units_per_run(total * tiles, p.runs);
-  const int64_t at = before * tiles + (int64_t)(h * p.row_tiles + tile) * units;
-  const int64_t first = at / per;
-  const int parts = (int)((at + units - 1) / per - first) + 1;
+  __shared__ float s_x[W > 1 ? W : 1][D], s_ml[W > 1 ? W : 1][2];
+  constexpr int N = D / 32, PER = kJoinWarps / W;  // rows per CTA
+  const int lane = threadIdx.x & 31, warp = (threadIdx.x >> 5) % W;
+  const int s = blockIdx.z, h = blockIdx.y, grow = blockIdx.x * PER + (threadIdx.x >> 5) / W;
+  const int tile = grow / (8 * NT), row = grow - tile * (8 * NT);
   // every block waits, so that this launch never ends before the one it follows
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  if (tile * 8 * NT + row >= seq.qn * p.group || parts == 1) return;
-  auto slot_of = [&](int k) { return ((first + k) * 2 + (k == 0)) * (8 * NT) + row; };
+  int qn = p.q_lens ? p.q_lens[s] : p.q.n;
+  if (qn < 0 || qn > p.q.n) qn = 0;
+  if (grow >= qn * p.group) return;
+  const int2 of = p.part_of[((int64_t)s * p.c.heads + h) * p.row_tiles + tile];
+  const int first = of.x, parts = of.y;
+  if (parts == 1) return;
+  auto slot_of = [&](int k) { return ((int64_t)(first + k) * 2 + (k == 0)) * (8 * NT) + row; };
   float m = -INFINITY, l = 0.0f, x[N];
 #pragma unroll
   for (int i = 0; i < N; i++) x[i] = 0.0f;
-  // a warp's parts: k = warp + 8 j; references of 32 of them at a time, then the sums, eight loads in flight
-  for (int k0 = warp; k0 < parts; k0 += 32 * kJoinWarps) {
-    const int n = min(32, (parts - k0 + kJoinWarps - 1) / kJoinWarps);
+  // a warp's parts: k = warp + W j; references of 32 of them at a time, then the sums, eight loads in flight
+  for (int k0 = warp; k0 < parts; k0 += 32 * W) {
+    const int n = min(32, (parts - k0 + W - 1) / W);
     float2 ml = make_float2(-INFINITY, 0.0f);
-    if (lane < n) ml = *reinterpret_cast<const float2*>(p.part_ml + slot_of(k0 + lane * kJoinWarps) * 2);
+    if (lane < n) ml = *reinterpret_cast<const float2*>(p.part_ml + slot_of(k0 + lane * W) * 2);
     float top = ml.x;
 #pragma unroll
     for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
@@ -799,7 +875,7 @@ kv4_combine_kernel(const __grid_constant__ AttendParams p) {
 #pragma unroll 8
     for (int j = 0; j < n; j++) {
       const float fj = __shfl_sync(0xffffffffu, f, j);
-      const float* src = p.part_o + slot_of(k0 + j * kJoinWarps) * D + lane * N;
+      const float* src = p.part_o + slot_of(k0 + j * W) * D + lane * N;
       float y[N];
       if constexpr (N == 4) {
         const float4 v = *reinterpret_cast<const float4*>(src);
@@ -812,31 +888,33 @@ kv4_combine_kernel(const __grid_constant__ AttendParams p) {
       for (int i = 0; i < N; i++) x[i] = __fmaf_rn(fj, y[i], x[i]);
     }
   }
+  if constexpr (W > 1) {
 #pragma unroll
-  for (int i = 0; i < N; i++) s_x[warp][lane * N + i] = x[i];
-  if (lane == 0) {
-    s_ml[warp][0] = m;
-    s_ml[warp][1] = l;
+    for (int i = 0; i < N; i++) s_x[warp][lane * N + i] = x[i];
+    if (lane == 0) {
+      s_ml[warp][0] = m;
+      s_ml[warp][1] = l;
+    }
+    __syncthreads();
+    if (warp) return;
+    const int w = lane & (W - 1);
+    m = s_ml[w][0];
+#pragma unroll
+    for (int o = W / 2; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    const float f = s_ml[w][0] == -INFINITY ? (s_ml[w][1] == 0.0f ? 0.0f : s_ml[w][1]) : exp2_fast(__fsub_rn(s_ml[w][0], m));
+    l = __fmul_rn(f, s_ml[w][1]);
+#pragma unroll
+    for (int o = W / 2; o; o >>= 1) l = __fadd_rn(l, __shfl_xor_sync(0xffffffffu, l, o));
+#pragma unroll
+    for (int i = 0; i < N; i++) x[i] = 0.0f;
+#pragma unroll
+    for (int k = 0; k < W; k++) {
+      const float fk = __shfl_sync(0xffffffffu, f, k);
+#pragma unroll
+      for (int i = 0; i < N; i++) x[i] = __fmaf_rn(fk, s_x[k][lane * N + i], x[i]);
+    }
   }
-  __syncthreads();
-  if (warp) return;
-  const int w = lane & (kJoinWarps - 1);
-  float top = s_ml[w][0];
-#pragma unroll
-  for (int o = kJoinWarps / 2; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-  const float f = s_ml[w][0] == -INFINITY ? (s_ml[w][1] == 0.0f ? 0.0f : s_ml[w][1]) : exp2_fast(__fsub_rn(s_ml[w][0], top));
-  float sum = __fmul_rn(f, s_ml[w][1]);
-#pragma unroll
-  for (int o = kJoinWarps / 2; o; o >>= 1) sum = __fadd_rn(sum, __shfl_xor_sync(0xffffffffu, sum, o));
-#pragma unroll
-  for (int i = 0; i < N; i++) x[i] = 0.0f;
-#pragma unroll
-  for (int k = 0; k < kJoinWarps; k++) {
-    const float fk = __shfl_sync(0xffffffffu, f, k);
-#pragma unroll
-    for (int i = 0; i < N; i++) x[i] = __fmaf_rn(fk, s_x[k][lane * N + i], x[i]);
-  }
-  write_row<T, N>(p, s, h, tile * 8 * NT + row, lane * N, x, top, sum, lane == 0);
+  write_row<T, N>(p, s, h, grow, lane * N, x, m, l, lane == 0);
 }
 
 // mass[key] += sum over the query rows of exp(score - lse).  A warp keeps the dequantised keys of 32 tokens in
@@ -883,8 +961,9 @@ kv4_mass_kernel(const __grid_constant__ AttendParams p) {
     if (!by_position && p.window > 0 && token0 >= p.sinks && pos0 + r0 / p.group - (token0 + kMassTokens - 1) >= p.window) break;
     uint32_t qhi[1][D / 16][2], qlo[1][D / 16][2];
     const int r = r0 + g, token = r / p.group, hq = h * p.group + (r - token * p.group);
-    const E* qp = reinterpret_cast<const E*>(p.q_ptr) + s * p.q.seq + (int64_t)token * p.q.token + hq * p.q.head;
-    const float inv = load_query<D, T>(qp, q4, r < rows, p.negate, qhi[0], qlo[0]);
+    float x[D / 4];
+    query_values<D, T>(p, s, h, r, rows, x);
+    const float inv = query_operand<D, T>(x, p.negate, qhi[0], qlo[0]);
     const float lse = r < rows ? p.lse[((int64_t)s * p.q.n + token) * p.q_heads + hq] : -INFINITY;
     const float f = __fmul_rn(__fmul_rn(__fmul_rn(p.scale, kLog2e), kScaleShift), inv);
     float factor[2], base[2];
@@ -930,7 +1009,8 @@ kv4_mass_kernel(const __grid_constant__ AttendParams p) {
 // ---- host ---------------------------------------------------------------------------------------------------------------
 struct Plan {
   int nt, row_tiles, runs;
-  int64_t part_rows;  // rows of partial sums
+  int64_t part_rows, tiles;  // rows of partial sums; row tiles of all
+  int64_t bytes(int dim) const { return runs ? part_rows * (dim + 2) * (int64_t)sizeof(float) + tiles * (int64_t)sizeof(int2) : 0; }
 };
 
 int sm_count() {
@@ -950,20 +1030,21 @@ Plan make_plan(const Cache& c, const pkv_kv4_rows* q, const pkv_kv4_attend_args*
     if (seen < longest) longest = seen;
   }
   const int64_t units = (longest + kUnitTokens - 1) / kUnitTokens;
-  // Rows of up to four units a warp are not worth a second launch.
+  // Rows of up to four units a warp are not worth a second launch, and with a row for every warp there is nothing to cut.
+  const int64_t tiles = (int64_t)c.heads * r.row_tiles * c.n_seqs, resident = (int64_t)sm_count() * kWarps * (r.nt == 1 ? 3 : 2);
   r.runs = 0;
-  if (units > 4 * kWarps) {
-    const int64_t all = (units * c.n_seqs * c.heads * r.row_tiles + kWarps - 1) / kWarps * kWarps;
-    const int64_t resident = sm_count() * kWarps * (r.nt == 1 ? 3 : 2);
-    r.runs = (int)(all < resident ? all : resident);
+  if (units > 4 * kWarps && tiles < kMaxRows && units * tiles < (1ll << 31)) {
+    const int64_t could = (units * tiles + kWarps - 1) / kWarps * kWarps;
+    r.runs = (int)(could < resident ? could : resident);
   }
   r.part_rows = (int64_t)r.runs * 2 * 8 * r.nt;
+  r.tiles = tiles;
   return r;
 }
 
 template <int D, int NT, int T>
 int launch_attend(const AttendParams& p, cudaStream_t s) {
-  auto kernel = kv4_attend_kernel<D, NT, T>;
+  auto kernel = p.runs ? kv4_attend_kernel<D, NT, T, false> : kv4_attend_kernel<D, NT, T, true>;
   constexpr int bytes = Shared<D, NT>::BYTES;
   if (bytes > 48 * 1024)
     if (cudaError_t ce = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes)) return pkv_cuda_status(ce);
@@ -975,14 +1056,16 @@ int launch_attend(const AttendParams& p, cudaStream_t s) {
     // its launch overlaps the end of the first kernel; it waits (griddepcontrol) before it reads the parts
     cudaLaunchConfig_t cfg = {};
     cudaLaunchAttribute attr = {};
-    cfg.gridDim = dim3(p.row_tiles * 8 * NT, p.c.heads, p.c.n_seqs);
+    const bool many = p.runs < 4 * p.row_tiles * p.c.heads * p.c.n_seqs;  // few parts a row
+    cfg.gridDim = dim3(p.row_tiles * 8 * NT / (many ? kJoinWarps : 1), p.c.heads, p.c.n_seqs);
     cfg.blockDim = dim3(kJoinWarps * 32);
     cfg.stream = s;
     attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr.val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = &attr;
     cfg.numAttrs = 1;
-    if (cudaError_t ce = cudaLaunchKernelEx(&cfg, kv4_combine_kernel<D, NT, T>, p)) return pkv_cuda_status(ce);
+    if (cudaError_t ce = cudaLaunchKernelEx(&cfg, many ? kv4_combine_kernel<D, NT, T, 1> : kv4_combine_kernel<D, NT, T, kJoinWarps>, p))
+      return pkv_cuda_status(ce);
     pkv_count_launch();
   }
   return pkv_cuda_status(cudaGetLastError());
@@ -1015,7 +1098,7 @@ extern "C" int64_t pkv_kv4_attend_workspace_bytes(const pkv_kv4_cache* cache, co
                                                   const pkv_kv4_attend_args* args) {
   Cache c;
   if (make_cache(cache, &c) || !q_rows || q_rows->n_tokens < 0 || check_args(c, q_rows, args)) return 0;
-  return make_plan(c, q_rows, args).part_rows * (cache->dim + 2) * (int64_t)sizeof(float);
+  return make_plan(c, q_rows, args).bytes(cache->dim);
 }
 
 extern "C" int pkv_kv4_attend_dev(const pkv_kv4_cache* cache, const void* q_dev, const pkv_kv4_rows* q_rows, void* out_dev,
@@ -1031,8 +1114,8 @@ extern "C" int pkv_kv4_attend_dev(const pkv_kv4_cache* cache, const void* q_dev,
   if (args->accumulate && (!lse_dev || !p.c.mass)) return PKV_ERR_INVALID_ARGUMENT;
   if (p.q.n == 0 || p.c.n_seqs == 0) return PKV_OK;
   const Plan plan = make_plan(p.c, q_rows, args);
-  if (plan.part_rows * (cache->dim + 2) * (int64_t)sizeof(float) > workspace_bytes) return PKV_ERR_BUFFER_TOO_SMALL;
-  if (plan.part_rows && (!workspace_dev || ((uintptr_t)workspace_dev & 15))) return PKV_ERR_INVALID_ARGUMENT;
+  if (plan.bytes(cache->dim) > workspace_bytes) return PKV_ERR_BUFFER_TOO_SMALL;
+  if (plan.runs && (!workspace_dev || ((uintptr_t)workspace_dev & 15))) return PKV_ERR_INVALID_ARGUMENT;
   p.q_ptr = q_dev;
   p.o_ptr = out_dev;
   p.lse = lse_dev;
@@ -1045,9 +1128,11 @@ extern "C" int pkv_kv4_attend_dev(const pkv_kv4_cache* cache, const void* q_dev,
   p.sinks = args->sinks;
   p.row_tiles = plan.row_tiles;
   p.runs = plan.runs;
+  p.tile_rows = 8 * plan.nt;
   p.whole_units = p.c.page_atoms % kUnitAtoms == 0;
   p.part_o = (float*)workspace_dev;
   p.part_ml = p.part_o + plan.part_rows * cache->dim;
+  p.part_of = (int2*)(p.part_ml + plan.part_rows * 2);
   p.err = err_dev;
   const int longest = args->max_len > 0 && args->max_len < p.c.capacity ? args->max_len : p.c.capacity;
   cudaStream_t s = (cudaStream_t)stream;
