@@ -187,7 +187,7 @@ _SIGS = {
     "pkv_tqb1_header_write": (C.c_int, [_V, C.c_uint32, _V]),
     "pkv_tqb1_header_parse": (C.c_int, [_V, _V, C.c_int64, C.POINTER(C.c_uint32)]),
     "pkv_kv4_append_dev": (C.c_int, [C.POINTER(Kv4CacheC), _V, C.POINTER(Kv4RowsC), _V, C.POINTER(Kv4RowsC), _V, _V, _V]),
-    "pkv_kv4_read_dev": (C.c_int, [C.POINTER(Kv4CacheC), _V, C.POINTER(Kv4RowsC), _V, C.POINTER(Kv4RowsC), _V, _V, _V]),
+    "pkv_kv4_read_dev": (C.c_int, [C.POINTER(Kv4CacheC), _V, C.POINTER(Kv4RowsC), _V, C.POINTER(Kv4RowsC), _V, C.c_int32, _V, _V]),
     "pkv_kv4_attend_workspace_bytes": (C.c_int64, [C.POINTER(Kv4CacheC), C.POINTER(Kv4RowsC), C.POINTER(Kv4AttendC)]),
     "pkv_kv4_attend_dev": (C.c_int, [C.POINTER(Kv4CacheC), _V, C.POINTER(Kv4RowsC), _V, C.POINTER(Kv4RowsC), _V, _V,
                                      C.POINTER(Kv4AttendC), _V, C.c_int64, _V, _V]),

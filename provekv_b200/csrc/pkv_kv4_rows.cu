@@ -143,17 +143,26 @@ kv4_append_kernel(Cache c, const typename PkvDst<T>::type* __restrict__ k, Rows 
 template <int D, int T>
 __global__ void __launch_bounds__(kThreads)
 kv4_read_kernel(Cache c, typename PkvDst<T>::type* __restrict__ k, Rows kr, typename PkvDst<T>::type* __restrict__ v,
-                Rows vr, const int32_t* __restrict__ new_lens, uint64_t* err) {
+                Rows vr, const int32_t* __restrict__ new_lens, int clear_rest, uint64_t* err) {
   using A = Atom<D>;
   constexpr int TOK = kThreads / A::SROW;
   const int b = threadIdx.x % A::SROW;
   const int s = blockIdx.z, h = blockIdx.y;
   const int i = blockIdx.x * TOK + threadIdx.x / A::SROW;
   if (i >= kr.n) return;
-  int slot, position;
-  if (!row_slot(c, s, i, kr.n, new_lens, err, &slot, &position)) return;
-  const uint8_t* atom = c.atom(s, h, slot / kAtomTokens, A::BYTES, err);
-  if (!atom) return;
+  int slot = 0, position;
+  const bool live = row_slot(c, s, i, kr.n, new_lens, err, &slot, &position);
+  const uint8_t* atom = live ? c.atom(s, h, slot / kAtomTokens, A::BYTES, err) : nullptr;
+  if (!atom) {
+    if (clear_rest) {
+      float x[16];
+#pragma unroll
+      for (int j = 0; j < 16; j++) x[j] = 0.0f;
+      store_f32<T, 16>(k + s * kr.seq + i * kr.token + h * kr.head + 16 * b, x);
+      store_f32<T, 16>(v + s * vr.seq + i * vr.token + h * vr.head + 16 * b, x);
+    }
+    return;
+  }
   const int t = slot % kAtomTokens;
 #pragma unroll
   for (int side = 0; side < 2; side++) {
@@ -171,32 +180,33 @@ kv4_read_kernel(Cache c, typename PkvDst<T>::type* __restrict__ k, Rows kr, type
 
 template <int D, int T>
 void launch_rows(bool append, const Cache& c, const void* k, const Rows& kr, const void* v, const Rows& vr,
-                 const int32_t* new_lens, uint64_t* err, cudaStream_t s) {
+                 const int32_t* new_lens, int clear_rest, uint64_t* err, cudaStream_t s) {
   using E = typename PkvDst<T>::type;
   constexpr int TOK = kThreads / Atom<D>::SROW;
   const dim3 grid((unsigned)((kr.n + TOK - 1) / TOK), (unsigned)c.heads, (unsigned)c.n_seqs);
   if (append)
     kv4_append_kernel<D, T><<<grid, kThreads, 0, s>>>(c, (const E*)k, kr, (const E*)v, vr, new_lens, err);
   else
-    kv4_read_kernel<D, T><<<grid, kThreads, 0, s>>>(c, (E*)const_cast<void*>(k), kr, (E*)const_cast<void*>(v), vr, new_lens, err);
+    kv4_read_kernel<D, T><<<grid, kThreads, 0, s>>>(c, (E*)const_cast<void*>(k), kr, (E*)const_cast<void*>(v), vr, new_lens,
+                                                clear_rest, err);
 }
 
 int rows_call(bool append, const pkv_kv4_cache* cache, const void* k, const pkv_kv4_rows* k_rows, const void* v,
-              const pkv_kv4_rows* v_rows, const int32_t* new_lens, uint64_t* err, void* stream) {
+              const pkv_kv4_rows* v_rows, const int32_t* new_lens, int clear_rest, uint64_t* err, void* stream) {
   Cache c;
   Rows kr, vr;
   if (int st = make_cache(cache, &c)) return st;
   if (int st = make_rows(k, k_rows, &kr)) return st;
   if (int st = make_rows(v, v_rows, &vr)) return st;
-  if (!err || kr.n != vr.n || k_rows->dtype != v_rows->dtype) return PKV_ERR_INVALID_ARGUMENT;
+  if (!err || kr.n != vr.n || k_rows->dtype != v_rows->dtype || (clear_rest != 0 && clear_rest != 1)) return PKV_ERR_INVALID_ARGUMENT;
   if (kr.n > c.capacity && !new_lens) return PKV_ERR_INVALID_ARGUMENT;
   if (kr.n == 0 || c.n_seqs == 0) return PKV_OK;
   cudaStream_t s = (cudaStream_t)stream;
 #define PKV_KV4_ROWS(D)                                                                                                    \
   switch (k_rows->dtype) {                                                                                                 \
-    case PKV_DST_F32: launch_rows<D, PKV_DST_F32>(append, c, k, kr, v, vr, new_lens, err, s); break;                       \
-    case PKV_DST_F16: launch_rows<D, PKV_DST_F16>(append, c, k, kr, v, vr, new_lens, err, s); break;                       \
-    default: launch_rows<D, PKV_DST_BF16>(append, c, k, kr, v, vr, new_lens, err, s); break;                               \
+    case PKV_DST_F32: launch_rows<D, PKV_DST_F32>(append, c, k, kr, v, vr, new_lens, clear_rest, err, s); break;                       \
+    case PKV_DST_F16: launch_rows<D, PKV_DST_F16>(append, c, k, kr, v, vr, new_lens, clear_rest, err, s); break;                       \
+    default: launch_rows<D, PKV_DST_BF16>(append, c, k, kr, v, vr, new_lens, clear_rest, err, s); break;                               \
   }
   if (cache->dim == 64) PKV_KV4_ROWS(64) else PKV_KV4_ROWS(128)
 #undef PKV_KV4_ROWS
@@ -209,10 +219,11 @@ int rows_call(bool append, const pkv_kv4_cache* cache, const void* k, const pkv_
 extern "C" int pkv_kv4_append_dev(const pkv_kv4_cache* cache, const void* k_dev, const pkv_kv4_rows* k_rows,
                                   const void* v_dev, const pkv_kv4_rows* v_rows, const int32_t* new_lens_dev,
                                   uint64_t* err_dev, void* stream) {
-  return rows_call(true, cache, k_dev, k_rows, v_dev, v_rows, new_lens_dev, err_dev, stream);
+  return rows_call(true, cache, k_dev, k_rows, v_dev, v_rows, new_lens_dev, 0, err_dev, stream);
 }
 
 extern "C" int pkv_kv4_read_dev(const pkv_kv4_cache* cache, void* k_dev, const pkv_kv4_rows* k_rows, void* v_dev,
-                                const pkv_kv4_rows* v_rows, const int32_t* new_lens_dev, uint64_t* err_dev, void* stream) {
-  return rows_call(false, cache, k_dev, k_rows, v_dev, v_rows, new_lens_dev, err_dev, stream);
+                                const pkv_kv4_rows* v_rows, const int32_t* new_lens_dev, int32_t clear_rest, uint64_t* err_dev,
+                                void* stream) {
+  return rows_call(false, cache, k_dev, k_rows, v_dev, v_rows, new_lens_dev, clear_rest, err_dev, stream);
 }

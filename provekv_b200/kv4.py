@@ -35,16 +35,11 @@ def atom_bytes(dim: int) -> int:
     return 18 * dim
 
 
-def _rows(t, name: str, cache: "Kv4Cache", heads: int | None = None) -> L.Kv4RowsC:
-    if t.dim() != 4 or t.shape[0] != cache.n_seqs or t.shape[3] != cache.dim:
-        raise ValueError(f"{name} must be [{cache.n_seqs}][tokens][heads][{cache.dim}], not {tuple(t.shape)}")
-    if heads is not None and t.shape[2] != heads:
-        raise ValueError(f"{name} has {t.shape[2]} heads, the cache {heads}")
-    if t.device != cache.device:
-        raise ValueError(f"{name} is on {t.device}, the cache on {cache.device}")
-    if t.stride(3) != 1 and t.numel():
-        raise ValueError(f"the values of a vector of {name} must be contiguous")
-    return L.Kv4RowsC(t.stride(0), t.stride(1), t.stride(2), t.shape[1], dst_dtype_of(t))
+def _raw_stream(index: int) -> int:
+    """The current stream of a device, without the Stream object torch.cuda.current_stream makes where torch can do that."""
+    import torch
+    raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+    return raw(index) if raw else torch.cuda.current_stream(index).cuda_stream
 
 
 class Kv4Cache:
@@ -90,6 +85,10 @@ class Kv4Cache:
         self._c = L.Kv4CacheC(ptr(pages), ptr(page_table), ptr(lens), ptr(ends), ptr(positions), ptr(mass), n_pages,
                               self.dim, self.n_kv_heads, self.page_tokens, self.n_seqs, max_pages, 0)
         self.error = torch.full((1,), -1, dtype=torch.int64, device=self.device)
+        # what a call needs besides its tensors' addresses, prepared once: a decode step makes few microseconds' calls
+        self._ref, self._err, self._index = C.byref(self._c), self.error.data_ptr(), self.device.index
+        self._rows_of, self._attend_of, self._evict_of = {}, {}, {}
+        self._lib = L.lib()
 
     @classmethod
     def allocate(cls, n_layers: int, n_seqs: int, n_kv_heads: int, dim: int, max_tokens: int, *, page_tokens: int = 64,
@@ -111,53 +110,69 @@ class Kv4Cache:
         return out
 
     # -- calls -----------------------------------------------------------------------------------------------------------
-    def _stream(self):
-        import torch
-        return torch.cuda.current_stream(self.device).cuda_stream
-
-    def _guard(self):
-        import torch
-        return torch.cuda.device(self.device)
+    def _rows(self, t, name: str, heads: int | None = None):
+        """A reference to the pkv_kv4_rows of a tensor's shape, strides and type (kept: they depend on nothing else)."""
+        key = (t.shape, t.stride(), t.dtype)
+        r = self._rows_of.get(key)
+        if r is None:
+            shape, stride = t.shape, t.stride()
+            if len(shape) != 4 or shape[0] != self.n_seqs or shape[3] != self.dim:
+                raise ValueError(f"{name} must be [{self.n_seqs}][tokens][heads][{self.dim}], not {tuple(shape)}")
+            if stride[3] != 1 and t.numel():
+                raise ValueError(f"the values of a vector of {name} must be contiguous")
+            if len(self._rows_of) >= 256:
+                self._rows_of.clear()
+            r = self._rows_of[key] = C.byref(L.Kv4RowsC(stride[0], stride[1], stride[2], shape[1], dst_dtype_of(t)))
+        if heads is not None and t.shape[2] != heads:
+            raise ValueError(f"{name} has {t.shape[2]} heads, the cache {heads}")
+        if t.get_device() != self._index:
+            raise ValueError(f"{name} is on {t.device}, the cache on {self.device}")
+        return r
 
     def _per_seq(self, t, name: str):
         import torch
         if t is None:
             return None
-        if t.dtype != torch.int32 or tuple(t.shape) != (self.n_seqs,) or not t.is_contiguous() or t.device != self.device:
+        if t.dtype != torch.int32 or tuple(t.shape) != (self.n_seqs,) or not t.is_contiguous() or t.get_device() != self._index:
             raise ValueError(f"{name} must be a contiguous int32 [{self.n_seqs}] tensor on {self.device}")
         return t.data_ptr()
+
+    def _call(self, fn, *args) -> None:
+        """fn(cache, *args, error word, stream) with the cache's device current."""
+        import torch
+        if torch.cuda.current_device() == self._index:
+            status = fn(self._ref, *args, self._err, _raw_stream(self._index))
+        else:
+            with torch.cuda.device(self._index):
+                status = fn(self._ref, *args, self._err, _raw_stream(self._index))
+        if status:
+            L.check(status)
 
     def append(self, k, v, new_lens=None) -> None:
         """Writes the newest tokens of each sequence: row i of ``k`` and ``v`` [n_seqs][n][n_kv_heads][dim] goes to slot
         lens - n + i (with ``new_lens`` int32 [n_seqs]: the first new_lens[s] rows to lens - new_lens + i)."""
-        kr, vr = _rows(k, "k", self, self.n_kv_heads), _rows(v, "v", self, self.n_kv_heads)
+        kr, vr = self._rows(k, "k", self.n_kv_heads), self._rows(v, "v", self.n_kv_heads)
         if k.shape != v.shape:
             raise ValueError("k and v must have the same shape")
         if k.numel() == 0:
             return
-        with self._guard():
-            L.check(L.lib().pkv_kv4_append_dev(C.byref(self._c), k.data_ptr(), C.byref(kr), v.data_ptr(), C.byref(vr),
-                                               self._per_seq(new_lens, "new_lens"), self.error.data_ptr(), self._stream()))
+        self._call(self._lib.pkv_kv4_append_dev, k.data_ptr(), kr, v.data_ptr(), vr, self._per_seq(new_lens, "new_lens"))
 
     def read(self, n: int, dtype=None, new_lens=None, out=None):
         """(k, v) [n_seqs][n][n_kv_heads][dim]: the values the newest tokens stand for, at the rows `append` would take
         them from.  Rows from new_lens[s] on are zeros, or as they were in ``out`` = (k, v)."""
         import torch
-        if out is None:
-            shape = (2, self.n_seqs, n, self.n_kv_heads, self.dim)
-            make = torch.empty if new_lens is None else torch.zeros
-            out = make(shape, dtype=dtype or torch.float32, device=self.device).unbind(0)
+        fresh = out is None
+        if fresh:
+            out = torch.empty((2, self.n_seqs, n, self.n_kv_heads, self.dim), dtype=dtype or torch.float32, device=self.device).unbind(0)
         k, v = out
         if k.shape[1] != n or (dtype is not None and k.dtype != dtype):
             raise ValueError("out does not have the rows or the type asked for")
-        kr, vr = _rows(k, "k", self, self.n_kv_heads), _rows(v, "v", self, self.n_kv_heads)
+        kr, vr = self._rows(k, "k", self.n_kv_heads), self._rows(v, "v", self.n_kv_heads)
         if k.shape != v.shape:
             raise ValueError("k and v must have the same shape")
-        if k.numel() == 0:
-            return k, v
-        with self._guard():
-            L.check(L.lib().pkv_kv4_read_dev(C.byref(self._c), k.data_ptr(), C.byref(kr), v.data_ptr(), C.byref(vr),
-                                             self._per_seq(new_lens, "new_lens"), self.error.data_ptr(), self._stream()))
+        if k.numel():
+            self._call(self._lib.pkv_kv4_read_dev, k.data_ptr(), kr, v.data_ptr(), vr, self._per_seq(new_lens, "new_lens"), int(fresh))
         return k, v
 
     def attend(self, q, *, scale: float | None = None, window: int = 0, sinks: int = 0, q_lens=None, accumulate: bool = False,
@@ -174,29 +189,31 @@ class Kv4Cache:
         lse         f32 [n_seqs][n][n_q_heads], natural logarithm; -inf where a query sees nothing (its out is zeros)
         """
         import torch
-        if accumulate and self.mass is None:
-            raise ValueError("accumulate needs a cache with mass")
-        qr = _rows(q, "q", self)
-        make = torch.empty if q_lens is None else torch.zeros
+        qr = self._rows(q, "q")
         if out is None:
-            out = make(q.shape, dtype=q.dtype, device=self.device)
+            out = (torch.empty if q_lens is None else torch.zeros)(q.shape, dtype=q.dtype, device=self.device)
         elif out.shape != q.shape or out.dtype != q.dtype:
             raise ValueError("out must have the shape and type of q")
-        outr = _rows(out, "out", self)
+        outr = self._rows(out, "out")
         if lse is None:
-            lse = make(q.shape[:3], dtype=torch.float32, device=self.device)
-        elif lse.shape != q.shape[:3] or lse.dtype != torch.float32 or not lse.is_contiguous() or lse.device != self.device:
+            lse = (torch.empty if q_lens is None else torch.zeros)(q.shape[:3], dtype=torch.float32, device=self.device)
+        elif lse.shape != q.shape[:3] or lse.dtype != torch.float32 or not lse.is_contiguous() or lse.get_device() != self._index:
             raise ValueError("lse must be contiguous f32 [n_seqs][tokens][heads] on the cache's device")
         if q.numel() == 0:
             return out, lse
-        args = L.Kv4AttendC(self.dim ** -0.5 if scale is None else scale, q.shape[2], window, sinks, int(accumulate), max_len)
-        lib = L.lib()
-        with self._guard():
-            need = lib.pkv_kv4_attend_workspace_bytes(C.byref(self._c), C.byref(qr), C.byref(args))
-            work = torch.empty(need, dtype=torch.uint8, device=self.device) if need else None
-            L.check(lib.pkv_kv4_attend_dev(C.byref(self._c), q.data_ptr(), C.byref(qr), out.data_ptr(), C.byref(outr), lse.data_ptr(),
-                                           self._per_seq(q_lens, "q_lens"), C.byref(args), work.data_ptr() if need else None, need,
-                                           self.error.data_ptr(), self._stream()))
+        key = (q.shape, q.dtype, scale, window, sinks, accumulate, max_len)
+        plan = self._attend_of.get(key)
+        if plan is None:
+            if accumulate and self.mass is None:
+                raise ValueError("accumulate needs a cache with mass")
+            args = L.Kv4AttendC(self.dim ** -0.5 if scale is None else scale, q.shape[2], window, sinks, int(accumulate), max_len)
+            if len(self._attend_of) >= 256:
+                self._attend_of.clear()
+            plan = self._attend_of[key] = (C.byref(args), self._lib.pkv_kv4_attend_workspace_bytes(self._ref, qr, C.byref(args)))
+        args, need = plan
+        work = torch.empty(need, dtype=torch.uint8, device=self.device) if need else None
+        self._call(self._lib.pkv_kv4_attend_dev, q.data_ptr(), qr, out.data_ptr(), outr, lse.data_ptr(),
+                   self._per_seq(q_lens, "q_lens"), args, work.data_ptr() if need else None, need)
         return out, lse
 
     def evict(self, budget: int, *, sinks: int = 0, recent: int = 0) -> None:
@@ -208,19 +225,21 @@ class Kv4Cache:
             raise ValueError("evict needs a cache with positions and mass")
         if self.n_seqs == 0:
             return
-        lib = L.lib()
-        with self._guard():
-            need = lib.pkv_kv4_evict_workspace_bytes(C.byref(self._c), budget)
-            work = torch.empty(need, dtype=torch.uint8, device=self.device) if need else None
-            L.check(lib.pkv_kv4_evict_dev(C.byref(self._c), budget, sinks, recent, work.data_ptr() if need else None, need,
-                                          self.error.data_ptr(), self._stream()))
+        need = self._evict_of.get(budget)
+        if need is None:
+            if len(self._evict_of) >= 256:
+                self._evict_of.clear()
+            need = self._evict_of[budget] = self._lib.pkv_kv4_evict_workspace_bytes(self._ref, budget)
+        work = torch.empty(need, dtype=torch.uint8, device=self.device) if need else None
+        self._call(self._lib.pkv_kv4_evict_dev, budget, sinks, recent, work.data_ptr() if need else None, need)
 
     def check(self) -> None:
         """Waits for the stream, raises PkvError for the first thing a kernel reported since the last check, and clears it."""
+        import torch
         code, index = C.c_int32(0), C.c_int64(-1)
-        with self._guard():
-            s = self._stream()
-            st = L.lib().pkv_error_word_read(self.error.data_ptr(), s, C.byref(code), C.byref(index))
+        with torch.cuda.device(self._index):
+            s = _raw_stream(self._index)
+            st = self._lib.pkv_error_word_read(self._err, s, C.byref(code), C.byref(index))
             if st != L.OK:
-                L.check(L.lib().pkv_error_word_reset(self.error.data_ptr(), s))
+                L.check(self._lib.pkv_error_word_reset(self._err, s))
                 raise L.PkvError(st, L.status_string(st), index.value)

@@ -25,7 +25,8 @@ def _rows(n=1, dtype=L.DST_BF16, strides=(1024, 512, 128)):
 
 def _append(cache, k=P, kr=None, v=P, vr=None, err=P, fn="pkv_kv4_append_dev"):
     kr, vr = kr or _rows(), vr or _rows()
-    return getattr(L.lib(), fn)(C.byref(cache), k, C.byref(kr), v, C.byref(vr), None, err, None)
+    rest = (0,) if fn == "pkv_kv4_read_dev" else ()
+    return getattr(L.lib(), fn)(C.byref(cache), k, C.byref(kr), v, C.byref(vr), None, *rest, err, None)
 
 
 @pytest.mark.parametrize("fn", ["pkv_kv4_append_dev", "pkv_kv4_read_dev"])
