@@ -19,51 +19,17 @@
 //                whatever the lengths.  The stream of units runs on from one row into the next.  A row that was cut is joined
 //                by a second launch from the warps' sums.
 //
-#include <math.h>
-
-#include "pkv_kv4.cuh"
+#include "pkv_kv4_attend.cuh"
 
 using namespace pkv_kv4;
 
 namespace {
 
 constexpr int kWarps = 4;
-constexpr int kUnitAtoms = 4, kUnitTokens = kUnitAtoms * kAtomTokens;
-constexpr int kBatch = 32 / kUnitAtoms;  // units whose page numbers a warp fetches at once
 constexpr int kStages = 2;
 constexpr int kMaxRows = 2048;           // (sequence, kv head, row tile)s that share runs
 constexpr int kJoinWarps = 8;
 constexpr int kMassTokens = 32;  // keys a warp of the mass kernel holds
-constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
-// Weights are kept times 2^7 and the running reference may lag the true maximum by 2^8: a weight in binary16 is at most
-// 2^15, and one 2^21 below the largest still has all its bits.
-constexpr float kWeightShift = 7.0f, kLag = 8.0f;
-
-struct AttendParams {
-  Cache c;
-  Rows q, o;
-  const void* q_ptr;
-  void* o_ptr;
-  float* lse;
-  const int32_t* q_lens;
-  float scale;        // its magnitude
-  int negate;         // its sign
-  int group, q_heads, window, sinks;
-  int row_tiles;      // tiles of 8 NT query rows per (sequence, kv head)
-  int runs;           // warps that share the units of all rows; 0: a CTA per row tile
-  int tile_rows;      // query rows of a tile, 8 NT
-  int whole_units;    // 1: a unit never crosses a page, one copy brings it
-  float* part_o;      // [run][2][8 NT][D] unnormalised sums of a run's first and last row, where it has only a part of it
-  float* part_ml;     // [run][2][8 NT][2] reference and sum
-  int2* part_of;      // [sequence][kv head][row tile] first run and number of runs that have a part of it
-  uint64_t* err;
-};
-
-__device__ __forceinline__ float exp2_fast(float x) {
-  float r;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
-  return r;
-}
 __device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
@@ -80,21 +46,7 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
   asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
   return r;
 }
-__device__ __forceinline__ uint32_t half2_of(float a, float b) {
-  const __half2 h = __floats2half2_rn(a, b);
-  return *reinterpret_cast<const uint32_t*>(&h);
-}
 __device__ __forceinline__ int tau(int m) { return (m & 8) | ((m & 1) ? 7 - ((m & 7) >> 1) : (m & 7) >> 1); }
-
-// A row's power of two that brings its largest magnitude to [2^13, 2^14): binary16 then holds a bfloat16 or
-// binary16 row exactly but for components below 2^-27 of the largest.
-__device__ __forceinline__ float row_power(float amax) {
-  if (!(amax > 0.0f) || !pkv_finite(amax)) return 1.0f;
-  const int e = (int)(__float_as_uint(amax) >> 23) - 127;
-  int x = 13 - e;
-  x = x > 120 ? 120 : x < -120 ? -120 : x;
-  return __uint_as_float((uint32_t)(x + 127) << 23);
-}
 
 // The B operand of S^T for query row `lane / 4` from its values of channels (lane % 4) D/4 .. (this lane's), in the
 // order nibbles() delivers the keys', odd channels divided by 16; negated for a negative softmax scale, so that scores
@@ -249,45 +201,6 @@ __device__ __forceinline__ void weigh(const uint8_t* atom, int lane, const uint3
     }
 }
 
-// Which tokens a tile of query rows can see, in units: `head` units from slot 0 (the sinks), then those from unit
-// `from` on, `count` in all.
-struct Span {
-  int head, from, count;
-  __device__ __forceinline__ int unit(int v) const { return v < head ? v : v - head + from; }
-};
-__device__ __forceinline__ Span visible_span(const AttendParams& p, int len, int pos_first, int pos_last) {
-  Span r;
-  int stop = len, lo = 0, sink = 0;
-  if (!p.c.positions) {  // slots are positions
-    stop = max(0, min(len, pos_last + 1));
-    if (p.window > 0) {
-      lo = max(0, pos_first - p.window + 1);
-      sink = min(p.sinks, stop);
-    }
-  }
-  const int last = (stop + kUnitTokens - 1) / kUnitTokens;
-  r.head = (sink + kUnitTokens - 1) / kUnitTokens;
-  r.from = lo / kUnitTokens;
-  if (r.from <= r.head) r.from = r.head;
-  r.count = r.from == r.head ? last : r.head + max(0, last - r.from);
-  return r;
-}
-
-// A sequence as the kernels see it: bad lengths are reported and count as empty.
-struct Sequence {
-  int len, end, qn;
-};
-__device__ __forceinline__ Sequence sequence_of(const AttendParams& p, int s) {
-  Sequence r;
-  r.len = p.c.length(s, p.err);
-  r.end = p.c.end(s, r.len);
-  r.qn = p.q_lens ? p.q_lens[s] : p.q.n;
-  if (r.qn < 0 || r.qn > p.q.n) {
-    pkv_report(p.err, 0, s, PKV_VEC_BAD_SEQUENCE);
-    r.qn = 0;
-  }
-  return r;
-}
 // Units of one (kv head, row tile) of a sequence: what its first to last query token see, at least one (a row that sees
 // nothing is written too), none without queries.
 __device__ __forceinline__ int units_of(const AttendParams& p, const Sequence& q) {
@@ -378,31 +291,6 @@ struct Sums {
   float o[D / 16][NT][4];            // channels (lane / 4) D/8 + 2 j + i / 2, row 2 (lane % 4) + i % 2
   float m[NT][2], l[NT][2];          // reference (log2) and sum of rows 2 (lane % 4) + e; l is this lane's part
 };
-
-// Writes N channels of a row, sums x (scale and the 16 of odd channels already undone) over l.
-template <int T, int N>
-__device__ __forceinline__ void write_row(const AttendParams& p, int s, int h, int row, int channel, const float (&x)[N], float m, float l,
-                                          bool first) {
-  using E = typename PkvDst<T>::type;
-  const int token = row / p.group, hq = h * p.group + (row - token * p.group);
-  const float inv = l > 0.0f ? __fdiv_rn(1.0f, l) : (l == 0.0f ? 0.0f : l);
-  E* dst = reinterpret_cast<E*>(p.o_ptr) + s * p.o.seq + (int64_t)token * p.o.token + hq * p.o.head + channel;
-  float y[N];
-#pragma unroll
-  for (int i = 0; i < N; i++) y[i] = __fmul_rn(x[i], inv);
-  if constexpr (T == PKV_DST_F32 ? N % 4 == 0 : N % 8 == 0) {
-    store_f32<T, N>(dst, y);
-  } else {
-#pragma unroll
-    for (int i = 0; i < N; i += 2) {
-      if constexpr (T == PKV_DST_F32) *reinterpret_cast<float2*>(dst + i) = make_float2(y[i], y[i + 1]);
-      else *reinterpret_cast<uint32_t*>(dst + i) = pkv_pack2<T>(y[i], y[i + 1]);
-    }
-  }
-  if (p.lse && first)
-    p.lse[((int64_t)s * p.q.n + token) * p.q_heads + hq] =
-        l == 0.0f ? -INFINITY : __fmul_rn(kLn2, __fadd_rn(m, __fsub_rn(log2f(l), kWeightShift)));
-}
 
 // Streams a warp's units; whole warp.  DIRECT: units v, v + kWarps, .. of row tile `t`; the sums stay in `r`.
 // Otherwise: `count` units from unit v of row tile `t` on (number `at` of all rows' units), into the next row tiles; every row tile's sums are written
@@ -1013,12 +901,6 @@ struct Plan {
   int64_t bytes(int dim) const { return runs ? part_rows * (dim + 2) * (int64_t)sizeof(float) + tiles * (int64_t)sizeof(int2) : 0; }
 };
 
-int sm_count() {
-  int dev = 0, sms = 148;
-  if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-  return sms;
-}
-
 Plan make_plan(const Cache& c, const pkv_kv4_rows* q, const pkv_kv4_attend_args* a) {
   Plan r;
   const int64_t rows = (int64_t)q->n_tokens * (a->n_q_heads / c.heads);
@@ -1073,7 +955,10 @@ int launch_attend(const AttendParams& p, cudaStream_t s) {
 
 template <int D, int T>
 int launch_all(const AttendParams& p, int nt, bool accumulate, int longest, cudaStream_t s) {
-  if (int st = nt == 1 ? launch_attend<D, 1, T>(p, s) : launch_attend<D, 2, T>(p, s)) return st;
+  if (nt == 0) {  // done by the kernel for many rows
+  } else if (int st = nt == 1 ? launch_attend<D, 1, T>(p, s) : launch_attend<D, 2, T>(p, s)) {
+    return st;
+  }
   if (accumulate && longest > 0) {
     const int per = kWarps * kMassTokens;
     kv4_mass_kernel<D, T><<<dim3((longest + per - 1) / per, p.c.heads, p.c.n_seqs), kWarps * 32, 0, s>>>(p);
@@ -1098,6 +983,7 @@ extern "C" int64_t pkv_kv4_attend_workspace_bytes(const pkv_kv4_cache* cache, co
                                                   const pkv_kv4_attend_args* args) {
   Cache c;
   if (make_cache(cache, &c) || !q_rows || q_rows->n_tokens < 0 || check_args(c, q_rows, args)) return 0;
+  if (chunk_takes(q_rows, args->n_q_heads / c.heads)) return chunk_workspace_bytes(c, cache->dim, q_rows, args);
   return make_plan(c, q_rows, args).bytes(cache->dim);
 }
 
@@ -1113,9 +999,12 @@ extern "C" int pkv_kv4_attend_dev(const pkv_kv4_cache* cache, const void* q_dev,
   if (!err_dev || p.q.n != p.o.n || q_rows->dtype != out_rows->dtype) return PKV_ERR_INVALID_ARGUMENT;
   if (args->accumulate && (!lse_dev || !p.c.mass)) return PKV_ERR_INVALID_ARGUMENT;
   if (p.q.n == 0 || p.c.n_seqs == 0) return PKV_OK;
-  const Plan plan = make_plan(p.c, q_rows, args);
-  if (plan.bytes(cache->dim) > workspace_bytes) return PKV_ERR_BUFFER_TOO_SMALL;
-  if (plan.runs && (!workspace_dev || ((uintptr_t)workspace_dev & 15))) return PKV_ERR_INVALID_ARGUMENT;
+  const bool chunk = chunk_takes(q_rows, args->n_q_heads / p.c.heads);
+  Plan plan = {};
+  if (!chunk) plan = make_plan(p.c, q_rows, args);
+  const int64_t need = chunk ? chunk_workspace_bytes(p.c, cache->dim, q_rows, args) : plan.bytes(cache->dim);
+  if (need > workspace_bytes) return PKV_ERR_BUFFER_TOO_SMALL;
+  if (need && (!workspace_dev || ((uintptr_t)workspace_dev & 15))) return PKV_ERR_INVALID_ARGUMENT;
   p.q_ptr = q_dev;
   p.o_ptr = out_dev;
   p.lse = lse_dev;
@@ -1137,6 +1026,8 @@ extern "C" int pkv_kv4_attend_dev(const pkv_kv4_cache* cache, const void* q_dev,
   const int longest = args->max_len > 0 && args->max_len < p.c.capacity ? args->max_len : p.c.capacity;
   cudaStream_t s = (cudaStream_t)stream;
   const bool acc = args->accumulate != 0;
+  if (chunk)
+    if (int st = launch_chunk(p, cache->dim, q_rows->dtype, q_rows, args, workspace_dev, s)) return st;
   if (cache->dim == 64) {
     switch (q_rows->dtype) {
       case PKV_DST_F32: return launch_all<64, PKV_DST_F32>(p, plan.nt, acc, longest, s);

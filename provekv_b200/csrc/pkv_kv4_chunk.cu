@@ -1,0 +1,568 @@
+// Attention over the 4-bit KV cache for many query rows per kv head (prompt chunks, drafts), 16-bit queries.
+//
+// A CTA takes up to 256 query rows of one kv head (two tiles of 128) over a run of units of 64 tokens, on the fifth-
+// generation tensor cores:
+//
+//   S = Q K^T    128 rows x 64 tokens, A = Q in tensor memory, B = dequantised keys in shared memory
+//   O += P V     128 rows x dim, A = P in tensor memory (over S), B = dequantised values, transposed, in shared memory
+//
+// Warps 0-3 and 4-7: the softmax of a tile each, a thread per row.  Warps 8-11 dequantise keys, 12-15 values; warp 16 brings
+// codes (bulk copies through a ring of three units), warp 17 issues the products.  The tiles alternate: while one's scores
+// become weights the tensor cores work for the other.
+//
+// A unit of 64 tokens costs the tensor cores 1024 cycles for 256 rows (dim 128), and the exponentials the same at 16 a
+// cycle; dequantising it takes about 900 warp instructions, shared by 256 rows.  Q and P are kept in tensor memory because
+// shared memory would otherwise be the bound: an operand of 128 x 128 read from there for every 64 tokens costs more than
+// the product.
+//
+// Both operands in shared memory are K-major with the 128-byte swizzle.  Row n of a unit's keys is token sigma(n), the same
+// order on the tokens' side of the values: it spreads the lanes that gather the values' codes over the banks.
+#include "pkv_kv4_attend.cuh"
+#include "pkv_tcgen05.cuh"
+
+using namespace pkv_kv4;
+
+namespace {
+
+constexpr int kThreads = 20 * 32;  // the last two warps only complete a warpgroup
+constexpr int kTileRows = 128, kTaskRows = 2 * kTileRows;
+constexpr int kCodeSlots = 3, kQuadSlots = 16;
+constexpr int kMinUnits = 8;  // a split of the tokens has at least this many units
+
+struct ChunkParams {
+  AttendParams a;
+  int tasks, splits;  // tasks of 256 rows of a kv head; splits of the tokens
+};
+
+// Token of row n of a unit's keys, of column n of its scores.
+__host__ __device__ constexpr int sigma(int n) { return (n & ~3) | ((n & 3) ^ ((n >> 3) & 3)); }
+
+// 128-byte swizzle: 16-byte piece c of row r of an operand with 128-byte rows.
+__device__ __forceinline__ uint32_t piece(int r, int c) { return (uint32_t)((r >> 3) * 1024 + (r & 7) * 128 + ((c ^ (r & 7)) << 4)); }
+
+// kind::f16: f32 accumulator, A and B binary16, both K-major
+__host__ __device__ constexpr uint32_t idesc_f16(int m, int n) {
+  return (1u << 4) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
+}
+// D[tmem] (+)= A[tmem] B[smem]^T, one step of 16 along K
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t"
+      ".reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, {%5, %5, %5, %5}, p;\n\t"
+      "}\n" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(0u)
+      : "memory");
+}
+__device__ __forceinline__ void arrive(uint64_t* bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(pkv_smem_u32(bar)) : "memory");
+}
+__device__ __forceinline__ void tmem_store8(uint32_t addr, const uint32_t (&r)[8]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(addr), "r"(r[0]), "r"(r[1]),
+               "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+               : "memory");
+}
+__device__ __forceinline__ void tmem_store_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// Registers move between the roles (whole warpgroups): 2 x 128 threads of 128, 2 x 128 of 80 and 128 of 64 are the 640 x 96
+// that the block was launched with.
+template <int N>
+__device__ __forceinline__ void more_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
+template <int N>
+__device__ __forceinline__ void fewer_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
+
+template <int D>
+struct Layout {
+  static constexpr int UNIT = kUnitAtoms * Atom<D>::BYTES;
+  static constexpr int KEYS = 64 * D * 2, VALUES = D * 64 * 2;  // a unit's operands
+  static constexpr int STAGE = KEYS + VALUES;
+  static constexpr int CODES = 2 * STAGE;                        // the ring of codes follows two stages of operands
+  static constexpr int BYTES = CODES + kCodeSlots * UNIT + 1024; // room to align the operands to 1024 bytes
+  // tensor memory columns of a tile: S (P over it), Q, O
+  static constexpr int S = 0, Q = 64, O = 128;
+};
+
+struct Barriers {
+  uint64_t codes_full[kCodeSlots], codes_empty[kCodeSlots];  // copies -> dequantising warps -> copies
+  uint64_t kv_full[2], kv_empty[2];                          // operands -> products -> operands
+  uint64_t q_full[2], s_full[2], p_full[2], o_done[2];       // per tile
+  uint64_t drain;
+};
+
+template <int D, int T>
+__global__ void __launch_bounds__(kThreads, 1)
+kv4_chunk_kernel(const __grid_constant__ ChunkParams cp) {
+  using A = Atom<D>;
+  using Y = Layout<D>;
+  using E = typename PkvDst<T>::type;
+  const AttendParams& p = cp.a;
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ __align__(8) Barriers bar;
+  __shared__ uint32_t s_tmem;
+  __shared__ uint32_t s_quad[kQuadSlots];  // which of a unit's atoms are there
+  uint8_t* smem = smem_raw + ((1024u - (pkv_smem_u32(smem_raw) & 1023u)) & 1023u);
+  const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
+
+  // ---- the task
+  const int split = blockIdx.x / cp.tasks, task = blockIdx.x - split * cp.tasks;
+  const int h = blockIdx.y, s = blockIdx.z;
+  const Sequence seq = sequence_of(p, s);
+  const int all_rows = seq.qn * p.group, row0 = task * kTaskRows;
+  if (row0 >= all_rows) return;
+  const int n_tiles = all_rows - row0 > kTileRows ? 2 : 1;
+  const int len = seq.len, pos0 = seq.end - seq.qn;
+  const int qpos_first = pos0 + row0 / p.group, qpos_last = pos0 + min(seq.qn - 1, (row0 + kTaskRows - 1) / p.group);
+  const Span span = visible_span(p, len, qpos_first, qpos_last);
+  const int first = (int)((int64_t)split * span.count / cp.splits), n = (int)((int64_t)(split + 1) * span.count / cp.splits) - first;
+
+  if (tid == 0) {
+    for (int i = 0; i < kCodeSlots; i++) {
+      pkv_mbar_init(&bar.codes_full[i], 1);
+      pkv_mbar_init(&bar.codes_empty[i], 8);
+    }
+    for (int i = 0; i < 2; i++) {
+      pkv_mbar_init(&bar.kv_full[i], 8);
+      pkv_mbar_init(&bar.kv_empty[i], 1);
+      pkv_mbar_init(&bar.q_full[i], kTileRows);
+      pkv_mbar_init(&bar.s_full[i], 1);
+      pkv_mbar_init(&bar.p_full[i], kTileRows);
+      pkv_mbar_init(&bar.o_done[i], 1);
+    }
+    pkv_mbar_init(&bar.drain, 1);
+  }
+  if (warp == 17) pkv_tc::tmem_alloc(&s_tmem, 512);
+  __syncthreads();
+  pkv_tc::fence_after_sync();
+  const uint32_t tmem = s_tmem;
+  bool fine = true;
+
+  if (warp >= 16) {
+    fewer_registers<64>();
+  } else if (warp >= 8) {
+    fewer_registers<80>();
+  } else {
+    more_registers<128>();
+  }
+  if (warp == 16) {
+    // ---- codes: page numbers of kBatch units at once, one atom per lane, a batch ahead of their use
+    auto atom_of = [&](int i0) -> int {
+      const int i = i0 + lane / kUnitAtoms;
+      if (i >= n) return -1;
+      const int a = span.unit(first + i) * kUnitAtoms + lane % kUnitAtoms;
+      return a * kAtomTokens < len ? a : -1;
+    };
+    auto page_of = [&](int a) -> int { return a < 0 ? -1 : __ldg(p.c.table + (int64_t)s * p.c.max_pages + a / p.c.page_atoms); };
+    int atom = atom_of(0), page = page_of(atom), issued = 0;
+    const uint8_t* src = nullptr;
+    unsigned live = 0;
+    for (int i = 0; i < n; i++) {
+      if (i % kBatch == 0) {
+        src = nullptr;
+        if (atom >= 0) {
+          if (page < 0 || page >= p.c.n_pages) pkv_report(p.err, 0, s, PKV_VEC_BAD_SEQUENCE);
+          else src = p.c.pages + (((int64_t)page * p.c.heads + h) * p.c.page_atoms + atom % p.c.page_atoms) * (int64_t)A::BYTES;
+        }
+        live = __ballot_sync(0xffffffffu, src != nullptr);
+        atom = atom_of(i + kBatch);
+        page = page_of(atom);
+      }
+      const int slot = i % kCodeSlots;
+      if (!__all_sync(0xffffffffu, pkv_mbar_wait(&bar.codes_empty[slot], ((i / kCodeSlots) & 1) ^ 1))) {
+        fine = false;
+        break;
+      }
+      const int l = kUnitAtoms * (i % kBatch);
+      const unsigned quad = (live >> l) & 15u;
+      if (lane == 0) {
+        s_quad[i % kQuadSlots] = quad;
+        pkv_mbar_expect_tx(&bar.codes_full[slot], (uint32_t)__popc(quad) * A::BYTES);
+      }
+      __syncwarp();
+      if (lane / kUnitAtoms == i % kBatch && src)
+        pkv_bulk_load(smem + Y::CODES + slot * Y::UNIT + lane % kUnitAtoms * A::BYTES, src, A::BYTES, &bar.codes_full[slot]);
+      issued = i + 1;
+    }
+    if (!fine)  // leave no copy behind
+      for (int i = max(0, issued - kCodeSlots); i < issued; i++) pkv_mbar_wait(&bar.codes_full[i % kCodeSlots], (i / kCodeSlots) & 1);
+  } else if (warp >= 17) {
+    // ---- products, one thread
+    if (warp == 17 && lane == 0) {
+      constexpr uint32_t id_s = idesc_f16(128, 64), id_o = idesc_f16(128, D);
+      auto scores = [&](int t, int i) {
+        const uint32_t keys = pkv_smem_u32(smem + (i & 1) * Y::STAGE);
+        const uint64_t b = pkv_tc::smem_desc_sw128(keys);
+        const uint32_t base = tmem + 256u * t;
+#pragma unroll
+        for (int k = 0; k < D / 16; k++)
+          mma_ts(base + Y::S, base + Y::Q + 8 * k, b + (uint64_t)(((k >> 2) * (64 * 128) + (k & 3) * 32) >> 4), id_s, k > 0);
+        pkv_tc::mma_commit(&bar.s_full[t]);
+      };
+      auto outputs = [&](int t, int i) {
+        const uint64_t b = pkv_tc::smem_desc_sw128(pkv_smem_u32(smem + (i & 1) * Y::STAGE + Y::KEYS));
+        const uint32_t base = tmem + 256u * t;
+#pragma unroll
+        for (int k = 0; k < 4; k++) mma_ts(base + Y::O, base + Y::S + 8 * k, b + (uint64_t)((k * 32) >> 4), id_o, i > 0 || k > 0);
+        pkv_tc::mma_commit(&bar.o_done[t]);
+      };
+      for (int i = 0; i < n && fine; i++) {
+        if (i == 0) {
+          fine = pkv_mbar_wait(&bar.kv_full[0], 0);
+          for (int t = 0; t < n_tiles && fine; t++) {
+            fine = pkv_mbar_wait(&bar.q_full[t], 0);
+            pkv_tc::fence_after_sync();
+            if (fine) scores(t, 0);
+          }
+        }
+        if (fine && i + 1 < n) fine = pkv_mbar_wait(&bar.kv_full[(i + 1) & 1], ((i + 1) >> 1) & 1);
+        for (int t = 0; t < n_tiles && fine; t++) {
+          fine = pkv_mbar_wait(&bar.p_full[t], i & 1);
+          if (!fine) break;
+          pkv_tc::fence_after_sync();
+          outputs(t, i);
+          if (i + 1 < n) scores(t, i + 1);
+        }
+        if (fine) pkv_tc::mma_commit(&bar.kv_empty[i & 1]);
+      }
+      pkv_tc::mma_commit(&bar.drain);
+      pkv_mbar_wait(&bar.drain, 0);
+    }
+  } else if (warp >= 8) {
+    // ---- codes to operands
+    const int w4 = warp & 3;
+    const bool values = warp >= 12;
+    for (int i = 0; i < n; i++) {
+      const int slot = i % kCodeSlots;
+      const bool ok = pkv_mbar_wait(&bar.codes_full[slot], (i / kCodeSlots) & 1) && pkv_mbar_wait(&bar.kv_empty[i & 1], ((i >> 1) & 1) ^ 1);
+      if (!__all_sync(0xffffffffu, ok)) {
+        fine = false;
+        break;
+      }
+      const uint8_t* codes = smem + Y::CODES + slot * Y::UNIT;
+      const unsigned quad = s_quad[i % kQuadSlots];
+      const int held = len - span.unit(first + i) * kUnitTokens;  // tokens of the unit below the sequence's length
+      const bool whole = quad == 15u && held >= kUnitTokens;
+      auto there = [&](int t) { return whole || (((quad >> (t >> 4)) & 1u) && t < held); };
+      if (!values) {
+        // a lane: one block of 16 channels of a token; four blocks x eight tokens a warp, so that the lanes of a store cover
+        // distinct banks
+        uint8_t* keys = smem + (i & 1) * Y::STAGE;
+        constexpr int BLOCKS = D / 16, PASSES = 64 * BLOCKS / 128;
+#pragma unroll 2
+        for (int k = 0; k < PASSES; k++) {
+          const int unit = k * 4 + w4;  // (group of 8 tokens, group of 4 blocks)
+          const int b = (lane & 3) + 4 * (unit % (BLOCKS / 4)), row = (lane >> 2) + 8 * (unit / (BLOCKS / 4)), t = sigma(row);
+          const uint8_t* atom = codes + (t >> 4) * A::BYTES;
+          uint2 w = make_uint2(0u, 0u);
+          uint32_t sb = 0u;
+          if (there(t)) {
+            w = *reinterpret_cast<const uint2*>(atom + A::KC + (t & 15) * A::ROW + 8 * b);
+            sb = atom[A::KS + (t & 15) * A::SROW + b];
+          }
+          const Scale sc = scale_of(sb * 0x00800080u);
+          uint32_t o0[4], o1[4];
+          nibbles(w.x, sc, o0);
+          nibbles(w.y, sc, o1);
+          uint8_t* slab = keys + (b >> 2) * (64 * 128);
+          *reinterpret_cast<uint4*>(slab + piece(row, 2 * (b & 3))) = make_uint4(o0[0], o0[1], o0[2], o0[3]);
+          *reinterpret_cast<uint4*>(slab + piece(row, 2 * (b & 3) + 1)) = make_uint4(o1[0], o1[1], o1[2], o1[3]);
+        }
+      } else {
+        // a lane: eight channels (a word of codes) of eight tokens, which become 16 bytes of eight rows of the transpose
+        uint8_t* vals = smem + (i & 1) * Y::STAGE + Y::KEYS;
+        constexpr int WORDS = D / 8;
+        for (int k = w4; k < WORDS / 4; k += 4) {
+          const int tg = lane & 7, word = 4 * k + (lane >> 3);
+          uint32_t m[4][8];  // [token pair][channel]
+#pragma unroll
+          for (int j = 0; j < 4; j++) {
+            uint32_t w[2], sb[2];
+#pragma unroll
+            for (int e = 0; e < 2; e++) {
+              const int t = 8 * tg + ((2 * j + e) ^ (tg & 3)), ta = t & 15;  // sigma(8 tg + 2 j + e)
+              const uint8_t* atom = codes + (t >> 4) * A::BYTES;
+              w[e] = sb[e] = 0u;
+              if (there(t)) {
+                w[e] = *reinterpret_cast<const uint32_t*>(atom + A::VC + ta * A::ROW + ((4 * word) ^ A::vswap(ta)));
+                sb[e] = atom[A::VS + ta * A::SROW + (word >> 1)];
+              }
+            }
+            const Scale sc = scale_of((sb[0] << 7) | (sb[1] << 23));
+            uint32_t lo[4], hi[4];
+            nibbles(__byte_perm(w[0], w[1], 0x5410), sc, lo);
+            nibbles(__byte_perm(w[0], w[1], 0x7632), sc, hi);
+#pragma unroll
+            for (int c = 0; c < 4; c++) {
+              m[j][c] = lo[c];
+              m[j][4 + c] = hi[c];
+            }
+          }
+#pragma unroll
+          for (int c = 0; c < 8; c++)
+            *reinterpret_cast<uint4*>(vals + piece(8 * word + c, tg)) = make_uint4(m[0][c], m[1][c], m[2][c], m[3][c]);
+        }
+      }
+      pkv_tc::fence_smem_to_async();
+      __syncwarp();
+      if (lane == 0) {
+        arrive(&bar.kv_full[i & 1]);
+        arrive(&bar.codes_empty[slot]);
+      }
+    }
+  } else if ((warp >> 2) < n_tiles) {
+    // ---- softmax of tile t, a thread per row
+    const int t = warp >> 2, row = row0 + kTileRows * t + (tid & 127);
+    const uint32_t base = tmem + 256u * t + ((uint32_t)(32 * (warp & 3)) << 16);
+    const bool live = row < all_rows;
+    const int token = row / p.group, hq = h * p.group + (row - token * p.group), qpos = pos0 + token;
+    float factor;
+    {  // the query, scaled by a power of two, odd channels divided by 16, in the order of the keys' channels
+      const E* q = reinterpret_cast<const E*>(p.q_ptr) + s * p.q.seq + (int64_t)token * p.q.token + hq * p.q.head;
+      float amax = 0.0f;
+#pragma unroll 2
+      for (int c = 0; c < D && live; c += 16) {
+        float x[16];
+        load_f32<T, 16>(q + c, x);
+#pragma unroll
+        for (int j = 0; j < 16; j++) amax = fmaxf(amax, fabsf(x[j]));
+      }
+      const float pw = p.negate ? -row_power(amax) : row_power(amax);
+      factor = __fmul_rn(__fmul_rn(__fmul_rn(p.scale, kLog2e), kScaleShift), 1.0f / row_power(amax));
+#pragma unroll 2
+      for (int c = 0; c < D; c += 16) {
+        float x[16];
+#pragma unroll
+        for (int j = 0; j < 16; j++) x[j] = 0.0f;
+        if (live) load_f32<T, 16>(q + c, x);
+        uint32_t r[8];
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+          const int at = 8 * (j >> 2) + (j & 3);
+          const float f = (j & 1) ? __fmul_rn(pw, 0.0625f) : pw;
+          r[j] = half2_of(__fmul_rn(x[at], f), __fmul_rn(x[at + 4], f));
+        }
+        __syncwarp();
+        tmem_store8(base + Y::Q + c / 2, r);
+      }
+      tmem_store_wait();
+      pkv_tc::fence_before_sync();
+      arrive(&bar.q_full[t]);
+    }
+    const bool by_position = p.c.positions != nullptr && (p.window > 0 || seq.qn > 1);
+    const int32_t* positions = by_position ? p.c.positions + p.c.stat(s, h) : nullptr;
+    const int tile_first = pos0 + (row0 + kTileRows * t) / p.group;
+    const int tile_last = pos0 + min(seq.qn - 1, (row0 + kTileRows * t + kTileRows - 1) / p.group);
+    float m = -INFINITY, l = 0.0f;
+    for (int i = 0; i < n; i++) {
+      if (!__all_sync(0xffffffffu, pkv_mbar_wait(&bar.s_full[t], i & 1))) {
+        fine = false;
+        break;
+      }
+      pkv_tc::fence_after_sync();
+      float x[2][32];
+      pkv_tc::tmem_load32(base + Y::S, x[0]);
+      pkv_tc::tmem_load32(base + Y::S + 32, x[1]);
+      const int token0 = span.unit(first + i) * kUnitTokens;
+      const unsigned quad = s_quad[i % kQuadSlots];
+      float fac = factor;
+      if (quad != 15u || token0 + kUnitTokens > len || by_position || token0 + kUnitTokens - 1 > tile_first ||
+          (p.window > 0 && tile_last - token0 >= p.window && token0 + kUnitTokens > p.sinks)) {
+        fac = 1.0f;
+#pragma unroll
+        for (int c = 0; c < 64; c++) {
+          const int k = sigma(c), at = token0 + k;
+          bool see = ((quad >> (k >> 4)) & 1u) && at < len;
+          int kp = at;
+          if (by_position) kp = see ? __ldg(positions + at) : 0;
+          const int d = qpos - kp;
+          see = see && d >= 0 && (p.window == 0 || d < p.window || kp < p.sinks);
+          x[c >> 5][c & 31] = see ? __fmul_rn(x[c >> 5][c & 31], factor) : -INFINITY;
+        }
+      }
+      float top = x[0][0];
+#pragma unroll
+      for (int c = 1; c < 64; c++) top = fmaxf(top, x[c >> 5][c & 31]);
+      top = __fmul_rn(top, fac);
+      // the sums up to the unit before are complete (their product was issued a whole turn ago)
+      if (i > 0 && !__all_sync(0xffffffffu, pkv_mbar_wait(&bar.o_done[t], (i - 1) & 1))) {
+        fine = false;
+        break;
+      }
+      if (__any_sync(0xffffffffu, top > __fadd_rn(m, kLag))) {
+        const float raised = fmaxf(m, top);
+        const float f = m == -INFINITY ? 0.0f : exp2_fast(__fsub_rn(m, raised));
+        m = raised;
+        l = __fmul_rn(l, f);
+        if (i > 0) {
+          pkv_tc::fence_after_sync();
+#pragma unroll 1
+          for (int c = 0; c < D; c += 8) {
+            float o[8];
+            pkv_tc::tmem_load<8>(base + Y::O + c, o);
+            uint32_t r[8];
+#pragma unroll
+            for (int j = 0; j < 8; j++) r[j] = __float_as_uint(__fmul_rn(o[j], f));
+            tmem_store8(base + Y::O + c, r);
+          }
+        }
+      }
+      const float shift = m == -INFINITY ? 0.0f : __fsub_rn(kWeightShift, m);
+      float sum[2] = {0.0f, 0.0f};
+#pragma unroll
+      for (int c = 0; c < 64; c += 16) {
+        uint32_t r[8];
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+          const float w0 = exp2_fast(__fmaf_rn(x[c >> 5][(c & 31) + 2 * j], fac, shift));
+          const float w1 = exp2_fast(__fmaf_rn(x[c >> 5][(c & 31) + 2 * j + 1], fac, shift));
+          sum[0] = __fadd_rn(sum[0], w0);
+          sum[1] = __fadd_rn(sum[1], w1);
+          r[j] = half2_of(w0, w1);
+        }
+        tmem_store8(base + Y::S + c / 2, r);
+      }
+      l = __fadd_rn(l, __fadd_rn(sum[0], sum[1]));
+      tmem_store_wait();
+      pkv_tc::fence_before_sync();
+      arrive(&bar.p_full[t]);
+    }
+    if (fine && n > 0) fine = __all_sync(0xffffffffu, pkv_mbar_wait(&bar.o_done[t], (n - 1) & 1));
+    pkv_tc::fence_after_sync();
+    if (!fine && lane == 0) pkv_report(p.err, 0, s, PKV_VEC_DEVICE_WAIT);
+    const int64_t part = (((((int64_t)s * p.c.heads + h) * cp.tasks + task) * cp.splits + split) * kTaskRows) + kTileRows * t + (tid & 127);
+    if (cp.splits > 1 && live) *reinterpret_cast<float2*>(p.part_ml + part * 2) = make_float2(m, l);
+    if (n > 0 || cp.splits == 1) {
+#pragma unroll 1
+      for (int c = 0; c < D; c += 32) {
+        float o[32];
+        __syncwarp();
+        if (n > 0) {
+          pkv_tc::tmem_load32(base + Y::O + c, o);
+        } else {
+#pragma unroll
+          for (int j = 0; j < 32; j++) o[j] = 0.0f;
+        }
+#pragma unroll
+        for (int j = 0; j < 32; j++) o[j] = __fmul_rn(o[j], (j & 1) ? kScaleShift / 16.0f : kScaleShift);
+        if (!live) continue;
+        if (cp.splits > 1) store_f32<PKV_DST_F32, 32>(p.part_o + part * D + c, o);
+        else write_row<T, 32>(p, s, h, row, c, o, m, l, c == 0);
+      }
+    }
+  }
+  // every product has been waited for (warp 17) and every read of tensor memory is done
+  pkv_tc::fence_before_sync();
+  __syncthreads();
+  if (warp == 17) {
+    pkv_tc::fence_after_sync();
+    pkv_tc::tmem_free(tmem, 512);
+  }
+}
+
+// Joins the splits of a query row; a warp per row.
+template <int D, int T>
+__global__ void __launch_bounds__(256)
+kv4_chunk_join_kernel(const __grid_constant__ ChunkParams cp) {
+  const AttendParams& p = cp.a;
+  constexpr int N = D / 32;
+  const int lane = threadIdx.x & 31;
+  const int h = blockIdx.y, s = blockIdx.z, row = blockIdx.x * 8 + (threadIdx.x >> 5);
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  int qn = p.q_lens ? p.q_lens[s] : p.q.n;
+  if (qn < 0 || qn > p.q.n) qn = 0;
+  if (row >= qn * p.group) return;
+  const int task = row / kTaskRows;
+  const int64_t first = ((((int64_t)s * p.c.heads + h) * cp.tasks + task) * cp.splits) * kTaskRows + (row - task * kTaskRows);
+  float m = -INFINITY, l = 0.0f, x[N];
+#pragma unroll
+  for (int i = 0; i < N; i++) x[i] = 0.0f;
+  for (int k = 0; k < cp.splits; k++) {
+    const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + (first + (int64_t)k * kTaskRows) * 2);
+    if (ml.x == -INFINITY && ml.y == 0.0f) continue;  // a split that sees nothing
+    const float top = fmaxf(m, ml.x);
+    const float fold = m == -INFINITY ? 0.0f : exp2_fast(__fsub_rn(m, top));
+    const float f = ml.x == -INFINITY ? ml.y : exp2_fast(__fsub_rn(ml.x, top));  // (NaN without a reference stays NaN)
+    m = top;
+    l = __fmaf_rn(l, fold, __fmul_rn(f, ml.y));
+    const float* src = p.part_o + (first + (int64_t)k * kTaskRows) * D + lane * N;
+#pragma unroll
+    for (int i = 0; i < N; i++) x[i] = __fmaf_rn(x[i], fold, __fmul_rn(f, src[i]));
+  }
+  write_row<T, N>(p, s, h, row, lane * N, x, m, l, lane == 0);
+}
+
+struct Plan {
+  int tasks, splits;
+  int64_t part_rows;
+};
+
+Plan make_plan(const Cache& c, const pkv_kv4_rows* q, const pkv_kv4_attend_args* a) {
+  Plan r;
+  const int64_t rows = (int64_t)q->n_tokens * (a->n_q_heads / c.heads);
+  r.tasks = (int)((rows + kTaskRows - 1) / kTaskRows);
+  int64_t longest = a->max_len > 0 && a->max_len < c.capacity ? a->max_len : c.capacity;
+  if (a->window > 0 && !c.positions) {
+    const int64_t seen = (int64_t)a->window + a->sinks + q->n_tokens + 3 * kUnitTokens;
+    if (seen < longest) longest = seen;
+  }
+  const int64_t units = (longest + kUnitTokens - 1) / kUnitTokens, ctas = (int64_t)r.tasks * c.heads * c.n_seqs;
+  // one CTA fits an SM; where the tasks leave SMs idle the tokens are split
+  int64_t splits = sm_count() / (ctas > 0 ? ctas : 1);
+  if (splits > units / kMinUnits) splits = units / kMinUnits;
+  r.splits = splits < 1 ? 1 : (int)splits;
+  r.part_rows = r.splits > 1 ? ctas * r.splits * kTaskRows : 0;
+  return r;
+}
+
+template <int D, int T>
+int launch(const ChunkParams& cp, int64_t rows, cudaStream_t s) {
+  auto kernel = kv4_chunk_kernel<D, T>;
+  constexpr int bytes = Layout<D>::BYTES;
+  if (cudaError_t ce = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes)) return pkv_cuda_status(ce);
+  kernel<<<dim3(cp.tasks * cp.splits, cp.a.c.heads, cp.a.c.n_seqs), kThreads, bytes, s>>>(cp);
+  pkv_count_launch();
+  if (cudaError_t ce = cudaGetLastError()) return pkv_cuda_status(ce);
+  if (cp.splits > 1) {
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr = {};
+    cfg.gridDim = dim3((unsigned)((rows + 7) / 8), cp.a.c.heads, cp.a.c.n_seqs);
+    cfg.blockDim = dim3(256);
+    cfg.stream = s;
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    if (cudaError_t ce = cudaLaunchKernelEx(&cfg, kv4_chunk_join_kernel<D, T>, cp)) return pkv_cuda_status(ce);
+    pkv_count_launch();
+  }
+  return pkv_cuda_status(cudaGetLastError());
+}
+
+}  // namespace
+
+namespace pkv_kv4 {
+
+// More rows than the other kernel's largest tile; f32 queries stay there (their two terms do not fit the tile).
+bool chunk_takes(const pkv_kv4_rows* q, int group) {
+  return q->dtype != PKV_DST_F32 && (int64_t)q->n_tokens * group > 16;
+}
+
+int64_t chunk_workspace_bytes(const Cache& c, int dim, const pkv_kv4_rows* q, const pkv_kv4_attend_args* a) {
+  return make_plan(c, q, a).part_rows * (dim + 2) * (int64_t)sizeof(float);
+}
+
+int launch_chunk(AttendParams p, int dim, int dtype, const pkv_kv4_rows* q, const pkv_kv4_attend_args* a, void* workspace,
+                 cudaStream_t s) {
+  const Plan plan = make_plan(p.c, q, a);
+  ChunkParams cp;
+  p.part_o = (float*)workspace;
+  p.part_ml = p.part_o + plan.part_rows * dim;
+  cp.a = p;
+  cp.tasks = plan.tasks;
+  cp.splits = plan.splits;
+  const int64_t rows = (int64_t)q->n_tokens * p.group;
+  if (dim == 64) return dtype == PKV_DST_F16 ? launch<64, PKV_DST_F16>(cp, rows, s) : launch<64, PKV_DST_BF16>(cp, rows, s);
+  return dtype == PKV_DST_F16 ? launch<128, PKV_DST_F16>(cp, rows, s) : launch<128, PKV_DST_BF16>(cp, rows, s);
+}
+
+}  // namespace pkv_kv4
