@@ -26,7 +26,7 @@ namespace {
 
 constexpr int kThreads = 20 * 32;  // the last two warps only complete a warpgroup
 constexpr int kTileRows = 128, kTaskRows = 2 * kTileRows;
-constexpr int kCodeSlots = 3, kQuadSlots = 16;
+constexpr int kCodeSlots = 3, kStagesKv = 4, kQuadSlots = 16;
 constexpr int kMinUnits = 8;  // a split of the tokens has at least this many units
 
 struct ChunkParams {
@@ -55,6 +55,17 @@ __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint3
       "r"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(0u)
       : "memory");
 }
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile(
+      "{\n\t"
+      ".reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t"
+      "}\n"
+      : "=r"(p));
+  return p != 0;
+}
 __device__ __forceinline__ void arrive(uint64_t* bar) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(pkv_smem_u32(bar)) : "memory");
 }
@@ -77,7 +88,7 @@ struct Layout {
   static constexpr int UNIT = kUnitAtoms * Atom<D>::BYTES;
   static constexpr int KEYS = 64 * D * 2, VALUES = D * 64 * 2;  // a unit's operands
   static constexpr int STAGE = KEYS + VALUES;
-  static constexpr int CODES = 2 * STAGE;                        // the ring of codes follows two stages of operands
+  static constexpr int CODES = kStagesKv * STAGE;                // the ring of codes follows the operands' stages
   static constexpr int BYTES = CODES + kCodeSlots * UNIT + 1024; // room to align the operands to 1024 bytes
   // tensor memory columns of a tile: S (P over it), Q, O
   static constexpr int S = 0, Q = 64, O = 128;
@@ -85,7 +96,7 @@ struct Layout {
 
 struct Barriers {
   uint64_t codes_full[kCodeSlots], codes_empty[kCodeSlots];  // copies -> dequantising warps -> copies
-  uint64_t kv_full[2], kv_empty[2];                          // operands -> products -> operands
+  uint64_t kv_full[kStagesKv], kv_empty[kStagesKv];                          // operands -> products -> operands
   uint64_t q_full[2], s_full[2], p_full[2], o_done[2];       // per tile
   uint64_t drain;
 };
@@ -121,9 +132,11 @@ kv4_chunk_kernel(const __grid_constant__ ChunkParams cp) {
       pkv_mbar_init(&bar.codes_full[i], 1);
       pkv_mbar_init(&bar.codes_empty[i], 8);
     }
-    for (int i = 0; i < 2; i++) {
+    for (int i = 0; i < kStagesKv; i++) {
       pkv_mbar_init(&bar.kv_full[i], 8);
       pkv_mbar_init(&bar.kv_empty[i], 1);
+    }
+    for (int i = 0; i < 2; i++) {
       pkv_mbar_init(&bar.q_full[i], kTileRows);
       pkv_mbar_init(&bar.s_full[i], 1);
       pkv_mbar_init(&bar.p_full[i], kTileRows);
@@ -134,7 +147,7 @@ kv4_chunk_kernel(const __grid_constant__ ChunkParams cp) {
   if (warp == 17) pkv_tc::tmem_alloc(&s_tmem, 512);
   __syncthreads();
   pkv_tc::fence_after_sync();
-  const uint32_t tmem = s_tmem;
+  const uint32_t tmem = __shfl_sync(0xffffffffu, s_tmem, 0);
   bool fine = true;
 
   if (warp >= 16) {
@@ -186,45 +199,58 @@ kv4_chunk_kernel(const __grid_constant__ ChunkParams cp) {
     if (!fine)  // leave no copy behind
       for (int i = max(0, issued - kCodeSlots); i < issued; i++) pkv_mbar_wait(&bar.codes_full[i % kCodeSlots], (i / kCodeSlots) & 1);
   } else if (warp >= 17) {
-    // ---- products, one thread
-    if (warp == 17 && lane == 0) {
+    // ---- products.  The whole warp walks through the units, so that descriptors and addresses stay in uniform registers
+    // (moving them there for every instruction costs a lone thread about 100 cycles a step); one lane issues.
+    if (warp == 17) {
       constexpr uint32_t id_s = idesc_f16(128, 64), id_o = idesc_f16(128, D);
+      const bool leader = elect_one();
+      const uint32_t operands = pkv_smem_u32(smem);
       auto scores = [&](int t, int i) {
-        const uint32_t keys = pkv_smem_u32(smem + (i & 1) * Y::STAGE);
-        const uint64_t b = pkv_tc::smem_desc_sw128(keys);
+        const uint64_t b = pkv_tc::smem_desc_sw128(operands + (i % kStagesKv) * Y::STAGE);
         const uint32_t base = tmem + 256u * t;
+        if (leader) {
 #pragma unroll
-        for (int k = 0; k < D / 16; k++)
-          mma_ts(base + Y::S, base + Y::Q + 8 * k, b + (uint64_t)(((k >> 2) * (64 * 128) + (k & 3) * 32) >> 4), id_s, k > 0);
-        pkv_tc::mma_commit(&bar.s_full[t]);
+          for (int k = 0; k < D / 16; k++)
+            mma_ts(base + Y::S, base + Y::Q + 8 * k, b + (uint64_t)(((k >> 2) * (64 * 128) + (k & 3) * 32) >> 4), id_s, k > 0);
+          pkv_tc::mma_commit(&bar.s_full[t]);
+        }
+        __syncwarp();
       };
       auto outputs = [&](int t, int i) {
-        const uint64_t b = pkv_tc::smem_desc_sw128(pkv_smem_u32(smem + (i & 1) * Y::STAGE + Y::KEYS));
+        const uint64_t b = pkv_tc::smem_desc_sw128(operands + (i % kStagesKv) * Y::STAGE + Y::KEYS);
         const uint32_t base = tmem + 256u * t;
+        if (leader) {
 #pragma unroll
-        for (int k = 0; k < 4; k++) mma_ts(base + Y::O, base + Y::S + 8 * k, b + (uint64_t)((k * 32) >> 4), id_o, i > 0 || k > 0);
-        pkv_tc::mma_commit(&bar.o_done[t]);
+          for (int k = 0; k < 4; k++) mma_ts(base + Y::O, base + Y::S + 8 * k, b + (uint64_t)((k * 32) >> 4), id_o, i > 0 || k > 0);
+          pkv_tc::mma_commit(&bar.o_done[t]);
+        }
+        __syncwarp();
       };
+      auto wait = [&](uint64_t* b, uint32_t parity) { return __all_sync(0xffffffffu, pkv_mbar_wait(b, parity)) != 0; };
       for (int i = 0; i < n && fine; i++) {
         if (i == 0) {
-          fine = pkv_mbar_wait(&bar.kv_full[0], 0);
+          fine = wait(&bar.kv_full[0], 0);
           for (int t = 0; t < n_tiles && fine; t++) {
-            fine = pkv_mbar_wait(&bar.q_full[t], 0);
+            fine = wait(&bar.q_full[t], 0);
             pkv_tc::fence_after_sync();
             if (fine) scores(t, 0);
           }
         }
-        if (fine && i + 1 < n) fine = pkv_mbar_wait(&bar.kv_full[(i + 1) & 1], ((i + 1) >> 1) & 1);
         for (int t = 0; t < n_tiles && fine; t++) {
-          fine = pkv_mbar_wait(&bar.p_full[t], i & 1);
+          fine = wait(&bar.p_full[t], i & 1);
           if (!fine) break;
           pkv_tc::fence_after_sync();
           outputs(t, i);
-          if (i + 1 < n) scores(t, i + 1);
+          if (i + 1 < n) {
+            if (t == 0) fine = wait(&bar.kv_full[(i + 1) % kStagesKv], ((i + 1) / kStagesKv) & 1);
+            if (fine) scores(t, i + 1);
+          }
         }
-        if (fine) pkv_tc::mma_commit(&bar.kv_empty[i & 1]);
+        if (fine && leader) pkv_tc::mma_commit(&bar.kv_empty[i % kStagesKv]);
+        __syncwarp();
       }
-      pkv_tc::mma_commit(&bar.drain);
+      if (leader) pkv_tc::mma_commit(&bar.drain);
+      __syncwarp();
       pkv_mbar_wait(&bar.drain, 0);
     }
   } else if (warp >= 8) {
@@ -233,7 +259,7 @@ kv4_chunk_kernel(const __grid_constant__ ChunkParams cp) {
     const bool values = warp >= 12;
     for (int i = 0; i < n; i++) {
       const int slot = i % kCodeSlots;
-      const bool ok = pkv_mbar_wait(&bar.codes_full[slot], (i / kCodeSlots) & 1) && pkv_mbar_wait(&bar.kv_empty[i & 1], ((i >> 1) & 1) ^ 1);
+      const bool ok = pkv_mbar_wait(&bar.codes_full[slot], (i / kCodeSlots) & 1) && pkv_mbar_wait(&bar.kv_empty[i % kStagesKv], ((i / kStagesKv) & 1) ^ 1);
       if (!__all_sync(0xffffffffu, ok)) {
         fine = false;
         break;
@@ -246,9 +272,9 @@ kv4_chunk_kernel(const __grid_constant__ ChunkParams cp) {
       if (!values) {
         // a lane: one block of 16 channels of a token; four blocks x eight tokens a warp, so that the lanes of a store cover
         // distinct banks
-        uint8_t* keys = smem + (i & 1) * Y::STAGE;
+        uint8_t* keys = smem + (i % kStagesKv) * Y::STAGE;
         constexpr int BLOCKS = D / 16, PASSES = 64 * BLOCKS / 128;
-#pragma unroll 2
+#pragma unroll
         for (int k = 0; k < PASSES; k++) {
           const int unit = k * 4 + w4;  // (group of 8 tokens, group of 4 blocks)
           const int b = (lane & 3) + 4 * (unit % (BLOCKS / 4)), row = (lane >> 2) + 8 * (unit / (BLOCKS / 4)), t = sigma(row);
@@ -269,7 +295,7 @@ kv4_chunk_kernel(const __grid_constant__ ChunkParams cp) {
         }
       } else {
         // a lane: eight channels (a word of codes) of eight tokens, which become 16 bytes of eight rows of the transpose
-        uint8_t* vals = smem + (i & 1) * Y::STAGE + Y::KEYS;
+        uint8_t* vals = smem + (i % kStagesKv) * Y::STAGE + Y::KEYS;
         constexpr int WORDS = D / 8;
         for (int k = w4; k < WORDS / 4; k += 4) {
           const int tg = lane & 7, word = 4 * k + (lane >> 3);
@@ -305,7 +331,7 @@ kv4_chunk_kernel(const __grid_constant__ ChunkParams cp) {
       pkv_tc::fence_smem_to_async();
       __syncwarp();
       if (lane == 0) {
-        arrive(&bar.kv_full[i & 1]);
+        arrive(&bar.kv_full[i % kStagesKv]);
         arrive(&bar.codes_empty[slot]);
       }
     }
