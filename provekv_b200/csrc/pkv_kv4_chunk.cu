@@ -3,17 +3,16 @@
 // A CTA takes up to 256 query rows of one kv head (two tiles of 128) over a run of units of 64 tokens, on the fifth-
 // generation tensor cores:
 //
-//   S = Q K^T    128 rows x 64 tokens, A = Q in tensor memory, B = dequantised keys in shared memory
+//   S = Q K^T    128 rows x 64 tokens, A = Q, B = dequantised keys, both in shared memory; two S per tile
 //   O += P V     128 rows x dim, A = P in tensor memory (over S), B = dequantised values, transposed, in shared memory
 //
 // Warps 0-3 and 4-7: the softmax of a tile each, a thread per row.  Warps 8-11 dequantise keys, 12-15 values; warp 16 brings
-// codes (bulk copies through a ring of three units), warp 17 issues the products.  The tiles alternate: while one's scores
-// become weights the tensor cores work for the other.
+// codes (bulk copies through a ring of three units), warp 17 issues the products.  The scores of the next unit are on
+// their way while a tile's softmax works on the last.
 //
 // A unit of 64 tokens costs the tensor cores 1024 cycles for 256 rows (dim 128), and the exponentials the same at 16 a
-// cycle; dequantising it takes about 900 warp instructions, shared by 256 rows.  Q and P are kept in tensor memory because
-// shared memory would otherwise be the bound: an operand of 128 x 128 read from there for every 64 tokens costs more than
-// the product.
+// cycle; shared memory gives the products their operands in another 1024, and the dequantised unit goes into it in about
+// 400.  Dequantising takes about 900 warp instructions, shared by 256 rows.
 //
 // Both operands in shared memory are K-major with the 128-byte swizzle.  Row n of a unit's keys is token sigma(n), the same
 // order on the tokens' side of the values: it spreads the lanes that gather the values' codes over the banks.
@@ -44,7 +43,18 @@ __device__ __forceinline__ uint32_t piece(int r, int c) { return (uint32_t)((r >
 __host__ __device__ constexpr uint32_t idesc_f16(int m, int n) {
   return (1u << 4) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
 }
-// D[tmem] (+)= A[tmem] B[smem]^T, one step of 16 along K
+// D[tmem] (+)= A[smem] B[smem]^T, one step of 16 along K
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t"
+      ".reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, {%5, %5, %5, %5}, p;\n\t"
+      "}\n" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(0u)
+      : "memory");
+}
+// D[tmem] (+)= A[tmem] B[smem]^T
 __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
       "{\n\t"
@@ -74,6 +84,56 @@ __device__ __forceinline__ void tmem_store8(uint32_t addr, const uint32_t (&r)[8
                "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
                : "memory");
 }
+// 64 columns of this thread's lane, one wait
+__device__ __forceinline__ void tmem_load32_async(uint32_t addr, uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];\n"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
+        "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]),
+        "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]),
+        "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(addr)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_load_wait(uint32_t (&r)[32]) {  // no use of the registers moves above it
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]),
+                 "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]), "+r"(r[16]), "+r"(r[17]), "+r"(r[18]),
+                 "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]),
+                 "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31])
+               :
+               : "memory");
+}
+__device__ __forceinline__ void tmem_load64(uint32_t addr, float (&x)[2][32]) {
+  uint32_t a[32], b[32];
+  tmem_load32_async(addr, a);
+  tmem_load32_async(addr + 32, b);
+  tmem_load_wait(a);
+  tmem_load_wait(b);
+#pragma unroll
+  for (int i = 0; i < 32; i++) {
+    x[0][i] = __uint_as_float(a[i]);
+    x[1][i] = __uint_as_float(b[i]);
+  }
+}
+// two f32 operations in one instruction
+__device__ __forceinline__ float2 fma2_f32(float2 a, float2 b, float2 c) {
+  unsigned long long r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;"
+      : "=l"(r)
+      : "l"(*reinterpret_cast<unsigned long long*>(&a)), "l"(*reinterpret_cast<unsigned long long*>(&b)),
+        "l"(*reinterpret_cast<unsigned long long*>(&c)));
+  return *reinterpret_cast<float2*>(&r);
+}
+__device__ __forceinline__ float2 add2_f32(float2 a, float2 b) {
+  unsigned long long r;
+  asm("add.rn.f32x2 %0, %1, %2;"
+      : "=l"(r)
+      : "l"(*reinterpret_cast<unsigned long long*>(&a)), "l"(*reinterpret_cast<unsigned long long*>(&b)));
+  return *reinterpret_cast<float2*>(&r);
+}
 __device__ __forceinline__ void tmem_store_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
 // Registers move between the roles (whole warpgroups): 2 x 128 threads of 128, 2 x 128 of 80 and 128 of 64 are the 640 x 96
@@ -88,16 +148,17 @@ struct Layout {
   static constexpr int UNIT = kUnitAtoms * Atom<D>::BYTES;
   static constexpr int KEYS = 64 * D * 2, VALUES = D * 64 * 2;  // a unit's operands
   static constexpr int STAGE = KEYS + VALUES;
-  static constexpr int CODES = kStagesKv * STAGE;                // the ring of codes follows the operands' stages
+  static constexpr int QUERY = kTileRows * D * 2;                // a tile's queries
+  static constexpr int QUERIES = kStagesKv * STAGE, CODES = QUERIES + 2 * QUERY;
   static constexpr int BYTES = CODES + kCodeSlots * UNIT + 1024; // room to align the operands to 1024 bytes
-  // tensor memory columns of a tile: S (P over it), Q, O
-  static constexpr int S = 0, Q = 64, O = 128;
+  // tensor memory columns of a tile: two S (P over each), O
+  static constexpr int S = 0, O = 128;
 };
 
 struct Barriers {
   uint64_t codes_full[kCodeSlots], codes_empty[kCodeSlots];  // copies -> dequantising warps -> copies
   uint64_t kv_full[kStagesKv], kv_empty[kStagesKv];                          // operands -> products -> operands
-  uint64_t q_full[2], s_full[2], p_full[2], o_done[2];       // per tile
+  uint64_t q_full[2], s_full[2][2], p_full[2][2], o_done[2]; // per tile (and S)
   uint64_t drain;
 };
 
@@ -138,8 +199,10 @@ kv4_chunk_kernel(const __grid_constant__ ChunkParams cp) {
     }
     for (int i = 0; i < 2; i++) {
       pkv_mbar_init(&bar.q_full[i], kTileRows);
-      pkv_mbar_init(&bar.s_full[i], 1);
-      pkv_mbar_init(&bar.p_full[i], kTileRows);
+      for (int b = 0; b < 2; b++) {
+        pkv_mbar_init(&bar.s_full[i][b], 1);
+        pkv_mbar_init(&bar.p_full[i][b], kTileRows);
+      }
       pkv_mbar_init(&bar.o_done[i], 1);
     }
     pkv_mbar_init(&bar.drain, 1);
@@ -206,13 +269,15 @@ kv4_chunk_kernel(const __grid_constant__ ChunkParams cp) {
       const bool leader = elect_one();
       const uint32_t operands = pkv_smem_u32(smem);
       auto scores = [&](int t, int i) {
+        const uint64_t a = pkv_tc::smem_desc_sw128(operands + Y::QUERIES + t * Y::QUERY);
         const uint64_t b = pkv_tc::smem_desc_sw128(operands + (i % kStagesKv) * Y::STAGE);
-        const uint32_t base = tmem + 256u * t;
+        const uint32_t d = tmem + 256u * t + Y::S + 64u * (i & 1);
         if (leader) {
 #pragma unroll
           for (int k = 0; k < D / 16; k++)
-            mma_ts(base + Y::S, base + Y::Q + 8 * k, b + (uint64_t)(((k >> 2) * (64 * 128) + (k & 3) * 32) >> 4), id_s, k > 0);
-          pkv_tc::mma_commit(&bar.s_full[t]);
+            mma_ss(d, a + (uint64_t)(((k >> 2) * (kTileRows * 128) + (k & 3) * 32) >> 4),
+                   b + (uint64_t)(((k >> 2) * (64 * 128) + (k & 3) * 32) >> 4), id_s, k > 0);
+          pkv_tc::mma_commit(&bar.s_full[t][i & 1]);
         }
         __syncwarp();
       };
@@ -221,7 +286,7 @@ kv4_chunk_kernel(const __grid_constant__ ChunkParams cp) {
         const uint32_t base = tmem + 256u * t;
         if (leader) {
 #pragma unroll
-          for (int k = 0; k < 4; k++) mma_ts(base + Y::O, base + Y::S + 8 * k, b + (uint64_t)((k * 32) >> 4), id_o, i > 0 || k > 0);
+          for (int k = 0; k < 4; k++) mma_ts(base + Y::O, base + Y::S + 64u * (i & 1) + 8 * k, b + (uint64_t)((k * 32) >> 4), id_o, i > 0 || k > 0);
           pkv_tc::mma_commit(&bar.o_done[t]);
         }
         __syncwarp();
@@ -236,15 +301,15 @@ kv4_chunk_kernel(const __grid_constant__ ChunkParams cp) {
             if (fine) scores(t, 0);
           }
         }
+        // the S that the next scores go into was read by the unit before's product, which is ahead of them in order
+        if (fine && i + 1 < n) {
+          fine = wait(&bar.kv_full[(i + 1) % kStagesKv], ((i + 1) / kStagesKv) & 1);
+          for (int t = 0; t < n_tiles && fine; t++) scores(t, i + 1);
+        }
         for (int t = 0; t < n_tiles && fine; t++) {
-          fine = wait(&bar.p_full[t], i & 1);
-          if (!fine) break;
+          fine = wait(&bar.p_full[t][i & 1], (i >> 1) & 1);
           pkv_tc::fence_after_sync();
-          outputs(t, i);
-          if (i + 1 < n) {
-            if (t == 0) fine = wait(&bar.kv_full[(i + 1) % kStagesKv], ((i + 1) / kStagesKv) & 1);
-            if (fine) scores(t, i + 1);
-          }
+          if (fine) outputs(t, i);
         }
         if (fine && leader) pkv_tc::mma_commit(&bar.kv_empty[i % kStagesKv]);
         __syncwarp();
@@ -354,6 +419,7 @@ kv4_chunk_kernel(const __grid_constant__ ChunkParams cp) {
       }
       const float pw = p.negate ? -row_power(amax) : row_power(amax);
       factor = __fmul_rn(__fmul_rn(__fmul_rn(p.scale, kLog2e), kScaleShift), 1.0f / row_power(amax));
+      uint8_t* to = smem + Y::QUERIES + t * Y::QUERY;
 #pragma unroll 2
       for (int c = 0; c < D; c += 16) {
         float x[16];
@@ -367,11 +433,11 @@ kv4_chunk_kernel(const __grid_constant__ ChunkParams cp) {
           const float f = (j & 1) ? __fmul_rn(pw, 0.0625f) : pw;
           r[j] = half2_of(__fmul_rn(x[at], f), __fmul_rn(x[at + 4], f));
         }
-        __syncwarp();
-        tmem_store8(base + Y::Q + c / 2, r);
+        uint8_t* slab = to + (c >> 6) * (kTileRows * 128);
+        *reinterpret_cast<uint4*>(slab + piece(tid & 127, (c >> 3) & 7)) = make_uint4(r[0], r[1], r[2], r[3]);
+        *reinterpret_cast<uint4*>(slab + piece(tid & 127, ((c >> 3) & 7) + 1)) = make_uint4(r[4], r[5], r[6], r[7]);
       }
-      tmem_store_wait();
-      pkv_tc::fence_before_sync();
+      pkv_tc::fence_smem_to_async();
       arrive(&bar.q_full[t]);
     }
     const bool by_position = p.c.positions != nullptr && (p.window > 0 || seq.qn > 1);
@@ -380,14 +446,14 @@ kv4_chunk_kernel(const __grid_constant__ ChunkParams cp) {
     const int tile_last = pos0 + min(seq.qn - 1, (row0 + kTileRows * t + kTileRows - 1) / p.group);
     float m = -INFINITY, l = 0.0f;
     for (int i = 0; i < n; i++) {
-      if (!__all_sync(0xffffffffu, pkv_mbar_wait(&bar.s_full[t], i & 1))) {
+      if (!__all_sync(0xffffffffu, pkv_mbar_wait(&bar.s_full[t][i & 1], (i >> 1) & 1))) {
         fine = false;
         break;
       }
       pkv_tc::fence_after_sync();
+      const uint32_t s_at = base + Y::S + 64u * (i & 1);
       float x[2][32];
-      pkv_tc::tmem_load32(base + Y::S, x[0]);
-      pkv_tc::tmem_load32(base + Y::S + 32, x[1]);
+      tmem_load64(s_at, x);
       const int token0 = span.unit(first + i) * kUnitTokens;
       const unsigned quad = s_quad[i % kQuadSlots];
       float fac = factor;
@@ -409,48 +475,51 @@ kv4_chunk_kernel(const __grid_constant__ ChunkParams cp) {
 #pragma unroll
       for (int c = 1; c < 64; c++) top = fmaxf(top, x[c >> 5][c & 31]);
       top = __fmul_rn(top, fac);
-      // the sums up to the unit before are complete (their product was issued a whole turn ago)
-      if (i > 0 && !__all_sync(0xffffffffu, pkv_mbar_wait(&bar.o_done[t], (i - 1) & 1))) {
-        fine = false;
-        break;
-      }
-      if (__any_sync(0xffffffffu, top > __fadd_rn(m, kLag))) {
+      const bool raise = __any_sync(0xffffffffu, top > __fadd_rn(m, kLag));
+      float f = 1.0f;
+      if (raise) {
         const float raised = fmaxf(m, top);
-        const float f = m == -INFINITY ? 0.0f : exp2_fast(__fsub_rn(m, raised));
+        f = m == -INFINITY ? 0.0f : exp2_fast(__fsub_rn(m, raised));
         m = raised;
         l = __fmul_rn(l, f);
-        if (i > 0) {
-          pkv_tc::fence_after_sync();
-#pragma unroll 1
-          for (int c = 0; c < D; c += 8) {
-            float o[8];
-            pkv_tc::tmem_load<8>(base + Y::O + c, o);
-            uint32_t r[8];
-#pragma unroll
-            for (int j = 0; j < 8; j++) r[j] = __float_as_uint(__fmul_rn(o[j], f));
-            tmem_store8(base + Y::O + c, r);
-          }
-        }
       }
       const float shift = m == -INFINITY ? 0.0f : __fsub_rn(kWeightShift, m);
-      float sum[2] = {0.0f, 0.0f};
+      float2 sum = make_float2(0.0f, 0.0f);
 #pragma unroll
       for (int c = 0; c < 64; c += 16) {
         uint32_t r[8];
 #pragma unroll
         for (int j = 0; j < 8; j++) {
-          const float w0 = exp2_fast(__fmaf_rn(x[c >> 5][(c & 31) + 2 * j], fac, shift));
-          const float w1 = exp2_fast(__fmaf_rn(x[c >> 5][(c & 31) + 2 * j + 1], fac, shift));
-          sum[0] = __fadd_rn(sum[0], w0);
-          sum[1] = __fadd_rn(sum[1], w1);
-          r[j] = half2_of(w0, w1);
+          float2 w = fma2_f32(make_float2(x[c >> 5][(c & 31) + 2 * j], x[c >> 5][(c & 31) + 2 * j + 1]), make_float2(fac, fac),
+                              make_float2(shift, shift));
+          w.x = exp2_fast(w.x);
+          w.y = exp2_fast(w.y);
+          sum = add2_f32(sum, w);
+          r[j] = half2_of(w.x, w.y);
         }
-        tmem_store8(base + Y::S + c / 2, r);
+        tmem_store8(s_at + c / 2, r);
       }
-      l = __fadd_rn(l, __fadd_rn(sum[0], sum[1]));
+      l = __fadd_rn(l, __fadd_rn(sum.x, sum.y));
+      // the sums up to the unit before are complete (their product was issued a turn ago)
+      if (i > 0 && !__all_sync(0xffffffffu, pkv_mbar_wait(&bar.o_done[t], (i - 1) & 1))) {
+        fine = false;
+        break;
+      }
+      if (raise && i > 0) {
+        pkv_tc::fence_after_sync();
+#pragma unroll 1
+        for (int c = 0; c < D; c += 8) {
+          float o[8];
+          pkv_tc::tmem_load<8>(base + Y::O + c, o);
+          uint32_t r[8];
+#pragma unroll
+          for (int j = 0; j < 8; j++) r[j] = __float_as_uint(__fmul_rn(o[j], f));
+          tmem_store8(base + Y::O + c, r);
+        }
+      }
       tmem_store_wait();
       pkv_tc::fence_before_sync();
-      arrive(&bar.p_full[t]);
+      arrive(&bar.p_full[t][i & 1]);
     }
     if (fine && n > 0) fine = __all_sync(0xffffffffu, pkv_mbar_wait(&bar.o_done[t], (n - 1) & 1));
     pkv_tc::fence_after_sync();
