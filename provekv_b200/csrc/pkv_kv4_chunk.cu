@@ -471,10 +471,14 @@ kv4_chunk_kernel(const __grid_constant__ ChunkParams cp) {
           x[c >> 5][c & 31] = see ? __fmul_rn(x[c >> 5][c & 31], factor) : -INFINITY;
         }
       }
-      float top = x[0][0];
+      float tops[4];  // four chains, their latencies side by side
 #pragma unroll
-      for (int c = 1; c < 64; c++) top = fmaxf(top, x[c >> 5][c & 31]);
-      top = __fmul_rn(top, fac);
+      for (int c = 0; c < 4; c++) tops[c] = fmaxf(x[0][c], x[0][c + 4]);
+#pragma unroll
+      for (int c = 8; c < 64; c += 8)
+#pragma unroll
+        for (int j = 0; j < 4; j++) tops[j] = fmaxf(tops[j], fmaxf(x[c >> 5][(c & 31) + j], x[c >> 5][(c & 31) + j + 4]));
+      const float top = __fmul_rn(fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])), fac);
       const bool raise = __any_sync(0xffffffffu, top > __fadd_rn(m, kLag));
       float f = 1.0f;
       if (raise) {
@@ -484,7 +488,7 @@ kv4_chunk_kernel(const __grid_constant__ ChunkParams cp) {
         l = __fmul_rn(l, f);
       }
       const float shift = m == -INFINITY ? 0.0f : __fsub_rn(kWeightShift, m);
-      float2 sum = make_float2(0.0f, 0.0f);
+      float2 sums[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
 #pragma unroll
       for (int c = 0; c < 64; c += 16) {
         uint32_t r[8];
@@ -494,11 +498,12 @@ kv4_chunk_kernel(const __grid_constant__ ChunkParams cp) {
                               make_float2(shift, shift));
           w.x = exp2_fast(w.x);
           w.y = exp2_fast(w.y);
-          sum = add2_f32(sum, w);
+          sums[j & 1] = add2_f32(sums[j & 1], w);
           r[j] = half2_of(w.x, w.y);
         }
         tmem_store8(s_at + c / 2, r);
       }
+      const float2 sum = add2_f32(sums[0], sums[1]);
       l = __fadd_rn(l, __fadd_rn(sum.x, sum.y));
       // the sums up to the unit before are complete (their product was issued a turn ago)
       if (i > 0 && !__all_sync(0xffffffffu, pkv_mbar_wait(&bar.o_done[t], (i - 1) & 1))) {
