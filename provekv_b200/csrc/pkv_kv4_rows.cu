@@ -1,16 +1,17 @@
 // Writing vectors into the 4-bit KV cache and reading them back.
 //
-// A thread owns one block of 16 channels of a token's key and of its value: the block's largest magnitude needs
-// no other thread, and both loads are in flight together.  A CTA covers 128 / (D / 16) tokens of one kv head, so that
-// its code and scale bytes form contiguous runs.  Both kernels are bound by HBM: a vector is read once and written
-// once.
+// Append: a thread owns one block of 16 channels of a token's key and of its value, so that the block's largest
+// magnitude needs no other thread and both loads are in flight together.  A CTA covers 128 / (D / 16) tokens of one kv head,
+// whose code and scale bytes form contiguous runs.
+// Read: a thread owns 16 bytes of the output, so that a warp's stores are contiguous.
+// Both kernels are bound by HBM: a vector is read once and written once.
 #include "pkv_kv4.cuh"
 
 using namespace pkv_kv4;
 
 namespace {
 
-constexpr int kThreads = 128;
+constexpr int kThreads = 128, kReadThreads = 256;
 
 // The nearest scale to amax / 7 (ties to the even code), as its byte; 256 if it is beyond kMaxScaleByte.  Decided
 // on exact products: the candidate below an approximate quotient, then amax against 7 x the midpoint above it.
@@ -36,21 +37,38 @@ __device__ __forceinline__ float scale_value(uint32_t byte) {
   return __half2float(__ushort_as_half((unsigned short)(byte << 7)));
 }
 
+// x / s to the nearest integer (ties to even), decided on the exact remainder, as 8 code bytes.
+__device__ __noinline__ uint2 codes_exactly(const float* x, float s) {
+  uint32_t w[2] = {0u, 0u};
+  const float r = __frcp_rn(s), half = __fmul_rn(0.5f, s);
+  for (int i = 0; i < 16; i++) {
+    const float q = rintf(fminf(fmaxf(__fmul_rn(x[i], r), -8.0f), 7.0f));
+    const float rest = __fmaf_rn(-q, s, x[i]);
+    const int qi = (int)q, odd = qi & 1;
+    const int up = rest > half || (rest == half && odd) ? 1 : 0;
+    const int down = rest < -half || (rest == -half && odd) ? 1 : 0;
+    w[i >> 3] |= (uint32_t)(min(7, max(-8, qi + up - down)) + 8) << (4 * (i & 7));
+  }
+  return make_uint2(w[0], w[1]);
+}
+
 // 16 channels -> 8 code bytes and the scale byte; false if they cannot be stored.
+//
+// With a scale of full precision (byte 8 and up) amax / s is below 7.44, so no quotient needs clamping.  x / s is rounded by
+// adding 1.5 x 2^23 + 8, which leaves n in the lowest byte of the sum's bits.  What the approximate reciprocal could spoil:
+//   16-bit types  at most 11 significant bits over 4: a quotient that is no tie is at least 2^-13 away from one, so rounding
+//                 it to a multiple of 2^-15 first (the sum with 384) restores exact ties and moves nothing across one;
+//   f32           a block with a quotient within 2^-16 of a tie (the quotient's error is below 2^-19) is done exactly.
 template <int T>
 __device__ __forceinline__ bool quantise(const float (&x)[16], uint2& codes, uint32_t& byte, int& why) {
-  float amax = 0.0f;
-  bool finite = true;
+  uint32_t top = 0u;  // magnitudes order like their bits, infinities and NaN above the finite ones
 #pragma unroll
-  for (int i = 0; i < 16; i++) {
-    finite = finite && pkv_finite(x[i]);
-    amax = fmaxf(amax, fabsf(x[i]));
-  }
-  if (!finite) {
+  for (int i = 0; i < 16; i++) top = max(top, __float_as_uint(x[i]) & 0x7fffffffu);
+  if (top >= 0x7f800000u) {
     why = PKV_VEC_NONFINITE_INPUT;
     return false;
   }
-  byte = scale_byte(amax);
+  byte = scale_byte(__uint_as_float(top));
   if (byte > 255u) {
     why = PKV_VEC_NORM_RANGE;
     return false;
@@ -60,26 +78,30 @@ __device__ __forceinline__ bool quantise(const float (&x)[16], uint2& codes, uin
     return true;
   }
   const float s = scale_value(byte), r = __frcp_rn(s);
-  uint32_t w[2] = {0u, 0u};
+  constexpr float kMagic = 12582912.0f + 8.0f;
+  uint32_t n[16];
+  float worst = byte < 8u ? 1.0f : 0.0f;  // the largest distance of a quotient from its integer
 #pragma unroll
   for (int i = 0; i < 16; i++) {
-    uint32_t n;
     if constexpr (T == PKV_DST_F32) {
-      // x / s to the nearest integer, decided on the exact remainder (an f32 quotient can round onto a tie)
-      const float q = rintf(fminf(fmaxf(__fmul_rn(x[i], r), -8.0f), 7.0f));
-      const float rest = __fmaf_rn(-q, s, x[i]), half = __fmul_rn(0.5f, s);
-      const int qi = (int)q, odd = qi & 1;
-      int up = rest > half || (rest == half && odd) ? 1 : 0;
-      int down = rest < -half || (rest == -half && odd) ? 1 : 0;
-      n = (uint32_t)(min(7, max(-8, qi + up - down)) + 8);
+      const float q = __fmul_rn(x[i], r), rounded = __fadd_rn(q, kMagic);
+      n[i] = __float_as_uint(rounded);
+      worst = fmaxf(worst, fabsf(__fsub_rn(q, __fsub_rn(rounded, kMagic))));
     } else {
-      // At most 11 significant bits over 4: a quotient that is no tie is at least 2^-13 away from one, so rounding it to
-      // a multiple of 2^-15 first (the sum with 384) restores exact ties and moves nothing across one.
-      const float q = fminf(fmaxf(__fmul_rn(x[i], r), -8.0f), 7.0f);
-      const float near = __fadd_rn(q, 384.0f);
-      n = __float_as_uint(__fadd_rn(near, 12582912.0f + 8.0f - 384.0f)) & 15u;
+      n[i] = __float_as_uint(__fadd_rn(__fmaf_rn(x[i], r, 384.0f), kMagic - 384.0f));
     }
-    w[i >> 3] |= n << (4 * (i & 7));
+  }
+  if (worst > 0.5f - 1.52587890625e-05f) {
+    codes = codes_exactly(x, s);
+    return true;
+  }
+  uint32_t w[2];
+#pragma unroll
+  for (int h = 0; h < 2; h++) {  // two codes a byte, four bytes a word; what is above the lowest byte falls away
+    uint32_t b[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) b[i] = n[8 * h + 2 * i + 1] * 16u + n[8 * h + 2 * i];
+    w[h] = __byte_perm(__byte_perm(b[0], b[1], 0x0040), __byte_perm(b[2], b[3], 0x0040), 0x5410);
   }
   codes = make_uint2(w[0], w[1]);
   return true;
@@ -109,11 +131,11 @@ kv4_append_kernel(Cache c, const typename PkvDst<T>::type* __restrict__ k, Rows 
   const int s = blockIdx.z, h = blockIdx.y;
   const int i = blockIdx.x * TOK + threadIdx.x / A::SROW;
   if (i >= kr.n) return;
+  int slot, position;
+  if (!row_slot(c, s, i, kr.n, new_lens, err, &slot, &position)) return;  // (padding is not fetched)
   float x[2][16];
   load_f32<T, 16>(k + s * kr.seq + i * kr.token + h * kr.head + 16 * b, x[0]);
   load_f32<T, 16>(v + s * vr.seq + i * vr.token + h * vr.head + 16 * b, x[1]);
-  int slot, position;
-  if (!row_slot(c, s, i, kr.n, new_lens, err, &slot, &position)) return;
   uint8_t* atom = c.atom(s, h, slot / kAtomTokens, A::BYTES, err);
   if (!atom) return;
   const int t = slot % kAtomTokens;
@@ -141,40 +163,61 @@ kv4_append_kernel(Cache c, const typename PkvDst<T>::type* __restrict__ k, Rows 
 }
 
 template <int D, int T>
-__global__ void __launch_bounds__(kThreads)
+struct ReadShape {
+  static constexpr int N = T == PKV_DST_F32 ? 4 : 8;   // channels of a 16-byte piece
+  static constexpr int PIECES = D / N;                 // of a row
+  static constexpr int ROWS = kReadThreads / PIECES;   // tokens a CTA covers at once
+  static constexpr int TURNS = 4;                      // tokens a thread has in flight
+};
+template <int D, int T>
+__global__ void __launch_bounds__(kReadThreads)
 kv4_read_kernel(Cache c, typename PkvDst<T>::type* __restrict__ k, Rows kr, typename PkvDst<T>::type* __restrict__ v,
                 Rows vr, const int32_t* __restrict__ new_lens, int clear_rest, uint64_t* err) {
   using A = Atom<D>;
-  constexpr int TOK = kThreads / A::SROW;
-  const int b = threadIdx.x % A::SROW;
+  using R = ReadShape<D, T>;
+  constexpr int N = R::N;
+  const int piece = threadIdx.x % R::PIECES;
   const int s = blockIdx.z, h = blockIdx.y;
-  const int i = blockIdx.x * TOK + threadIdx.x / A::SROW;
-  if (i >= kr.n) return;
-  int slot = 0, position;
-  const bool live = row_slot(c, s, i, kr.n, new_lens, err, &slot, &position);
-  const uint8_t* atom = live ? c.atom(s, h, slot / kAtomTokens, A::BYTES, err) : nullptr;
-  if (!atom) {
-    if (clear_rest) {
-      float x[16];
+  const int i0 = blockIdx.x * R::ROWS * R::TURNS + threadIdx.x / R::PIECES;
+  uint32_t codes[R::TURNS][2], scale[R::TURNS][2];
 #pragma unroll
-      for (int j = 0; j < 16; j++) x[j] = 0.0f;
-      store_f32<T, 16>(k + s * kr.seq + i * kr.token + h * kr.head + 16 * b, x);
-      store_f32<T, 16>(v + s * vr.seq + i * vr.token + h * vr.head + 16 * b, x);
+  for (int u = 0; u < R::TURNS; u++) {
+    const int i = i0 + u * R::ROWS;
+    int slot = 0, position;
+    codes[u][0] = codes[u][1] = scale[u][0] = scale[u][1] = 0u;
+    const bool live = i < kr.n && row_slot(c, s, i, kr.n, new_lens, err, &slot, &position);
+    const uint8_t* atom = live ? c.atom(s, h, slot / kAtomTokens, A::BYTES, err) : nullptr;
+    if (!atom) {
+      if (!clear_rest || i >= kr.n) scale[u][0] = 0x100u;  // nothing to write
+      continue;
     }
-    return;
+    const int t = slot % kAtomTokens, at = piece * N / 2;
+    const uint8_t* kc = atom + A::KC + t * A::ROW + at;
+    const uint8_t* vc = atom + A::VC + t * A::ROW + (at ^ A::vswap(t));
+    if constexpr (N == 8) {
+      codes[u][0] = *reinterpret_cast<const uint32_t*>(kc);
+      codes[u][1] = *reinterpret_cast<const uint32_t*>(vc);
+    } else {
+      codes[u][0] = *reinterpret_cast<const uint16_t*>(kc);
+      codes[u][1] = *reinterpret_cast<const uint16_t*>(vc);
+    }
+    scale[u][0] = atom[A::KS + t * A::SROW + piece * N / 16];
+    scale[u][1] = atom[A::VS + t * A::SROW + piece * N / 16];
   }
-  const int t = slot % kAtomTokens;
 #pragma unroll
-  for (int side = 0; side < 2; side++) {
-    const int at = side ? A::VC + t * A::ROW + ((8 * b) ^ A::vswap(t)) : A::KC + t * A::ROW + 8 * b;
-    const uint2 codes = *reinterpret_cast<const uint2*>(atom + at);
-    const float scale = scale_value(atom[(side ? A::VS : A::KS) + t * A::SROW + b]);
-    float x[16];
+  for (int u = 0; u < R::TURNS; u++) {
+    const int i = i0 + u * R::ROWS;
+    if (scale[u][0] == 0x100u) continue;
 #pragma unroll
-    for (int j = 0; j < 16; j++)
-      x[j] = __fmul_rn((float)((int)(((j < 8 ? codes.x : codes.y) >> (4 * (j & 7))) & 15u) - 8), scale);
-    if (side == 0) store_f32<T, 16>(k + s * kr.seq + i * kr.token + h * kr.head + 16 * b, x);
-    else store_f32<T, 16>(v + s * vr.seq + i * vr.token + h * vr.head + 16 * b, x);
+    for (int side = 0; side < 2; side++) {
+      const float f = scale_value(scale[u][side]);
+      float x[N];
+#pragma unroll
+      for (int j = 0; j < N; j++)  // 2^23 + n as bits, less 2^23 + 8
+        x[j] = __fmul_rn(__fadd_rn(__uint_as_float(((codes[u][side] >> (4 * j)) & 15u) | 0x4b000000u), -8388616.0f), f);
+      if (side == 0) store_f32<T, N>(k + s * kr.seq + i * kr.token + h * kr.head + piece * N, x);
+      else store_f32<T, N>(v + s * vr.seq + i * vr.token + h * vr.head + piece * N, x);
+    }
   }
 }
 
@@ -182,13 +225,14 @@ template <int D, int T>
 void launch_rows(bool append, const Cache& c, const void* k, const Rows& kr, const void* v, const Rows& vr,
                  const int32_t* new_lens, int clear_rest, uint64_t* err, cudaStream_t s) {
   using E = typename PkvDst<T>::type;
-  constexpr int TOK = kThreads / Atom<D>::SROW;
-  const dim3 grid((unsigned)((kr.n + TOK - 1) / TOK), (unsigned)c.heads, (unsigned)c.n_seqs);
+  constexpr int TOK = kThreads / Atom<D>::SROW, READ = ReadShape<D, T>::ROWS * ReadShape<D, T>::TURNS;
+  const int per = append ? TOK : READ;
+  const dim3 grid((unsigned)((kr.n + per - 1) / per), (unsigned)c.heads, (unsigned)c.n_seqs);
   if (append)
     kv4_append_kernel<D, T><<<grid, kThreads, 0, s>>>(c, (const E*)k, kr, (const E*)v, vr, new_lens, err);
   else
-    kv4_read_kernel<D, T><<<grid, kThreads, 0, s>>>(c, (E*)const_cast<void*>(k), kr, (E*)const_cast<void*>(v), vr, new_lens,
-                                                clear_rest, err);
+    kv4_read_kernel<D, T><<<grid, kReadThreads, 0, s>>>(c, (E*)const_cast<void*>(k), kr, (E*)const_cast<void*>(v), vr, new_lens,
+                                                        clear_rest, err);
 }
 
 int rows_call(bool append, const pkv_kv4_cache* cache, const void* k, const pkv_kv4_rows* k_rows, const void* v,
