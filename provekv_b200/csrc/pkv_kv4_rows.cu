@@ -107,58 +107,145 @@ __device__ __forceinline__ bool quantise(const float (&x)[16], uint2& codes, uin
   return true;
 }
 
-// Where row i of a call goes; false if it is not one of the sequence's.
-__device__ __forceinline__ bool row_slot(const Cache& c, int s, int i, int n_tokens, const int32_t* new_lens, uint64_t* err,
-                                         int* slot, int* position) {
+// The rows of a sequence in a call: row i < fresh goes to slot first + i, whose token has position `position` + i.
+struct Fresh {
+  int fresh, first, position;
+};
+__device__ __forceinline__ Fresh fresh_of(const Cache& c, int s, int n_tokens, const int32_t* new_lens, uint64_t* err) {
+  Fresh r;
   const int n = c.length(s, err);
-  const int fresh = new_lens ? new_lens[s] : n_tokens;
-  if (fresh < 0 || fresh > n_tokens || fresh > n) {
+  r.fresh = new_lens ? new_lens[s] : n_tokens;
+  if (r.fresh < 0 || r.fresh > n_tokens || r.fresh > n) {
     pkv_report(err, 0, s, PKV_VEC_BAD_SEQUENCE);
-    return false;
+    r.fresh = 0;
   }
-  *slot = n - fresh + i;
-  *position = c.end(s, n) - fresh + i;
-  return i < fresh;
+  r.first = n - r.fresh;
+  r.position = c.end(s, n) - r.fresh;
+  return r;
 }
+
+// 16 values as they lie in memory, and as f32.
+template <int T>
+struct Raw {
+  static constexpr int N = T == PKV_DST_F32 ? 4 : 2;
+  uint4 v[N];
+  __device__ __forceinline__ void load(const typename PkvDst<T>::type* p) {
+#pragma unroll
+    for (int i = 0; i < N; i++) v[i] = __ldg(reinterpret_cast<const uint4*>(p) + i);
+  }
+  __device__ __forceinline__ void to_f32(float (&x)[16]) const {
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+      const uint32_t w[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
+#pragma unroll
+      for (int j = 0; j < 4; j++) {
+        if constexpr (T == PKV_DST_F32) {
+          x[4 * i + j] = __uint_as_float(w[j]);
+        } else if constexpr (T == PKV_DST_F16) {
+          const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[j]));
+          x[8 * i + 2 * j] = f.x;
+          x[8 * i + 2 * j + 1] = f.y;
+        } else {  // a bfloat16 is the upper half of an f32
+          x[8 * i + 2 * j] = __uint_as_float(w[j] << 16);
+          x[8 * i + 2 * j + 1] = __uint_as_float(w[j] & 0xffff0000u);
+        }
+      }
+    }
+  }
+};
+
+// Tokens a thread has in flight: 128 bytes of loads in either case.
+template <int T>
+constexpr int kAppendTurns = T == PKV_DST_F32 ? 1 : 2;
 
 template <int D, int T>
 __global__ void __launch_bounds__(kThreads)
 kv4_append_kernel(Cache c, const typename PkvDst<T>::type* __restrict__ k, Rows kr,
                   const typename PkvDst<T>::type* __restrict__ v, Rows vr, const int32_t* __restrict__ new_lens, uint64_t* err) {
   using A = Atom<D>;
-  constexpr int TOK = kThreads / A::SROW;
+  constexpr int TOK = kThreads / A::SROW, TURNS = kAppendTurns<T>;
   const int b = threadIdx.x % A::SROW;  // block of 16 channels
   const int s = blockIdx.z, h = blockIdx.y;
-  const int i = blockIdx.x * TOK + threadIdx.x / A::SROW;
-  if (i >= kr.n) return;
-  int slot, position;
-  if (!row_slot(c, s, i, kr.n, new_lens, err, &slot, &position)) return;  // (padding is not fetched)
-  float x[2][16];
-  load_f32<T, 16>(k + s * kr.seq + i * kr.token + h * kr.head + 16 * b, x[0]);
-  load_f32<T, 16>(v + s * vr.seq + i * vr.token + h * vr.head + 16 * b, x[1]);
-  uint8_t* atom = c.atom(s, h, slot / kAtomTokens, A::BYTES, err);
-  if (!atom) return;
-  const int t = slot % kAtomTokens;
+  const int i0 = blockIdx.x * TOK * TURNS + threadIdx.x / A::SROW;
   const unsigned row_lanes = ((1u << A::SROW) - 1u) << ((threadIdx.x & 31) / A::SROW * A::SROW);
+  Raw<T> raw[TURNS][2];
+  uint8_t* atom[TURNS];
+  const Fresh f = fresh_of(c, s, kr.n, new_lens, err);
+  k += s * kr.seq + h * kr.head + 16 * b;
+  v += s * vr.seq + h * vr.head + 16 * b;
 #pragma unroll
-  for (int side = 0; side < 2; side++) {
-    uint2 codes = make_uint2(0u, 0u);
-    uint32_t byte = 0u;
-    int why = 0;
-    const bool ok = quantise<T>(x[side], codes, byte, why);
-    // one block that cannot be stored empties the whole row; the row's threads are neighbours in a warp
-    if (!__all_sync(row_lanes, ok)) {
-      codes = make_uint2(0u, 0u);
-      byte = 0u;
-      if (!ok) pkv_report(err, 0, (((int64_t)s * kr.n + i) * c.heads + h) * 2 + side, why);
+  for (int u = 0; u < TURNS; u++) {
+    const int i = i0 + u * TOK;
+    atom[u] = nullptr;
+    if (i < f.fresh) {  // (padding is not fetched)
+      raw[u][0].load(k + i * kr.token);
+      raw[u][1].load(v + i * vr.token);
+      atom[u] = c.atom(s, h, (f.first + i) / kAtomTokens, A::BYTES, err);
     }
-    const int at = side ? A::VC + t * A::ROW + ((8 * b) ^ A::vswap(t)) : A::KC + t * A::ROW + 8 * b;
-    *reinterpret_cast<uint2*>(atom + at) = codes;
-    atom[(side ? A::VS : A::KS) + t * A::SROW + b] = (uint8_t)byte;
   }
-  if (b == 0) {
-    if (c.positions) c.positions[c.stat(s, h) + slot] = position;
-    if (c.mass) c.mass[c.stat(s, h) + slot] = 0.0f;
+#pragma unroll
+  for (int u = 0; u < TURNS; u++) {
+    if (!atom[u]) continue;
+    const int slot = f.first + i0 + u * TOK, t = slot % kAtomTokens;
+#pragma unroll
+    for (int side = 0; side < 2; side++) {
+      float x[16];
+      raw[u][side].to_f32(x);
+      uint2 codes = make_uint2(0u, 0u);
+      uint32_t byte = 0u;
+      int why = 0;
+      const bool ok = quantise<T>(x, codes, byte, why);
+      // one block that cannot be stored empties the whole row; the row's threads are neighbours in a warp
+      if (!__all_sync(row_lanes, ok)) {
+        codes = make_uint2(0u, 0u);
+        byte = 0u;
+        if (!ok) pkv_report(err, 0, (((int64_t)s * kr.n + i0 + u * TOK) * c.heads + h) * 2 + side, why);
+      }
+      const int at = side ? A::VC + t * A::ROW + ((8 * b) ^ A::vswap(t)) : A::KC + t * A::ROW + 8 * b;
+      *reinterpret_cast<uint2*>(atom[u] + at) = codes;
+      atom[u][(side ? A::VS : A::KS) + t * A::SROW + b] = (uint8_t)byte;
+    }
+    if (b == 0) {
+      if (c.positions) c.positions[c.stat(s, h) + slot] = f.position + i0 + u * TOK;
+      if (c.mass) c.mass[c.stat(s, h) + slot] = 0.0f;
+    }
+  }
+}
+
+// 16 bytes of output from their codes (16 or 32 bits) and scale.
+template <int T>
+__device__ __forceinline__ uint4 values_of(uint32_t w, uint32_t byte) {
+  if constexpr (T == PKV_DST_F32) {
+    const float f = scale_value(byte);
+    float x[4];
+#pragma unroll
+    for (int j = 0; j < 4; j++)  // 2^23 + n as bits, less 2^23 + 8
+      x[j] = __fmul_rn(__fadd_rn(__uint_as_float(and_or(w >> (4 * j), 15u, 0x4b000000u)), -8388616.0f), f);
+    return make_uint4(__float_as_uint(x[0]), __float_as_uint(x[1]), __float_as_uint(x[2]), __float_as_uint(x[3]));
+  } else {
+    uint32_t p[4];  // channels (j, j + 4)
+    if constexpr (T == PKV_DST_F16) {
+      // 1024 + n as bits, less 1032, times s: every step exact
+      const uint32_t s2 = byte * 0x00800080u;
+#pragma unroll
+      for (int j = 0; j < 4; j++) {
+        const uint32_t u = and_or(w >> (4 * j), 0x000f000fu, 0x64006400u);
+        const __half2 d = __hadd2(*reinterpret_cast<const __half2*>(&u), __float2half2_rn(-1032.0f));
+        const __half2 r = __hmul2(d, *reinterpret_cast<const __half2*>(&s2));
+        p[j] = *reinterpret_cast<const uint32_t*>(&r);
+      }
+    } else {
+      const __nv_bfloat162 s2 = __float2bfloat162_rn(scale_value(byte));
+#pragma unroll
+      for (int j = 0; j < 4; j++) {  // 128 + n as bits, less 136, times s
+        const uint32_t u = and_or(w >> (4 * j), 0x000f000fu, 0x43004300u);
+        const __nv_bfloat162 d = __hadd2(*reinterpret_cast<const __nv_bfloat162*>(&u), __float2bfloat162_rn(-136.0f));
+        const __nv_bfloat162 r = __hmul2(d, s2);
+        p[j] = *reinterpret_cast<const uint32_t*>(&r);
+      }
+    }
+    return make_uint4(__byte_perm(p[0], p[1], 0x5410), __byte_perm(p[2], p[3], 0x5410), __byte_perm(p[0], p[1], 0x7632),
+                      __byte_perm(p[2], p[3], 0x7632));
   }
 }
 
@@ -179,18 +266,17 @@ kv4_read_kernel(Cache c, typename PkvDst<T>::type* __restrict__ k, Rows kr, type
   const int piece = threadIdx.x % R::PIECES;
   const int s = blockIdx.z, h = blockIdx.y;
   const int i0 = blockIdx.x * R::ROWS * R::TURNS + threadIdx.x / R::PIECES;
+  const Fresh f = fresh_of(c, s, kr.n, new_lens, err);
+  k += s * kr.seq + h * kr.head + piece * N;
+  v += s * vr.seq + h * vr.head + piece * N;
   uint32_t codes[R::TURNS][2], scale[R::TURNS][2];
+  bool live[R::TURNS];
 #pragma unroll
   for (int u = 0; u < R::TURNS; u++) {
-    const int i = i0 + u * R::ROWS;
-    int slot = 0, position;
-    codes[u][0] = codes[u][1] = scale[u][0] = scale[u][1] = 0u;
-    const bool live = i < kr.n && row_slot(c, s, i, kr.n, new_lens, err, &slot, &position);
-    const uint8_t* atom = live ? c.atom(s, h, slot / kAtomTokens, A::BYTES, err) : nullptr;
-    if (!atom) {
-      if (!clear_rest || i >= kr.n) scale[u][0] = 0x100u;  // nothing to write
-      continue;
-    }
+    const int i = i0 + u * R::ROWS, slot = f.first + i;
+    const uint8_t* atom = i < f.fresh ? c.atom(s, h, slot / kAtomTokens, A::BYTES, err) : nullptr;
+    live[u] = atom != nullptr;
+    if (!live[u]) continue;
     const int t = slot % kAtomTokens, at = piece * N / 2;
     const uint8_t* kc = atom + A::KC + t * A::ROW + at;
     const uint8_t* vc = atom + A::VC + t * A::ROW + (at ^ A::vswap(t));
@@ -207,17 +293,15 @@ kv4_read_kernel(Cache c, typename PkvDst<T>::type* __restrict__ k, Rows kr, type
 #pragma unroll
   for (int u = 0; u < R::TURNS; u++) {
     const int i = i0 + u * R::ROWS;
-    if (scale[u][0] == 0x100u) continue;
-#pragma unroll
-    for (int side = 0; side < 2; side++) {
-      const float f = scale_value(scale[u][side]);
-      float x[N];
-#pragma unroll
-      for (int j = 0; j < N; j++)  // 2^23 + n as bits, less 2^23 + 8
-        x[j] = __fmul_rn(__fadd_rn(__uint_as_float(((codes[u][side] >> (4 * j)) & 15u) | 0x4b000000u), -8388616.0f), f);
-      if (side == 0) store_f32<T, N>(k + s * kr.seq + i * kr.token + h * kr.head + piece * N, x);
-      else store_f32<T, N>(v + s * vr.seq + i * vr.token + h * vr.head + piece * N, x);
+    uint4 out[2] = {make_uint4(0u, 0u, 0u, 0u), make_uint4(0u, 0u, 0u, 0u)};
+    if (live[u]) {
+      out[0] = values_of<T>(codes[u][0], scale[u][0]);
+      out[1] = values_of<T>(codes[u][1], scale[u][1]);
+    } else if (!clear_rest || i >= kr.n) {
+      continue;
     }
+    *reinterpret_cast<uint4*>(k + i * kr.token) = out[0];
+    *reinterpret_cast<uint4*>(v + i * vr.token) = out[1];
   }
 }
 
@@ -225,7 +309,7 @@ template <int D, int T>
 void launch_rows(bool append, const Cache& c, const void* k, const Rows& kr, const void* v, const Rows& vr,
                  const int32_t* new_lens, int clear_rest, uint64_t* err, cudaStream_t s) {
   using E = typename PkvDst<T>::type;
-  constexpr int TOK = kThreads / Atom<D>::SROW, READ = ReadShape<D, T>::ROWS * ReadShape<D, T>::TURNS;
+  constexpr int TOK = kThreads / Atom<D>::SROW * kAppendTurns<T>, READ = ReadShape<D, T>::ROWS * ReadShape<D, T>::TURNS;
   const int per = append ? TOK : READ;
   const dim3 grid((unsigned)((kr.n + per - 1) / per), (unsigned)c.heads, (unsigned)c.n_seqs);
   if (append)
