@@ -37,11 +37,16 @@ __device__ __forceinline__ float scale_value(uint32_t byte) {
   return __half2float(__ushort_as_half((unsigned short)(byte << 7)));
 }
 
-// x / s to the nearest integer (ties to even), decided on the exact remainder, as 8 code bytes.
-__device__ __noinline__ uint2 codes_exactly(const float* x, float s) {
+// A block done step by step, every decision on exact values: (codes, codes, scale byte or 256).
+__device__ __forceinline__ uint3 quantise_exactly(const float (&x)[16], float amax) {
+  const uint32_t byte = scale_byte(amax);
+  if (byte > 255u) return make_uint3(0u, 0u, 256u);
+  if (byte == 0u) return make_uint3(0x88888888u, 0x88888888u, 0u);  // below half the smallest scale: zeros (code 8)
   uint32_t w[2] = {0u, 0u};
-  const float r = __frcp_rn(s), half = __fmul_rn(0.5f, s);
-  for (int i = 0; i < 16; i++) {
+  const float s = scale_value(byte), r = __frcp_rn(s), half = __fmul_rn(0.5f, s);
+#pragma unroll
+  for (int i = 0; i < 16; i++) {  // (inline and unrolled: the values stay in registers on the common way too)
+    // x / s to the nearest integer, ties to even, by the remainder
     const float q = rintf(fminf(fmaxf(__fmul_rn(x[i], r), -8.0f), 7.0f));
     const float rest = __fmaf_rn(-q, s, x[i]);
     const int qi = (int)q, odd = qi & 1;
@@ -49,16 +54,21 @@ __device__ __noinline__ uint2 codes_exactly(const float* x, float s) {
     const int down = rest < -half || (rest == -half && odd) ? 1 : 0;
     w[i >> 3] |= (uint32_t)(min(7, max(-8, qi + up - down)) + 8) << (4 * (i & 7));
   }
-  return make_uint2(w[0], w[1]);
+  return make_uint3(w[0], w[1], byte);
 }
 
 // 16 channels -> 8 code bytes and the scale byte; false if they cannot be stored.
 //
-// With a scale of full precision (byte 8 and up) amax / s is below 7.44, so no quotient needs clamping.  x / s is rounded by
-// adding 1.5 x 2^23 + 8, which leaves n in the lowest byte of the sum's bits.  What the approximate reciprocal could spoil:
-//   16-bit types  at most 11 significant bits over 4: a quotient that is no tie is at least 2^-13 away from one, so rounding
-//                 it to a multiple of 2^-15 first (the sum with 384) restores exact ties and moves nothing across one;
-//   f32           a block with a quotient within 2^-16 of a tie (the quotient's error is below 2^-19) is done exactly.
+// The common way takes approximate quotients; what that could spoil:
+//   the scale     amax / 7 is rounded to 4 significant bits on its bits.  16-bit types: at most 11 significant bits over 7, a
+//                 quotient that is no tie is at least 2^-13 (relative) away from one, so rounding it to 18 bits first
+//                 restores exact ties and moves nothing across one.  f32: a quotient within 2^-21 of a tie (its error is below
+//                 2^-22) has the block done exactly, as does any below the scales of full precision;
+//   the codes     amax / s is below 7.44, so no quotient needs clamping.  x / s is rounded by adding 1.5 x 2^23 + 8, which
+//                 leaves n in the lowest byte of the sum's bits.  16-bit types: at most 11 significant bits over 4, no
+//                 quotient but a tie is within 2^-13 of one, and rounding to a multiple of 2^-15 first (the sum with 384)
+//                 restores those.  f32: a block with a quotient within 2^-16 of a tie (the error is below 2^-18) is done
+//                 exactly.
 template <int T>
 __device__ __forceinline__ bool quantise(const float (&x)[16], uint2& codes, uint32_t& byte, int& why) {
   uint32_t top = 0u;  // magnitudes order like their bits, infinities and NaN above the finite ones
@@ -68,19 +78,17 @@ __device__ __forceinline__ bool quantise(const float (&x)[16], uint2& codes, uin
     why = PKV_VEC_NONFINITE_INPUT;
     return false;
   }
-  byte = scale_byte(__uint_as_float(top));
-  if (byte > 255u) {
-    why = PKV_VEC_NORM_RANGE;
-    return false;
-  }
-  if (byte == 0u) {  // every value below half the smallest scale: zeros (code 8)
-    codes = make_uint2(0x88888888u, 0x88888888u);
-    return true;
-  }
-  const float s = scale_value(byte), r = __frcp_rn(s);
+  uint32_t q7 = __float_as_uint(__fmul_rn(__uint_as_float(top), 0.142857149f));
+  if constexpr (T != PKV_DST_F32) q7 = (q7 + 16u) & ~31u;
+  bool unsure = q7 < 0x38800000u;  // 2^-14
+  if constexpr (T == PKV_DST_F32) unsure = unsure || ((q7 - 0x7fffcu) & 0xfffffu) <= 8u;
+  byte = ((q7 + 0x7ffffu + ((q7 >> 20) & 1u)) >> 20) - (112u << 3);
+  const float s = __uint_as_float((byte + (112u << 3)) << 20);
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(s));
   constexpr float kMagic = 12582912.0f + 8.0f;
   uint32_t n[16];
-  float worst = byte < 8u ? 1.0f : 0.0f;  // the largest distance of a quotient from its integer
+  float worst = 0.0f;  // the largest distance of a quotient from its integer
 #pragma unroll
   for (int i = 0; i < 16; i++) {
     if constexpr (T == PKV_DST_F32) {
@@ -91,10 +99,6 @@ __device__ __forceinline__ bool quantise(const float (&x)[16], uint2& codes, uin
       n[i] = __float_as_uint(__fadd_rn(__fmaf_rn(x[i], r, 384.0f), kMagic - 384.0f));
     }
   }
-  if (worst > 0.5f - 1.52587890625e-05f) {
-    codes = codes_exactly(x, s);
-    return true;
-  }
   uint32_t w[2];
 #pragma unroll
   for (int h = 0; h < 2; h++) {  // two codes a byte, four bytes a word; what is above the lowest byte falls away
@@ -102,6 +106,20 @@ __device__ __forceinline__ bool quantise(const float (&x)[16], uint2& codes, uin
 #pragma unroll
     for (int i = 0; i < 4; i++) b[i] = n[8 * h + 2 * i + 1] * 16u + n[8 * h + 2 * i];
     w[h] = __byte_perm(__byte_perm(b[0], b[1], 0x0040), __byte_perm(b[2], b[3], 0x0040), 0x5410);
+  }
+  if (unsure || worst > 0.5f - 1.52587890625e-05f) {
+    w[0] = w[1] = 0x88888888u;
+    byte = 0u;
+    if (top != 0u) {
+      const uint3 e = quantise_exactly(x, __uint_as_float(top));
+      w[0] = e.x;
+      w[1] = e.y;
+      byte = e.z;
+    }
+  }
+  if (byte > (uint32_t)kMaxScaleByte) {
+    why = PKV_VEC_NORM_RANGE;
+    return false;
   }
   codes = make_uint2(w[0], w[1]);
   return true;
@@ -132,6 +150,10 @@ struct Raw {
   __device__ __forceinline__ void load(const typename PkvDst<T>::type* p) {
 #pragma unroll
     for (int i = 0; i < N; i++) v[i] = __ldg(reinterpret_cast<const uint4*>(p) + i);
+  }
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int i = 0; i < N; i++) v[i] = make_uint4(0u, 0u, 0u, 0u);
   }
   __device__ __forceinline__ void to_f32(float (&x)[16]) const {
 #pragma unroll
@@ -185,27 +207,31 @@ kv4_append_kernel(Cache c, const typename PkvDst<T>::type* __restrict__ k, Rows 
   }
 #pragma unroll
   for (int u = 0; u < TURNS; u++) {
-    if (!atom[u]) continue;
+    if (!__any_sync(0xffffffffu, atom[u] != nullptr)) continue;
     const int slot = f.first + i0 + u * TOK, t = slot % kAtomTokens;
 #pragma unroll
     for (int side = 0; side < 2; side++) {
       float x[16];
+      if (!atom[u]) raw[u][side].clear();
       raw[u][side].to_f32(x);
       uint2 codes = make_uint2(0u, 0u);
       uint32_t byte = 0u;
       int why = 0;
       const bool ok = quantise<T>(x, codes, byte, why);
       // one block that cannot be stored empties the whole row; the row's threads are neighbours in a warp
-      if (!__all_sync(row_lanes, ok)) {
+      const unsigned bad = __ballot_sync(0xffffffffu, !ok);
+      if (bad & row_lanes) {
         codes = make_uint2(0u, 0u);
         byte = 0u;
         if (!ok) pkv_report(err, 0, (((int64_t)s * kr.n + i0 + u * TOK) * c.heads + h) * 2 + side, why);
       }
       const int at = side ? A::VC + t * A::ROW + ((8 * b) ^ A::vswap(t)) : A::KC + t * A::ROW + 8 * b;
-      *reinterpret_cast<uint2*>(atom[u] + at) = codes;
-      atom[u][(side ? A::VS : A::KS) + t * A::SROW + b] = (uint8_t)byte;
+      if (atom[u]) {
+        *reinterpret_cast<uint2*>(atom[u] + at) = codes;
+        atom[u][(side ? A::VS : A::KS) + t * A::SROW + b] = (uint8_t)byte;
+      }
     }
-    if (b == 0) {
+    if (b == 0 && atom[u]) {
       if (c.positions) c.positions[c.stat(s, h) + slot] = f.position + i0 + u * TOK;
       if (c.mass) c.mass[c.stat(s, h) + slot] = 0.0f;
     }
