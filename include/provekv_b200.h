@@ -439,7 +439,7 @@ int pkv_tqb1_header_parse(const pkv_turbo_profile* p, const uint8_t* bytes, int6
  * all layers, before its first call.  ends[s] is the number of tokens the sequence has had (a query's position is
  * counted from it); null = lens.  positions[s][h][j] is the position of the token in a slot, below ends[s]; null = the slot's
  * own number, as long as nothing was evicted.  mass[s][h][j] is the attention weight a token has received.  Both are
- * [n_seqs][n_kv_heads][max_pages * page_tokens].
+ * [n_seqs][n_kv_heads][max_pages * page_tokens], 16-byte aligned.
  *
  * A sequence whose length is negative or above max_pages * page_tokens, or that has a page number outside [0, n_pages) among the
  * entries a call reads, is reported as PKV_VEC_BAD_SEQUENCE with its index.  A sequence with a bad length counts as empty,

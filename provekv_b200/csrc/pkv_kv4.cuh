@@ -63,7 +63,7 @@ inline int make_cache(const pkv_kv4_cache* c, Cache* out) {
   if (!c || !c->pages || !c->page_table || !c->lens || c->reserved != 0) return PKV_ERR_INVALID_ARGUMENT;
   if (c->n_pages < 0 || c->n_kv_heads < 1 || c->n_seqs < 0 || c->max_pages < 0 || c->page_tokens < 1)
     return PKV_ERR_INVALID_ARGUMENT;
-  if ((uintptr_t)c->pages & 15) return PKV_ERR_INVALID_ARGUMENT;
+  if (((uintptr_t)c->pages | (uintptr_t)c->positions | (uintptr_t)c->mass) & 15) return PKV_ERR_INVALID_ARGUMENT;
   if ((c->dim != 64 && c->dim != 128) || c->page_tokens % kAtomTokens) return PKV_ERR_UNSUPPORTED;
   // slots are 32-bit numbers with room for a tile behind the last one; sequences and heads go into grid dimensions
   if ((int64_t)c->max_pages * c->page_tokens > 0x7fff0000ll || c->n_kv_heads > 65535 || c->n_seqs > 65535)

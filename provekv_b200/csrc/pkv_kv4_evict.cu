@@ -19,6 +19,7 @@ struct EvictParams {
   Cache c;
   int budget, sinks, recent;
   int list;         // entries of each of a list's halves
+  int fused;        // 1: the first launch moves the rows too
   int shared_keys;  // 1: the keys of a sequence fit in shared memory
   int32_t* lists;   // [n_seqs][heads][2][list]: destinations, sources
   int32_t* counts;  // [n_seqs][heads]
@@ -31,21 +32,89 @@ __device__ __forceinline__ uint32_t key_of(int position, float mass, int sinks, 
   return mass > 0.0f ? __float_as_uint(mass) : 0u;
 }
 
-// THREADS: 256 for caches of a few thousand slots (eight CTAs an SM), 1024 for long ones.
-template <int THREADS>
-__global__ void __launch_bounds__(THREADS)
+// 16 lanes move a row: K codes, V codes (their halves swap places where the two slots differ in bit 1), scales,
+// position and mass.  Rows first, first + step, .. of the lists.
+template <int D, int TURNS>  // TURNS: rows that 16 lanes have in flight
+__device__ __forceinline__ void move_rows(const EvictParams& p, int s, int h, const int32_t* dst, const int32_t* src, int count, int first,
+                                          int step) {
+  using A = Atom<D>;
+  const int part = threadIdx.x & 15;
+  constexpr int PIECES = A::ROW / 16, WORDS = A::SROW / 4;  // 16-byte pieces of a code row, words of a scale row
+  const int64_t stat = p.c.stat(s, h);
+  // what this lane moves: bytes into the atom, per token, and whether the token swaps halves
+  const bool wide = part < 2 * PIECES, scale = !wide && part < 2 * PIECES + 2 * WORDS, swaps = wide && part >= PIECES;
+  int base, per_token;
+  if (wide) {
+    base = part < PIECES ? A::KC + 16 * part : A::VC;
+    per_token = A::ROW;
+  } else {
+    const int o = part - 2 * PIECES;
+    base = (o / WORDS ? A::VS : A::KS) + 4 * (o % WORDS);
+    per_token = A::SROW;
+  }
+  const int half = swaps ? 16 * (part - PIECES) : 0;
+  auto at = [&](int slot) { return base + (slot % kAtomTokens) * per_token + (swaps ? half ^ A::vswap(slot) : 0); };
+  auto page_of = [&](int slot) { return __ldg(p.c.table + (int64_t)s * p.c.max_pages + slot / p.c.page_tokens); };
+  auto atom_of = [&](int page, int slot) {
+    return p.c.pages + (((int64_t)page * p.c.heads + h) * p.c.page_atoms + slot % p.c.page_tokens / kAtomTokens) * (int64_t)A::BYTES;
+  };
+#pragma unroll 1
+  for (int i0 = first; i0 < count; i0 += step * TURNS) {
+    int from[TURNS], to[TURNS], from_page[TURNS], to_page[TURNS];
+    bool live[TURNS];
+    uint4 v[TURNS];
+    // step by step for all rows, so that their loads are in flight together
+#pragma unroll
+    for (int u = 0; u < TURNS; u++) {
+      const int i = min(i0 + step * u, count - 1);
+      live[u] = i0 + step * u < count;
+      from[u] = src[i];
+      to[u] = dst[i];
+    }
+#pragma unroll
+    for (int u = 0; u < TURNS; u++) {
+      from_page[u] = page_of(from[u]);
+      to_page[u] = page_of(to[u]);
+    }
+#pragma unroll
+    for (int u = 0; u < TURNS; u++) {
+      if (from_page[u] < 0 || from_page[u] >= p.c.n_pages || to_page[u] < 0 || to_page[u] >= p.c.n_pages) {
+        if (live[u] && part == 0) pkv_report(p.err, 0, s, PKV_VEC_BAD_SEQUENCE);
+        live[u] = false;
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < TURNS; u++) {
+      if (live[u] && wide) v[u] = *reinterpret_cast<const uint4*>(atom_of(from_page[u], from[u]) + at(from[u]));
+      if (live[u] && scale) v[u].x = *reinterpret_cast<const uint32_t*>(atom_of(from_page[u], from[u]) + at(from[u]));
+      if (live[u] && part == 14) v[u].x = (uint32_t)p.c.positions[stat + from[u]];
+      if (live[u] && part == 15) v[u].x = __float_as_uint(p.c.mass[stat + from[u]]);
+    }
+#pragma unroll
+    for (int u = 0; u < TURNS; u++) {
+      if (live[u] && wide) *reinterpret_cast<uint4*>(atom_of(to_page[u], to[u]) + at(to[u])) = v[u];
+      if (live[u] && scale) *reinterpret_cast<uint32_t*>(atom_of(to_page[u], to[u]) + at(to[u])) = v[u].x;
+      if (live[u] && part == 14) p.c.positions[stat + to[u]] = (int32_t)v[u].x;
+      if (live[u] && part == 15) p.c.mass[stat + to[u]] = __uint_as_float(v[u].x);
+    }
+  }
+}
+
+// THREADS: 256 for caches of a few thousand slots (several CTAs an SM), 1024 for long ones.
+template <int D, int THREADS>
+__global__ void __launch_bounds__(THREADS, THREADS == 256 ? 6 : 1)
 kv4_select_kernel(const __grid_constant__ EvictParams p) {
   constexpr int WARPS = THREADS / 32, PER = kBins / THREADS;
   extern __shared__ uint32_t s_keys[];
   __shared__ uint32_t s_hist[kBins];
   __shared__ uint32_t s_warp[2][WARPS];
-  __shared__ uint32_t s_pick[2];  // digit, how many are left to take within it
+  __shared__ uint32_t s_pick[3];  // digit, how many are left to take within it, how many there are
   const int h = blockIdx.x, s = blockIdx.y;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int n = p.c.length(s, p.err);
   const int64_t at = (int64_t)s * p.c.heads + h;
   if (n <= p.budget) {
-    if (tid == 0) p.counts[at] = 0;
+    if (tid == 0 && !p.fused) p.counts[at] = 0;
     return;
   }
   const int recent_from = p.c.end(s, n) - p.recent;
@@ -63,8 +132,17 @@ kv4_select_kernel(const __grid_constant__ EvictParams p) {
     return __reduce_add_sync(0xffffffffu, lane < warp ? v : 0u);
   };
   if (p.shared_keys) {
+    // four slots a load; the last one may reach behind the sequence, never behind its capacity (a multiple of 16)
+    const int4* pos4 = reinterpret_cast<const int4*>(pos);
+    const float4* mass4 = reinterpret_cast<const float4*>(mass);
 #pragma unroll 4
-    for (int j = tid; j < n; j += THREADS) s_keys[j] = key_of(__ldg(pos + j), __ldg(mass + j), p.sinks, recent_from);
+    for (int j = tid; j < (n + 3) / 4; j += THREADS) {
+      const int4 q = __ldg(pos4 + j);
+      const float4 m = __ldg(mass4 + j);
+      reinterpret_cast<uint4*>(s_keys)[j] =
+          make_uint4(key_of(q.x, m.x, p.sinks, recent_from), key_of(q.y, m.y, p.sinks, recent_from),
+                     key_of(q.z, m.z, p.sinks, recent_from), key_of(q.w, m.w, p.sinks, recent_from));
+    }
   }
   // the budget-th largest key, digit by digit: `prefix` are the digits found, `left` how many of the keys that
   // share them are still to be taken
@@ -104,108 +182,113 @@ kv4_select_kernel(const __grid_constant__ EvictParams p) {
         }
       s_pick[0] = (uint32_t)(kBins - 1 - tid * PER - i);
       s_pick[1] = left - have;
+      s_pick[2] = 0u;
+#pragma unroll
+      for (int k = 0; k < PER; k++)
+        if (k == i) s_pick[2] = c[k];
     }
     __syncthreads();
     prefix = (prefix << bits) | s_pick[0];
     left = s_pick[1];
   }
-  // slots in order, a contiguous part per warp; of the keys equal to `prefix` the first `left` stay
+  // Slots in order, a contiguous part per warp.  Of the keys equal to `prefix` the first `left` stay: all of them, unless the
+  // budget cuts through equal weights.
+  const bool cut = left < s_pick[2];
   const int part = (n + THREADS - 1) / THREADS * 32, j0 = warp * part, j1 = min(n, j0 + part);
   const unsigned below = (1u << lane) - 1u;
-  uint32_t equal = 0, all;
-  for (int j = j0 + lane; j - lane < j1; j += 32) equal += __popc(__ballot_sync(0xffffffffu, j < j1 && key(j) == prefix));
-  const uint32_t equal0 = before_warp(0, equal, &all);
-  auto walk = [&](auto each) {  // each(slot, hole, move, lanes with a hole, lanes with a move)
+  uint32_t equal0 = 0, all;
+  if (cut) {
+    uint32_t equal = 0;
+    for (int j = j0 + lane; j - lane < j1; j += 32) equal += __popc(__ballot_sync(0xffffffffu, j < j1 && key(j) == prefix));
+    equal0 = before_warp(0, equal, &all);
+  }
+  // each(slot, whether it is in its list, the row's lanes that are, the row's lanes below the budget): a slot below the
+  // budget is listed when it is freed, one above when it is kept
+  auto walk = [&](auto each) {
     uint32_t e = equal0;
-    for (int j = j0 + lane; j - lane < j1; j += 32) {
+    for (int j = j0 + lane, row = j0; row < j1; j += 32, row += 32) {
       const uint32_t k = j < j1 ? key(j) : 0u;
-      const bool same = j < j1 && k == prefix;
-      const unsigned eq = __ballot_sync(0xffffffffu, same);
-      const bool kept = j < j1 && (k > prefix || (same && e + __popc(eq & below) < left));
-      e += __popc(eq);
-      const bool hole = j < j1 && !kept && j < p.budget, move = kept && j >= p.budget;
-      each(j, hole, move, __ballot_sync(0xffffffffu, hole), __ballot_sync(0xffffffffu, move));
+      bool kept = k >= prefix;
+      if (cut) {
+        const unsigned eq = __ballot_sync(0xffffffffu, j < j1 && k == prefix);
+        kept = k > prefix || (k == prefix && e + __popc(eq & below) < left);
+        e += __popc(eq);
+      }
+      const bool listed = j < j1 && (j < p.budget) != kept;
+      const unsigned low = row + 32 <= p.budget ? 0xffffffffu : row >= p.budget ? 0u : (1u << (p.budget - row)) - 1u;
+      each(j, listed, __ballot_sync(0xffffffffu, listed), low);
     }
   };
   uint32_t holes = 0, moves = 0, all_moves;
-  walk([&](int, bool, bool, unsigned hb, unsigned mb) {
-    holes += __popc(hb);
-    moves += __popc(mb);
+  walk([&](int, bool, unsigned rows, unsigned low) {
+    holes += __popc(rows & low);
+    moves += __popc(rows & ~low);
   });
   uint32_t hole_at = before_warp(1, holes, &all);
   uint32_t move_at = before_warp(0, moves, &all_moves);
   int32_t* dst = p.lists + at * 2 * p.list;
   int32_t* src = dst + p.list;
-  walk([&](int j, bool hole, bool move, unsigned hb, unsigned mb) {
-    const uint32_t a = hole_at + __popc(hb & below), b = move_at + __popc(mb & below);
-    if (hole && a < (uint32_t)p.list) dst[a] = j;
-    if (move && b < (uint32_t)p.list) src[b] = j;
-    hole_at += __popc(hb);
-    move_at += __popc(mb);
+  walk([&](int j, bool listed, unsigned rows, unsigned low) {
+    if (listed) {
+      const bool hole = j < p.budget;
+      const uint32_t i = hole ? hole_at + __popc(rows & low & below) : move_at + __popc(rows & ~low & below);
+      if (i < (uint32_t)p.list) (hole ? dst : src)[i] = j;
+    }
+    hole_at += __popc(rows & low);
+    move_at += __popc(rows & ~low);
   });
-  if (tid == 0) p.counts[at] = min(min((int)all, (int)all_moves), p.list);
-}
-
-// 16 lanes move a row: K codes, V codes (their halves swap places where the two slots differ in bit 1), scales,
-// position and mass.
-template <int D>
-__global__ void __launch_bounds__(256)
-kv4_move_kernel(const __grid_constant__ EvictParams p) {
-  using A = Atom<D>;
-  const int h = blockIdx.y, s = blockIdx.z;
-  const int64_t at = (int64_t)s * p.c.heads + h;
-  const int count = p.counts[at];
-  const int32_t* dst = p.lists + at * 2 * p.list;
-  const int32_t* src = dst + p.list;
-  const int part = threadIdx.x & 15;
-  constexpr int PIECES = A::ROW / 16, WORDS = A::SROW / 4;  // 16-byte pieces of a code row, words of a scale row
-  constexpr int TURNS = 4;                                  // rows that 16 lanes have in flight
-  const int64_t stat = p.c.stat(s, h);
-  for (int i0 = blockIdx.x * 16 * TURNS + (threadIdx.x >> 4); i0 < count; i0 += gridDim.x * 16 * TURNS) {
-    uint8_t* to[TURNS];
-    uint4 v[TURNS];
-    int slot[TURNS];
-#pragma unroll
-    for (int u = 0; u < TURNS; u++) {
-      to[u] = nullptr;
-      const int i = i0 + 16 * u;
-      if (i >= count) continue;
-      const int a = src[i], b = dst[i];
-      const uint8_t* from = p.c.atom(s, h, a / kAtomTokens, A::BYTES, p.err);
-      uint8_t* into = p.c.atom(s, h, b / kAtomTokens, A::BYTES, p.err);
-      if (!from || !into) continue;
-      const int ta = a % kAtomTokens, tb = b % kAtomTokens;
-      slot[u] = b;
-      if (part < PIECES) {
-        v[u] = *reinterpret_cast<const uint4*>(from + A::KC + ta * A::ROW + 16 * part);
-        to[u] = into + A::KC + tb * A::ROW + 16 * part;
-      } else if (part < 2 * PIECES) {
-        const int o = 16 * (part - PIECES);
-        v[u] = *reinterpret_cast<const uint4*>(from + A::VC + ta * A::ROW + (o ^ A::vswap(ta)));
-        to[u] = into + A::VC + tb * A::ROW + (o ^ A::vswap(tb));
-      } else if (part < 2 * PIECES + 2 * WORDS) {
-        const int o = part - 2 * PIECES, base = o / WORDS ? A::VS : A::KS, w = 4 * (o % WORDS);
-        v[u].x = *reinterpret_cast<const uint32_t*>(from + base + ta * A::SROW + w);
-        to[u] = into + base + tb * A::SROW + w;
-      } else if (part >= 14) {
-        v[u].x = part == 14 ? (uint32_t)p.c.positions[stat + a] : __float_as_uint(p.c.mass[stat + a]);
-        to[u] = into;
-      }
-    }
-#pragma unroll
-    for (int u = 0; u < TURNS; u++) {
-      if (!to[u]) continue;
-      if (part < 2 * PIECES) *reinterpret_cast<uint4*>(to[u]) = v[u];
-      else if (part < 14) *reinterpret_cast<uint32_t*>(to[u]) = v[u].x;
-      else if (part == 14) p.c.positions[stat + slot[u]] = (int32_t)v[u].x;
-      else p.c.mass[stat + slot[u]] = __uint_as_float(v[u].x);
-    }
+  const int count = min(min((int)all, (int)all_moves), p.list);
+  if (p.fused) {  // few rows: this CTA moves them, without a second launch
+    __syncthreads();
+    move_rows<D, 1>(p, s, h, dst, src, count, tid >> 4, THREADS / 16);
+  } else if (tid == 0) {
+    p.counts[at] = count;
   }
 }
+
+template <int D>
+__global__ void __launch_bounds__(256, 5)
+kv4_move_kernel(const __grid_constant__ EvictParams p) {
+  const int h = blockIdx.y, s = blockIdx.z;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int64_t at = (int64_t)s * p.c.heads + h;
+  const int count = min(p.counts[at], (int)blockIdx.x * 32 + 32);
+  const int32_t* dst = p.lists + at * 2 * p.list;
+  move_rows<D, 2>(p, s, h, dst, dst + p.list, count, blockIdx.x * 32 + (threadIdx.x >> 4), 16);
+}
+
 
 int list_entries(const Cache& c, int budget) {
   const int above = c.capacity - budget;
   return above <= 0 ? 0 : (above < budget ? above : budget);
+}
+
+template <int D>
+int launch(const EvictParams& p, cudaStream_t s) {
+  const int bytes = p.shared_keys ? p.c.capacity * 4 : 0;
+  const dim3 select(p.c.heads, p.c.n_seqs);
+  if (p.c.capacity <= 8192) {
+    kv4_select_kernel<D, 256><<<select, 256, bytes, s>>>(p);
+  } else {
+    if (cudaError_t ce = cudaFuncSetAttribute(kv4_select_kernel<D, 1024>, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSharedKeys * 4))
+      return pkv_cuda_status(ce);
+    kv4_select_kernel<D, 1024><<<select, 1024, bytes, s>>>(p);
+  }
+  pkv_count_launch();
+  if (cudaError_t ce = cudaGetLastError()) return pkv_cuda_status(ce);
+  if (p.fused) return PKV_OK;
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr = {};
+  cfg.gridDim = dim3((p.list + 31) / 32, p.c.heads, p.c.n_seqs);  // every move in flight at once
+  cfg.blockDim = dim3(256);
+  cfg.stream = s;
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  if (cudaError_t ce = cudaLaunchKernelEx(&cfg, kv4_move_kernel<D>, p)) return pkv_cuda_status(ce);
+  pkv_count_launch();
+  return pkv_cuda_status(cudaGetLastError());
 }
 
 }  // namespace
@@ -230,25 +313,10 @@ extern "C" int pkv_kv4_evict_dev(const pkv_kv4_cache* cache, int32_t budget, int
   p.sinks = sinks;
   p.recent = recent;
   p.shared_keys = p.c.capacity <= kMaxSharedKeys;
+  p.fused = p.list <= 256;  // a few turns of a CTA's 16-lane groups
   p.lists = (int32_t*)workspace_dev;
   p.counts = p.lists + (int64_t)p.c.n_seqs * p.c.heads * 2 * p.list;
   p.err = err_dev;
   cudaStream_t s = (cudaStream_t)stream;
-  const int bytes = p.shared_keys ? p.c.capacity * 4 : 0;
-  const dim3 select(p.c.heads, p.c.n_seqs);
-  if (p.c.capacity <= 8192) {
-    kv4_select_kernel<256><<<select, 256, bytes, s>>>(p);
-  } else {
-    if (cudaError_t ce = cudaFuncSetAttribute(kv4_select_kernel<1024>, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSharedKeys * 4))
-      return pkv_cuda_status(ce);
-    kv4_select_kernel<1024><<<select, 1024, bytes, s>>>(p);
-  }
-  pkv_count_launch();
-  if (cudaError_t ce = cudaGetLastError()) return pkv_cuda_status(ce);
-  const int ctas = (p.list + 63) / 64;  // every move in flight at once
-  const dim3 grid(ctas, p.c.heads, p.c.n_seqs);
-  if (cache->dim == 64) kv4_move_kernel<64><<<grid, 256, 0, s>>>(p);
-  else kv4_move_kernel<128><<<grid, 256, 0, s>>>(p);
-  pkv_count_launch();
-  return pkv_cuda_status(cudaGetLastError());
+  return cache->dim == 64 ? launch<64>(p, s) : launch<128>(p, s);
 }

@@ -32,7 +32,7 @@ def _append(cache, k=P, kr=None, v=P, vr=None, err=P, fn="pkv_kv4_append_dev"):
 @pytest.mark.parametrize("fn", ["pkv_kv4_append_dev", "pkv_kv4_read_dev"])
 def test_append_and_read_refuse(fn):
     bad, unsup = L.ERR_INVALID_ARGUMENT, L.ERR_UNSUPPORTED
-    for kw, want in ((dict(pages=None), bad), (dict(pages=P + 8), bad), (dict(lens=None), bad), (dict(page_table=None), bad),
+    for kw, want in ((dict(pages=None), bad), (dict(pages=P + 8), bad), (dict(lens=None), bad), (dict(positions=P + 4), bad), (dict(mass=P + 8), bad), (dict(page_table=None), bad),
                      (dict(reserved=1), bad), (dict(n_kv_heads=0), bad), (dict(n_seqs=-1), bad), (dict(max_pages=-1), bad),
                      (dict(page_tokens=0), bad), (dict(n_pages=-1), bad), (dict(dim=96), unsup), (dict(dim=256), unsup),
                      (dict(page_tokens=24), unsup), (dict(max_pages=1 << 26), unsup), (dict(n_seqs=70000), unsup)):
