@@ -29,6 +29,7 @@ constexpr int kWarps = 4;
 constexpr int kStages = 2;
 constexpr int kMaxRows = 2048;           // (sequence, kv head, row tile)s that share runs
 constexpr int kJoinWarps = 8;
+constexpr int64_t kMostScores = 1ll << 26;  // 256 MiB
 constexpr int kMassTokens = 32;  // keys a warp of the mass kernel holds
 __device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
@@ -527,6 +528,20 @@ __device__ __forceinline__ void stream_units(const AttendParams& p, Cursor t, in
                 }
             }
         }
+        if (__builtin_expect(p.scores != nullptr, 0)) {  // for the weights to accumulate, once their sums are known
+          float* to = p.scores + (p.c.stat(t.s, t.h) + token0 + 32 * k) * (8 * NT) + 2 * q4;
+#pragma unroll
+          for (int a = 0; a < 2; a++)
+#pragma unroll
+            for (int hh = 0; hh < 2; hh++) {
+              const int at = 16 * a + 8 * hh + tau(g);
+#pragma unroll
+              for (int n = 0; n < NT; n++)
+                if (token0 + 32 * k + at < len)
+                  *reinterpret_cast<float2*>(to + at * (8 * NT) + 8 * n) =
+                      make_float2(__fmul_rn(sc[a][n][2 * hh], fac[n][0]), __fmul_rn(sc[a][n][2 * hh + 1], fac[n][1]));
+            }
+        }
         float top[NT][2];
         bool raise = false;
 #pragma unroll
@@ -616,8 +631,11 @@ __device__ __forceinline__ void stream_units(const AttendParams& p, Cursor t, in
   }
 }
 
+// CTAs an SM holds: as many as the registers of the sums, the queries and (f32) their second terms leave room for.
+__host__ __device__ constexpr int ctas_per_sm(int dim, int nt, bool f32) { return nt == 1 && !(f32 && dim == 128) ? 3 : 2; }
+
 template <int D, int NT, int T, bool DIRECT>
-__global__ void __launch_bounds__(kWarps * 32, (NT == 1 ? 3 : 2))
+__global__ void __launch_bounds__(kWarps * 32, ctas_per_sm(D, NT, T == PKV_DST_F32))
 kv4_attend_kernel(const __grid_constant__ AttendParams p) {
   using S = Shared<D, NT>;
   extern __shared__ __align__(128) uint8_t smem[];
@@ -805,7 +823,41 @@ kv4_combine_kernel(const __grid_constant__ AttendParams p) {
   write_row<T, N>(p, s, h, grow, lane * N, x, m, l, lane == 0);
 }
 
-// mass[key] += sum over the query rows of exp(score - lse).  A warp keeps the dequantised keys of 32 tokens in
+// mass[key] += sum over the query rows of exp(score - lse), from the scores that the attention kernel left behind; a thread
+// per slot.  One row tile, so a slot's rows are 32 or 64 consecutive bytes.
+template <int NT>
+__global__ void __launch_bounds__(256)
+kv4_mass_of_scores_kernel(const __grid_constant__ AttendParams p) {
+  __shared__ float s_lse[8 * NT];
+  const int s = blockIdx.z, h = blockIdx.y;
+  const Sequence seq = sequence_of(p, s);
+  const int rows = seq.qn * p.group, pos0 = seq.end - seq.qn;
+  const Span span = visible_span(p, seq.len, pos0, seq.end - 1);
+  if (threadIdx.x < 8 * NT) {
+    const int r = threadIdx.x, token = r / p.group, hq = h * p.group + (r - token * p.group);
+    s_lse[r] = r < rows ? __fmul_rn(kLog2e, p.lse[((int64_t)s * p.q.n + token) * p.q_heads + hq]) : -INFINITY;
+  }
+  __syncthreads();
+  for (int slot = blockIdx.x * 256 + threadIdx.x; slot < seq.len; slot += gridDim.x * 256) {
+    const int unit = slot / kUnitTokens;
+    if (unit >= span.head && (unit < span.from || unit >= span.from + span.count - span.head)) continue;  // not visited
+    const float* x = p.scores + (p.c.stat(s, h) + slot) * (8 * NT);
+    float sum = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 8 * NT; i += 4) {
+      if (i >= rows) break;
+      const float4 v = *reinterpret_cast<const float4*>(x + i);
+      const float y[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+      for (int j = 0; j < 4; j++)  // (a row that sees nothing has no lse; rows behind the last one neither)
+        if (s_lse[i + j] != -INFINITY) sum = __fadd_rn(sum, exp2_fast(__fsub_rn(y[j], s_lse[i + j])));
+    }
+    float* m = p.c.mass + p.c.stat(s, h) + slot;
+    *m = __fadd_rn(*m, sum);
+  }
+}
+
+// The same by a second pass over the keys, for more query rows (or where the scores would not fit the workspace).  A warp keeps the dequantised keys of 32 tokens in
 // registers and walks over the rows, so every sum has one owner and one order.
 template <int D, int T>
 __global__ void __launch_bounds__(kWarps * 32)
@@ -898,10 +950,14 @@ kv4_mass_kernel(const __grid_constant__ AttendParams p) {
 struct Plan {
   int nt, row_tiles, runs;
   int64_t part_rows, tiles;  // rows of partial sums; row tiles of all
-  int64_t bytes(int dim) const { return runs ? part_rows * (dim + 2) * (int64_t)sizeof(float) + tiles * (int64_t)sizeof(int2) : 0; }
+  int64_t scores;            // of kv4_mass_of_scores_kernel
+  int64_t bytes(int dim) const {
+    return scores * (int64_t)sizeof(float) +
+           (runs ? part_rows * (dim + 2) * (int64_t)sizeof(float) + tiles * (int64_t)sizeof(int2) : 0);
+  }
 };
 
-Plan make_plan(const Cache& c, const pkv_kv4_rows* q, const pkv_kv4_attend_args* a) {
+Plan make_plan(const Cache& c, int dim, const pkv_kv4_rows* q, const pkv_kv4_attend_args* a) {
   Plan r;
   const int64_t rows = (int64_t)q->n_tokens * (a->n_q_heads / c.heads);
   r.nt = rows > 8 ? 2 : 1;
@@ -914,7 +970,7 @@ Plan make_plan(const Cache& c, const pkv_kv4_rows* q, const pkv_kv4_attend_args*
   const int64_t units = (longest + kUnitTokens - 1) / kUnitTokens;
   // Rows of up to six units a warp are not worth a second launch (32 sequences with a window of 1024, 8 kv heads: 17.2 us
   // against 24.4), and with a row for every warp there is nothing to cut.
-  const int64_t tiles = (int64_t)c.heads * r.row_tiles * c.n_seqs, resident = (int64_t)sm_count() * kWarps * (r.nt == 1 ? 3 : 2);
+  const int64_t tiles = (int64_t)c.heads * r.row_tiles * c.n_seqs, resident = (int64_t)sm_count() * kWarps * ctas_per_sm(dim, r.nt, q->dtype == PKV_DST_F32);
   r.runs = 0;
   if (units > 6 * kWarps && tiles < kMaxRows && units * tiles < (1ll << 31)) {
     const int64_t could = (units * tiles + kWarps - 1) / kWarps * kWarps;
@@ -922,6 +978,10 @@ Plan make_plan(const Cache& c, const pkv_kv4_rows* q, const pkv_kv4_attend_args*
   }
   r.part_rows = (int64_t)r.runs * 2 * 8 * r.nt;
   r.tiles = tiles;
+  // keeping the scores costs 32 bytes a token and kv head each way (eight rows), a second pass over the keys 72 (dim 128) and
+  // their dequantisation
+  r.scores = a->accumulate && r.row_tiles == 1 ? (int64_t)c.n_seqs * c.heads * c.capacity * 8 * r.nt : 0;
+  if (r.scores > kMostScores) r.scores = 0;
   return r;
 }
 
@@ -960,7 +1020,12 @@ int launch_all(const AttendParams& p, int nt, bool accumulate, int longest, cuda
   } else if (int st = nt == 1 ? launch_attend<D, 1, T>(p, s) : launch_attend<D, 2, T>(p, s)) {
     return st;
   }
-  if (accumulate && longest > 0) {
+  if (p.scores && longest > 0) {
+    const dim3 grid((longest + 255) / 256, p.c.heads, p.c.n_seqs);
+    if (nt == 1) kv4_mass_of_scores_kernel<1><<<grid, 256, 0, s>>>(p);
+    else kv4_mass_of_scores_kernel<2><<<grid, 256, 0, s>>>(p);
+    pkv_count_launch();
+  } else if (accumulate && longest > 0) {
     const int per = kWarps * kMassTokens;
     kv4_mass_kernel<D, T><<<dim3((longest + per - 1) / per, p.c.heads, p.c.n_seqs), kWarps * 32, 0, s>>>(p);
     pkv_count_launch();
@@ -985,7 +1050,7 @@ extern "C" int64_t pkv_kv4_attend_workspace_bytes(const pkv_kv4_cache* cache, co
   Cache c;
   if (make_cache(cache, &c) || !q_rows || q_rows->n_tokens < 0 || check_args(c, q_rows, args)) return 0;
   if (chunk_takes(q_rows, args->n_q_heads / c.heads)) return chunk_workspace_bytes(c, cache->dim, q_rows, args);
-  return make_plan(c, q_rows, args).bytes(cache->dim);
+  return make_plan(c, cache->dim, q_rows, args).bytes(cache->dim);
 }
 
 extern "C" int pkv_kv4_attend_dev(const pkv_kv4_cache* cache, const void* q_dev, const pkv_kv4_rows* q_rows, void* out_dev,
@@ -1002,7 +1067,7 @@ extern "C" int pkv_kv4_attend_dev(const pkv_kv4_cache* cache, const void* q_dev,
   if (p.q.n == 0 || p.c.n_seqs == 0) return PKV_OK;
   const bool chunk = chunk_takes(q_rows, args->n_q_heads / p.c.heads);
   Plan plan = {};
-  if (!chunk) plan = make_plan(p.c, q_rows, args);
+  if (!chunk) plan = make_plan(p.c, cache->dim, q_rows, args);
   const int64_t need = chunk ? chunk_workspace_bytes(p.c, cache->dim, q_rows, args) : plan.bytes(cache->dim);
   if (need > workspace_bytes) return PKV_ERR_BUFFER_TOO_SMALL;
   if (need && (!workspace_dev || ((uintptr_t)workspace_dev & 15))) return PKV_ERR_INVALID_ARGUMENT;
@@ -1020,7 +1085,8 @@ extern "C" int pkv_kv4_attend_dev(const pkv_kv4_cache* cache, const void* q_dev,
   p.runs = plan.runs;
   p.tile_rows = 8 * plan.nt;
   p.whole_units = p.c.page_atoms % kUnitAtoms == 0;
-  p.part_o = (float*)workspace_dev;
+  p.scores = plan.scores ? (float*)workspace_dev : nullptr;
+  p.part_o = (float*)workspace_dev + plan.scores;
   p.part_ml = p.part_o + plan.part_rows * cache->dim;
   p.part_of = (int2*)(p.part_ml + plan.part_rows * 2);
   p.err = err_dev;

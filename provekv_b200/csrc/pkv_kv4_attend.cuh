@@ -32,6 +32,7 @@ struct AttendParams {
   float* part_o;      // [run][2][8 NT][D] unnormalised sums of a run's first and last row, where it has only a part of it
   float* part_ml;     // [run][2][8 NT][2] reference and sum
   int2* part_of;      // [sequence][kv head][row tile] first run and number of runs that have a part of it
+  float* scores;      // accumulating, one row tile: [sequence][kv head][slot][8 NT] scaled scores (log2), else null
   uint64_t* err;
 };
 
