@@ -279,6 +279,56 @@ def test_long_rows_are_split_and_joined(dtype):
     _attend_case(14, dtype, 64, 1, 2, 64, [1700, 3], 1, 0, 0, False, True, max_len=600)
 
 
+@pytest.mark.parametrize("dtype", ["float32", "float16"])
+@pytest.mark.parametrize("page,moved,window,sinks", [(48, False, 0, 0), (16, True, 500, 30), (48, False, 1200, 100), (64, True, 0, 0)])
+def test_rows_share_runs_whatever_their_lengths(dtype, page, moved, window, sinks):
+    """More than 32 sequences, some empty, of lengths that cut units and pages anywhere; the longest decides that rows share runs."""
+    rng = np.random.default_rng(page + window)
+    lens = [1700, 0, 1] + rng.integers(1, 400, 34).tolist() + [1650]
+    _attend_case(15, dtype, 64, 1, 3, page, lens, 1, window, sinks, moved, True)
+
+
+def test_runs_skip_sequences_without_queries():
+    lens = [1700, 1650, 30, 800, 64]
+    _attend_case(16, "bfloat16", 128, 2, 2, 64, lens, 3, 0, 0, False, True, q_lens=[0, 2, 3, 0, 1])
+    _attend_case(17, "float32", 64, 1, 9, 64, lens, 2, 0, 0, False, True, q_lens=[1, 0, 0, 2, 0])
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("scale", [0.0, -0.2, 1e-3])
+@pytest.mark.parametrize("lens,q_len", [([45, 70], 1), ([1700], 1), ([90], 30)])
+def test_scales_that_are_zero_negative_or_small(dtype, scale, lens, q_len):
+    _attend_case(18, dtype, 64, 2, 2, 16, lens, q_len, 40, 3, False, True, scale=float(np.float32(scale)))
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("page,lens,q_len,group,window,sinks,moved", [(48, [700], 60, 2, 0, 0, False), (16, [1300, 5, 0], 20, 1, 300, 70, False),
+                                                                      (64, [1100, 1024], 18, 1, 0, 0, True), (48, [640], 300, 1, 50, 0, True)])
+def test_chunks_split_over_the_tokens(dim, page, lens, q_len, group, window, sinks, moved):
+    _attend_case(19 + page, "bfloat16", dim, 1, group, page, lens, q_len, window, sinks, moved, True,
+                 q_lens=[min(q_len, n + 2) for n in lens])
+
+
+def test_pages_missing_from_a_chunk_and_from_a_long_row():
+    import torch
+    for q_len, n in ((20, 300), (1, 1700)):
+        rng = np.random.default_rng(n)
+        pages, table, values = kv4ref.fill(rng, 2, 1, 128, 16, [n, 40])
+        table[0, 3], table[0, 9] = -1, pages.shape[0] + 7
+        cache = kv4.Kv4Cache(_dev(pages), _ints(table), _ints([n, 40]), mass=torch.zeros((2, 1, table.shape[1] * 16), device="cuda"))
+        q = _dev(rng.standard_normal((2, q_len, 2, 128)), torch.float16)
+        out, lse = cache.attend(q, accumulate=True)
+        with pytest.raises(pk.PkvError) as e:
+            cache.check()
+        assert (e.value.status, e.value.vector_index) == (L.VEC_BAD_SEQUENCE, 0)
+        gone = np.r_[48:64, 144:160]
+        pos = np.tile(np.arange(n, dtype=np.int64), (2, 1, 1))
+        pos[0, 0, gone] = 1 << 30  # beyond every query: not seen
+        w = kv4ref.attend(q.double().cpu().numpy(), values, [n, 40], [n, 40], pos, 2, 128 ** -0.5, 0, 0, [q_len] * 2)
+        _close(out, lse, w[0], w[1], *w[3:])
+        assert (cache.mass[0, 0, 48:64] == 0).all() and (cache.mass[0, 0, 64:100] > 0).all()
+
+
 def test_a_longer_query_chunk():
     _attend_case(21, "bfloat16", 128, 1, 4, 64, [300], 200, 0, 0, False, True)
     _attend_case(22, "float16", 64, 2, 2, 48, [150, 260], 130, 50, 5, False, False, q_lens=[130, 77])
