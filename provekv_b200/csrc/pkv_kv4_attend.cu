@@ -648,6 +648,7 @@ kv4_attend_kernel(const __grid_constant__ AttendParams p) {
 #pragma unroll
     for (int i = 0; i < kStages; i++) pkv_mbar_init(&bars[warp][i], 1);
   __syncwarp();
+  wait_for_stream();
   Sums<D, NT> r;
 
   if constexpr (DIRECT) {
@@ -747,8 +748,7 @@ kv4_combine_kernel(const __grid_constant__ AttendParams p) {
   const int lane = threadIdx.x & 31, warp = (threadIdx.x >> 5) % W;
   const int s = blockIdx.z, h = blockIdx.y, grow = blockIdx.x * PER + (threadIdx.x >> 5) / W;
   const int tile = grow / (8 * NT), row = grow - tile * (8 * NT);
-  // every block waits, so that this launch never ends before the one it follows
-  asm volatile("griddepcontrol.wait;" ::: "memory");
+  wait_for_stream();
   int qn = p.q_lens ? p.q_lens[s] : p.q.n;
   if (qn < 0 || qn > p.q.n) qn = 0;
   if (grow >= qn * p.group) return;
@@ -830,6 +830,7 @@ __global__ void __launch_bounds__(256)
 kv4_mass_of_scores_kernel(const __grid_constant__ AttendParams p) {
   __shared__ float s_lse[8 * NT];
   const int s = blockIdx.z, h = blockIdx.y;
+  wait_for_stream();
   const Sequence seq = sequence_of(p, s);
   const int rows = seq.qn * p.group, pos0 = seq.end - seq.qn;
   const Span span = visible_span(p, seq.len, pos0, seq.end - 1);
@@ -868,6 +869,7 @@ kv4_mass_kernel(const __grid_constant__ AttendParams p) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int g = lane >> 2, q4 = lane & 3;
   const int s = blockIdx.z, h = blockIdx.y;
+  wait_for_stream();
   const int len = p.c.length(s, p.err), end = p.c.end(s, len);
   int qn = p.q_lens ? p.q_lens[s] : p.q.n;
   if (qn < 0 || qn > p.q.n) qn = 0;
@@ -992,26 +994,12 @@ int launch_attend(const AttendParams& p, cudaStream_t s) {
   if (bytes > 48 * 1024)
     if (cudaError_t ce = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes)) return pkv_cuda_status(ce);
   const dim3 rows(p.row_tiles, p.c.heads, p.c.n_seqs);
-  kernel<<<p.runs ? dim3(p.runs / kWarps) : rows, kWarps * 32, bytes, s>>>(p);
-  pkv_count_launch();
-  if (cudaError_t ce = cudaGetLastError()) return pkv_cuda_status(ce);
-  if (p.runs) {
-    // its launch overlaps the end of the first kernel; it waits (griddepcontrol) before it reads the parts
-    cudaLaunchConfig_t cfg = {};
-    cudaLaunchAttribute attr = {};
-    const bool many = p.runs < 16ll * p.row_tiles * p.c.heads * p.c.n_seqs;  // few parts a row
-    cfg.gridDim = dim3(p.row_tiles * 8 * NT / (many ? kJoinWarps : 1), p.c.heads, p.c.n_seqs);
-    cfg.blockDim = dim3(kJoinWarps * 32);
-    cfg.stream = s;
-    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr.val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = &attr;
-    cfg.numAttrs = 1;
-    if (cudaError_t ce = cudaLaunchKernelEx(&cfg, many ? kv4_combine_kernel<D, NT, T, 1> : kv4_combine_kernel<D, NT, T, kJoinWarps>, p))
-      return pkv_cuda_status(ce);
-    pkv_count_launch();
-  }
-  return pkv_cuda_status(cudaGetLastError());
+  if (cudaError_t ce = launch_early(kernel, p.runs ? dim3(p.runs / kWarps) : rows, kWarps * 32, bytes, s, p)) return pkv_cuda_status(ce);
+  if (!p.runs) return PKV_OK;
+  const bool many = p.runs < 16ll * p.row_tiles * p.c.heads * p.c.n_seqs;  // few parts a row
+  return pkv_cuda_status(launch_early(many ? kv4_combine_kernel<D, NT, T, 1> : kv4_combine_kernel<D, NT, T, kJoinWarps>,
+                                      dim3(p.row_tiles * 8 * NT / (many ? kJoinWarps : 1), p.c.heads, p.c.n_seqs), kJoinWarps * 32, 0, s,
+                                      p));
 }
 
 template <int D, int T>
@@ -1020,17 +1008,13 @@ int launch_all(const AttendParams& p, int nt, bool accumulate, int longest, cuda
   } else if (int st = nt == 1 ? launch_attend<D, 1, T>(p, s) : launch_attend<D, 2, T>(p, s)) {
     return st;
   }
-  if (p.scores && longest > 0) {
-    const dim3 grid((longest + 255) / 256, p.c.heads, p.c.n_seqs);
-    if (nt == 1) kv4_mass_of_scores_kernel<1><<<grid, 256, 0, s>>>(p);
-    else kv4_mass_of_scores_kernel<2><<<grid, 256, 0, s>>>(p);
-    pkv_count_launch();
-  } else if (accumulate && longest > 0) {
-    const int per = kWarps * kMassTokens;
-    kv4_mass_kernel<D, T><<<dim3((longest + per - 1) / per, p.c.heads, p.c.n_seqs), kWarps * 32, 0, s>>>(p);
-    pkv_count_launch();
-  }
-  return pkv_cuda_status(cudaGetLastError());
+  if (!accumulate || longest <= 0) return PKV_OK;
+  if (p.scores)
+    return pkv_cuda_status(launch_early(nt == 1 ? kv4_mass_of_scores_kernel<1> : kv4_mass_of_scores_kernel<2>,
+                                        dim3((longest + 255) / 256, p.c.heads, p.c.n_seqs), 256, 0, s, p));
+  const int per = kWarps * kMassTokens;
+  return pkv_cuda_status(
+      launch_early(kv4_mass_kernel<D, T>, dim3((longest + per - 1) / per, p.c.heads, p.c.n_seqs), kWarps * 32, 0, s, p));
 }
 
 int check_args(const Cache& c, const pkv_kv4_rows* q, const pkv_kv4_attend_args* a) {

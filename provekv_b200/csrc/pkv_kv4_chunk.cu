@@ -176,6 +176,8 @@ kv4_chunk_kernel(const __grid_constant__ ChunkParams cp) {
   uint8_t* smem = smem_raw + ((1024u - (pkv_smem_u32(smem_raw) & 1023u)) & 1023u);
   const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
 
+  wait_for_stream();
+
   // ---- the task
   const int split = blockIdx.x / cp.tasks, task = blockIdx.x - split * cp.tasks;
   const int h = blockIdx.y, s = blockIdx.z;
@@ -567,7 +569,7 @@ kv4_chunk_join_kernel(const __grid_constant__ ChunkParams cp) {
   constexpr int N = D / 32;
   const int lane = threadIdx.x & 31;
   const int h = blockIdx.y, s = blockIdx.z, row = blockIdx.x * 8 + (threadIdx.x >> 5);
-  asm volatile("griddepcontrol.wait;" ::: "memory");
+  wait_for_stream();
   int qn = p.q_lens ? p.q_lens[s] : p.q.n;
   if (qn < 0 || qn > p.q.n) qn = 0;
   if (row >= qn * p.group) return;
@@ -619,23 +621,11 @@ int launch(const ChunkParams& cp, int64_t rows, cudaStream_t s) {
   auto kernel = kv4_chunk_kernel<D, T>;
   constexpr int bytes = Layout<D>::BYTES;
   if (cudaError_t ce = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes)) return pkv_cuda_status(ce);
-  kernel<<<dim3(cp.tasks * cp.splits, cp.a.c.heads, cp.a.c.n_seqs), kThreads, bytes, s>>>(cp);
-  pkv_count_launch();
-  if (cudaError_t ce = cudaGetLastError()) return pkv_cuda_status(ce);
-  if (cp.splits > 1) {
-    cudaLaunchConfig_t cfg = {};
-    cudaLaunchAttribute attr = {};
-    cfg.gridDim = dim3((unsigned)((rows + 7) / 8), cp.a.c.heads, cp.a.c.n_seqs);
-    cfg.blockDim = dim3(256);
-    cfg.stream = s;
-    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr.val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = &attr;
-    cfg.numAttrs = 1;
-    if (cudaError_t ce = cudaLaunchKernelEx(&cfg, kv4_chunk_join_kernel<D, T>, cp)) return pkv_cuda_status(ce);
-    pkv_count_launch();
-  }
-  return pkv_cuda_status(cudaGetLastError());
+  if (cudaError_t ce = launch_early(kernel, dim3(cp.tasks * cp.splits, cp.a.c.heads, cp.a.c.n_seqs), kThreads, bytes, s, cp))
+    return pkv_cuda_status(ce);
+  if (cp.splits == 1) return PKV_OK;
+  return pkv_cuda_status(launch_early(kv4_chunk_join_kernel<D, T>, dim3((unsigned)((rows + 7) / 8), cp.a.c.heads, cp.a.c.n_seqs), 256,
+                                      0, s, cp));
 }
 
 }  // namespace

@@ -111,6 +111,7 @@ kv4_select_kernel(const __grid_constant__ EvictParams p) {
   __shared__ uint32_t s_pick[3];  // digit, how many are left to take within it, how many there are
   const int h = blockIdx.x, s = blockIdx.y;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  wait_for_stream();
   const int n = p.c.length(s, p.err);
   const int64_t at = (int64_t)s * p.c.heads + h;
   if (n <= p.budget) {
@@ -250,7 +251,7 @@ template <int D>
 __global__ void __launch_bounds__(256, 5)
 kv4_move_kernel(const __grid_constant__ EvictParams p) {
   const int h = blockIdx.y, s = blockIdx.z;
-  asm volatile("griddepcontrol.wait;" ::: "memory");
+  wait_for_stream();
   const int64_t at = (int64_t)s * p.c.heads + h;
   const int count = min(p.counts[at], (int)blockIdx.x * 32 + 32);
   const int32_t* dst = p.lists + at * 2 * p.list;
@@ -267,28 +268,15 @@ template <int D>
 int launch(const EvictParams& p, cudaStream_t s) {
   const int bytes = p.shared_keys ? p.c.capacity * 4 : 0;
   const dim3 select(p.c.heads, p.c.n_seqs);
-  if (p.c.capacity <= 8192) {
-    kv4_select_kernel<D, 256><<<select, 256, bytes, s>>>(p);
-  } else {
+  if (p.c.capacity > 8192)
     if (cudaError_t ce = cudaFuncSetAttribute(kv4_select_kernel<D, 1024>, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSharedKeys * 4))
       return pkv_cuda_status(ce);
-    kv4_select_kernel<D, 1024><<<select, 1024, bytes, s>>>(p);
-  }
-  pkv_count_launch();
-  if (cudaError_t ce = cudaGetLastError()) return pkv_cuda_status(ce);
+  if (cudaError_t ce = p.c.capacity <= 8192 ? launch_early(kv4_select_kernel<D, 256>, select, 256, bytes, s, p)
+                                            : launch_early(kv4_select_kernel<D, 1024>, select, 1024, bytes, s, p))
+    return pkv_cuda_status(ce);
   if (p.fused) return PKV_OK;
-  cudaLaunchConfig_t cfg = {};
-  cudaLaunchAttribute attr = {};
-  cfg.gridDim = dim3((p.list + 31) / 32, p.c.heads, p.c.n_seqs);  // every move in flight at once
-  cfg.blockDim = dim3(256);
-  cfg.stream = s;
-  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr.val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = &attr;
-  cfg.numAttrs = 1;
-  if (cudaError_t ce = cudaLaunchKernelEx(&cfg, kv4_move_kernel<D>, p)) return pkv_cuda_status(ce);
-  pkv_count_launch();
-  return pkv_cuda_status(cudaGetLastError());
+  return pkv_cuda_status(
+      launch_early(kv4_move_kernel<D>, dim3((p.list + 31) / 32, p.c.heads, p.c.n_seqs), 256, 0, s, p));  // every move in flight at once
 }
 
 }  // namespace

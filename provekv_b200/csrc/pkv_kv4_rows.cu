@@ -192,6 +192,7 @@ kv4_append_kernel(Cache c, const typename PkvDst<T>::type* __restrict__ k, Rows 
   const unsigned row_lanes = ((1u << A::SROW) - 1u) << ((threadIdx.x & 31) / A::SROW * A::SROW);
   Raw<T> raw[TURNS][2];
   uint8_t* atom[TURNS];
+  wait_for_stream();
   const Fresh f = fresh_of(c, s, kr.n, new_lens, err);
   k += s * kr.seq + h * kr.head + 16 * b;
   v += s * vr.seq + h * vr.head + 16 * b;
@@ -292,6 +293,7 @@ kv4_read_kernel(Cache c, typename PkvDst<T>::type* __restrict__ k, Rows kr, type
   const int piece = threadIdx.x % R::PIECES;
   const int s = blockIdx.z, h = blockIdx.y;
   const int i0 = blockIdx.x * R::ROWS * R::TURNS + threadIdx.x / R::PIECES;
+  wait_for_stream();
   const Fresh f = fresh_of(c, s, kr.n, new_lens, err);
   k += s * kr.seq + h * kr.head + piece * N;
   v += s * vr.seq + h * vr.head + piece * N;
@@ -332,17 +334,15 @@ kv4_read_kernel(Cache c, typename PkvDst<T>::type* __restrict__ k, Rows kr, type
 }
 
 template <int D, int T>
-void launch_rows(bool append, const Cache& c, const void* k, const Rows& kr, const void* v, const Rows& vr,
+cudaError_t launch_rows(bool append, const Cache& c, const void* k, const Rows& kr, const void* v, const Rows& vr,
                  const int32_t* new_lens, int clear_rest, uint64_t* err, cudaStream_t s) {
   using E = typename PkvDst<T>::type;
   constexpr int TOK = kThreads / Atom<D>::SROW * kAppendTurns<T>, READ = ReadShape<D, T>::ROWS * ReadShape<D, T>::TURNS;
   const int per = append ? TOK : READ;
   const dim3 grid((unsigned)((kr.n + per - 1) / per), (unsigned)c.heads, (unsigned)c.n_seqs);
-  if (append)
-    kv4_append_kernel<D, T><<<grid, kThreads, 0, s>>>(c, (const E*)k, kr, (const E*)v, vr, new_lens, err);
-  else
-    kv4_read_kernel<D, T><<<grid, kReadThreads, 0, s>>>(c, (E*)const_cast<void*>(k), kr, (E*)const_cast<void*>(v), vr, new_lens,
-                                                        clear_rest, err);
+  if (append) return launch_early(kv4_append_kernel<D, T>, grid, kThreads, 0, s, c, (const E*)k, kr, (const E*)v, vr, new_lens, err);
+  return launch_early(kv4_read_kernel<D, T>, grid, kReadThreads, 0, s, c, (E*)const_cast<void*>(k), kr, (E*)const_cast<void*>(v), vr,
+                      new_lens, clear_rest, err);
 }
 
 int rows_call(bool append, const pkv_kv4_cache* cache, const void* k, const pkv_kv4_rows* k_rows, const void* v,
@@ -356,16 +356,16 @@ int rows_call(bool append, const pkv_kv4_cache* cache, const void* k, const pkv_
   if (kr.n > c.capacity && !new_lens) return PKV_ERR_INVALID_ARGUMENT;
   if (kr.n == 0 || c.n_seqs == 0) return PKV_OK;
   cudaStream_t s = (cudaStream_t)stream;
+  cudaError_t ce;
 #define PKV_KV4_ROWS(D)                                                                                                    \
   switch (k_rows->dtype) {                                                                                                 \
-    case PKV_DST_F32: launch_rows<D, PKV_DST_F32>(append, c, k, kr, v, vr, new_lens, clear_rest, err, s); break;                       \
-    case PKV_DST_F16: launch_rows<D, PKV_DST_F16>(append, c, k, kr, v, vr, new_lens, clear_rest, err, s); break;                       \
-    default: launch_rows<D, PKV_DST_BF16>(append, c, k, kr, v, vr, new_lens, clear_rest, err, s); break;                               \
+    case PKV_DST_F32: ce = launch_rows<D, PKV_DST_F32>(append, c, k, kr, v, vr, new_lens, clear_rest, err, s); break;                       \
+    case PKV_DST_F16: ce = launch_rows<D, PKV_DST_F16>(append, c, k, kr, v, vr, new_lens, clear_rest, err, s); break;                       \
+    default: ce = launch_rows<D, PKV_DST_BF16>(append, c, k, kr, v, vr, new_lens, clear_rest, err, s); break;                               \
   }
   if (cache->dim == 64) PKV_KV4_ROWS(64) else PKV_KV4_ROWS(128)
 #undef PKV_KV4_ROWS
-  pkv_count_launch();
-  return pkv_cuda_status(cudaGetLastError());
+  return pkv_cuda_status(ce);
 }
 
 }  // namespace

@@ -35,11 +35,12 @@ def atom_bytes(dim: int) -> int:
     return 18 * dim
 
 
-def _raw_stream(index: int) -> int:
-    """The current stream of a device, without the Stream object torch.cuda.current_stream makes where torch can do that."""
-    import torch
-    raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
-    return raw(index) if raw else torch.cuda.current_stream(index).cuda_stream
+def _raw_queries(torch):
+    """(current device, current stream of a device) as plain numbers: torch's own accessors without the Python objects around
+    them where this torch has them (a decode step's call is a few microseconds long)."""
+    device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
+    stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda i: torch.cuda.current_stream(i).cuda_stream)
+    return device, stream
 
 
 class Kv4Cache:
@@ -88,7 +89,8 @@ class Kv4Cache:
         # what a call needs besides its tensors' addresses, prepared once: a decode step makes few microseconds' calls
         self._ref, self._err, self._index = C.byref(self._c), self.error.data_ptr(), self.device.index
         self._rows_of, self._attend_of, self._evict_of = {}, {}, {}
-        self._lib = L.lib()
+        self._lib, self._torch = L.lib(), torch
+        self._current_device, self._current_stream = _raw_queries(torch)
 
     @classmethod
     def allocate(cls, n_layers: int, n_seqs: int, n_kv_heads: int, dim: int, max_tokens: int, *, page_tokens: int = 64,
@@ -130,21 +132,19 @@ class Kv4Cache:
         return r
 
     def _per_seq(self, t, name: str):
-        import torch
         if t is None:
             return None
-        if t.dtype != torch.int32 or tuple(t.shape) != (self.n_seqs,) or not t.is_contiguous() or t.get_device() != self._index:
+        if t.dtype != self._torch.int32 or tuple(t.shape) != (self.n_seqs,) or not t.is_contiguous() or t.get_device() != self._index:
             raise ValueError(f"{name} must be a contiguous int32 [{self.n_seqs}] tensor on {self.device}")
         return t.data_ptr()
 
     def _call(self, fn, *args) -> None:
         """fn(cache, *args, error word, stream) with the cache's device current."""
-        import torch
-        if torch.cuda.current_device() == self._index:
-            status = fn(self._ref, *args, self._err, _raw_stream(self._index))
+        if self._current_device() == self._index:
+            status = fn(self._ref, *args, self._err, self._current_stream(self._index))
         else:
-            with torch.cuda.device(self._index):
-                status = fn(self._ref, *args, self._err, _raw_stream(self._index))
+            with self._torch.cuda.device(self._index):
+                status = fn(self._ref, *args, self._err, self._current_stream(self._index))
         if status:
             L.check(status)
 
@@ -161,16 +161,19 @@ class Kv4Cache:
     def read(self, n: int, dtype=None, new_lens=None, out=None):
         """(k, v) [n_seqs][n][n_kv_heads][dim]: the values the newest tokens stand for, at the rows `append` would take
         them from.  Rows from new_lens[s] on are zeros, or as they were in ``out`` = (k, v)."""
-        import torch
+        torch = self._torch
         fresh = out is None
         if fresh:
-            out = torch.empty((2, self.n_seqs, n, self.n_kv_heads, self.dim), dtype=dtype or torch.float32, device=self.device).unbind(0)
-        k, v = out
-        if k.shape[1] != n or (dtype is not None and k.dtype != dtype):
-            raise ValueError("out does not have the rows or the type asked for")
-        kr, vr = self._rows(k, "k", self.n_kv_heads), self._rows(v, "v", self.n_kv_heads)
-        if k.shape != v.shape:
-            raise ValueError("k and v must have the same shape")
+            shape, dtype = (self.n_seqs, n, self.n_kv_heads, self.dim), dtype or torch.float32
+            k, v = (torch.empty(shape, dtype=dtype, device=self.device) for _ in range(2))
+        else:
+            k, v = out
+            if k.shape[1] != n or (dtype is not None and k.dtype != dtype):
+                raise ValueError("out does not have the rows or the type asked for")
+            if k.shape != v.shape:
+                raise ValueError("k and v must have the same shape")
+        kr = self._rows(k, "k", self.n_kv_heads)
+        vr = kr if fresh else self._rows(v, "v", self.n_kv_heads)
         if k.numel():
             self._call(self._lib.pkv_kv4_read_dev, k.data_ptr(), kr, v.data_ptr(), vr, self._per_seq(new_lens, "new_lens"), int(fresh))
         return k, v
@@ -188,29 +191,31 @@ class Kv4Cache:
         max_len     a bound on the lengths that the host knows (sizes the split of the work; any value is correct)
         lse         f32 [n_seqs][n][n_q_heads], natural logarithm; -inf where a query sees nothing (its out is zeros)
         """
-        import torch
+        torch = self._torch
         qr = self._rows(q, "q")
+        shape = q.shape
         if out is None:
-            out = (torch.empty if q_lens is None else torch.zeros)(q.shape, dtype=q.dtype, device=self.device)
-        elif out.shape != q.shape or out.dtype != q.dtype:
+            out = q.new_empty(shape) if q_lens is None else q.new_zeros(shape)
+        elif out.shape != shape or out.dtype != q.dtype:
             raise ValueError("out must have the shape and type of q")
         outr = self._rows(out, "out")
         if lse is None:
-            lse = (torch.empty if q_lens is None else torch.zeros)(q.shape[:3], dtype=torch.float32, device=self.device)
-        elif lse.shape != q.shape[:3] or lse.dtype != torch.float32 or not lse.is_contiguous() or lse.get_device() != self._index:
+            lse = (q.new_empty if q_lens is None else q.new_zeros)(shape[:3], dtype=torch.float32)
+        elif lse.shape != shape[:3] or lse.dtype != torch.float32 or not lse.is_contiguous() or lse.get_device() != self._index:
             raise ValueError("lse must be contiguous f32 [n_seqs][tokens][heads] on the cache's device")
-        if q.numel() == 0:
-            return out, lse
-        key = (q.shape, q.dtype, scale, window, sinks, accumulate, max_len)
+        key = (shape, q.dtype, scale, window, sinks, accumulate, max_len)
         plan = self._attend_of.get(key)
         if plan is None:
             if accumulate and self.mass is None:
                 raise ValueError("accumulate needs a cache with mass")
-            args = L.Kv4AttendC(self.dim ** -0.5 if scale is None else scale, q.shape[2], window, sinks, int(accumulate), max_len)
+            args = L.Kv4AttendC(self.dim ** -0.5 if scale is None else scale, shape[2], window, sinks, int(accumulate), max_len)
             if len(self._attend_of) >= 256:
                 self._attend_of.clear()
-            plan = self._attend_of[key] = (C.byref(args), self._lib.pkv_kv4_attend_workspace_bytes(self._ref, qr, C.byref(args)))
-        args, need = plan
+            plan = self._attend_of[key] = (C.byref(args), self._lib.pkv_kv4_attend_workspace_bytes(self._ref, qr, C.byref(args)),
+                                           q.numel() == 0)
+        args, need, empty = plan
+        if empty:
+            return out, lse
         work = torch.empty(need, dtype=torch.uint8, device=self.device) if need else None
         self._call(self._lib.pkv_kv4_attend_dev, q.data_ptr(), qr, out.data_ptr(), outr, lse.data_ptr(),
                    self._per_seq(q_lens, "q_lens"), args, work.data_ptr() if need else None, need)
@@ -220,7 +225,7 @@ class Kv4Cache:
         """Cuts every sequence longer than `budget` down to it, per kv head: positions below `sinks`, the `recent` newest
         positions, and the heaviest of the others stay (ties: the lowest slot).  Then ``lens.clamp_(max=budget)``, once
         all layers are done."""
-        import torch
+        torch = self._torch
         if self.positions is None or self.mass is None:
             raise ValueError("evict needs a cache with positions and mass")
         if self.n_seqs == 0:
@@ -235,10 +240,9 @@ class Kv4Cache:
 
     def check(self) -> None:
         """Waits for the stream, raises PkvError for the first thing a kernel reported since the last check, and clears it."""
-        import torch
         code, index = C.c_int32(0), C.c_int64(-1)
-        with torch.cuda.device(self._index):
-            s = _raw_stream(self._index)
+        with self._torch.cuda.device(self._index):
+            s = self._current_stream(self._index)
             st = self._lib.pkv_error_word_read(self._err, s, C.byref(code), C.byref(index))
             if st != L.OK:
                 L.check(self._lib.pkv_error_word_reset(self._err, s))
