@@ -165,7 +165,8 @@ class Kv4Cache:
         fresh = out is None
         if fresh:
             shape, dtype = (self.n_seqs, n, self.n_kv_heads, self.dim), dtype or torch.float32
-            k, v = (torch.empty(shape, dtype=dtype, device=self.device) for _ in range(2))
+            k = self.pages.new_empty(shape, dtype=dtype)
+            v = torch.empty_like(k)
         else:
             k, v = out
             if k.shape[1] != n or (dtype is not None and k.dtype != dtype):
@@ -195,7 +196,7 @@ class Kv4Cache:
         qr = self._rows(q, "q")
         shape = q.shape
         if out is None:
-            out = q.new_empty(shape) if q_lens is None else q.new_zeros(shape)
+            out = (torch.empty_like if q_lens is None else torch.zeros_like)(q, memory_format=torch.contiguous_format)
         elif out.shape != shape or out.dtype != q.dtype:
             raise ValueError("out must have the shape and type of q")
         outr = self._rows(out, "out")
@@ -216,7 +217,7 @@ class Kv4Cache:
         args, need, empty = plan
         if empty:
             return out, lse
-        work = torch.empty(need, dtype=torch.uint8, device=self.device) if need else None
+        work = self.pages.new_empty(need) if need else None
         self._call(self._lib.pkv_kv4_attend_dev, q.data_ptr(), qr, out.data_ptr(), outr, lse.data_ptr(),
                    self._per_seq(q_lens, "q_lens"), args, work.data_ptr() if need else None, need)
         return out, lse
@@ -225,7 +226,6 @@ class Kv4Cache:
         """Cuts every sequence longer than `budget` down to it, per kv head: positions below `sinks`, the `recent` newest
         positions, and the heaviest of the others stay (ties: the lowest slot).  Then ``lens.clamp_(max=budget)``, once
         all layers are done."""
-        torch = self._torch
         if self.positions is None or self.mass is None:
             raise ValueError("evict needs a cache with positions and mass")
         if self.n_seqs == 0:
@@ -235,7 +235,7 @@ class Kv4Cache:
             if len(self._evict_of) >= 256:
                 self._evict_of.clear()
             need = self._evict_of[budget] = self._lib.pkv_kv4_evict_workspace_bytes(self._ref, budget)
-        work = torch.empty(need, dtype=torch.uint8, device=self.device) if need else None
+        work = self.pages.new_empty(need) if need else None
         self._call(self._lib.pkv_kv4_evict_dev, budget, sinks, recent, work.data_ptr() if need else None, need)
 
     def check(self) -> None:
