@@ -94,7 +94,10 @@ __device__ __forceinline__ void query_values(const AttendParams& p, int s, int h
 }
 
 // One atom's scores: S^T[16 keys][8 NT rows] from its K codes and scales in shared memory.
-template <int D, int NT, bool F32>
+//
+// F32 (queries of two binary16 terms): 0 one term, 1 the terms in operands of their own, 2 side by side in one operand
+// (up to four rows: rows 0..3 the first terms, 4..7 the second; half the products).
+template <int D, int NT, int F32>
 __device__ __forceinline__ void scores_of(const uint8_t* atom, int lane, const uint32_t (&qhi)[NT][D / 16][2],
                                           const uint32_t (&qlo)[NT][D / 16][2], float (&s)[NT][4]) {
   using A = Atom<D>;
@@ -134,7 +137,11 @@ __device__ __forceinline__ void scores_of(const uint8_t* atom, int lane, const u
 #pragma unroll
       for (int n = 0; n < NT; n++) {
         const uint32_t h0 = qhi[n][2 * j + u][0], h1 = qhi[n][2 * j + u][1];
-        if constexpr (F32) {
+        if constexpr (F32 == 2) {
+          float(&hi)[4] = 2 * j < D / 32 ? s[n] : part[n][0];
+          if (2 * j % (D / 32) == 0 && u == 0) mma_first(hi, a[2 * u], b[2 * u], a[2 * u + 1], b[2 * u + 1], h0, h1);
+          else mma(hi, a[2 * u], b[2 * u], a[2 * u + 1], b[2 * u + 1], h0, h1);
+        } else if constexpr (F32 == 1) {
           float(&hi)[4] = 2 * j < D / 32 ? s[n] : part[n][0];
           const uint32_t l0 = qlo[n][2 * j + u][0], l1 = qlo[n][2 * j + u][1];
           if (2 * j % (D / 32) == 0 && u == 0) mma_first(hi, a[2 * u], b[2 * u], a[2 * u + 1], b[2 * u + 1], h0, h1);
@@ -147,17 +154,26 @@ __device__ __forceinline__ void scores_of(const uint8_t* atom, int lane, const u
         }
       }
   }
-  if constexpr (F32) {
+  if constexpr (F32 == 1) {
 #pragma unroll
     for (int n = 0; n < NT; n++)
 #pragma unroll
       for (int i = 0; i < 4; i++) s[n][i] = __fadd_rn(__fadd_rn(s[n][i], part[n][0][i]), part[n][1][i]);
   }
+  if constexpr (F32 == 2) {  // rows r and r + 4 are in lanes that differ in bit 1: both get their sum
+#pragma unroll
+    for (int n = 0; n < NT; n++)
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        const float x = __fadd_rn(s[n][i], part[n][0][i]);
+        s[n][i] = __fadd_rn(x, __shfl_xor_sync(0xffffffffu, x, 2));
+      }
+  }
 }
 
 // O^T += V^T P^T for one atom; p[n][0..1] is the B operand (f32 queries: p[n][2..3] its remainder).
-template <int D, int NT, bool F32, bool FIRST>
-__device__ __forceinline__ void weigh(const uint8_t* atom, int lane, const uint32_t (&p)[NT][F32 ? 4 : 2], float (&o)[D / 16][NT][4]) {
+template <int D, int NT, int F32, bool FIRST>
+__device__ __forceinline__ void weigh(const uint8_t* atom, int lane, const uint32_t (&p)[NT][F32 == 1 ? 4 : 2], float (&o)[D / 16][NT][4]) {
   using A = Atom<D>;
   const int q4 = lane & 3, g = lane >> 2;
   uint32_t m[2][D / 16 * 2];  // [key pair][channel of this lane]: two keys' values of one channel
@@ -198,7 +214,7 @@ __device__ __forceinline__ void weigh(const uint8_t* atom, int lane, const uint3
     for (int n = 0; n < NT; n++) {
       if constexpr (FIRST) mma_first(o[j][n], m[0][2 * j], m[0][2 * j + 1], m[1][2 * j], m[1][2 * j + 1], p[n][0], p[n][1]);
       else mma(o[j][n], m[0][2 * j], m[0][2 * j + 1], m[1][2 * j], m[1][2 * j + 1], p[n][0], p[n][1]);
-      if constexpr (F32) mma(o[j][n], m[0][2 * j], m[0][2 * j + 1], m[1][2 * j], m[1][2 * j + 1], p[n][2], p[n][3]);
+      if constexpr (F32 == 1) mma(o[j][n], m[0][2 * j], m[0][2 * j + 1], m[1][2 * j], m[1][2 * j + 1], p[n][2], p[n][3]);
     }
 }
 
@@ -293,13 +309,14 @@ struct Sums {
   float m[NT][2], l[NT][2];          // reference (log2) and sum of rows 2 (lane % 4) + e; l is this lane's part
 };
 
-// Streams a warp's units; whole warp.  DIRECT: units v, v + kWarps, .. of row tile `t`; the sums stay in `r`.
+// Streams a warp's units; whole warp.  PAIRED: f32 queries, at most four rows in all, the two terms of queries and weights
+// side by side in operands of eight rows.  DIRECT: units v, v + kWarps, .. of row tile `t`; the sums stay in `r`.
 // Otherwise: `count` units from unit v of row tile `t` on (number `at` of all rows' units), into the next row tiles; every row tile's sums are written
 // when it ends, into out if the run has all of it, else into the run's parts.
-template <int D, int NT, int T, bool DIRECT>
+template <int D, int NT, int T, bool DIRECT, bool PAIRED>
 __device__ __forceinline__ void stream_units(const AttendParams& p, Cursor t, int v, int count, Ring& ring, Sums<D, NT>& r,
                                              Runs runs = Runs(), unsigned at = 0) {
-  constexpr bool F32 = T == PKV_DST_F32;
+  constexpr int F32 = T != PKV_DST_F32 ? 0 : PAIRED ? 2 : 1;
   constexpr int STEP = DIRECT ? kWarps : 1;
   using A = Atom<D>;
   using S = Shared<D, NT>;
@@ -307,7 +324,7 @@ __device__ __forceinline__ void stream_units(const AttendParams& p, Cursor t, in
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0);
   float qx[NT][D / 4];  // the queries' values are on their way while the first page numbers and units are
 #pragma unroll
-  for (int n = 0; n < NT; n++) query_values<D, T>(p, t.s, t.h, t.tile * 8 * NT + 8 * n + g, t.rows(p), qx[n]);
+  for (int n = 0; n < NT; n++) query_values<D, T>(p, t.s, t.h, t.tile * 8 * NT + 8 * n + (PAIRED ? g & 3 : g), t.rows(p), qx[n]);
 
   // ---- the stream.  Page numbers are fetched for up to kBatch units of a row tile at once, one atom per lane, a batch ahead
   // of their use.
@@ -380,6 +397,12 @@ __device__ __forceinline__ void stream_units(const AttendParams& p, Cursor t, in
 #pragma unroll
     for (int n = 0; n < NT; n++) {
       const float inv = query_operand<D, T>(qx[n], p.negate, qhi[n], qlo[n]);
+      if constexpr (PAIRED) {
+#pragma unroll
+        for (int j = 0; j < D / 16; j++)
+#pragma unroll
+          for (int e = 0; e < 2; e++) qhi[n][j][e] = g < 4 ? qhi[n][j][e] : qlo[n][j][e];
+      }
       const float f = __fmul_rn(__fmul_rn(p.scale, kLog2e), kScaleShift);
 #pragma unroll
       for (int e = 0; e < 2; e++) factor[n][e] = __fmul_rn(f, __shfl_sync(0xffffffffu, inv, 4 * (2 * q4 + e)));
@@ -407,6 +430,14 @@ __device__ __forceinline__ void stream_units(const AttendParams& p, Cursor t, in
       }
   };
   auto join_lanes = [&]() {
+    if constexpr (PAIRED) {  // what the first and the second terms of the weights gave
+#pragma unroll
+      for (int j = 0; j < D / 16; j++)
+#pragma unroll
+        for (int n = 0; n < NT; n++)
+#pragma unroll
+          for (int i = 0; i < 4; i++) r.o[j][n][i] = __fadd_rn(r.o[j][n][i], __shfl_xor_sync(0xffffffffu, r.o[j][n][i], 2));
+    }
 #pragma unroll
     for (int n = 0; n < NT; n++)
 #pragma unroll
@@ -434,7 +465,7 @@ __device__ __forceinline__ void stream_units(const AttendParams& p, Cursor t, in
           x[2 * j] = __fmul_rn(r.o[j][n][e], kScaleShift);
           x[2 * j + 1] = __fmul_rn(r.o[j][n][2 + e], kScaleShift / 16.0f);
         }
-        if (row0 + row < t.rows(p)) {
+        if (row0 + row < t.rows(p) && (!PAIRED || q4 < 2)) {
           if (n_units < t.units) {  // a row that starts here and goes on has the run's second place
             const int64_t slot = ((int64_t)run * 2 + (v0 == 0)) * (8 * NT) + row;
             store_f32<PKV_DST_F32, D / 8>(p.part_o + slot * D + g * (D / 8), x);
@@ -521,7 +552,7 @@ __device__ __forceinline__ void stream_units(const AttendParams& p, Cursor t, in
               for (int n = 0; n < NT; n++)
 #pragma unroll
                 for (int e = 0; e < 2; e++) {
-                  const int d = pos0 + (row0 + 8 * n + 2 * q4 + e) / p.group - kp;
+                  const int d = pos0 + (row0 + 8 * n + (PAIRED ? 2 * q4 & 3 : 2 * q4) + e) / p.group - kp;
                   const bool see = held && d >= 0 && (p.window == 0 || d < p.window || kp < p.sinks);
                   float& x = sc[a][n][2 * hh + e];
                   x = see ? __fmul_rn(x, factor[n][e]) : -INFINITY;
@@ -537,7 +568,7 @@ __device__ __forceinline__ void stream_units(const AttendParams& p, Cursor t, in
               const int at = 16 * a + 8 * hh + tau(g);
 #pragma unroll
               for (int n = 0; n < NT; n++)
-                if (token0 + 32 * k + at < len)
+                if (token0 + 32 * k + at < len && (!PAIRED || q4 < 2))
                   *reinterpret_cast<float2*>(to + at * (8 * NT) + 8 * n) =
                       make_float2(__fmul_rn(sc[a][n][2 * hh], fac[n][0]), __fmul_rn(sc[a][n][2 * hh + 1], fac[n][1]));
             }
@@ -571,7 +602,7 @@ __device__ __forceinline__ void stream_units(const AttendParams& p, Cursor t, in
               }
             }
         }
-        uint32_t pb[2][NT][F32 ? 4 : 2];
+        uint32_t pb[2][NT][F32 == 1 ? 4 : 2];
 #pragma unroll
         for (int n = 0; n < NT; n++) {
           float base[2];
@@ -585,9 +616,14 @@ __device__ __forceinline__ void stream_units(const AttendParams& p, Cursor t, in
               const float w1 = exp2_fast(__fmaf_rn(sc[a][n][2 * hh + 1], fac[n][1], base[1]));
               r.l[n][0] = __fadd_rn(r.l[n][0], w0);
               r.l[n][1] = __fadd_rn(r.l[n][1], w1);
-              const uint32_t hw = half2_of(w0, w1);
+              uint32_t hw = half2_of(w0, w1);
+              if constexpr (F32 == 2) {  // lanes of rows 4..7 hold the second terms
+                const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&hw));
+                const uint32_t rest = half2_of(__fsub_rn(w0, f.x), __fsub_rn(w1, f.y));
+                hw = q4 < 2 ? hw : rest;
+              }
               pb[a][n][hh] = transpose8(hw);
-              if constexpr (F32) {
+              if constexpr (F32 == 1) {
                 const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&hw));
                 pb[a][n][2 + hh] = transpose8(half2_of(__fsub_rn(w0, f.x), __fsub_rn(w1, f.y)));
               }
@@ -626,7 +662,7 @@ __device__ __forceinline__ void stream_units(const AttendParams& p, Cursor t, in
       t.next(p);
       v = 0;
 #pragma unroll
-      for (int n = 0; n < NT; n++) query_values<D, T>(p, t.s, t.h, t.tile * 8 * NT + 8 * n + g, t.rows(p), qx[n]);
+      for (int n = 0; n < NT; n++) query_values<D, T>(p, t.s, t.h, t.tile * 8 * NT + 8 * n + (PAIRED ? g & 3 : g), t.rows(p), qx[n]);
     }
   }
 }
@@ -634,7 +670,7 @@ __device__ __forceinline__ void stream_units(const AttendParams& p, Cursor t, in
 // CTAs an SM holds: as many as the registers of the sums, the queries and (f32) their second terms leave room for.
 __host__ __device__ constexpr int ctas_per_sm(int dim, int nt, bool f32) { return nt == 1 && !(f32 && dim == 128) ? 3 : 2; }
 
-template <int D, int NT, int T, bool DIRECT>
+template <int D, int NT, int T, bool DIRECT, bool PAIRED>
 __global__ void __launch_bounds__(kWarps * 32, ctas_per_sm(D, NT, T == PKV_DST_F32))
 kv4_attend_kernel(const __grid_constant__ AttendParams p) {
   using S = Shared<D, NT>;
@@ -661,7 +697,7 @@ kv4_attend_kernel(const __grid_constant__ AttendParams p) {
     t.place(p);
     const int row0 = tile * 8 * NT, rows = t.rows(p) - row0;  // rows of this tile that exist (may be more than it holds)
     if (rows <= 0) return;
-    stream_units<D, NT, T, true>(p, t, warp, t.span.count > warp ? (t.span.count - warp + kWarps - 1) / kWarps : 0, ring, r);
+    stream_units<D, NT, T, true, PAIRED>(p, t, warp, t.span.count > warp ? (t.span.count - warp + kWarps - 1) / kWarps : 0, ring, r);
     if (g == 0)
 #pragma unroll
       for (int n = 0; n < NT; n++)
@@ -734,7 +770,7 @@ kv4_attend_kernel(const __grid_constant__ AttendParams p) {
   t.h = ht / (unsigned)t.tiles;
   t.tile = ht - t.h * t.tiles;
   t.place(p);
-  stream_units<D, NT, T, false>(p, t, (int)(off - ht * t.units), count, ring, r, runs, at);
+  stream_units<D, NT, T, false, PAIRED>(p, t, (int)(off - ht * t.units), count, ring, r, runs, at);
   }
 }
 
@@ -989,7 +1025,11 @@ Plan make_plan(const Cache& c, int dim, const pkv_kv4_rows* q, const pkv_kv4_att
 
 template <int D, int NT, int T>
 int launch_attend(const AttendParams& p, cudaStream_t s) {
-  auto kernel = p.runs ? kv4_attend_kernel<D, NT, T, false> : kv4_attend_kernel<D, NT, T, true>;
+  auto kernel = p.runs ? kv4_attend_kernel<D, NT, T, false, false> : kv4_attend_kernel<D, NT, T, true, false>;
+  // f32 with up to four rows a kv head: paired terms, half the matrix instructions.  8 sequences of 4096 tokens, 32 heads of 64,
+  // one row: 32.5 us, 35.5 with the terms in operands of their own; 16 of 8192, 8 heads of 128, four rows: 47.6, 51.9.
+  if constexpr (T == PKV_DST_F32 && NT == 1)
+    if (p.q.n * p.group <= 4) kernel = p.runs ? kv4_attend_kernel<D, NT, T, false, true> : kv4_attend_kernel<D, NT, T, true, true>;
   constexpr int bytes = Shared<D, NT>::BYTES;
   if (bytes > 48 * 1024)
     if (cudaError_t ce = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes)) return pkv_cuda_status(ce);
