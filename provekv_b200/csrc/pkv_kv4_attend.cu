@@ -19,6 +19,8 @@
 //                whatever the lengths.  The stream of units runs on from one row into the next.  A row that was cut is joined
 //                by a second launch from the warps' sums.
 //
+#include <limits.h>
+
 #include "pkv_kv4_attend.cuh"
 
 using namespace pkv_kv4;
@@ -28,9 +30,8 @@ namespace {
 constexpr int kWarps = 4;
 constexpr int kStages = 2;
 constexpr int kMaxRows = 2048;           // (sequence, kv head, row tile)s that share runs
-constexpr int kJoinWarps = 8;
 constexpr int64_t kMostScores = 1ll << 26;  // 256 MiB
-constexpr int kMassTokens = 32;  // keys a warp of the mass kernel holds
+constexpr int kMassTokens = 32, kMassWarps = 8;  // keys a warp of the mass kernel holds; its warps
 __device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
@@ -93,6 +94,37 @@ __device__ __forceinline__ void query_values(const AttendParams& p, int s, int h
   }
 }
 
+// A lane's part of an atom's keys: tokens tau(lane / 4) and 8 on, channels (lane % 4) D/4 ..
+template <int D>
+struct KeyCodes {
+  uint32_t w0[D / 32], w1[D / 32];
+  Scale sc0[D / 64], sc1[D / 64];
+  __device__ __forceinline__ KeyCodes(const uint8_t* atom, int lane) {
+    using A = Atom<D>;
+    const int q4 = lane & 3, t0 = tau(lane >> 2), t1 = t0 + 8;
+    if constexpr (D == 128) {
+      const uint4 a = *reinterpret_cast<const uint4*>(atom + A::KC + t0 * A::ROW + 16 * q4);
+      const uint4 b = *reinterpret_cast<const uint4*>(atom + A::KC + t1 * A::ROW + 16 * q4);
+      w0[0] = a.x; w0[1] = a.y; w0[2] = a.z; w0[3] = a.w;
+      w1[0] = b.x; w1[1] = b.y; w1[2] = b.z; w1[3] = b.w;
+      const uint32_t u0 = *reinterpret_cast<const uint16_t*>(atom + A::KS + t0 * A::SROW + 2 * q4);
+      const uint32_t u1 = *reinterpret_cast<const uint16_t*>(atom + A::KS + t1 * A::SROW + 2 * q4);
+      const Scale p0 = scale_of(__byte_perm(u0, 0u, 0x4140) << 7), p1 = scale_of(__byte_perm(u1, 0u, 0x4140) << 7);
+      sc0[0] = p0.low();
+      sc0[1] = p0.high();
+      sc1[0] = p1.low();
+      sc1[1] = p1.high();
+    } else {
+      const uint2 a = *reinterpret_cast<const uint2*>(atom + A::KC + t0 * A::ROW + 8 * q4);
+      const uint2 b = *reinterpret_cast<const uint2*>(atom + A::KC + t1 * A::ROW + 8 * q4);
+      w0[0] = a.x; w0[1] = a.y;
+      w1[0] = b.x; w1[1] = b.y;
+      sc0[0] = scale_of((uint32_t)atom[A::KS + t0 * A::SROW + q4] * 0x00800080u);
+      sc1[0] = scale_of((uint32_t)atom[A::KS + t1 * A::SROW + q4] * 0x00800080u);
+    }
+  }
+};
+
 // One atom's scores: S^T[16 keys][8 NT rows] from its K codes and scales in shared memory.
 //
 // F32 (queries of two binary16 terms): 0 one term, 1 the terms in operands of their own, 2 side by side in one operand
@@ -100,38 +132,15 @@ __device__ __forceinline__ void query_values(const AttendParams& p, int s, int h
 template <int D, int NT, int F32>
 __device__ __forceinline__ void scores_of(const uint8_t* atom, int lane, const uint32_t (&qhi)[NT][D / 16][2],
                                           const uint32_t (&qlo)[NT][D / 16][2], float (&s)[NT][4]) {
-  using A = Atom<D>;
-  const int q4 = lane & 3, t0 = tau(lane >> 2), t1 = t0 + 8;
-  uint32_t w0[D / 32], w1[D / 32];
-  Scale sc0[D / 64], sc1[D / 64];
-  if constexpr (D == 128) {
-    const uint4 a = *reinterpret_cast<const uint4*>(atom + A::KC + t0 * A::ROW + 16 * q4);
-    const uint4 b = *reinterpret_cast<const uint4*>(atom + A::KC + t1 * A::ROW + 16 * q4);
-    w0[0] = a.x; w0[1] = a.y; w0[2] = a.z; w0[3] = a.w;
-    w1[0] = b.x; w1[1] = b.y; w1[2] = b.z; w1[3] = b.w;
-    const uint32_t u0 = *reinterpret_cast<const uint16_t*>(atom + A::KS + t0 * A::SROW + 2 * q4);
-    const uint32_t u1 = *reinterpret_cast<const uint16_t*>(atom + A::KS + t1 * A::SROW + 2 * q4);
-    const Scale p0 = scale_of(__byte_perm(u0, 0u, 0x4140) << 7), p1 = scale_of(__byte_perm(u1, 0u, 0x4140) << 7);
-    sc0[0] = p0.low();
-    sc0[1] = p0.high();
-    sc1[0] = p1.low();
-    sc1[1] = p1.high();
-  } else {
-    const uint2 a = *reinterpret_cast<const uint2*>(atom + A::KC + t0 * A::ROW + 8 * q4);
-    const uint2 b = *reinterpret_cast<const uint2*>(atom + A::KC + t1 * A::ROW + 8 * q4);
-    w0[0] = a.x; w0[1] = a.y;
-    w1[0] = b.x; w1[1] = b.y;
-    sc0[0] = scale_of((uint32_t)atom[A::KS + t0 * A::SROW + q4] * 0x00800080u);
-    sc1[0] = scale_of((uint32_t)atom[A::KS + t1 * A::SROW + q4] * 0x00800080u);
-  }
+  const KeyCodes<D> k(atom, lane);
   // F32: the tensor cores cut their sums off instead of rounding them; chains of at most D / 32 products of the queries' first
   // terms, the second terms apart, keep that below the f32 error of the sum
   float part[F32 ? NT : 1][2][4];
 #pragma unroll
   for (int j = 0; j < D / 32; j++) {
     uint32_t a[4], b[4];
-    nibbles(w0[j], sc0[j >> 1], a);
-    nibbles(w1[j], sc1[j >> 1], b);
+    nibbles(k.w0[j], k.sc0[j >> 1], a);
+    nibbles(k.w1[j], k.sc1[j >> 1], b);
 #pragma unroll
     for (int u = 0; u < 2; u++)
 #pragma unroll
@@ -779,9 +788,7 @@ kv4_attend_kernel(const __grid_constant__ AttendParams p) {
 template <int D, int NT, int T, int W>
 __global__ void __launch_bounds__(kJoinWarps * 32)
 kv4_combine_kernel(const __grid_constant__ AttendParams p) {
-  __shared__ float s_x[W > 1 ? W : 1][D], s_ml[W > 1 ? W : 1][2];
-  constexpr int N = D / 32, PER = kJoinWarps / W;  // rows per CTA
-  const int lane = threadIdx.x & 31, warp = (threadIdx.x >> 5) % W;
+  constexpr int PER = kJoinWarps / W;  // rows per CTA
   const int s = blockIdx.z, h = blockIdx.y, grow = blockIdx.x * PER + (threadIdx.x >> 5) / W;
   const int tile = grow / (8 * NT), row = grow - tile * (8 * NT);
   wait_for_stream();
@@ -789,74 +796,8 @@ kv4_combine_kernel(const __grid_constant__ AttendParams p) {
   if (qn < 0 || qn > p.q.n) qn = 0;
   if (grow >= qn * p.group) return;
   const int2 of = p.part_of[((int64_t)s * p.c.heads + h) * p.row_tiles + tile];
-  const int first = of.x, parts = of.y;
-  if (parts == 1) return;
-  auto slot_of = [&](int k) { return ((int64_t)(first + k) * 2 + (k == 0)) * (8 * NT) + row; };
-  float m = -INFINITY, l = 0.0f, x[N];
-#pragma unroll
-  for (int i = 0; i < N; i++) x[i] = 0.0f;
-  // a warp's parts: k = warp + W j; references of 32 of them at a time, then the sums, eight loads in flight
-  for (int k0 = warp; k0 < parts; k0 += 32 * W) {
-    const int n = min(32, (parts - k0 + W - 1) / W);
-    float2 ml = make_float2(-INFINITY, 0.0f);
-    if (lane < n) ml = *reinterpret_cast<const float2*>(p.part_ml + slot_of(k0 + lane * W) * 2);
-    float top = ml.x;
-#pragma unroll
-    for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-    top = fmaxf(top, m);
-    const float fold = m == -INFINITY ? 0.0f : exp2_fast(__fsub_rn(m, top));
-    // (a part without a visible key, or with nothing but NaN, has no reference)
-    const float f = ml.x == -INFINITY ? (ml.y == 0.0f ? 0.0f : ml.y) : exp2_fast(__fsub_rn(ml.x, top));
-    float sum = __fmul_rn(f, ml.y);
-#pragma unroll
-    for (int o = 16; o; o >>= 1) sum = __fadd_rn(sum, __shfl_xor_sync(0xffffffffu, sum, o));
-    l = __fmaf_rn(l, fold, sum);
-    m = top;
-#pragma unroll
-    for (int i = 0; i < N; i++) x[i] = __fmul_rn(x[i], fold);
-#pragma unroll 8
-    for (int j = 0; j < n; j++) {
-      const float fj = __shfl_sync(0xffffffffu, f, j);
-      const float* src = p.part_o + slot_of(k0 + j * W) * D + lane * N;
-      float y[N];
-      if constexpr (N == 4) {
-        const float4 v = *reinterpret_cast<const float4*>(src);
-        y[0] = v.x; y[1] = v.y; y[2] = v.z; y[3] = v.w;
-      } else {
-        const float2 v = *reinterpret_cast<const float2*>(src);
-        y[0] = v.x; y[1] = v.y;
-      }
-#pragma unroll
-      for (int i = 0; i < N; i++) x[i] = __fmaf_rn(fj, y[i], x[i]);
-    }
-  }
-  if constexpr (W > 1) {
-#pragma unroll
-    for (int i = 0; i < N; i++) s_x[warp][lane * N + i] = x[i];
-    if (lane == 0) {
-      s_ml[warp][0] = m;
-      s_ml[warp][1] = l;
-    }
-    __syncthreads();
-    if (warp) return;
-    const int w = lane & (W - 1);
-    m = s_ml[w][0];
-#pragma unroll
-    for (int o = W / 2; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-    const float f = s_ml[w][0] == -INFINITY ? (s_ml[w][1] == 0.0f ? 0.0f : s_ml[w][1]) : exp2_fast(__fsub_rn(s_ml[w][0], m));
-    l = __fmul_rn(f, s_ml[w][1]);
-#pragma unroll
-    for (int o = W / 2; o; o >>= 1) l = __fadd_rn(l, __shfl_xor_sync(0xffffffffu, l, o));
-#pragma unroll
-    for (int i = 0; i < N; i++) x[i] = 0.0f;
-#pragma unroll
-    for (int k = 0; k < W; k++) {
-      const float fk = __shfl_sync(0xffffffffu, f, k);
-#pragma unroll
-      for (int i = 0; i < N; i++) x[i] = __fmaf_rn(fk, s_x[k][lane * N + i], x[i]);
-    }
-  }
-  write_row<T, N>(p, s, h, grow, lane * N, x, m, l, lane == 0);
+  if (of.y == 1) return;
+  join_parts<D, T, W>(p, s, h, grow, of.y, [&](int k) { return ((int64_t)(of.x + k) * 2 + (k == 0)) * (8 * NT) + row; });
 }
 
 // mass[key] += sum over the query rows of exp(score - lse), from the scores that the attention kernel left behind; a thread
@@ -894,93 +835,169 @@ kv4_mass_of_scores_kernel(const __grid_constant__ AttendParams p) {
   }
 }
 
-// The same by a second pass over the keys, for more query rows (or where the scores would not fit the workspace).  A warp keeps the dequantised keys of 32 tokens in
-// registers and walks over the rows, so every sum has one owner and one order.
+// The same by a second pass over the keys, for more query rows (or where the scores would not fit the workspace).
+//
+// A warp keeps 32 tokens' dequantised keys in registers as the A operand of S^T = K Q^T and walks over the rows, so every sum
+// has one owner and one order.  The queries come as B operands from shared memory, 64 rows at a time, eight converted by each
+// warp: rows are read and converted once for 256 tokens, keys once in all.  Two exponentials, two multiply-adds and two
+// additions a score pair are left besides the products.  512 rows over 8192 tokens, 8 heads of 128: 54 us (142 with the keys dequantised
+// again for every eight rows).
 template <int D, int T>
-__global__ void __launch_bounds__(kWarps * 32)
+__global__ void __launch_bounds__(kMassWarps * 32, T == PKV_DST_F32 && D == 128 ? 1 : 2)
 kv4_mass_kernel(const __grid_constant__ AttendParams p) {
   constexpr bool F32 = T == PKV_DST_F32;
+  constexpr int TERMS = F32 ? 2 : 1, PER = kMassWarps * kMassTokens;
   using A = Atom<D>;
-  using E = typename PkvDst<T>::type;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  __shared__ uint4 s_q[kMassWarps][TERMS][D / 32][32];
+  __shared__ __align__(16) float2 s_row[kMassWarps][8];  // what turns a product into log2 of a weight: factor, offset
+  const int lane = threadIdx.x & 31, warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0);
   const int g = lane >> 2, q4 = lane & 3;
   const int s = blockIdx.z, h = blockIdx.y;
   wait_for_stream();
-  const int len = p.c.length(s, p.err), end = p.c.end(s, len);
-  int qn = p.q_lens ? p.q_lens[s] : p.q.n;
-  if (qn < 0 || qn > p.q.n) qn = 0;
+  const Sequence seq = sequence_of(p, s);
+  const int len = seq.len, qn = seq.qn;
   if (qn == 0) return;
-  const int pos0 = end - qn, rows = qn * p.group;
-  for (int token0 = (blockIdx.x * kWarps + warp) * kMassTokens; token0 < len; token0 += gridDim.x * kWarps * kMassTokens) {
-  const uint8_t* atom[2];
-  unsigned there = token0 + kMassTokens <= len ? 0xffffffffu : (1u << (len - token0)) - 1u;
-#pragma unroll
-  for (int a = 0; a < 2; a++) {
-    atom[a] = token0 + 16 * a < len ? p.c.atom(s, h, token0 / 16 + a, A::BYTES, p.err) : nullptr;
-    if (!atom[a]) there &= a ? 0x0000ffffu : 0xffff0000u;
-  }
-  if (!there) continue;
+  const int pos0 = seq.end - qn, rows = qn * p.group;
   const bool by_position = p.c.positions != nullptr && (p.window > 0 || qn > 1);
-  int kp[2][2];
-  bool held[2][2];
-#pragma unroll
-  for (int a = 0; a < 2; a++)
-#pragma unroll
-    for (int hh = 0; hh < 2; hh++) {
-      const int t = 16 * a + 8 * hh + tau(g);
-      held[a][hh] = (there >> t) & 1u;
-      kp[a][hh] = by_position && held[a][hh] ? p.c.positions[p.c.stat(s, h) + token0 + t] : token0 + t;
-    }
-  float sum[2][2] = {{0.0f, 0.0f}, {0.0f, 0.0f}};
-  // rows of 8 at a time; a causal row before every key of this warp is passed over
-  int r_first = 0;
-  if (!by_position && qn > 1) r_first = max(0, token0 - pos0) * p.group / 8 * 8;
-  for (int r0 = r_first; r0 < rows; r0 += 8) {
-    if (!by_position && p.window > 0 && token0 >= p.sinks && pos0 + r0 / p.group - (token0 + kMassTokens - 1) >= p.window) break;
-    uint32_t qhi[1][D / 16][2], qlo[1][D / 16][2];
-    const int r = r0 + g, token = r / p.group, hq = h * p.group + (r - token * p.group);
-    float x[D / 4];
-    query_values<D, T>(p, s, h, r, rows, x);
-    const float inv = query_operand<D, T>(x, p.negate, qhi[0], qlo[0]);
-    const float lse = r < rows ? p.lse[((int64_t)s * p.q.n + token) * p.q_heads + hq] : -INFINITY;
-    const float f = __fmul_rn(__fmul_rn(__fmul_rn(p.scale, kLog2e), kScaleShift), inv);
-    float factor[2], base[2];
-    int qpos[2];
-#pragma unroll
-    for (int e = 0; e < 2; e++) {
-      factor[e] = __shfl_sync(0xffffffffu, f, 4 * (2 * q4 + e));
-      base[e] = __fmul_rn(kLog2e, __shfl_sync(0xffffffffu, lse, 4 * (2 * q4 + e)));
-      qpos[e] = pos0 + (r0 + 2 * q4 + e) / p.group;
-    }
+  for (int cta0 = blockIdx.x * PER; cta0 < len; cta0 += gridDim.x * PER) {
+    const int token0 = cta0 + warp * kMassTokens;
+    unsigned there = token0 >= len ? 0u : token0 + kMassTokens <= len ? 0xffffffffu : (1u << (len - token0)) - 1u;
+    uint32_t key[2][D / 32][2][4];  // [atom][16 channels of a lane's D / 4][half atom]
 #pragma unroll
     for (int a = 0; a < 2; a++) {
-      if (!atom[a]) continue;
-      float sc[1][4];
-      scores_of<D, 1, F32>(atom[a], lane, qhi, qlo, sc);
+      const uint8_t* atom = token0 + 16 * a < len ? p.c.atom(s, h, token0 / 16 + a, A::BYTES, p.err) : nullptr;
+      if (atom) {
+        const KeyCodes<D> k(atom, lane);
 #pragma unroll
-      for (int hh = 0; hh < 2; hh++)
-#pragma unroll
-        for (int e = 0; e < 2; e++) {
-          const int d = qpos[e] - kp[a][hh];
-          const bool see = r0 + 2 * q4 + e < rows && held[a][hh] && d >= 0 &&
-                           (p.window == 0 || d < p.window || kp[a][hh] < p.sinks);
-          const float w = see ? exp2_fast(__fsub_rn(__fmul_rn(sc[0][2 * hh + e], factor[e]), base[e])) : 0.0f;
-          sum[a][hh] = __fadd_rn(sum[a][hh], w);
+        for (int j = 0; j < D / 32; j++) {
+          nibbles(k.w0[j], k.sc0[j >> 1], key[a][j][0]);
+          nibbles(k.w1[j], k.sc1[j >> 1], key[a][j][1]);
         }
-    }
-  }
+      } else {
+        there &= a ? 0x0000ffffu : 0xffff0000u;
 #pragma unroll
-  for (int a = 0; a < 2; a++)
+        for (int j = 0; j < D / 32; j++)
 #pragma unroll
-    for (int hh = 0; hh < 2; hh++) {
-      float t = sum[a][hh];
-      t = __fadd_rn(t, __shfl_xor_sync(0xffffffffu, t, 1));
-      t = __fadd_rn(t, __shfl_xor_sync(0xffffffffu, t, 2));
-      if (q4 == 0 && held[a][hh]) {
-        float* m = p.c.mass + p.c.stat(s, h) + token0 + 16 * a + 8 * hh + tau(g);
-        *m = __fadd_rn(*m, t);
+          for (int i = 0; i < 4; i++) key[a][j][0][i] = key[a][j][1][i] = 0u;
       }
     }
+    // positions of the keys, their least and greatest
+    int kp[2][2], k_min = INT_MAX, k_max = INT_MIN;
+    bool held[2][2];
+#pragma unroll
+    for (int a = 0; a < 2; a++)
+#pragma unroll
+      for (int hh = 0; hh < 2; hh++) {
+        const int t = 16 * a + 8 * hh + tau(g);
+        held[a][hh] = (there >> t) & 1u;
+        kp[a][hh] = by_position && held[a][hh] ? __ldg(p.c.positions + p.c.stat(s, h) + token0 + t) : token0 + t;
+        if (held[a][hh]) {
+          k_min = min(k_min, kp[a][hh]);
+          k_max = max(k_max, kp[a][hh]);
+        }
+      }
+    k_min = __reduce_min_sync(0xffffffffu, k_min);
+    k_max = __reduce_max_sync(0xffffffffu, k_max);
+    float sum[2][2] = {{0.0f, 0.0f}, {0.0f, 0.0f}};
+    // causal rows before every key of this CTA are passed over
+    int r_first = 0;
+    if (!by_position && qn > 1) r_first = max(0, cta0 - pos0) * p.group / 8 * 8;
+    for (int r0 = r_first; r0 < rows; r0 += 8 * kMassWarps) {
+      if (!by_position && p.window > 0 && cta0 >= p.sinks && pos0 + r0 / p.group - (cta0 + PER - 1) >= p.window) break;
+      __syncthreads();  // the rows before these have been used
+      if (r0 + 8 * warp < rows) {
+        uint32_t hi[D / 16][2], lo[D / 16][2];
+        float x[D / 4];
+        const int r = r0 + 8 * warp + g, token = r / p.group, hq = h * p.group + (r - token * p.group);
+        const float lse = r < rows ? p.lse[((int64_t)s * p.q.n + token) * p.q_heads + hq] : -INFINITY;
+        query_values<D, T>(p, s, h, r, rows, x);
+        const float inv = query_operand<D, T>(x, p.negate, hi, lo);
+#pragma unroll
+        for (int i = 0; i < D / 32; i++) {
+          s_q[warp][0][i][lane] = make_uint4(hi[2 * i][0], hi[2 * i][1], hi[2 * i + 1][0], hi[2 * i + 1][1]);
+          if constexpr (F32) s_q[warp][TERMS - 1][i][lane] = make_uint4(lo[2 * i][0], lo[2 * i][1], lo[2 * i + 1][0], lo[2 * i + 1][1]);
+        }
+        // (a row that sees nothing, or behind the last one, weighs nothing)
+        if (q4 == 0)
+          s_row[warp][g] = lse == -INFINITY ? make_float2(0.0f, -INFINITY)
+                                            : make_float2(__fmul_rn(__fmul_rn(__fmul_rn(p.scale, kLog2e), kScaleShift), inv),
+                                                          -__fmul_rn(kLog2e, lse));
+      }
+      __syncthreads();
+      if (!there) continue;
+#pragma unroll 1
+      for (int k = 0; k < kMassWarps; k++) {
+        const int ra = r0 + 8 * k;
+        if (ra >= rows) break;
+        const int first = pos0 + ra / p.group, last = pos0 + min(rows - 1, ra + 7) / p.group;
+        if (last < k_min || (p.window > 0 && first - k_max >= p.window && k_min >= p.sinks)) continue;
+        float sc[2][4], part[2][2][4];
+#pragma unroll
+        for (int j = 0; j < D / 32; j++) {
+          const uint4 q = s_q[k][0][j][lane];
+#pragma unroll
+          for (int a = 0; a < 2; a++) {
+            const uint32_t(&w)[2][4] = key[a][j];
+            // f32 queries: chains as in scores_of
+            float(&c)[4] = F32 && 2 * j >= D / 32 ? part[a][0] : sc[a];
+            if (j == 0 || (F32 && 2 * j == D / 32)) mma_first(c, w[0][0], w[1][0], w[0][1], w[1][1], q.x, q.y);
+            else mma(c, w[0][0], w[1][0], w[0][1], w[1][1], q.x, q.y);
+            mma(c, w[0][2], w[1][2], w[0][3], w[1][3], q.z, q.w);
+          }
+          if constexpr (F32) {
+            const uint4 q2 = s_q[k][1][j][lane];
+#pragma unroll
+            for (int a = 0; a < 2; a++) {
+              const uint32_t(&w)[2][4] = key[a][j];
+              if (j == 0) mma_first(part[a][1], w[0][0], w[1][0], w[0][1], w[1][1], q2.x, q2.y);
+              else mma(part[a][1], w[0][0], w[1][0], w[0][1], w[1][1], q2.x, q2.y);
+              mma(part[a][1], w[0][2], w[1][2], w[0][3], w[1][3], q2.z, q2.w);
+            }
+          }
+        }
+        if constexpr (F32) {
+#pragma unroll
+          for (int a = 0; a < 2; a++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) sc[a][i] = __fadd_rn(__fadd_rn(sc[a][i], part[a][0][i]), part[a][1][i]);
+        }
+        const float4 f = *reinterpret_cast<const float4*>(&s_row[k][2 * q4]);
+        const bool all = there == 0xffffffffu && first >= k_max && (p.window == 0 || last - k_min < p.window) && ra + 8 <= rows;
+        if (all) {
+#pragma unroll
+          for (int a = 0; a < 2; a++)
+#pragma unroll
+            for (int hh = 0; hh < 2; hh++)
+              sum[a][hh] = __fadd_rn(sum[a][hh], __fadd_rn(exp2_fast(__fmaf_rn(sc[a][2 * hh], f.x, f.y)),
+                                                           exp2_fast(__fmaf_rn(sc[a][2 * hh + 1], f.z, f.w))));
+        } else {
+#pragma unroll
+          for (int e = 0; e < 2; e++) {
+            const int row = ra + 2 * q4 + e, qpos = pos0 + row / p.group;
+#pragma unroll
+            for (int a = 0; a < 2; a++)
+#pragma unroll
+              for (int hh = 0; hh < 2; hh++) {
+                const int d = qpos - kp[a][hh];
+                const bool see = row < rows && held[a][hh] && d >= 0 && (p.window == 0 || d < p.window || kp[a][hh] < p.sinks);
+                if (see) sum[a][hh] = __fadd_rn(sum[a][hh], exp2_fast(__fmaf_rn(sc[a][2 * hh + e], e ? f.z : f.x, e ? f.w : f.y)));
+              }
+          }
+        }
+      }
+    }
+#pragma unroll
+    for (int a = 0; a < 2; a++)
+#pragma unroll
+      for (int hh = 0; hh < 2; hh++) {
+        float t = sum[a][hh];
+        t = __fadd_rn(t, __shfl_xor_sync(0xffffffffu, t, 1));
+        t = __fadd_rn(t, __shfl_xor_sync(0xffffffffu, t, 2));
+        if (q4 == 0 && held[a][hh]) {
+          float* m = p.c.mass + p.c.stat(s, h) + token0 + 16 * a + 8 * hh + tau(g);
+          *m = __fadd_rn(*m, t);
+        }
+      }
   }
 }
 
@@ -1052,9 +1069,9 @@ int launch_all(const AttendParams& p, int nt, bool accumulate, int longest, cuda
   if (p.scores)
     return pkv_cuda_status(launch_early(nt == 1 ? kv4_mass_of_scores_kernel<1> : kv4_mass_of_scores_kernel<2>,
                                         dim3((longest + 255) / 256, p.c.heads, p.c.n_seqs), 256, 0, s, p));
-  const int per = kWarps * kMassTokens;
+  const int per = kMassWarps * kMassTokens;
   return pkv_cuda_status(
-      launch_early(kv4_mass_kernel<D, T>, dim3((longest + per - 1) / per, p.c.heads, p.c.n_seqs), kWarps * 32, 0, s, p));
+      launch_early(kv4_mass_kernel<D, T>, dim3((longest + per - 1) / per, p.c.heads, p.c.n_seqs), kMassWarps * 32, 0, s, p));
 }
 
 int check_args(const Cache& c, const pkv_kv4_rows* q, const pkv_kv4_attend_args* a) {

@@ -9,6 +9,7 @@
 namespace pkv_kv4 {
 
 constexpr int kUnitAtoms = 4, kUnitTokens = kUnitAtoms * kAtomTokens;
+constexpr int kJoinWarps = 8;
 constexpr int kBatch = 32 / kUnitAtoms;  // units whose page numbers a warp fetches at once
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 // Weights are kept times 2^7 and the running reference may lag the true maximum by 2^8: a weight in binary16 is at most
@@ -117,6 +118,80 @@ __device__ __forceinline__ void write_row(const AttendParams& p, int s, int h, i
   if (p.lse && first)
     p.lse[((int64_t)s * p.q.n + token) * p.q_heads + hq] =
         l == 0.0f ? -INFINITY : __fmul_rn(kLn2, __fadd_rn(m, __fsub_rn(log2f(l), kWeightShift)));
+}
+
+// Joins the parts of query row `row` and writes it: W warps of a CTA (all of it, or one warp alone), each every W-th part.
+// slot_of(k): which row of part_o and part_ml is part k's.
+template <int D, int T, int W, typename SlotOf>
+__device__ __forceinline__ void join_parts(const AttendParams& p, int s, int h, int row, int parts, SlotOf slot_of) {
+  constexpr int N = D / 32;
+  __shared__ float s_x[W > 1 ? W : 1][D], s_ml[W > 1 ? W : 1][2];
+  const int lane = threadIdx.x & 31, warp = W > 1 ? threadIdx.x >> 5 : 0;
+  float m = -INFINITY, l = 0.0f, x[N];
+#pragma unroll
+  for (int i = 0; i < N; i++) x[i] = 0.0f;
+  // a warp's parts: k = warp + W j; references of 32 of them at a time, then the sums, eight loads in flight
+  for (int k0 = warp; k0 < parts; k0 += 32 * W) {
+    const int n = min(32, (parts - k0 + W - 1) / W);
+    float2 ml = make_float2(-INFINITY, 0.0f);
+    if (lane < n) ml = *reinterpret_cast<const float2*>(p.part_ml + slot_of(k0 + lane * W) * 2);
+    float top = ml.x;
+#pragma unroll
+    for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    top = fmaxf(top, m);
+    const float fold = m == -INFINITY ? 0.0f : exp2_fast(__fsub_rn(m, top));
+    // (a part without a visible key, or with nothing but NaN, has no reference)
+    const float f = ml.x == -INFINITY ? (ml.y == 0.0f ? 0.0f : ml.y) : exp2_fast(__fsub_rn(ml.x, top));
+    float sum = __fmul_rn(f, ml.y);
+#pragma unroll
+    for (int o = 16; o; o >>= 1) sum = __fadd_rn(sum, __shfl_xor_sync(0xffffffffu, sum, o));
+    l = __fmaf_rn(l, fold, sum);
+    m = top;
+#pragma unroll
+    for (int i = 0; i < N; i++) x[i] = __fmul_rn(x[i], fold);
+#pragma unroll 8
+    for (int j = 0; j < n; j++) {
+      const float fj = __shfl_sync(0xffffffffu, f, j);
+      const float* src = p.part_o + slot_of(k0 + j * W) * D + lane * N;
+      float y[N];
+      if constexpr (N == 4) {
+        const float4 v = *reinterpret_cast<const float4*>(src);
+        y[0] = v.x; y[1] = v.y; y[2] = v.z; y[3] = v.w;
+      } else {
+        const float2 v = *reinterpret_cast<const float2*>(src);
+        y[0] = v.x; y[1] = v.y;
+      }
+#pragma unroll
+      for (int i = 0; i < N; i++) x[i] = __fmaf_rn(fj, y[i], x[i]);
+    }
+  }
+  if constexpr (W > 1) {
+#pragma unroll
+    for (int i = 0; i < N; i++) s_x[warp][lane * N + i] = x[i];
+    if (lane == 0) {
+      s_ml[warp][0] = m;
+      s_ml[warp][1] = l;
+    }
+    __syncthreads();
+    if (warp) return;
+    const int w = lane & (W - 1);
+    m = s_ml[w][0];
+#pragma unroll
+    for (int o = W / 2; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    const float f = s_ml[w][0] == -INFINITY ? (s_ml[w][1] == 0.0f ? 0.0f : s_ml[w][1]) : exp2_fast(__fsub_rn(s_ml[w][0], m));
+    l = __fmul_rn(f, s_ml[w][1]);
+#pragma unroll
+    for (int o = W / 2; o; o >>= 1) l = __fadd_rn(l, __shfl_xor_sync(0xffffffffu, l, o));
+#pragma unroll
+    for (int i = 0; i < N; i++) x[i] = 0.0f;
+#pragma unroll
+    for (int k = 0; k < W; k++) {
+      const float fk = __shfl_sync(0xffffffffu, f, k);
+#pragma unroll
+      for (int i = 0; i < N; i++) x[i] = __fmaf_rn(fk, s_x[k][lane * N + i], x[i]);
+    }
+  }
+  write_row<T, N>(p, s, h, row, lane * N, x, m, l, lane == 0);
 }
 
 inline int sm_count() {

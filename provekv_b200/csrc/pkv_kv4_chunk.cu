@@ -1,4 +1,4 @@
-// Attention over the 4-bit KV cache for many query rows per kv head (prompt chunks, drafts), 16-bit queries.
+// Attention over the 4-bit KV cache for many query rows per kv head (prompt chunks), 16-bit queries.
 //
 // A CTA takes up to 256 query rows of one kv head (two tiles of 128) over a run of units of 64 tokens, on the fifth-
 // generation tensor cores:
@@ -446,8 +446,19 @@ kv4_chunk_kernel(const __grid_constant__ ChunkParams cp) {
     const int32_t* positions = by_position ? p.c.positions + p.c.stat(s, h) : nullptr;
     const int tile_first = pos0 + (row0 + kTileRows * t) / p.group;
     const int tile_last = pos0 + min(seq.qn - 1, (row0 + kTileRows * t + kTileRows - 1) / p.group);
+    // positions of a unit's tokens, two a lane, loaded a unit ahead.  Only units with a token that some row of the tile must not
+    // see are masked token by token.
+    int kp[2] = {0, 0};
+    auto load_positions = [&](int i) {
+      const int at = i < n ? span.unit(first + i) * kUnitTokens + lane : len;
+#pragma unroll
+      for (int e = 0; e < 2; e++) kp[e] = at + 32 * e < len ? __ldg(positions + at + 32 * e) : 0;
+    };
+    if (by_position) load_positions(0);
     float m = -INFINITY, l = 0.0f;
     for (int i = 0; i < n; i++) {
+      int at[2] = {kp[0], kp[1]};
+      if (by_position) load_positions(i + 1);
       if (!__all_sync(0xffffffffu, pkv_mbar_wait(&bar.s_full[t][i & 1], (i >> 1) & 1))) {
         fine = false;
         break;
@@ -459,15 +470,19 @@ kv4_chunk_kernel(const __grid_constant__ ChunkParams cp) {
       const int token0 = span.unit(first + i) * kUnitTokens;
       const unsigned quad = s_quad[i % kQuadSlots];
       float fac = factor;
-      if (quad != 15u || token0 + kUnitTokens > len || by_position || token0 + kUnitTokens - 1 > tile_first ||
-          (p.window > 0 && tile_last - token0 >= p.window && token0 + kUnitTokens > p.sinks)) {
+      int newest = token0 + kUnitTokens - 1, oldest = token0;
+      if (by_position) {
+        newest = __reduce_max_sync(0xffffffffu, max(at[0], at[1]));
+        oldest = __reduce_min_sync(0xffffffffu, min(at[0], at[1]));
+      }
+      if (quad != 15u || token0 + kUnitTokens > len || newest > tile_first ||
+          (p.window > 0 && tile_last - oldest >= p.window && newest >= p.sinks)) {
         fac = 1.0f;
 #pragma unroll
         for (int c = 0; c < 64; c++) {
-          const int k = sigma(c), at = token0 + k;
-          bool see = ((quad >> (k >> 4)) & 1u) && at < len;
-          int kp = at;
-          if (by_position) kp = see ? __ldg(positions + at) : 0;
+          const int k = sigma(c);
+          bool see = ((quad >> (k >> 4)) & 1u) && token0 + k < len;
+          const int kp = by_position ? __shfl_sync(0xffffffffu, at[k >> 5], k & 31) : token0 + k;
           const int d = qpos - kp;
           see = see && d >= 0 && (p.window == 0 || d < p.window || kp < p.sinks);
           x[c >> 5][c & 31] = see ? __fmul_rn(x[c >> 5][c & 31], factor) : -INFINITY;
@@ -533,23 +548,21 @@ kv4_chunk_kernel(const __grid_constant__ ChunkParams cp) {
     if (!fine && lane == 0) pkv_report(p.err, 0, s, PKV_VEC_DEVICE_WAIT);
     const int64_t part = (((((int64_t)s * p.c.heads + h) * cp.tasks + task) * cp.splits + split) * kTaskRows) + kTileRows * t + (tid & 127);
     if (cp.splits > 1 && live) *reinterpret_cast<float2*>(p.part_ml + part * 2) = make_float2(m, l);
-    if (n > 0 || cp.splits == 1) {
 #pragma unroll 1
-      for (int c = 0; c < D; c += 32) {
-        float o[32];
-        __syncwarp();
-        if (n > 0) {
-          pkv_tc::tmem_load32(base + Y::O + c, o);
-        } else {
+    for (int c = 0; c < D; c += 32) {
+      float o[32];
+      __syncwarp();
+      if (n > 0) {
+        pkv_tc::tmem_load32(base + Y::O + c, o);
+      } else {
 #pragma unroll
-          for (int j = 0; j < 32; j++) o[j] = 0.0f;
-        }
-#pragma unroll
-        for (int j = 0; j < 32; j++) o[j] = __fmul_rn(o[j], (j & 1) ? kScaleShift / 16.0f : kScaleShift);
-        if (!live) continue;
-        if (cp.splits > 1) store_f32<PKV_DST_F32, 32>(p.part_o + part * D + c, o);
-        else write_row<T, 32>(p, s, h, row, c, o, m, l, c == 0);
+        for (int j = 0; j < 32; j++) o[j] = 0.0f;
       }
+#pragma unroll
+      for (int j = 0; j < 32; j++) o[j] = __fmul_rn(o[j], (j & 1) ? kScaleShift / 16.0f : kScaleShift);
+      if (!live) continue;
+      if (cp.splits > 1) store_f32<PKV_DST_F32, 32>(p.part_o + part * D + c, o);
+      else write_row<T, 32>(p, s, h, row, c, o, m, l, c == 0);
     }
   }
   // every product has been waited for (warp 17) and every read of tensor memory is done
@@ -561,36 +574,19 @@ kv4_chunk_kernel(const __grid_constant__ ChunkParams cp) {
   }
 }
 
-// Joins the splits of a query row; a warp per row.
-template <int D, int T>
-__global__ void __launch_bounds__(256)
+// Joins the splits of a query row; a warp per row, or (W = kJoinWarps) a CTA.
+template <int D, int T, int W>
+__global__ void __launch_bounds__(kJoinWarps * 32)
 kv4_chunk_join_kernel(const __grid_constant__ ChunkParams cp) {
   const AttendParams& p = cp.a;
-  constexpr int N = D / 32;
-  const int lane = threadIdx.x & 31;
-  const int h = blockIdx.y, s = blockIdx.z, row = blockIdx.x * 8 + (threadIdx.x >> 5);
+  const int h = blockIdx.y, s = blockIdx.z, row = blockIdx.x * (kJoinWarps / W) + (threadIdx.x >> 5) / W;
   wait_for_stream();
   int qn = p.q_lens ? p.q_lens[s] : p.q.n;
   if (qn < 0 || qn > p.q.n) qn = 0;
   if (row >= qn * p.group) return;
   const int task = row / kTaskRows;
   const int64_t first = ((((int64_t)s * p.c.heads + h) * cp.tasks + task) * cp.splits) * kTaskRows + (row - task * kTaskRows);
-  float m = -INFINITY, l = 0.0f, x[N];
-#pragma unroll
-  for (int i = 0; i < N; i++) x[i] = 0.0f;
-  for (int k = 0; k < cp.splits; k++) {
-    const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + (first + (int64_t)k * kTaskRows) * 2);
-    if (ml.x == -INFINITY && ml.y == 0.0f) continue;  // a split that sees nothing
-    const float top = fmaxf(m, ml.x);
-    const float fold = m == -INFINITY ? 0.0f : exp2_fast(__fsub_rn(m, top));
-    const float f = ml.x == -INFINITY ? ml.y : exp2_fast(__fsub_rn(ml.x, top));  // (NaN without a reference stays NaN)
-    m = top;
-    l = __fmaf_rn(l, fold, __fmul_rn(f, ml.y));
-    const float* src = p.part_o + (first + (int64_t)k * kTaskRows) * D + lane * N;
-#pragma unroll
-    for (int i = 0; i < N; i++) x[i] = __fmaf_rn(x[i], fold, __fmul_rn(f, src[i]));
-  }
-  write_row<T, N>(p, s, h, row, lane * N, x, m, l, lane == 0);
+  join_parts<D, T, W>(p, s, h, row, cp.splits, [&](int k) { return first + (int64_t)k * kTaskRows; });
 }
 
 struct Plan {
@@ -624,17 +620,21 @@ int launch(const ChunkParams& cp, int64_t rows, cudaStream_t s) {
   if (cudaError_t ce = launch_early(kernel, dim3(cp.tasks * cp.splits, cp.a.c.heads, cp.a.c.n_seqs), kThreads, bytes, s, cp))
     return pkv_cuda_status(ce);
   if (cp.splits == 1) return PKV_OK;
-  return pkv_cuda_status(launch_early(kv4_chunk_join_kernel<D, T>, dim3((unsigned)((rows + 7) / 8), cp.a.c.heads, cp.a.c.n_seqs), 256,
-                                      0, s, cp));
+  const bool many = cp.splits <= 16;  // few splits a row
+  return pkv_cuda_status(launch_early(many ? kv4_chunk_join_kernel<D, T, 1> : kv4_chunk_join_kernel<D, T, kJoinWarps>,
+                                      dim3((unsigned)(many ? (rows + kJoinWarps - 1) / kJoinWarps : rows), cp.a.c.heads, cp.a.c.n_seqs),
+                                      kJoinWarps * 32, 0, s, cp));
 }
 
 }  // namespace
 
 namespace pkv_kv4 {
 
-// More rows than the other kernel's largest tile; f32 queries stay there (their two terms do not fit the tile).
+// More rows than three of the other kernel's largest tiles; f32 queries stay there (their two terms do not fit the tile).
+// 8 kv heads of 128, 48 rows, here and there: 32 sequences of 8192 tokens 253 and 244 us, one of 131,071 122 and 127, four of
+// 1024 22.5 and 14.9; 64 rows: 254 and 320, 121 and 165, 23 and 15.
 bool chunk_takes(const pkv_kv4_rows* q, int group) {
-  return q->dtype != PKV_DST_F32 && (int64_t)q->n_tokens * group > 16;
+  return q->dtype != PKV_DST_F32 && (int64_t)q->n_tokens * group > 48;
 }
 
 int64_t chunk_workspace_bytes(const Cache& c, int dim, const pkv_kv4_rows* q, const pkv_kv4_attend_args* a) {

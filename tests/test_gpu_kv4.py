@@ -309,6 +309,41 @@ def test_chunks_split_over_the_tokens(dim, page, lens, q_len, group, window, sin
                  q_lens=[min(q_len, n + 2) for n in lens])
 
 
+@pytest.mark.parametrize("dtype,q_len,group", [("bfloat16", 30, 2), ("float16", 150, 2), ("float32", 20, 1), ("bfloat16", 9, 4)])
+@pytest.mark.parametrize("window,sinks", [(0, 0), (200, 20)])
+def test_queries_over_a_cache_that_was_thinned_out(dtype, q_len, group, window, sinks):
+    """Ascending positions with gaps, as an eviction leaves them: most units are seen by every row, the last by some."""
+    import torch
+    rng = np.random.default_rng(q_len)
+    lens, ends = [700, 330], np.array([900, 345])
+    pages, table, values = kv4ref.fill(rng, 2, 2, 64, 32, lens)
+    cap = table.shape[1] * 32
+    pos = np.full((2, 2, cap), -5, np.int32)  # behind the length: anything
+    for s, n in enumerate(lens):
+        for h in range(2):
+            old = np.sort(rng.permutation(int(ends[s]) - q_len)[:n - q_len])
+            pos[s, h, :n] = np.r_[old, np.arange(ends[s] - q_len, ends[s])]
+    cache = kv4.Kv4Cache(_dev(pages), _ints(table), _ints(lens), ends=_ints(ends), positions=_ints(pos),
+                         mass=torch.zeros((2, 2, cap), device="cuda"))
+    q = _dev(rng.standard_normal((2, q_len, 2 * group, 64)), _dt(dtype))
+    out, lse = cache.attend(q, window=window, sinks=sinks, accumulate=True)
+    cache.check()
+    want = kv4ref.attend(q.double().cpu().numpy(), values, lens, ends, pos, group, 64 ** -0.5, window, sinks, [q_len] * 2)
+    _close(out, lse, want[0], want[1], *want[3:])
+    # a weight is off by its score's error and its sum's, and rounded once a row
+    got = cache.mass.double().cpu().numpy()[:, :, :want[2].shape[2]]
+    eps = 2.0 ** -18 * want[4].max() + 2.0 ** -22 * np.abs(want[1]).max() + 2.0 ** -19
+    _within(got, want[2], (2 * eps + 2.0 ** -24 * q_len * group) * want[2], "mass")
+
+
+@pytest.mark.parametrize("dtype", ["float16", "bfloat16"])
+@pytest.mark.parametrize("q_len,group,heads,n", [(17, 1, 2, 300), (12, 4, 1, 700), (7, 7, 1, 500), (64, 1, 1, 1700), (50, 1, 1, 2500)])
+def test_rows_on_both_sides_of_a_tile(dtype, q_len, group, heads, n):
+    """17, 48, 49, 64 and 50 query rows a kv head; the last two in many splits."""
+    _attend_case(23 + q_len, dtype, 128, heads, group, 64, [n], q_len, 0, 0, False, True)
+    _attend_case(24 + q_len, dtype, 64, heads, group, 16, [n, 3], q_len, 130, 7, True, False)
+
+
 def test_pages_missing_from_a_chunk_and_from_a_long_row():
     import torch
     for q_len, n in ((20, 300), (1, 1700)):
