@@ -901,7 +901,7 @@ kv4_mass_kernel(const __grid_constant__ AttendParams p) {
     float sum[2][2] = {{0.0f, 0.0f}, {0.0f, 0.0f}};
     // causal rows before every key of this CTA are passed over
     int r_first = 0;
-    if (!by_position && qn > 1) r_first = max(0, cta0 - pos0) * p.group / 8 * 8;
+    if (!by_position && qn > 1) r_first = (int)min((long long)rows, max(0ll, (long long)cta0 - pos0) * p.group / 8 * 8);
     for (int r0 = r_first; r0 < rows; r0 += 8 * kMassWarps) {
       if (!by_position && p.window > 0 && cta0 >= p.sinks && pos0 + r0 / p.group - (cta0 + PER - 1) >= p.window) break;
       __syncthreads();  // the rows before these have been used

@@ -68,7 +68,7 @@ __device__ __forceinline__ Span visible_span(const AttendParams& p, int len, int
   if (!p.c.positions) {  // slots are positions
     stop = max(0, min(len, pos_last + 1));
     if (p.window > 0) {
-      lo = max(0, pos_first - p.window + 1);
+      lo = (int)max(0ll, (long long)pos_first - p.window + 1);
       sink = min(p.sinks, stop);
     }
   }

@@ -35,6 +35,13 @@ def atom_bytes(dim: int) -> int:
     return 18 * dim
 
 
+def _int32(name: str, x: int) -> int:
+    """A count as the library takes it (ctypes would cut off what is above 32 bits)."""
+    if not 0 <= x < 1 << 31:
+        raise ValueError(f"{name} must be at least 0 and below 2**31, not {x}")
+    return x
+
+
 def _raw_queries(torch):
     """(current device, current stream of a device) as plain numbers: torch's own accessors without the Python objects around
     them where this torch has them (a decode step's call is a few microseconds long)."""
@@ -98,6 +105,8 @@ class Kv4Cache:
         """Empty caches for `n_layers` layers that share page table, `lens` and `ends`; each sequence owns the pages of
         `max_tokens` tokens.  `evictable`: with positions and mass."""
         import torch
+        if page_tokens < 1 or page_tokens % ATOM_TOKENS:
+            raise ValueError(f"page_tokens must be a multiple of {ATOM_TOKENS}, not {page_tokens}")
         max_pages = -(-max_tokens // page_tokens)
         table = torch.arange(n_seqs * max_pages, dtype=torch.int32, device=device).view(n_seqs, max_pages)
         lens, ends = (torch.zeros(n_seqs, dtype=torch.int32, device=device) for _ in range(2))
@@ -112,9 +121,9 @@ class Kv4Cache:
         return out
 
     # -- calls -----------------------------------------------------------------------------------------------------------
-    def _rows(self, t, name: str, heads: int | None = None):
+    def _rows(self, t, name: str, heads: int | None = None, written: bool = False):
         """A reference to the pkv_kv4_rows of a tensor's shape, strides and type (kept: they depend on nothing else)."""
-        key = (t.shape, t.stride(), t.dtype)
+        key = (t.shape, t.stride(), t.dtype, written)
         r = self._rows_of.get(key)
         if r is None:
             shape, stride = t.shape, t.stride()
@@ -122,9 +131,12 @@ class Kv4Cache:
                 raise ValueError(f"{name} must be [{self.n_seqs}][tokens][heads][{self.dim}], not {tuple(shape)}")
             if stride[3] != 1 and t.numel():
                 raise ValueError(f"the values of a vector of {name} must be contiguous")
+            if written and any(n > 1 and st == 0 for n, st in zip(shape, stride)):
+                raise ValueError(f"{name} is written: its vectors must not lie over one another")
             if len(self._rows_of) >= 256:
                 self._rows_of.clear()
-            r = self._rows_of[key] = C.byref(L.Kv4RowsC(stride[0], stride[1], stride[2], shape[1], dst_dtype_of(t)))
+            # (the stride of a dimension of one says nothing)
+            r = self._rows_of[key] = C.byref(L.Kv4RowsC(*(stride[i] if shape[i] > 1 else 0 for i in range(3)), shape[1], dst_dtype_of(t)))
         if heads is not None and t.shape[2] != heads:
             raise ValueError(f"{name} has {t.shape[2]} heads, the cache {heads}")
         if t.get_device() != self._index:
@@ -173,8 +185,8 @@ class Kv4Cache:
                 raise ValueError("out does not have the rows or the type asked for")
             if k.shape != v.shape:
                 raise ValueError("k and v must have the same shape")
-        kr = self._rows(k, "k", self.n_kv_heads)
-        vr = kr if fresh else self._rows(v, "v", self.n_kv_heads)
+        kr = self._rows(k, "k", self.n_kv_heads, True)
+        vr = kr if fresh else self._rows(v, "v", self.n_kv_heads, True)
         if k.numel():
             self._call(self._lib.pkv_kv4_read_dev, k.data_ptr(), kr, v.data_ptr(), vr, self._per_seq(new_lens, "new_lens"), int(fresh))
         return k, v
@@ -199,7 +211,7 @@ class Kv4Cache:
             out = (torch.empty_like if q_lens is None else torch.zeros_like)(q, memory_format=torch.contiguous_format)
         elif out.shape != shape or out.dtype != q.dtype:
             raise ValueError("out must have the shape and type of q")
-        outr = self._rows(out, "out")
+        outr = self._rows(out, "out", written=True)
         if lse is None:
             lse = (q.new_empty if q_lens is None else q.new_zeros)(shape[:3], dtype=torch.float32)
         elif lse.shape != shape[:3] or lse.dtype != torch.float32 or not lse.is_contiguous() or lse.get_device() != self._index:
@@ -209,7 +221,8 @@ class Kv4Cache:
         if plan is None:
             if accumulate and self.mass is None:
                 raise ValueError("accumulate needs a cache with mass")
-            args = L.Kv4AttendC(self.dim ** -0.5 if scale is None else scale, shape[2], window, sinks, int(accumulate), max_len)
+            args = L.Kv4AttendC(self.dim ** -0.5 if scale is None else scale, shape[2], _int32("window", window), _int32("sinks", sinks),
+                                int(accumulate), _int32("max_len", max_len))
             if len(self._attend_of) >= 256:
                 self._attend_of.clear()
             plan = self._attend_of[key] = (C.byref(args), self._lib.pkv_kv4_attend_workspace_bytes(self._ref, qr, C.byref(args)),
@@ -228,6 +241,8 @@ class Kv4Cache:
         all layers are done."""
         if self.positions is None or self.mass is None:
             raise ValueError("evict needs a cache with positions and mass")
+        for name, x in (("budget", budget), ("sinks", sinks), ("recent", recent)):
+            _int32(name, x)
         if self.n_seqs == 0:
             return
         need = self._evict_of.get(budget)

@@ -432,6 +432,60 @@ def test_strided_queries_and_outputs():
     assert (room[..., :4] == 7).all() and (room[..., 68:] == 7).all() and (room[:, :, 3] == 7).all()
 
 
+def test_what_would_wrap_or_overlap_is_refused():
+    import torch
+    rng = np.random.default_rng(41)
+    pages, table, _ = kv4ref.fill(rng, 2, 2, 64, 16, [30, 55])
+    cap = table.shape[1] * 16
+    cache = kv4.Kv4Cache(_dev(pages), _ints(table), _ints([30, 55]), positions=torch.zeros((2, 2, cap), dtype=torch.int32, device="cuda"),
+                         mass=torch.zeros((2, 2, cap), device="cuda"))
+    q = torch.zeros((2, 1, 4, 64), device="cuda")
+    wide = (1 << 32) + 5
+    for bad in (dict(window=wide), dict(sinks=wide), dict(max_len=wide), dict(window=-1), dict(out=q[:1].expand(2, 1, 4, 64))):
+        with pytest.raises(ValueError):
+            cache.attend(q, **bad)
+    for bad in ((wide, 0, 0), (20, wide, 0), (20, 0, wide), (-1, 0, 0)):
+        with pytest.raises(ValueError):
+            cache.evict(bad[0], sinks=bad[1], recent=bad[2])
+    k = torch.zeros((2, 1, 2, 64), device="cuda")
+    with pytest.raises(ValueError):
+        cache.read(1, out=(k, k[:, :, :1].expand(2, 1, 2, 64)))
+    assert (cache.mass == 0).all() and (cache.pages.cpu().numpy() == pages).all()
+
+
+def test_strides_of_dimensions_of_one_do_not_count():
+    import torch
+    rng = np.random.default_rng(42)
+    pages, table, values = kv4ref.fill(rng, 1, 1, 64, 16, [30])
+    cache = kv4.Kv4Cache(_dev(pages), _ints(table), _ints([30]))
+    q = _dev(rng.standard_normal(64), torch.float32).as_strided((1, 1, 1, 64), (1, 3, 5, 1))
+    out, lse = cache.attend(q)
+    want = kv4ref.attend(q.double().cpu().numpy(), values, [30], [30], None, 1, 0.125, 0, 0, [1])
+    _close(out, lse, want[0], want[1], *want[3:])
+
+
+@pytest.mark.parametrize("dtype,q_len", [("float32", 6), ("bfloat16", 6), ("bfloat16", 70)])
+def test_the_widest_window_with_more_queries_than_tokens(dtype, q_len):
+    # positions below zero minus the window do not fit 32 bits
+    _attend_case(43, dtype, 64, 1, 2, 16, [4, 66], q_len, (1 << 31) - 1, 0, False, True)
+    _attend_case(44, dtype, 64, 1, 2, 16, [4, 66], q_len, (1 << 31) - 1, 2, True, True)
+
+
+def test_ends_below_the_lengths_read_and_write_nothing_else():
+    """Ends that were never raised: whatever the queries see, no row before the first is read and mass stays finite."""
+    import torch
+    rng = np.random.default_rng(45)
+    pages, table, _ = kv4ref.fill(rng, 2, 1, 64, 64, [700, 700])
+    mass = torch.zeros((2, 1, table.shape[1] * 64), device="cuda")
+    cache = kv4.Kv4Cache(_dev(pages), _ints(table), _ints([700, 700]), ends=_ints([-(1 << 31) + 200, 3]), mass=mass)
+    for q_len, dtype in ((70, torch.bfloat16), (20, torch.float32)):
+        q = _dev(rng.standard_normal((2, q_len, 2, 64)), dtype)
+        out, lse = cache.attend(q, accumulate=True)
+        cache.check()
+        assert (out[0] == 0).all() and torch.isneginf(lse[0]).all() and (out[1, :-3] == 0).all()
+        assert (mass[0] == 0).all() and (mass[1, :, 3:] == 0).all() and torch.isfinite(mass).all()
+
+
 def test_the_class_refuses():
     import torch
     rng = np.random.default_rng(35)

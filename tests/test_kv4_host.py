@@ -163,3 +163,16 @@ def test_rows_come_back_from_a_page():
         for (h, t, side), (c, s) in want.items():
             gc, gs = kv4ref.get_row(page, h, t, side, dim)
             assert np.array_equal(c, gc) and np.array_equal(s, gs)
+
+
+def test_allocate_refuses_pages_of_no_whole_atoms():
+    for page in (0, 8, 40, -16):
+        with pytest.raises(ValueError, match="multiple of 16"):
+            kv4.Kv4Cache.allocate(1, 1, 1, 64, 100, page_tokens=page, device="cpu")
+
+
+def test_counts_do_not_wrap():
+    assert kv4._int32("window", (1 << 31) - 1) == (1 << 31) - 1
+    for x in (-1, 1 << 31, (1 << 32) + 5):
+        with pytest.raises(ValueError, match="window"):
+            kv4._int32("window", x)
