@@ -841,7 +841,7 @@ kv4_mass_of_scores_kernel(const __grid_constant__ AttendParams p) {
 // has one owner and one order.  The queries come as B operands from shared memory, 64 rows at a time, eight converted by each
 // warp: rows are read and converted once for 256 tokens, keys once in all.  Two exponentials, two multiply-adds and two
 // additions a score pair are left besides the products.  512 rows over 8192 tokens, 8 heads of 128: 54 us (142 with the keys dequantised
-// again for every eight rows).
+// again for every eight rows); 4096 rows 347 us, 380 with one chain of products an atom and divisions for the rows' positions.
 template <int D, int T>
 __global__ void __launch_bounds__(kMassWarps * 32, T == PKV_DST_F32 && D == 128 ? 1 : 2)
 kv4_mass_kernel(const __grid_constant__ AttendParams p) {
@@ -850,6 +850,7 @@ kv4_mass_kernel(const __grid_constant__ AttendParams p) {
   using A = Atom<D>;
   __shared__ uint4 s_q[kMassWarps][TERMS][D / 32][32];
   __shared__ __align__(16) float2 s_row[kMassWarps][8];  // what turns a product into log2 of a weight: factor, offset
+  __shared__ int2 s_span[kMassWarps];                    // positions of the first and the last of eight rows
   const int lane = threadIdx.x & 31, warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0);
   const int g = lane >> 2, q4 = lane & 3;
   const int s = blockIdx.z, h = blockIdx.y;
@@ -917,6 +918,7 @@ kv4_mass_kernel(const __grid_constant__ AttendParams p) {
           s_q[warp][0][i][lane] = make_uint4(hi[2 * i][0], hi[2 * i][1], hi[2 * i + 1][0], hi[2 * i + 1][1]);
           if constexpr (F32) s_q[warp][TERMS - 1][i][lane] = make_uint4(lo[2 * i][0], lo[2 * i][1], lo[2 * i + 1][0], lo[2 * i + 1][1]);
         }
+        if (lane == 0) s_span[warp] = make_int2(pos0 + (r0 + 8 * warp) / p.group, pos0 + min(rows - 1, r0 + 8 * warp + 7) / p.group);
         // (a row that sees nothing, or behind the last one, weighs nothing)
         if (q4 == 0)
           s_row[warp][g] = lse == -INFINITY ? make_float2(0.0f, -INFINITY)
@@ -929,38 +931,43 @@ kv4_mass_kernel(const __grid_constant__ AttendParams p) {
       for (int k = 0; k < kMassWarps; k++) {
         const int ra = r0 + 8 * k;
         if (ra >= rows) break;
-        const int first = pos0 + ra / p.group, last = pos0 + min(rows - 1, ra + 7) / p.group;
+        const int first = s_span[k].x, last = s_span[k].y;
         if (last < k_min || (p.window > 0 && first - k_max >= p.window && k_min >= p.sinks)) continue;
+        // two chains of products an atom (f32 queries: the second terms a third, as in scores_of)
         float sc[2][4], part[2][2][4];
 #pragma unroll
-        for (int j = 0; j < D / 32; j++) {
-          const uint4 q = s_q[k][0][j][lane];
+        for (int j = 0; j < D / 64; j++) {
 #pragma unroll
-          for (int a = 0; a < 2; a++) {
-            const uint32_t(&w)[2][4] = key[a][j];
-            // f32 queries: chains as in scores_of
-            float(&c)[4] = F32 && 2 * j >= D / 32 ? part[a][0] : sc[a];
-            if (j == 0 || (F32 && 2 * j == D / 32)) mma_first(c, w[0][0], w[1][0], w[0][1], w[1][1], q.x, q.y);
-            else mma(c, w[0][0], w[1][0], w[0][1], w[1][1], q.x, q.y);
-            mma(c, w[0][2], w[1][2], w[0][3], w[1][3], q.z, q.w);
-          }
-          if constexpr (F32) {
-            const uint4 q2 = s_q[k][1][j][lane];
+          for (int half = 0; half < 2; half++) {
+            const int at = j + half * (D / 64);
+            const uint4 q = s_q[k][0][at][lane];
 #pragma unroll
             for (int a = 0; a < 2; a++) {
-              const uint32_t(&w)[2][4] = key[a][j];
-              if (j == 0) mma_first(part[a][1], w[0][0], w[1][0], w[0][1], w[1][1], q2.x, q2.y);
-              else mma(part[a][1], w[0][0], w[1][0], w[0][1], w[1][1], q2.x, q2.y);
-              mma(part[a][1], w[0][2], w[1][2], w[0][3], w[1][3], q2.z, q2.w);
+              const uint32_t(&w)[2][4] = key[a][at];
+              float(&c)[4] = half ? part[a][0] : sc[a];
+              if (j == 0) mma_first(c, w[0][0], w[1][0], w[0][1], w[1][1], q.x, q.y);
+              else mma(c, w[0][0], w[1][0], w[0][1], w[1][1], q.x, q.y);
+              mma(c, w[0][2], w[1][2], w[0][3], w[1][3], q.z, q.w);
+            }
+            if constexpr (F32) {
+              const uint4 q2 = s_q[k][TERMS - 1][at][lane];
+#pragma unroll
+              for (int a = 0; a < 2; a++) {
+                const uint32_t(&w)[2][4] = key[a][at];
+                if (at == 0) mma_first(part[a][1], w[0][0], w[1][0], w[0][1], w[1][1], q2.x, q2.y);
+                else mma(part[a][1], w[0][0], w[1][0], w[0][1], w[1][1], q2.x, q2.y);
+                mma(part[a][1], w[0][2], w[1][2], w[0][3], w[1][3], q2.z, q2.w);
+              }
             }
           }
         }
-        if constexpr (F32) {
 #pragma unroll
-          for (int a = 0; a < 2; a++)
+        for (int a = 0; a < 2; a++)
 #pragma unroll
-            for (int i = 0; i < 4; i++) sc[a][i] = __fadd_rn(__fadd_rn(sc[a][i], part[a][0][i]), part[a][1][i]);
-        }
+          for (int i = 0; i < 4; i++) {
+            sc[a][i] = __fadd_rn(sc[a][i], part[a][0][i]);
+            if constexpr (F32) sc[a][i] = __fadd_rn(sc[a][i], part[a][1][i]);
+          }
         const float4 f = *reinterpret_cast<const float4*>(&s_row[k][2 * q4]);
         const bool all = there == 0xffffffffu && first >= k_max && (p.window == 0 || last - k_min < p.window) && ra + 8 <= rows;
         if (all) {
