@@ -542,6 +542,15 @@ int pkv_test_capture_rotated(float* rotated_dev);
  * can compare the two routes byte for byte.  Process-wide. */
 int pkv_test_turbo_encode_legacy(int on);
 
+/* Test hook, no counterpart in the reference.  Only the last launch of a pkv_kv4_attend_dev call with the same arguments, the
+ * one that joins the parts of rows that were cut, over the workspace as it is: tests spoil its table of parts the way a
+ * bounded wait that ran out would leave it.  Rows of such entries are reported as PKV_VEC_DEVICE_WAIT and not written.
+ * PKV_ERR_UNSUPPORTED for calls without that launch, and for others than dim 64, f32, at most 8 query rows a kv head. */
+int pkv_test_kv4_join_dev(const pkv_kv4_cache* cache, const void* q_dev, const pkv_kv4_rows* q_rows, void* out_dev,
+                          const pkv_kv4_rows* out_rows, float* lse_dev, const int32_t* q_lens_dev,
+                          const pkv_kv4_attend_args* args, void* workspace_dev, int64_t workspace_bytes, uint64_t* err_dev,
+                          void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -191,6 +191,8 @@ _SIGS = {
     "pkv_kv4_attend_workspace_bytes": (C.c_int64, [C.POINTER(Kv4CacheC), C.POINTER(Kv4RowsC), C.POINTER(Kv4AttendC)]),
     "pkv_kv4_attend_dev": (C.c_int, [C.POINTER(Kv4CacheC), _V, C.POINTER(Kv4RowsC), _V, C.POINTER(Kv4RowsC), _V, _V,
                                      C.POINTER(Kv4AttendC), _V, C.c_int64, _V, _V]),
+    "pkv_test_kv4_join_dev": (C.c_int, [C.POINTER(Kv4CacheC), _V, C.POINTER(Kv4RowsC), _V, C.POINTER(Kv4RowsC), _V, _V,
+                                        C.POINTER(Kv4AttendC), _V, C.c_int64, _V, _V]),
     "pkv_kv4_evict_workspace_bytes": (C.c_int64, [C.POINTER(Kv4CacheC), C.c_int32]),
     "pkv_kv4_evict_dev": (C.c_int, [C.POINTER(Kv4CacheC), C.c_int32, C.c_int32, C.c_int32, _V, C.c_int64, _V, _V]),
     "pkv_host_libm_exceptions": (C.c_int, [C.c_int32, _V, C.c_int64, C.POINTER(C.c_int64), C.POINTER(C.c_int32)]),

@@ -457,12 +457,9 @@ __device__ __forceinline__ void stream_units(const AttendParams& p, Cursor t, in
         r.l[n][e] = __fadd_rn(x, __shfl_xor_sync(0xffffffffu, x, 16));
       }
   };
-  auto end_tile = [&](int v0, int n_units) {  // units v0 .. v0 + n_units - 1 of tile t are in r; `at` is the first one's number
+  const int run = blockIdx.x * kWarps + warp;
+  auto end_tile = [&](int v0, int n_units) {  // units v0 .. v0 + n_units - 1 of tile t are in r
     join_lanes();
-    const int run = blockIdx.x * kWarps + warp;
-    if (v0 == 0 && lane == 0)
-      p.part_of[((int64_t)t.s * p.c.heads + t.h) * p.row_tiles + t.tile] =
-          make_int2(run, n_units == t.units ? 1 : (int)runs.of(at + t.units - 1) - run + 1);
 #pragma unroll
     for (int n = 0; n < NT; n++)
 #pragma unroll
@@ -490,6 +487,10 @@ __device__ __forceinline__ void stream_units(const AttendParams& p, Cursor t, in
   for (;;) {
     begin_tile();
     const int v0 = v, n_here = DIRECT ? count : min(left_here, t.units - v);
+    if constexpr (!DIRECT)  // (before the first wait, which may give up)
+      if (v0 == 0 && lane == 0)
+        p.part_of[((int64_t)t.s * p.c.heads + t.h) * p.row_tiles + t.tile] =
+            make_int2(run, n_here == t.units ? 1 : (int)runs.of(at + t.units - 1) - run + 1);
 #pragma unroll 1
     for (int i = 0; i < n_here; i++, v += STEP) {
       const int token0 = t.span.unit(v) * kUnitTokens;
@@ -797,6 +798,12 @@ kv4_combine_kernel(const __grid_constant__ AttendParams p) {
   if (grow >= qn * p.group) return;
   const int2 of = p.part_of[((int64_t)s * p.c.heads + h) * p.row_tiles + tile];
   if (of.y == 1) return;
+  // A warp that gave up leaves the entries of the row tiles it never came to as they were in the workspace.  Its parts are
+  // not valid, which it has reported, and only entries inside the table are followed.
+  if (of.x < 0 || of.y < 1 || of.y > p.runs || of.x > p.runs - of.y) {
+    if ((threadIdx.x & 31) == 0) pkv_report(p.err, 0, s, PKV_VEC_DEVICE_WAIT);
+    return;
+  }
   join_parts<D, T, W>(p, s, h, grow, of.y, [&](int k) { return ((int64_t)(of.x + k) * 2 + (k == 0)) * (8 * NT) + row; });
 }
 
@@ -1048,6 +1055,14 @@ Plan make_plan(const Cache& c, int dim, const pkv_kv4_rows* q, const pkv_kv4_att
 }
 
 template <int D, int NT, int T>
+int launch_join(const AttendParams& p, cudaStream_t s) {
+  const bool many = p.runs < 16ll * p.row_tiles * p.c.heads * p.c.n_seqs;  // few parts a row
+  return pkv_cuda_status(launch_early(many ? kv4_combine_kernel<D, NT, T, 1> : kv4_combine_kernel<D, NT, T, kJoinWarps>,
+                                      dim3(p.row_tiles * 8 * NT / (many ? kJoinWarps : 1), p.c.heads, p.c.n_seqs), kJoinWarps * 32, 0, s,
+                                      p));
+}
+
+template <int D, int NT, int T>
 int launch_attend(const AttendParams& p, cudaStream_t s) {
   auto kernel = p.runs ? kv4_attend_kernel<D, NT, T, false, false> : kv4_attend_kernel<D, NT, T, true, false>;
   // f32 with up to four rows a kv head: paired terms, half the matrix instructions.  8 sequences of 4096 tokens, 32 heads of 64,
@@ -1059,11 +1074,7 @@ int launch_attend(const AttendParams& p, cudaStream_t s) {
     if (cudaError_t ce = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes)) return pkv_cuda_status(ce);
   const dim3 rows(p.row_tiles, p.c.heads, p.c.n_seqs);
   if (cudaError_t ce = launch_early(kernel, p.runs ? dim3(p.runs / kWarps) : rows, kWarps * 32, bytes, s, p)) return pkv_cuda_status(ce);
-  if (!p.runs) return PKV_OK;
-  const bool many = p.runs < 16ll * p.row_tiles * p.c.heads * p.c.n_seqs;  // few parts a row
-  return pkv_cuda_status(launch_early(many ? kv4_combine_kernel<D, NT, T, 1> : kv4_combine_kernel<D, NT, T, kJoinWarps>,
-                                      dim3(p.row_tiles * 8 * NT / (many ? kJoinWarps : 1), p.c.heads, p.c.n_seqs), kJoinWarps * 32, 0, s,
-                                      p));
+  return p.runs ? launch_join<D, NT, T>(p, s) : PKV_OK;
 }
 
 template <int D, int T>
@@ -1101,11 +1112,17 @@ extern "C" int64_t pkv_kv4_attend_workspace_bytes(const pkv_kv4_cache* cache, co
   return make_plan(c, cache->dim, q_rows, args).bytes(cache->dim);
 }
 
-extern "C" int pkv_kv4_attend_dev(const pkv_kv4_cache* cache, const void* q_dev, const pkv_kv4_rows* q_rows, void* out_dev,
-                                  const pkv_kv4_rows* out_rows, float* lse_dev, const int32_t* q_lens_dev,
-                                  const pkv_kv4_attend_args* args, void* workspace_dev, int64_t workspace_bytes,
-                                  uint64_t* err_dev, void* stream) {
+namespace {
+
+// What the calls check and set up alike.  `nt`: of the kernel for few rows, 0 where the other takes the call.
+struct Call {
   AttendParams p;
+  int nt, longest;
+};
+int make_call(const pkv_kv4_cache* cache, const void* q_dev, const pkv_kv4_rows* q_rows, void* out_dev, const pkv_kv4_rows* out_rows,
+              float* lse_dev, const int32_t* q_lens_dev, const pkv_kv4_attend_args* args, void* workspace_dev, int64_t workspace_bytes,
+              uint64_t* err_dev, Call* c) {
+  AttendParams& p = c->p;
   if (int st = make_cache(cache, &p.c)) return st;
   if (int st = make_rows(q_dev, q_rows, &p.q)) return st;
   if (int st = make_rows(out_dev, out_rows, &p.o)) return st;
@@ -1138,21 +1155,48 @@ extern "C" int pkv_kv4_attend_dev(const pkv_kv4_cache* cache, const void* q_dev,
   p.part_ml = p.part_o + plan.part_rows * cache->dim;
   p.part_of = (int2*)(p.part_ml + plan.part_rows * 2);
   p.err = err_dev;
-  const int longest = args->max_len > 0 && args->max_len < p.c.capacity ? args->max_len : p.c.capacity;
+  c->nt = plan.nt;
+  c->longest = args->max_len > 0 && args->max_len < p.c.capacity ? args->max_len : p.c.capacity;
+  return PKV_OK;
+}
+
+}  // namespace
+
+extern "C" int pkv_kv4_attend_dev(const pkv_kv4_cache* cache, const void* q_dev, const pkv_kv4_rows* q_rows, void* out_dev,
+                                  const pkv_kv4_rows* out_rows, float* lse_dev, const int32_t* q_lens_dev,
+                                  const pkv_kv4_attend_args* args, void* workspace_dev, int64_t workspace_bytes,
+                                  uint64_t* err_dev, void* stream) {
+  Call c;
+  if (int st = make_call(cache, q_dev, q_rows, out_dev, out_rows, lse_dev, q_lens_dev, args, workspace_dev, workspace_bytes, err_dev, &c))
+    return st;
+  const AttendParams& p = c.p;
+  if (p.q.n == 0 || p.c.n_seqs == 0) return PKV_OK;
   cudaStream_t s = (cudaStream_t)stream;
   const bool acc = args->accumulate != 0;
-  if (chunk)
+  if (c.nt == 0)
     if (int st = launch_chunk(p, cache->dim, q_rows->dtype, q_rows, args, workspace_dev, s)) return st;
   if (cache->dim == 64) {
     switch (q_rows->dtype) {
-      case PKV_DST_F32: return launch_all<64, PKV_DST_F32>(p, plan.nt, acc, longest, s);
-      case PKV_DST_F16: return launch_all<64, PKV_DST_F16>(p, plan.nt, acc, longest, s);
-      default: return launch_all<64, PKV_DST_BF16>(p, plan.nt, acc, longest, s);
+      case PKV_DST_F32: return launch_all<64, PKV_DST_F32>(p, c.nt, acc, c.longest, s);
+      case PKV_DST_F16: return launch_all<64, PKV_DST_F16>(p, c.nt, acc, c.longest, s);
+      default: return launch_all<64, PKV_DST_BF16>(p, c.nt, acc, c.longest, s);
     }
   }
   switch (q_rows->dtype) {
-    case PKV_DST_F32: return launch_all<128, PKV_DST_F32>(p, plan.nt, acc, longest, s);
-    case PKV_DST_F16: return launch_all<128, PKV_DST_F16>(p, plan.nt, acc, longest, s);
-    default: return launch_all<128, PKV_DST_BF16>(p, plan.nt, acc, longest, s);
+    case PKV_DST_F32: return launch_all<128, PKV_DST_F32>(p, c.nt, acc, c.longest, s);
+    case PKV_DST_F16: return launch_all<128, PKV_DST_F16>(p, c.nt, acc, c.longest, s);
+    default: return launch_all<128, PKV_DST_BF16>(p, c.nt, acc, c.longest, s);
   }
+}
+
+extern "C" int pkv_test_kv4_join_dev(const pkv_kv4_cache* cache, const void* q_dev, const pkv_kv4_rows* q_rows, void* out_dev,
+                                     const pkv_kv4_rows* out_rows, float* lse_dev, const int32_t* q_lens_dev,
+                                     const pkv_kv4_attend_args* args, void* workspace_dev, int64_t workspace_bytes,
+                                     uint64_t* err_dev, void* stream) {
+  Call c;
+  if (int st = make_call(cache, q_dev, q_rows, out_dev, out_rows, lse_dev, q_lens_dev, args, workspace_dev, workspace_bytes, err_dev, &c))
+    return st;
+  if (c.p.q.n == 0 || c.p.c.n_seqs == 0 || c.nt != 1 || !c.p.runs || cache->dim != 64 || q_rows->dtype != PKV_DST_F32)
+    return PKV_ERR_UNSUPPORTED;
+  return launch_join<64, 1, PKV_DST_F32>(c.p, (cudaStream_t)stream);
 }

@@ -745,3 +745,48 @@ def test_far_pages_and_sums_do_not_wrap():
     out, lse = cache.attend(q)
     w = kv4ref.attend(q.double().cpu().numpy(), np.stack([want.transpose(0, 2, 1, 3)] * 2, 1), [150], [150], None, 1, d ** -0.5, 0, 0, [1])
     _close(out, lse, w[0], w[1], *w[3:])
+
+
+# -- what must not go unnoticed ------------------------------------------------------------------------------------------
+def test_the_join_follows_no_entry_that_was_not_written():
+    """The table of parts as a copy that never arrives leaves it: whatever lay in the workspace.  Rows of such entries are
+    reported and stay as they were, the others are joined."""
+    import ctypes as C
+    import torch
+    rng = np.random.default_rng(61)
+    heads, group, n = 8, 2, 2500
+    pages, table, _ = kv4ref.fill(rng, 1, heads, 64, 64, [n])
+    cache = kv4.Kv4Cache(_dev(pages), _ints(table), _ints([n]))
+    q = _dev(rng.standard_normal((1, 1, heads * group, 64)), torch.float32)
+    want, wlse = cache.attend(q)
+    cache.check()
+    lib, rows, args = L.lib(), cache._rows(q, "q"), L.Kv4AttendC(64 ** -0.5, heads * group, 0, 0, 0, 0)
+    need = lib.pkv_kv4_attend_workspace_bytes(cache._ref, rows, C.byref(args))
+    work = torch.zeros(need, dtype=torch.uint8, device="cuda")
+    out, lse = torch.empty_like(q), torch.empty((1, 1, heads * group), device="cuda")
+
+    def call(f):
+        L.check(f(cache._ref, q.data_ptr(), rows, out.data_ptr(), rows, lse.data_ptr(), None, C.byref(args), work.data_ptr(), need,
+                  cache.error.data_ptr(), torch.cuda.current_stream().cuda_stream))
+
+    call(lib.pkv_kv4_attend_dev)
+    cache.check()
+    assert torch.equal(out, want) and torch.equal(lse, wlse)
+    entries = work[-8 * heads:].view(torch.int32).view(heads, 2)  # (first run, runs) of each kv head
+    runs = 4 * -(-heads * -(-cache.capacity // 64) // 4)
+    assert (entries[:, 1] > 1).all() and int(entries.sum(1).max()) <= runs
+    good = entries.clone()
+    bad = torch.tensor([[-1, 3], [0, 0], [0, -5], [0, runs + 1], [runs - 1, 2], [0x7f7f7f7f, 0x7f7f7f7f]], dtype=torch.int32, device="cuda")
+    for first in (0, 2):
+        entries.copy_(good)
+        entries[first:first + 6] = bad
+        out.fill_(7.0)
+        lse.fill_(7.0)
+        call(lib.pkv_test_kv4_join_dev)
+        with pytest.raises(pk.PkvError) as e:
+            cache.check()
+        assert (e.value.status, e.value.vector_index) == (L.VEC_DEVICE_WAIT, 0)
+        spoilt = torch.zeros(heads * group, dtype=torch.bool, device="cuda")
+        spoilt[first * group:(first + 6) * group] = True
+        assert (out[0, 0, spoilt] == 7).all() and (lse[0, 0, spoilt] == 7).all()
+        assert torch.equal(out[0, 0, ~spoilt], want[0, 0, ~spoilt]) and torch.equal(lse[0, 0, ~spoilt], wlse[0, 0, ~spoilt])

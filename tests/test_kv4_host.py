@@ -176,3 +176,12 @@ def test_counts_do_not_wrap():
     for x in (-1, 1 << 31, (1 << 32) + 5):
         with pytest.raises(ValueError, match="window"):
             kv4._int32("window", x)
+
+
+def test_the_join_alone_is_there_for_split_rows_only():
+    f = L.lib().pkv_test_kv4_join_dev
+    row = _rows(dtype=L.DST_F32)
+    call = lambda c, n: f(C.byref(c), P, C.byref(row), P, C.byref(row), P, None, C.byref(_args()), P, n, P, None)  # noqa: E731
+    assert call(_cache(dim=64), 1 << 30) == L.ERR_UNSUPPORTED                                # short rows: nothing is cut
+    assert call(_cache(dim=128, max_pages=4096, n_seqs=1), 1 << 30) == L.ERR_UNSUPPORTED
+    assert call(_cache(dim=64, max_pages=4096, n_seqs=1), 8) == L.ERR_BUFFER_TOO_SMALL
