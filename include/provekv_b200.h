@@ -490,7 +490,8 @@ typedef struct pkv_kv4_attend_args {
 /* out = softmax(scale * q K^T) V over the visible tokens of each sequence, read from the pages.  The queries are the
  * newest tokens: row i of sequence s has position ends[s] - q_lens[s] + i (q_lens null: n_tokens for every sequence)
  * and sees the cached tokens of positions up to it.  Rows from q_lens[s] on are neither read nor written.  A query that
- * sees nothing gets zeros.  lse_dev (may be null unless accumulating): [n_seqs][n_tokens][n_q_heads] f32, the natural logarithm of
+ * sees nothing gets zeros.  out may be q itself unless weights are accumulated; anything else of q it must not overlap (refused;
+ * looked for exactly where both have the same strides, by the ranges otherwise).  lse_dev (may be null unless accumulating): [n_seqs][n_tokens][n_q_heads] f32, the natural logarithm of
  * the sum of exponentials, -inf where nothing is visible.  q and out have the same type.
  * Products, softmax statistics and sums are f32; weights enter the second product in binary16 (f32 queries: as two
  * binary16 terms).  The result does not depend on the order in which blocks run.

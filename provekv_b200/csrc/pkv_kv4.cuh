@@ -97,6 +97,49 @@ inline int make_rows(const void* base, const pkv_kv4_rows* r, Rows* out) {
   return PKV_OK;
 }
 
+// Whether two sets of vectors [n_seqs][n][heads][dim] of one type share memory.  Equal strides: looked for exactly, largest
+// stride first (a slice and its neighbours in one buffer are apart); others: by their ranges, so perhaps for nothing.
+enum { kApart, kSame, kOverlap };
+struct Axis {
+  int64_t stride, n;
+};
+// whether `delta` is within `row` of a difference of two of the axes' offsets
+inline bool meets(int64_t delta, const Axis* axis, int axes, int64_t row) {
+  if (axes == 0) return delta > -row && delta < row;
+  int64_t e = axis->stride ? delta / axis->stride : 0;
+  for (int64_t k = e - 1; k <= e + 1; k++)
+    if (k > -axis->n && k < axis->n && meets(delta - k * axis->stride, axis + 1, axes - 1, row)) return true;
+  return false;
+}
+inline int overlap(const void* a, const Rows& ra, const void* b, const Rows& rb, int n_seqs, int heads, int dim, int dtype) {
+  const int64_t size = dtype == PKV_DST_F32 ? 4 : 2, row = dim * size, delta = (int64_t)((uintptr_t)b - (uintptr_t)a);
+  Axis x[3] = {{ra.seq, n_seqs}, {ra.token, ra.n}, {ra.head, heads}}, y[3] = {{rb.seq, n_seqs}, {rb.token, rb.n}, {rb.head, heads}};
+  bool equal = true;
+  int64_t low = 0, high = row;  // from the first byte of a to behind its last, and of both where they meet
+  int64_t low_b = delta, high_b = delta + row;
+  for (int i = 0; i < 3; i++) {
+    if (x[i].n <= 1) x[i].stride = y[i].stride = 0;  // says nothing
+    x[i].stride *= size;
+    y[i].stride *= size;
+    equal = equal && x[i].stride == y[i].stride;
+    const int64_t ea = x[i].stride * (x[i].n - 1), eb = y[i].stride * (y[i].n - 1);
+    (ea < 0 ? low : high) += ea;
+    (eb < 0 ? low_b : high_b) += eb;
+  }
+  if (high <= low_b || high_b <= low) return kApart;
+  if (!equal) return kOverlap;
+  if (delta == 0) return kSame;
+  auto size_of = [](const Axis& v) { return v.stride < 0 ? -v.stride : v.stride; };
+  for (int i = 0; i < 2; i++)
+    for (int j = 0; j + 1 < 3 - i; j++)
+      if (size_of(x[j]) < size_of(x[j + 1])) {
+        const Axis t = x[j];
+        x[j] = x[j + 1];
+        x[j + 1] = t;
+      }
+  return meets(delta, x, 3, row) ? kOverlap : kApart;
+}
+
 // Every kernel over this cache is launched so that it may come up while the one before it in the stream ends, and waits
 // here, before its first access to memory (saves about 1 us between two short kernels).
 __device__ __forceinline__ void wait_for_stream() { asm volatile("griddepcontrol.wait;" ::: "memory"); }

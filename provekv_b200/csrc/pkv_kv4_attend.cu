@@ -1130,6 +1130,10 @@ int make_call(const pkv_kv4_cache* cache, const void* q_dev, const pkv_kv4_rows*
   if (!err_dev || p.q.n != p.o.n || q_rows->dtype != out_rows->dtype) return PKV_ERR_INVALID_ARGUMENT;
   if (args->accumulate && (!lse_dev || !p.c.mass)) return PKV_ERR_INVALID_ARGUMENT;
   if (p.q.n == 0 || p.c.n_seqs == 0) return PKV_OK;
+  // A row tile's queries are read before its outputs are written, by the same CTA or a launch earlier, so out may be q.  The weights
+  // of a second pass over the keys are made from the queries after that.
+  const int shared = overlap(q_dev, p.q, out_dev, p.o, p.c.n_seqs, args->n_q_heads, cache->dim, q_rows->dtype);
+  if (shared == kOverlap || (shared == kSame && args->accumulate)) return PKV_ERR_INVALID_ARGUMENT;
   const bool chunk = chunk_takes(q_rows, args->n_q_heads / p.c.heads);
   Plan plan = {};
   if (!chunk) plan = make_plan(p.c, cache->dim, q_rows, args);

@@ -150,13 +150,15 @@ class Kv4Cache:
             raise ValueError(f"{name} must be a contiguous int32 [{self.n_seqs}] tensor on {self.device}")
         return t.data_ptr()
 
-    def _call(self, fn, *args) -> None:
+    def _status(self, fn, *args) -> int:
         """fn(cache, *args, error word, stream) with the cache's device current."""
         if self._current_device() == self._index:
-            status = fn(self._ref, *args, self._err, self._current_stream(self._index))
-        else:
-            with self._torch.cuda.device(self._index):
-                status = fn(self._ref, *args, self._err, self._current_stream(self._index))
+            return fn(self._ref, *args, self._err, self._current_stream(self._index))
+        with self._torch.cuda.device(self._index):
+            return fn(self._ref, *args, self._err, self._current_stream(self._index))
+
+    def _call(self, fn, *args) -> None:
+        status = self._status(fn, *args)
         if status:
             L.check(status)
 
@@ -202,6 +204,7 @@ class Kv4Cache:
                     ``out``, untouched in a given one; the same for ``lse``)
         accumulate  adds the weights of these queries to ``mass``
         max_len     a bound on the lengths that the host knows (sizes the split of the work; any value is correct)
+        out         where to write, of q's shape and type; may be q, or lie over it
         lse         f32 [n_seqs][n][n_q_heads], natural logarithm; -inf where a query sees nothing (its out is zeros)
         """
         torch = self._torch
@@ -231,8 +234,13 @@ class Kv4Cache:
         if empty:
             return out, lse
         work = self.pages.new_empty(need) if need else None
-        self._call(self._lib.pkv_kv4_attend_dev, q.data_ptr(), qr, out.data_ptr(), outr, lse.data_ptr(),
-                   self._per_seq(q_lens, "q_lens"), args, work.data_ptr() if need else None, need)
+        rest = (out.data_ptr(), outr, lse.data_ptr(), self._per_seq(q_lens, "q_lens"), args, work.data_ptr() if need else None, need)
+        status = self._status(self._lib.pkv_kv4_attend_dev, q.data_ptr(), qr, *rest)
+        if status == L.ERR_INVALID_ARGUMENT and out.untyped_storage().data_ptr() == q.untyped_storage().data_ptr():
+            q = q.clone()  # out lies over queries that are still to be read
+            status = self._status(self._lib.pkv_kv4_attend_dev, q.data_ptr(), self._rows(q, "q"), *rest)
+        if status:
+            L.check(status)
         return out, lse
 
     def evict(self, budget: int, *, sinks: int = 0, recent: int = 0) -> None:

@@ -790,3 +790,27 @@ def test_the_join_follows_no_entry_that_was_not_written():
         spoilt[first * group:(first + 6) * group] = True
         assert (out[0, 0, spoilt] == 7).all() and (lse[0, 0, spoilt] == 7).all()
         assert torch.equal(out[0, 0, ~spoilt], want[0, 0, ~spoilt]) and torch.equal(lse[0, 0, ~spoilt], wlse[0, 0, ~spoilt])
+
+
+@pytest.mark.parametrize("dtype,q_len,group", [("bfloat16", 1, 4), ("float16", 10, 2), ("float32", 10, 3), ("bfloat16", 35, 2)])
+def test_outputs_in_the_place_of_the_queries(dtype, q_len, group):
+    """Weights from stored scores, from a second pass over the keys, and behind a chunk: written over q they are the same."""
+    import torch
+    rng = np.random.default_rng(62)
+    pages, table, _ = kv4ref.fill(rng, 2, 2, 64, 16, [130, 71])
+    make = lambda: kv4.Kv4Cache(_dev(pages), _ints(table), _ints([130, 71]),  # noqa: E731
+                                mass=torch.zeros((2, 2, table.shape[1] * 16), device="cuda"))
+    buf = _dev(rng.standard_normal((2, q_len + 1, 2 * group, 64)), _dt(dtype))
+    for accumulate in (False, True):
+        for at in (1, 0):  # exactly over the queries, and a token beside them
+            plain, over = make(), make()
+            b = buf.clone()
+            q = b[:, 1:]
+            want, wlse = plain.attend(q.clone(), accumulate=accumulate)
+            out, lse = over.attend(q, accumulate=accumulate, out=b[:, at:at + q_len])
+            plain.check()
+            over.check()
+            assert out.data_ptr() == b[:, at:].data_ptr()
+            assert torch.equal(out, want) and torch.equal(lse, wlse) and torch.equal(over.mass, plain.mass)
+            assert (over.mass != 0).any() == accumulate
+            assert torch.equal(b[:, 0 if at else q_len], buf[:, 0 if at else q_len])

@@ -185,3 +185,40 @@ def test_the_join_alone_is_there_for_split_rows_only():
     assert call(_cache(dim=64), 1 << 30) == L.ERR_UNSUPPORTED                                # short rows: nothing is cut
     assert call(_cache(dim=128, max_pages=4096, n_seqs=1), 1 << 30) == L.ERR_UNSUPPORTED
     assert call(_cache(dim=64, max_pages=4096, n_seqs=1), 8) == L.ERR_BUFFER_TOO_SMALL
+
+
+def test_attend_refuses_outputs_over_its_queries():
+    """By the vectors, not by the ranges: q, k and v of one buffer lie between one another without meeting."""
+    bad = L.ERR_INVALID_ARGUMENT
+    full = _cache(mass=P, max_pages=4096, n_seqs=2)           # needs a workspace: where nothing is refused the call ends there
+    rows = lambda s: _rows(3, strides=s)  # noqa: E731
+    packed = (3 * 12 * 128, 12 * 128, 128)                     # 12 heads side by side, 4 of them queries
+    for shift, strides, acc, want in ((0, packed, 0, None), (0, packed, 1, bad), (4 * 128 * 2, packed, 1, None), (3 * 128 * 2, packed, 0, bad),
+                                      (-8 * 128 * 2, packed, 1, None), (-9 * 128 * 2, packed, 1, bad), (12 * 128 * 2, packed, 0, bad),
+                                      (3 * 12 * 128 * 2, packed, 0, bad), (6 * 12 * 128 * 2, packed, 1, None),
+                                      (16, packed, 0, bad), (-16, packed, 0, bad), (4 * 128 * 2 - 16, packed, 0, bad),
+                                      (0, (3 * 512, 512, 128), 0, bad), (6 * 12 * 128 * 2, (3 * 512, 512, 128), 1, None),
+                                      (-6 * 512 * 2, (3 * 512, 512, 128), 1, None), (-6 * 512 * 2 + 16, (3 * 512, 512, 128), 0, bad)):
+        got = _attend(full, _args(accumulate=acc), q=P, out=P + shift, qr=rows(packed), outr=rows(strides))
+        assert got == (want or L.ERR_BUFFER_TOO_SMALL), (shift, strides, acc)
+
+
+def test_overlap_against_a_list_of_bytes():
+    rng = np.random.default_rng(3)
+    full = _cache(dim=64, max_pages=4096, n_seqs=3, n_kv_heads=1)
+    seen = set()
+    for _ in range(400):
+        counts = (3, int(rng.integers(1, 5)), int(rng.integers(1, 4)))
+        order, step, strides = rng.permutation(3), 64, [0, 0, 0]
+        for i in order:  # axes in any order with gaps of whole vectors between them
+            strides[i] = int(step + 64 * rng.integers(0, 3))
+            step = strides[i] * counts[i]
+        shift = int(rng.integers(-step // 8 - 8, step // 8 + 8)) * 8 * 2
+        at = np.add.outer(np.add.outer(np.arange(counts[0]) * strides[0], np.arange(counts[1]) * strides[1]), np.arange(counts[2]) * strides[2])
+        q = (at.reshape(-1, 1) + np.arange(64)).ravel()
+        want = shift != 0 and np.isin(q, q + shift // 2).any()
+        row = _rows(counts[1], strides=tuple(strides))
+        got = _attend(full, _args(n_q_heads=counts[2]), q=P, out=P + shift, qr=row, outr=row)
+        assert (got == L.ERR_INVALID_ARGUMENT) == want and got in (L.ERR_INVALID_ARGUMENT, L.ERR_BUFFER_TOO_SMALL), (counts, strides, shift)
+        seen.add(bool(want))
+    assert seen == {False, True}
