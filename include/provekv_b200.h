@@ -494,7 +494,8 @@ typedef struct pkv_kv4_attend_args {
  * looked for exactly where both have the same strides, by the ranges otherwise).  lse_dev (may be null unless accumulating): [n_seqs][n_tokens][n_q_heads] f32, the natural logarithm of
  * the sum of exponentials, -inf where nothing is visible.  q and out have the same type.
  * Products, softmax statistics and sums are f32; weights enter the second product in binary16 (f32 queries: as two
- * binary16 terms).  The result does not depend on the order in which blocks run.
+ * binary16 terms).  The result does not depend on the order in which blocks run.  A row of queries that are not finite gives
+ * NaN; accumulating, it weighs nothing and is reported as PKV_VEC_NONFINITE_INPUT with the index of its lse.
  * workspace_dev: pkv_kv4_attend_workspace_bytes bytes (may be 0), 16-byte aligned, not shared with a call that can
  * overlap. */
 int64_t pkv_kv4_attend_workspace_bytes(const pkv_kv4_cache* cache, const pkv_kv4_rows* q_rows,

@@ -807,6 +807,16 @@ kv4_combine_kernel(const __grid_constant__ AttendParams p) {
   join_parts<D, T, W>(p, s, h, grow, of.y, [&](int k) { return ((int64_t)(of.x + k) * 2 + (k == 0)) * (8 * NT) + row; });
 }
 
+// A row's lse where its weights are accumulated.  A row that is not finite (reported) weighs nothing, like one that sees nothing:
+// a single one would otherwise spoil the sums of every token for good.
+__device__ __forceinline__ float weighing_lse(const AttendParams& p, int s, int token, int hq) {
+  const int64_t at = ((int64_t)s * p.q.n + token) * p.q_heads + hq;
+  const float lse = p.lse[at];
+  if (pkv_finite(lse) || lse == -INFINITY) return lse;
+  pkv_report(p.err, 0, at, PKV_VEC_NONFINITE_INPUT);
+  return -INFINITY;
+}
+
 // mass[key] += sum over the query rows of exp(score - lse), from the scores that the attention kernel left behind; a thread
 // per slot.  One row tile, so a slot's rows are 32 or 64 consecutive bytes.
 template <int NT>
@@ -820,7 +830,7 @@ kv4_mass_of_scores_kernel(const __grid_constant__ AttendParams p) {
   const Span span = visible_span(p, seq.len, pos0, seq.end - 1);
   if (threadIdx.x < 8 * NT) {
     const int r = threadIdx.x, token = r / p.group, hq = h * p.group + (r - token * p.group);
-    s_lse[r] = r < rows ? __fmul_rn(kLog2e, p.lse[((int64_t)s * p.q.n + token) * p.q_heads + hq]) : -INFINITY;
+    s_lse[r] = r < rows ? __fmul_rn(kLog2e, weighing_lse(p, s, token, hq)) : -INFINITY;
   }
   __syncthreads();
   for (int slot = blockIdx.x * 256 + threadIdx.x; slot < seq.len; slot += gridDim.x * 256) {
@@ -917,11 +927,15 @@ kv4_mass_kernel(const __grid_constant__ AttendParams p) {
         uint32_t hi[D / 16][2], lo[D / 16][2];
         float x[D / 4];
         const int r = r0 + 8 * warp + g, token = r / p.group, hq = h * p.group + (r - token * p.group);
-        const float lse = r < rows ? p.lse[((int64_t)s * p.q.n + token) * p.q_heads + hq] : -INFINITY;
+        const float lse = r < rows ? weighing_lse(p, s, token, hq) : -INFINITY;
         query_values<D, T>(p, s, h, r, rows, x);
         const float inv = query_operand<D, T>(x, p.negate, hi, lo);
 #pragma unroll
         for (int i = 0; i < D / 32; i++) {
+          if (lse == -INFINITY) {  // a product of 0, whatever the queries are
+            hi[2 * i][0] = hi[2 * i][1] = hi[2 * i + 1][0] = hi[2 * i + 1][1] = 0u;
+            if constexpr (F32) lo[2 * i][0] = lo[2 * i][1] = lo[2 * i + 1][0] = lo[2 * i + 1][1] = 0u;
+          }
           s_q[warp][0][i][lane] = make_uint4(hi[2 * i][0], hi[2 * i][1], hi[2 * i + 1][0], hi[2 * i + 1][1]);
           if constexpr (F32) s_q[warp][TERMS - 1][i][lane] = make_uint4(lo[2 * i][0], lo[2 * i][1], lo[2 * i + 1][0], lo[2 * i + 1][1]);
         }

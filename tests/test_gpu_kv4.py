@@ -814,3 +814,39 @@ def test_outputs_in_the_place_of_the_queries(dtype, q_len, group):
             assert torch.equal(out, want) and torch.equal(lse, wlse) and torch.equal(over.mass, plain.mass)
             assert (over.mass != 0).any() == accumulate
             assert torch.equal(b[:, 0 if at else q_len], buf[:, 0 if at else q_len])
+
+
+@pytest.mark.parametrize("dtype,q_len,group,lens", [("bfloat16", 1, 4, [50, 90]), ("float32", 1, 2, [50, 3000]), ("float32", 10, 2, [50, 90]),
+                                                    ("float16", 10, 2, [50, 300]), ("bfloat16", 30, 4, [50, 300])])
+def test_queries_that_are_not_finite_weigh_nothing(dtype, q_len, group, lens):
+    """mass is that of the other rows, from stored scores and from a second pass over the keys; the first such row is reported."""
+    import torch
+    rng = np.random.default_rng(63)
+    pages, table, values = kv4ref.fill(rng, 2, 2, 64, 16, lens)
+    mass = torch.zeros((2, 2, table.shape[1] * 16), device="cuda")
+    cache = kv4.Kv4Cache(_dev(pages), _ints(table), _ints(lens), mass=mass)
+    q = _dev(rng.standard_normal((2, q_len, 2 * group, 64)), _dt(dtype))
+    clean, _ = cache.attend(q)
+    heads, last = 2 * group, q_len - 1
+    rows = [(0, last, 1), (1, 0, heads - 1), (1, last, 0)]
+    spoilt = torch.zeros((2, q_len, heads), dtype=torch.bool, device="cuda")
+    q2 = q.clone()
+    for (s, i, h), x in zip(rows, ("nan", "inf", "-inf")):
+        q2[s, i, h, 7] = float(x)
+        q2[s, i, h, 8] = -float(x)  # whatever the keys' signs, products of either
+        spoilt[s, i, h] = True
+    out, lse = cache.attend(q2, accumulate=True)
+    with pytest.raises(pk.PkvError) as e:
+        cache.check()
+    assert (e.value.status, e.value.vector_index) == (L.VEC_NONFINITE_INPUT, (0 * q_len + last) * heads + 1)
+    assert torch.isnan(out[spoilt]).all() and torch.equal(out[~spoilt], clean[~spoilt])
+    ref = q.double().cpu().numpy()
+    want = kv4ref.attend(ref, values, lens, lens, None, group, 0.125, 0, 0, [q_len] * 2)
+    added = want[2].copy()
+    for s, i, h in rows:  # less what those rows would have added
+        n = lens[s] - q_len + i + 1
+        added[s, h // group, :n] -= np.exp(0.125 * (values[s, 0, h // group, :n] @ ref[s, i, h]) - want[1][s, i, h])
+    got = mass.double().cpu().numpy()[:, :, :added.shape[2]]
+    # a weight is off by its score's error and its sum's, and rounded once a row; the difference above is of 64-bit numbers
+    eps = 2.0 ** -18 * want[4].max() + 2.0 ** -22 * np.abs(want[1]).max() + 2.0 ** -19
+    _within(got, added, (2 * eps + 2.0 ** -24 * q_len * group) * added + 1e-12, "mass")
