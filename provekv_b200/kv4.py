@@ -21,6 +21,7 @@ cache's error word: `check` reads it.
 from __future__ import annotations
 
 import ctypes as C
+from operator import index
 
 from . import _lib as L
 from .patch import dst_dtype_of
@@ -36,7 +37,9 @@ def atom_bytes(dim: int) -> int:
 
 
 def _int32(name: str, x: int) -> int:
-    """A count as the library takes it (ctypes would cut off what is above 32 bits)."""
+    """A count as the library takes it (ctypes would cut off what is above 32 bits), as a plain number: what is kept by it
+    must not change when the caller's object does."""
+    x = index(x)
     if not 0 <= x < 1 << 31:
         raise ValueError(f"{name} must be at least 0 and below 2**31, not {x}")
     return x
@@ -219,6 +222,11 @@ class Kv4Cache:
             lse = (q.new_empty if q_lens is None else q.new_zeros)(shape[:3], dtype=torch.float32)
         elif lse.shape != shape[:3] or lse.dtype != torch.float32 or not lse.is_contiguous() or lse.get_device() != self._index:
             raise ValueError("lse must be contiguous f32 [n_seqs][tokens][heads] on the cache's device")
+        if scale is not None and type(scale) is not float:
+            scale = float(scale)
+        if not type(window) is type(sinks) is type(max_len) is int:
+            window, sinks, max_len = _int32("window", window), _int32("sinks", sinks), _int32("max_len", max_len)
+        accumulate = bool(accumulate)
         key = (shape, q.dtype, scale, window, sinks, accumulate, max_len)
         plan = self._attend_of.get(key)
         if plan is None:
@@ -249,8 +257,7 @@ class Kv4Cache:
         all layers are done."""
         if self.positions is None or self.mass is None:
             raise ValueError("evict needs a cache with positions and mass")
-        for name, x in (("budget", budget), ("sinks", sinks), ("recent", recent)):
-            _int32(name, x)
+        budget, sinks, recent = _int32("budget", budget), _int32("sinks", sinks), _int32("recent", recent)
         if self.n_seqs == 0:
             return
         need = self._evict_of.get(budget)

@@ -850,3 +850,29 @@ def test_queries_that_are_not_finite_weigh_nothing(dtype, q_len, group, lens):
     # a weight is off by its score's error and its sum's, and rounded once a row; the difference above is of 64-bit numbers
     eps = 2.0 ** -18 * want[4].max() + 2.0 ** -22 * np.abs(want[1]).max() + 2.0 ** -19
     _within(got, added, (2 * eps + 2.0 ** -24 * q_len * group) * added + 1e-12, "mass")
+
+
+def test_arguments_that_change_in_place_are_read_at_every_call():
+    """A scale or a count may be a tensor of one value: nothing is kept by the tensor itself."""
+    import torch
+    rng = np.random.default_rng(64)
+    pages, table, _ = kv4ref.fill(rng, 1, 2, 64, 16, [90])
+    cap = table.shape[1] * 16
+    cache = kv4.Kv4Cache(_dev(pages), _ints(table), _ints([90]), positions=torch.arange(cap, device="cuda").int().expand(1, 2, cap).contiguous(),
+                         mass=_dev(rng.random((1, 2, cap)), torch.float32))
+    q = _dev(rng.standard_normal((1, 1, 4, 64)), torch.float32)
+    scale, window, sinks = torch.tensor(0.125), torch.tensor(20), torch.tensor(3)
+    for change in (None, (scale, -0.3), (window, 7), (sinks, 30), (window, 0)):
+        if change:
+            change[0].fill_(change[1])
+        want = cache.attend(q, scale=float(scale), window=int(window), sinks=int(sinks))
+        got = cache.attend(q, scale=scale, window=window, sinks=sinks)
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    with pytest.raises(TypeError):
+        cache.attend(q, window=7.0)
+    budget = torch.tensor(80)
+    cache.evict(budget)  # its workspace is smaller than that of the next
+    cache.lens.clamp_(max=80)
+    budget.fill_(40)
+    cache.evict(budget)
+    cache.check()

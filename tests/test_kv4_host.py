@@ -222,3 +222,12 @@ def test_overlap_against_a_list_of_bytes():
         assert (got == L.ERR_INVALID_ARGUMENT) == want and got in (L.ERR_INVALID_ARGUMENT, L.ERR_BUFFER_TOO_SMALL), (counts, strides, shift)
         seen.add(bool(want))
     assert seen == {False, True}
+
+
+def test_counts_become_plain_numbers():
+    import torch
+    for x in (np.int64(7), torch.tensor(7), True):
+        assert type(kv4._int32("sinks", x)) is int and kv4._int32("sinks", x) == int(x)
+    for x in (1.0, torch.tensor(1.5), "3"):
+        with pytest.raises(TypeError):
+            kv4._int32("sinks", x)
