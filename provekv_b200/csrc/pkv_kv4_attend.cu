@@ -1045,17 +1045,19 @@ Plan make_plan(const Cache& c, int dim, const pkv_kv4_rows* q, const pkv_kv4_att
   const int64_t rows = (int64_t)q->n_tokens * (a->n_q_heads / c.heads);
   r.nt = rows > 8 ? 2 : 1;
   r.row_tiles = (int)((rows + 8 * r.nt - 1) / (8 * r.nt));
-  int64_t longest = a->max_len > 0 && a->max_len < c.capacity ? a->max_len : c.capacity;
+  int64_t most = c.capacity, longest = a->max_len > 0 && a->max_len < c.capacity ? a->max_len : c.capacity;
   if (a->window > 0 && !c.positions) {  // slots outside the sinks and the window of the query tokens are never visited
     const int64_t seen = (int64_t)a->window + a->sinks + q->n_tokens + 3 * kUnitTokens;
     if (seen < longest) longest = seen;
+    if (seen < most) most = seen;
   }
-  const int64_t units = (longest + kUnitTokens - 1) / kUnitTokens;
+  const int64_t units = (longest + kUnitTokens - 1) / kUnitTokens, most_units = (most + kUnitTokens - 1) / kUnitTokens;
   // Rows of up to six units a warp are not worth a second launch (32 sequences with a window of 1024, 8 kv heads: 17.2 us
   // against 24.4), and with a row for every warp there is nothing to cut.
   const int64_t tiles = (int64_t)c.heads * r.row_tiles * c.n_seqs, resident = (int64_t)sm_count() * kWarps * ctas_per_sm(dim, r.nt, q->dtype == PKV_DST_F32);
   r.runs = 0;
-  if (units > 6 * kWarps && tiles < kMaxRows && units * tiles < (1ll << 31)) {
+  // (the kernel numbers the units of all rows in 32 bits, and max_len may be below the lengths)
+  if (units > 6 * kWarps && tiles < kMaxRows && most_units * tiles < (1ll << 31)) {
     const int64_t could = (units * tiles + kWarps - 1) / kWarps * kWarps;
     r.runs = (int)(could < resident ? could : resident);
   }

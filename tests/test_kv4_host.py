@@ -231,3 +231,14 @@ def test_counts_become_plain_numbers():
     for x in (1.0, torch.tensor(1.5), "3"):
         with pytest.raises(TypeError):
             kv4._int32("sinks", x)
+
+
+def test_rows_share_runs_only_where_their_units_can_be_numbered():
+    """2^24 units of 64 tokens in the table, 1024 row tiles: 2^34 units, whatever bound on the lengths the caller gives."""
+    need = lambda c, **kw: L.lib().pkv_kv4_attend_workspace_bytes(C.byref(c), C.byref(_rows()), C.byref(_args(n_q_heads=16, **kw)))  # noqa: E731
+    huge = dict(max_pages=1 << 24, n_seqs=64, n_kv_heads=16)
+    assert need(_cache(**huge)) == 0
+    assert need(_cache(**huge), max_len=1 << 17) == 0
+    assert need(_cache(**huge), window=1 << 17) > 0                    # a window bounds what is visited
+    assert need(_cache(**huge, positions=P), window=1 << 17) == 0      # unless any slot may be in it
+    assert need(_cache(**{**huge, "max_pages": 1 << 20}), max_len=1 << 17) > 0
