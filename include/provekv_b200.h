@@ -462,8 +462,8 @@ typedef struct pkv_kv4_cache {
  * the base 16-byte aligned), the dim values of a vector contiguous. */
 typedef struct pkv_kv4_rows {
   int64_t seq_stride, token_stride, head_stride;
-  int32_t n_tokens;
-  int32_t dtype;  /* PKV_DST_* */
+  int32_t n_tokens;  /* PKV_ERR_UNSUPPORTED above 0x7fff0000 */
+  int32_t dtype;     /* PKV_DST_* */
 } pkv_kv4_rows;
 
 /* Writes the keys and values of each sequence's newest tokens: row i of sequence s goes to slot

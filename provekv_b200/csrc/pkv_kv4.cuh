@@ -7,6 +7,7 @@
 namespace pkv_kv4 {
 
 constexpr int kAtomTokens = 16;
+constexpr int64_t kMostSlots = 0x7fff0000;  // of a sequence, and tokens of a call: 32-bit numbers with room for a tile behind the last
 constexpr int kMaxScaleByte = 0xDE;  // 7168: the largest scale for which the dequantisation below stays in range
 
 // Byte offsets inside an atom (16 tokens of one kv head).
@@ -65,8 +66,8 @@ inline int make_cache(const pkv_kv4_cache* c, Cache* out) {
     return PKV_ERR_INVALID_ARGUMENT;
   if (((uintptr_t)c->pages | (uintptr_t)c->positions | (uintptr_t)c->mass) & 15) return PKV_ERR_INVALID_ARGUMENT;
   if ((c->dim != 64 && c->dim != 128) || c->page_tokens % kAtomTokens) return PKV_ERR_UNSUPPORTED;
-  // slots are 32-bit numbers with room for a tile behind the last one; sequences and heads go into grid dimensions
-  if ((int64_t)c->max_pages * c->page_tokens > 0x7fff0000ll || c->n_kv_heads > 65535 || c->n_seqs > 65535)
+  // sequences and heads go into grid dimensions
+  if ((int64_t)c->max_pages * c->page_tokens > kMostSlots || c->n_kv_heads > 65535 || c->n_seqs > 65535)
     return PKV_ERR_UNSUPPORTED;
   out->pages = c->pages;
   out->table = c->page_table;
@@ -90,6 +91,7 @@ inline int make_rows(const void* base, const pkv_kv4_rows* r, Rows* out) {
   const int unit = r->dtype == PKV_DST_F32 ? 4 : 8;
   if (((uintptr_t)base & 15) || r->seq_stride % unit || r->token_stride % unit || r->head_stride % unit)
     return PKV_ERR_INVALID_ARGUMENT;
+  if (r->n_tokens > kMostSlots) return PKV_ERR_UNSUPPORTED;
   out->seq = r->seq_stride;
   out->token = r->token_stride;
   out->head = r->head_stride;

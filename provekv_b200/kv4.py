@@ -139,7 +139,8 @@ class Kv4Cache:
             if len(self._rows_of) >= 256:
                 self._rows_of.clear()
             # (the stride of a dimension of one says nothing)
-            r = self._rows_of[key] = C.byref(L.Kv4RowsC(*(stride[i] if shape[i] > 1 else 0 for i in range(3)), shape[1], dst_dtype_of(t)))
+            r = self._rows_of[key] = C.byref(L.Kv4RowsC(*(stride[i] if shape[i] > 1 else 0 for i in range(3)), _int32(f"the tokens of {name}", shape[1]),
+                                                       dst_dtype_of(t)))
         if heads is not None and t.shape[2] != heads:
             raise ValueError(f"{name} has {t.shape[2]} heads, the cache {heads}")
         if t.get_device() != self._index:

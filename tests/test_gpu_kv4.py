@@ -876,3 +876,20 @@ def test_arguments_that_change_in_place_are_read_at_every_call():
     budget.fill_(40)
     cache.evict(budget)
     cache.check()
+
+
+def test_more_tokens_than_32_bits_are_refused():
+    """An expanded tensor has as many tokens as its view says, not those of the count's lower 32 bits."""
+    import torch
+    rng = np.random.default_rng(65)
+    cache = _empty_cache(1, 2, 64, 16, 4, rng, [5])
+    before = cache.pages.clone()
+    x = torch.ones((1, 1, 2, 64), device="cuda")
+    for n in ((1 << 32) + 1, 1 << 31):
+        with pytest.raises(ValueError, match="tokens"):
+            cache.append(x.expand(1, n, 2, 64), x.expand(1, n, 2, 64), _ints([1]))
+    assert torch.equal(cache.pages, before)
+    cache.append(x.expand(1, 5, 2, 64), x.expand(1, 5, 2, 64))
+    cache.check()
+    want = kv4ref.dequantise(*kv4ref.quantise(np.ones((1, 5, 2, 64))))  # 7 x 0.140625, the scale nearest to 1 / 7
+    assert np.array_equal(cache.read(5)[0].double().cpu().numpy(), want)

@@ -242,3 +242,13 @@ def test_rows_share_runs_only_where_their_units_can_be_numbered():
     assert need(_cache(**huge), window=1 << 17) > 0                    # a window bounds what is visited
     assert need(_cache(**huge, positions=P), window=1 << 17) == 0      # unless any slot may be in it
     assert need(_cache(**{**huge, "max_pages": 1 << 20}), max_len=1 << 17) > 0
+
+
+@pytest.mark.parametrize("fn", ["pkv_kv4_append_dev", "pkv_kv4_read_dev"])
+def test_token_numbers_stay_in_32_bits(fn):
+    """Rows up to the last tile's end are numbered; n_seqs = 0 would end the call before anything is launched."""
+    f = getattr(L.lib(), fn)
+    rest = (0,) if fn == "pkv_kv4_read_dev" else ()
+    for n, want in ((0x7fff0000, L.OK), (0x7fff0001, L.ERR_UNSUPPORTED), (0x7fffffff, L.ERR_UNSUPPORTED)):
+        row = _rows(n, strides=(0, 0, 128))
+        assert f(C.byref(_cache(n_seqs=0)), P, C.byref(row), P, C.byref(row), P, *rest, P, None) == want
