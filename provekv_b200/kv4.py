@@ -62,13 +62,19 @@ class Kv4Cache:
     ends        int32 [n_seqs]: tokens the sequence has had (None: as many as it holds)
     positions   int32 [n_seqs][n_kv_heads][max_pages * page_tokens]: position of the token in a slot (None: the slot's number)
     mass        f32, the same shape: attention weight received
+
+    They are attributes under these names; one that is assigned another tensor of the same kind uses it from the next call on.
     """
+    pages, page_table, lens, ends, positions, mass = (
+        property(lambda self, name=name: getattr(self, "_" + name), lambda self, t, name=name: self._rebind(name, t))
+        for name in ("pages", "page_table", "lens", "ends", "positions", "mass"))
+    error = property(lambda self: self._error, doc="The error word that the kernels report to (see `check`).")
 
     def __init__(self, pages, page_table, lens, *, ends=None, positions=None, mass=None):
         import torch
         if pages.dim() != 4 or pages.dtype != torch.uint8:
             raise ValueError("pages must be uint8 [n_pages][n_kv_heads][page_tokens / 16][18 * dim]")
-        n_pages, self.n_kv_heads, atoms, width = pages.shape
+        _, self.n_kv_heads, atoms, width = pages.shape
         self.dim, self.page_tokens, self.device = width // 18, atoms * ATOM_TOKENS, pages.device
         if width not in (atom_bytes(64), atom_bytes(128)):
             raise ValueError(f"an atom has 18 * 64 or 18 * 128 bytes, not {width}")
@@ -77,30 +83,51 @@ class Kv4Cache:
         self.n_seqs, max_pages = page_table.shape
         self.capacity = max_pages * self.page_tokens
         stats = (self.n_seqs, self.n_kv_heads, self.capacity)
-        for name, t, dtype, shape in (("pages", pages, torch.uint8, pages.shape), ("page_table", page_table, torch.int32, page_table.shape),
-                                      ("lens", lens, torch.int32, (self.n_seqs,)), ("ends", ends, torch.int32, (self.n_seqs,)),
-                                      ("positions", positions, torch.int32, stats), ("mass", mass, torch.float32, stats)):
-            if t is None:
-                continue
-            if t.dtype != dtype or tuple(t.shape) != tuple(shape):
-                raise ValueError(f"{name} must be {dtype} of shape {tuple(shape)}, not {t.dtype} of {tuple(t.shape)}")
-            if not t.is_contiguous():
-                raise ValueError(f"{name} must be contiguous")
-            if t.device != self.device:
-                raise ValueError(f"{name} is on {t.device}, the pages on {self.device}")
+        self._like = {"pages": (torch.uint8, pages.shape[1:]), "page_table": (torch.int32, page_table.shape),
+                      "lens": (torch.int32, (self.n_seqs,)), "ends": (torch.int32, (self.n_seqs,)),
+                      "positions": (torch.int32, stats), "mass": (torch.float32, stats)}
+        tensors = dict(pages=pages, page_table=page_table, lens=lens, ends=ends, positions=positions, mass=mass)
+        for name, t in tensors.items():
+            self._check_tensor(name, t)
         if self.device.type != "cuda":
             raise ValueError("a Kv4Cache lives on a CUDA device")
-        self.pages, self.page_table, self.lens, self.ends, self.positions, self.mass = (
-            pages, page_table, lens, ends, positions, mass)
-        ptr = lambda t: None if t is None else t.data_ptr()  # noqa: E731
-        self._c = L.Kv4CacheC(ptr(pages), ptr(page_table), ptr(lens), ptr(ends), ptr(positions), ptr(mass), n_pages,
-                              self.dim, self.n_kv_heads, self.page_tokens, self.n_seqs, max_pages, 0)
-        self.error = torch.full((1,), -1, dtype=torch.int64, device=self.device)
-        # what a call needs besides its tensors' addresses, prepared once: a decode step makes few microseconds' calls
-        self._ref, self._err, self._index = C.byref(self._c), self.error.data_ptr(), self.device.index
+        self._c = L.Kv4CacheC(dim=self.dim, n_kv_heads=self.n_kv_heads, page_tokens=self.page_tokens, n_seqs=self.n_seqs,
+                              max_pages=max_pages)
         self._rows_of, self._attend_of, self._evict_of = {}, {}, {}
+        for name, t in tensors.items():
+            self._bind(name, t)
+        self._error = torch.full((1,), -1, dtype=torch.int64, device=self.device)
+        # what a call needs besides its tensors' addresses, prepared once: a decode step makes few microseconds' calls
+        self._ref, self._err, self._index = C.byref(self._c), self._error.data_ptr(), self.device.index
         self._lib, self._torch = L.lib(), torch
         self._current_device, self._current_stream = _raw_queries(torch)
+
+    def _check_tensor(self, name: str, t) -> None:
+        dtype, shape = self._like[name]
+        if t is None:
+            if name in ("pages", "page_table", "lens"):
+                raise ValueError(f"{name} must be a tensor")
+            return
+        if t.dtype != dtype or tuple(t.shape[1:] if name == "pages" else t.shape) != tuple(shape):
+            raise ValueError(f"{name} must be {dtype} of shape {tuple(shape)}, not {t.dtype} of {tuple(t.shape)}")
+        if not t.is_contiguous():
+            raise ValueError(f"{name} must be contiguous")
+        if t.device != self.device:
+            raise ValueError(f"{name} is on {t.device}, the pages on {self.device}")
+
+    def _bind(self, name: str, t) -> None:
+        """Makes a checked tensor the one that later calls use."""
+        setattr(self, "_" + name, t)
+        setattr(self._c, name, None if t is None else t.data_ptr())
+        if name == "pages":
+            self._c.n_pages = t.shape[0]
+        self._attend_of.clear()  # workspaces go by which statistics there are
+        self._evict_of.clear()
+
+    def _rebind(self, name: str, t) -> None:
+        if t is not getattr(self, "_" + name):  # (`cache.lens += 1` assigns the tensor that it changed)
+            self._check_tensor(name, t)
+            self._bind(name, t)
 
     @classmethod
     def allocate(cls, n_layers: int, n_seqs: int, n_kv_heads: int, dim: int, max_tokens: int, *, page_tokens: int = 64,
@@ -183,7 +210,7 @@ class Kv4Cache:
         fresh = out is None
         if fresh:
             shape, dtype = (self.n_seqs, n, self.n_kv_heads, self.dim), dtype or torch.float32
-            k = self.pages.new_empty(shape, dtype=dtype)
+            k = self._pages.new_empty(shape, dtype=dtype)
             v = torch.empty_like(k)
         else:
             k, v = out
@@ -231,7 +258,7 @@ class Kv4Cache:
         key = (shape, q.dtype, scale, window, sinks, accumulate, max_len)
         plan = self._attend_of.get(key)
         if plan is None:
-            if accumulate and self.mass is None:
+            if accumulate and self._mass is None:
                 raise ValueError("accumulate needs a cache with mass")
             args = L.Kv4AttendC(self.dim ** -0.5 if scale is None else scale, shape[2], _int32("window", window), _int32("sinks", sinks),
                                 int(accumulate), _int32("max_len", max_len))
@@ -242,7 +269,7 @@ class Kv4Cache:
         args, need, empty = plan
         if empty:
             return out, lse
-        work = self.pages.new_empty(need) if need else None
+        work = self._pages.new_empty(need) if need else None
         rest = (out.data_ptr(), outr, lse.data_ptr(), self._per_seq(q_lens, "q_lens"), args, work.data_ptr() if need else None, need)
         status = self._status(self._lib.pkv_kv4_attend_dev, q.data_ptr(), qr, *rest)
         if status == L.ERR_INVALID_ARGUMENT and out.untyped_storage().data_ptr() == q.untyped_storage().data_ptr():
@@ -256,7 +283,7 @@ class Kv4Cache:
         """Cuts every sequence longer than `budget` down to it, per kv head: positions below `sinks`, the `recent` newest
         positions, and the heaviest of the others stay (ties: the lowest slot).  Then ``lens.clamp_(max=budget)``, once
         all layers are done."""
-        if self.positions is None or self.mass is None:
+        if self._positions is None or self._mass is None:
             raise ValueError("evict needs a cache with positions and mass")
         budget, sinks, recent = _int32("budget", budget), _int32("sinks", sinks), _int32("recent", recent)
         if self.n_seqs == 0:
@@ -266,7 +293,7 @@ class Kv4Cache:
             if len(self._evict_of) >= 256:
                 self._evict_of.clear()
             need = self._evict_of[budget] = self._lib.pkv_kv4_evict_workspace_bytes(self._ref, budget)
-        work = self.pages.new_empty(need) if need else None
+        work = self._pages.new_empty(need) if need else None
         self._call(self._lib.pkv_kv4_evict_dev, budget, sinks, recent, work.data_ptr() if need else None, need)
 
     def check(self) -> None:

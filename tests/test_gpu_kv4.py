@@ -893,3 +893,38 @@ def test_more_tokens_than_32_bits_are_refused():
     cache.check()
     want = kv4ref.dequantise(*kv4ref.quantise(np.ones((1, 5, 2, 64))))  # 7 x 0.140625, the scale nearest to 1 / 7
     assert np.array_equal(cache.read(5)[0].double().cpu().numpy(), want)
+
+
+def test_tensors_that_are_replaced_are_used():
+    import torch
+    rng = np.random.default_rng(66)
+    pages, table, _ = kv4ref.fill(rng, 2, 2, 64, 16, [40, 70])
+    cap = table.shape[1] * 16
+    q = _dev(rng.standard_normal((2, 1, 4, 64)), torch.float32)
+    make = lambda p, lens, **kw: kv4.Kv4Cache(p, _ints(table), lens, **kw)  # noqa: E731
+    cache = make(_dev(pages), _ints([40, 70]))
+    first = cache.attend(q)
+    cache.lens += 1  # in place, then assigned to itself
+    assert cache.lens.tolist() == [41, 71]
+    lens = cache.lens = cache.lens - 9
+    assert cache.lens is lens
+    want = make(_dev(pages), _ints([32, 62])).attend(q)
+    got = cache.attend(q)
+    assert torch.equal(got[0], want[0]) and not torch.equal(got[0], first[0])
+    more = torch.cat([_dev(pages), _dev(pages).flip(0)])  # a pool of another size
+    cache.pages, cache.page_table = more, _ints(more.shape[0] - 1 - table)
+    assert torch.equal(cache.attend(q)[0], want[0])
+    cache.mass, cache.positions = torch.zeros((2, 2, cap), device="cuda"), torch.arange(cap, device="cuda").int().expand(2, 2, cap).contiguous()
+    got = cache.attend(q, accumulate=True)
+    assert torch.equal(got[0], want[0]) and (cache.mass[0, :, :32] > 0).all() and (cache.mass[0, :, 32:] == 0).all()
+    cache.mass = None
+    with pytest.raises(ValueError, match="mass"):
+        cache.attend(q, accumulate=True)
+    cache.check()
+    for name, t in (("lens", _ints([1, 2, 3])), ("lens", lens.long()), ("lens", lens.cpu()), ("lens", None), ("pages", more[:, :1]),
+                    ("page_table", _ints(table)[:, :1]), ("positions", torch.zeros((2, 2, 2 * cap), dtype=torch.int32, device="cuda")[:, :, ::2])):
+        with pytest.raises(ValueError, match=name):
+            setattr(cache, name, t)
+    assert torch.equal(cache.attend(q)[0], want[0])
+    with pytest.raises(AttributeError):
+        cache.error = cache.error.clone()
