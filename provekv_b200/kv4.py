@@ -181,12 +181,15 @@ class Kv4Cache:
             raise ValueError(f"{name} must be a contiguous int32 [{self.n_seqs}] tensor on {self.device}")
         return t.data_ptr()
 
-    def _status(self, fn, *args) -> int:
-        """fn(cache, *args, error word, stream) with the cache's device current."""
+    def _on_device(self, fn, *args) -> int:
+        """fn(cache, *args) with the cache's device current (plans go by its size)."""
         if self._current_device() == self._index:
-            return fn(self._ref, *args, self._err, self._current_stream(self._index))
+            return fn(self._ref, *args)
         with self._torch.cuda.device(self._index):
-            return fn(self._ref, *args, self._err, self._current_stream(self._index))
+            return fn(self._ref, *args)
+
+    def _status(self, fn, *args) -> int:
+        return self._on_device(fn, *args, self._err, self._current_stream(self._index))
 
     def _call(self, fn, *args) -> None:
         status = self._status(fn, *args)
@@ -264,7 +267,7 @@ class Kv4Cache:
                                 int(accumulate), _int32("max_len", max_len))
             if len(self._attend_of) >= 256:
                 self._attend_of.clear()
-            plan = self._attend_of[key] = (C.byref(args), self._lib.pkv_kv4_attend_workspace_bytes(self._ref, qr, C.byref(args)),
+            plan = self._attend_of[key] = (C.byref(args), self._on_device(self._lib.pkv_kv4_attend_workspace_bytes, qr, C.byref(args)),
                                            q.numel() == 0)
         args, need, empty = plan
         if empty:

@@ -928,3 +928,37 @@ def test_tensors_that_are_replaced_are_used():
     assert torch.equal(cache.attend(q)[0], want[0])
     with pytest.raises(AttributeError):
         cache.error = cache.error.clone()
+
+
+def test_calls_are_planned_and_made_on_the_caches_device(monkeypatch):
+    """As if another device were current: workspace and launch are asked for inside the guard, the device of the cache in it."""
+    import torch
+    rng = np.random.default_rng(67)
+    pages, table, _ = kv4ref.fill(rng, 1, 1, 64, 64, [2500])
+    cache = kv4.Kv4Cache(_dev(pages), _ints(table), _ints([2500]))
+    q = _dev(rng.standard_normal((1, 1, 4, 64)), torch.float32)
+    events = []
+
+    class Guard(torch.cuda.device):
+        def __enter__(self):
+            events.append(self.idx)
+            return super().__enter__()
+
+        def __exit__(self, *args):
+            events.append("out")
+            return super().__exit__(*args)
+
+    class Recorder:
+        def __getattr__(self, name):
+            def call(*args):
+                events.append(name)
+                return getattr(L.lib(), name)(*args)
+            return call
+
+    want = cache.attend(q)
+    cache = kv4.Kv4Cache(_dev(pages), _ints(table), _ints([2500]))
+    monkeypatch.setattr(torch.cuda, "device", Guard)
+    cache._lib, cache._current_device = Recorder(), lambda: cache._index + 1
+    got = cache.attend(q)
+    assert events == [cache._index, "pkv_kv4_attend_workspace_bytes", "out", cache._index, "pkv_kv4_attend_dev", "out"]
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
