@@ -230,7 +230,7 @@ class Kv4Cache:
     def attend(self, q, *, scale: float | None = None, window: int = 0, sinks: int = 0, q_lens=None, accumulate: bool = False,
                max_len: int = 0, out=None, lse=None):
         """(out, lse): attention of the newest tokens' queries ``q`` [n_seqs][n][n_q_heads][dim] over what their
-        sequences hold, each up to its own position.
+        sequences hold, each up to its own position.  Not differentiable.
 
         scale       of the products; None: dim ** -0.5
         window      > 0: only the `window` newest positions, and those below `sinks`
@@ -242,6 +242,8 @@ class Kv4Cache:
         lse         f32 [n_seqs][n][n_q_heads], natural logarithm; -inf where a query sees nothing (its out is zeros)
         """
         torch = self._torch
+        if q.requires_grad and torch.is_grad_enabled():
+            raise ValueError("attend has no gradient: detach q, or call it under torch.no_grad()")
         qr = self._rows(q, "q")
         shape = q.shape
         if out is None:

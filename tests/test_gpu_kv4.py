@@ -962,3 +962,18 @@ def test_calls_are_planned_and_made_on_the_caches_device(monkeypatch):
     got = cache.attend(q)
     assert events == [cache._index, "pkv_kv4_attend_workspace_bytes", "out", cache._index, "pkv_kv4_attend_dev", "out"]
     assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+def test_attention_refuses_to_drop_a_gradient():
+    import torch
+    rng = np.random.default_rng(68)
+    pages, table, _ = kv4ref.fill(rng, 1, 1, 64, 16, [20])
+    cache = kv4.Kv4Cache(_dev(pages), _ints(table), _ints([20]))
+    q = _dev(rng.standard_normal((1, 1, 2, 64)), torch.float32)
+    want, _ = cache.attend(q)
+    q.requires_grad_()
+    with pytest.raises(ValueError, match="gradient"):
+        cache.attend(q)
+    with torch.no_grad():
+        assert torch.equal(cache.attend(q)[0], want)
+    assert torch.equal(cache.attend(q.detach())[0], want)
