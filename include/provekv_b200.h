@@ -475,7 +475,7 @@ int pkv_kv4_append_dev(const pkv_kv4_cache* cache, const void* k_dev, const pkv_
                        const pkv_kv4_rows* v_rows, const int32_t* new_lens_dev, uint64_t* err_dev, void* stream);
 /* The inverse: the values the newest tokens of each sequence stand for, at the rows an append would take them from;
  * new_lens = lens reads everything.  Rows from new_lens[s] on stay as they were (clear_rest = 0) or become zeros
- * (clear_rest = 1), as do the rows of a bad page or sequence. */
+ * (clear_rest = 1), as do the rows of a bad page or sequence.  k and v must not overlap (refused). */
 int pkv_kv4_read_dev(const pkv_kv4_cache* cache, void* k_dev, const pkv_kv4_rows* k_rows, void* v_dev,
                      const pkv_kv4_rows* v_rows, const int32_t* new_lens_dev, int32_t clear_rest, uint64_t* err_dev, void* stream);
 

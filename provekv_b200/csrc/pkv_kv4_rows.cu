@@ -355,6 +355,8 @@ int rows_call(bool append, const pkv_kv4_cache* cache, const void* k, const pkv_
   if (!err || kr.n != vr.n || k_rows->dtype != v_rows->dtype || (clear_rest != 0 && clear_rest != 1)) return PKV_ERR_INVALID_ARGUMENT;
   if (kr.n > c.capacity && !new_lens) return PKV_ERR_INVALID_ARGUMENT;
   if (kr.n == 0 || c.n_seqs == 0) return PKV_OK;
+  // both are written; sets of vectors that are only between one another are apart
+  if (!append && overlap(k, kr, v, vr, c.n_seqs, c.heads, cache->dim, k_rows->dtype) != kApart) return PKV_ERR_INVALID_ARGUMENT;
   cudaStream_t s = (cudaStream_t)stream;
   cudaError_t ce;
 #define PKV_KV4_ROWS(D)                                                                                                    \

@@ -977,3 +977,23 @@ def test_attention_refuses_to_drop_a_gradient():
     with torch.no_grad():
         assert torch.equal(cache.attend(q)[0], want)
     assert torch.equal(cache.attend(q.detach())[0], want)
+
+
+def test_read_into_slices_of_one_buffer():
+    """k and v side by side in it are apart; in one place, or a head's width off, they are refused."""
+    import torch
+    rng = np.random.default_rng(69)
+    cache = _empty_cache(2, 3, 64, 16, 3, rng, [9, 40])
+    k, v = (_dev(rng.standard_normal((2, 9, 3, 64)), torch.bfloat16) for _ in range(2))
+    cache.append(k, v)
+    wk, wv = cache.read(9, torch.bfloat16)
+    buf = torch.full((2, 9, 8, 64), 3.0, dtype=torch.bfloat16, device="cuda")
+    cache.read(9, out=(buf[:, :, 4:7], buf[:, :, :3]))
+    cache.check()
+    assert torch.equal(buf[:, :, 4:7], wk) and torch.equal(buf[:, :, :3], wv) and (buf[:, :, 3] == 3).all() and (buf[:, :, 7] == 3).all()
+    before = buf.clone()
+    for a, b in ((0, 0), (0, 2), (3, 1)):
+        with pytest.raises(pk.PkvError) as e:
+            cache.read(9, out=(buf[:, :, a:a + 3], buf[:, :, b:b + 3]))
+        assert e.value.status == L.ERR_INVALID_ARGUMENT
+    assert torch.equal(buf, before)

@@ -252,3 +252,11 @@ def test_token_numbers_stay_in_32_bits(fn):
     for n, want in ((0x7fff0000, L.OK), (0x7fff0001, L.ERR_UNSUPPORTED), (0x7fffffff, L.ERR_UNSUPPORTED)):
         row = _rows(n, strides=(0, 0, 128))
         assert f(C.byref(_cache(n_seqs=0)), P, C.byref(row), P, C.byref(row), P, *rest, P, None) == want
+
+
+def test_read_refuses_outputs_over_one_another():
+    packed = (2 * 5 * 6 * 128, 6 * 128, 128)  # k and v heads side by side, three sequences
+    call = lambda shift: L.lib().pkv_kv4_read_dev(C.byref(_cache(n_kv_heads=3)), P, C.byref(_rows(5, strides=packed)), P + shift,  # noqa: E731
+                                                  C.byref(_rows(5, strides=packed)), None, 0, P, None)
+    for shift in (0, 128 * 2, -2 * 128 * 2, 16, 6 * 128 * 2):
+        assert call(shift) == L.ERR_INVALID_ARGUMENT, shift
