@@ -161,7 +161,8 @@ class Kv4Cache:
                 raise ValueError(f"{name} must be [{self.n_seqs}][tokens][heads][{self.dim}], not {tuple(shape)}")
             if stride[3] != 1 and t.numel():
                 raise ValueError(f"the values of a vector of {name} must be contiguous")
-            if written and any(n > 1 and st == 0 for n, st in zip(shape, stride)):
+            steps = [st for n, st in zip(shape[:3], stride) if n > 1]
+            if written and (any(st < self.dim for st in steps) or len(set(steps)) < len(steps)):
                 raise ValueError(f"{name} is written: its vectors must not lie over one another")
             if len(self._rows_of) >= 256:
                 self._rows_of.clear()

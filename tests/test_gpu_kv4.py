@@ -997,3 +997,25 @@ def test_read_into_slices_of_one_buffer():
             cache.read(9, out=(buf[:, :, a:a + 3], buf[:, :, b:b + 3]))
         assert e.value.status == L.ERR_INVALID_ARGUMENT
     assert torch.equal(buf, before)
+
+
+def test_written_vectors_that_lie_over_one_another_are_refused():
+    import torch
+    rng = np.random.default_rng(70)
+    pages, table, _ = kv4ref.fill(rng, 2, 2, 64, 16, [30, 55])
+    cache = kv4.Kv4Cache(_dev(pages), _ints(table), _ints([30, 55]))
+    q = torch.ones((2, 3, 4, 64), device="cuda")
+    buf = torch.zeros(4096, device="cuda")
+    for strides in ((768, 256, 0), (768, 256, 32), (768, 64, 64), (256, 256, 64), (0, 256, 64)):  # broadcast, half, sliding windows
+        with pytest.raises(ValueError, match="over one another"):
+            cache.attend(q, out=buf.as_strided((2, 3, 4, 64), (*strides, 1)))
+    assert (buf == 0).all()
+    want, _ = cache.attend(q)
+    for strides in ((768, 256, 64), (64, 128, 512), (1024, 320, 68)):  # any order, gaps
+        out = buf.as_strided((2, 3, 4, 64), (*strides, 1))
+        cache.attend(q, out=out)
+        assert torch.equal(out, want)
+    one = torch.zeros(256, device="cuda").as_strided((1, 1, 4, 64), (0, 0, 64, 1))  # strides of dimensions of one say nothing
+    few = kv4.Kv4Cache(_dev(pages), _ints(table[:1]), _ints([30]))
+    few.attend(q[:1, :1], out=one)
+    cache.check()
