@@ -441,6 +441,9 @@ int pkv_tqb1_header_parse(const pkv_turbo_profile* p, const uint8_t* bytes, int6
  * own number, as long as nothing was evicted.  mass[s][h][j] is the attention weight a token has received.  Both are
  * [n_seqs][n_kv_heads][max_pages * page_tokens], 16-byte aligned.
  *
+ * A sequence with positions whose ends[s] is below lens[s] is reported as PKV_VEC_BAD_SEQUENCE too (raise both for a step's tokens).
+ * Without positions, ends only says where the queries stand.
+ *
  * A sequence whose length is negative or above max_pages * page_tokens, or that has a page number outside [0, n_pages) among the
  * entries a call reads, is reported as PKV_VEC_BAD_SEQUENCE with its index.  A sequence with a bad length counts as empty,
  * the tokens of a bad page as absent; nothing is read or written through either.

@@ -87,7 +87,7 @@ struct Sequence {
 __device__ __forceinline__ Sequence sequence_of(const AttendParams& p, int s) {
   Sequence r;
   r.len = p.c.length(s, p.err);
-  r.end = p.c.end(s, r.len);
+  r.end = p.c.end(s, r.len, p.err);
   r.qn = p.q_lens ? p.q_lens[s] : p.q.n;
   if (r.qn < 0 || r.qn > p.q.n) {
     pkv_report(p.err, 0, s, PKV_VEC_BAD_SEQUENCE);

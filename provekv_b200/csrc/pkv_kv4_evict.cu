@@ -118,7 +118,7 @@ kv4_select_kernel(const __grid_constant__ EvictParams p) {
     if (tid == 0 && !p.fused) p.counts[at] = 0;
     return;
   }
-  const int recent_from = p.c.end(s, n) - p.recent;
+  const int recent_from = p.c.end(s, n, p.err) - p.recent;
   const int32_t* pos = p.c.positions + p.c.stat(s, h);
   const float* mass = p.c.mass + p.c.stat(s, h);
   auto key = [&](int j) {

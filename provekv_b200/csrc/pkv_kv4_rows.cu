@@ -138,7 +138,7 @@ __device__ __forceinline__ Fresh fresh_of(const Cache& c, int s, int n_tokens, c
     r.fresh = 0;
   }
   r.first = n - r.fresh;
-  r.position = c.end(s, n) - r.fresh;
+  r.position = c.end(s, n, err) - r.fresh;
   return r;
 }
 

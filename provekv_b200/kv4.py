@@ -7,9 +7,10 @@ codecs decoded), `attend` is attention straight from the pages (shared kv heads,
 window with sinks), `evict` cuts a cache down to a budget by the attention weight its tokens received, and `read` gives
 values back.  The format and the exact meaning of each call are in include/provekv_b200.h (``pkv_kv4_*``).
 
-The lengths belong to the step, not to the layer: raise ``lens`` (and ``ends``) once, then call the layers::
+The lengths belong to the step, not to the layer: raise ``lens`` and ``ends`` once, then call the layers::
 
     lens += 1                                   # int32 [n_seqs], on the device, shared by all layers
+    ends += 1                                   # (caches made without ends have as many tokens as they hold)
     for layer, cache in enumerate(caches):
         cache.append(k, v)                      # [n_seqs, 1, n_kv_heads, dim]
         out, lse = cache.attend(q)              # [n_seqs, 1, n_q_heads, dim]

@@ -1019,3 +1019,25 @@ def test_written_vectors_that_lie_over_one_another_are_refused():
     few = kv4.Kv4Cache(_dev(pages), _ints(table[:1]), _ints([30]))
     few.attend(q[:1, :1], out=one)
     cache.check()
+
+
+def test_ends_that_were_not_raised_are_reported_where_positions_are_kept():
+    """lens += n alone: every call says so; with both raised none does."""
+    import torch
+    (cache,) = kv4.Kv4Cache.allocate(1, 3, 2, 64, 64, page_tokens=16, evictable=True)
+    x = torch.ones((3, 20, 2, 64), device="cuda")
+    q = torch.ones((3, 1, 4, 64), device="cuda")
+    cache.lens += 20
+    cache.ends += torch.tensor([20, 19, 25], dtype=torch.int32, device="cuda")
+    cache.ends[2] += 5
+    calls = (lambda: cache.append(x, x), lambda: cache.read(20), lambda: cache.attend(q), lambda: cache.attend(x[:, :, :1].expand(3, 20, 8, 64).bfloat16()),
+             lambda: cache.evict(16))
+    for call in calls:
+        call()
+        with pytest.raises(pk.PkvError) as e:
+            cache.check()
+        assert (e.value.status, e.value.vector_index) == (L.VEC_BAD_SEQUENCE, 1)
+    cache.ends[1] += 1
+    for call in calls:
+        call()
+        cache.check()
