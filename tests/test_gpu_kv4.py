@@ -1041,3 +1041,183 @@ def test_ends_that_were_not_raised_are_reported_where_positions_are_kept():
     for call in calls:
         call()
         cache.check()
+
+
+# -- the other forms, with their choice checked ---------------------------------------------------------------------------
+def _launches(f):
+    before = L.lib().pkv_launch_count()
+    r = f()
+    return r, L.lib().pkv_launch_count() - before
+
+
+def _workspace(cache, q, **kw):
+    import ctypes as C
+    f = dict(scale=1.0, n_q_heads=q.shape[2], window=0, sinks=0, accumulate=0, max_len=0)
+    f.update(kw)
+    args = L.Kv4AttendC(*[f[n] for n, _ in L.Kv4AttendC._fields_])
+    return L.lib().pkv_kv4_attend_workspace_bytes(cache._ref, cache._rows(q, "q"), C.byref(args))
+
+
+def _splits(cache, q, **kw):
+    """Of a chunk's tokens: 256 rows of partial sums each; 1 if it has no partial sums."""
+    tasks = -(-q.shape[1] * q.shape[2] // cache.n_kv_heads // 256)
+    return max(1, _workspace(cache, q, **kw) // (tasks * cache.n_seqs * cache.n_kv_heads * 256 * (cache.dim + 2) * 4))
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("page,lens,q_len,group,window,sinks,moved", [(48, [1150], 60, 2, 0, 0, False), (16, [1300, 5, 0], 60, 1, 300, 70, True),
+                                                                      (64, [1100, 1124], 25, 2, 0, 0, True), (32, [2100], 300, 1, 900, 9, False)])
+def test_chunks_in_splits(dim, page, lens, q_len, group, window, sinks, moved):
+    """More than 48 rows, long enough for two splits and more."""
+    cache, q, _, _ = _attend_case(71 + page, "bfloat16", dim, 1, group, page, lens, q_len, window, sinks, moved, True,
+                                  q_lens=[min(q_len, n + 2) for n in lens])
+    assert q_len * group > 48 and _splits(cache, q, window=window, sinks=sinks) >= 2
+    assert _launches(lambda: cache.attend(q, window=window, sinks=sinks))[1] == 2
+
+
+def test_a_chunk_in_more_than_sixteen_splits():
+    """Each row is joined by a CTA."""
+    cache, q, _, _ = _attend_case(72, "float16", 64, 1, 1, 64, [9100], 50, 0, 0, False, True)
+    assert _splits(cache, q) > 16
+    cache, q, _, _ = _attend_case(73, "bfloat16", 128, 1, 1, 48, [9050, 100], 52, 0, 0, True, False)
+    assert _splits(cache, q) > 16
+
+
+@pytest.mark.parametrize("dim,dtype", [(64, "bfloat16"), (128, "float16")])
+def test_a_chunk_of_many_units_in_one_cta(dim, dtype):
+    """40 units and more through the rings of a CTA: enough sequences that nothing is split, a missing page far behind."""
+    import torch
+    rng = np.random.default_rng(74)
+    S, n, q_len = 75, 2700, 50
+    lens = [n] + [60] * (S - 1)
+    pages, table, values = kv4ref.fill(rng, 1, 1, dim, 64, [n])
+    table[0, 30] = -1
+    full = np.repeat(table, S, 0)  # the others hold the first tokens of the same pages
+    cache = kv4.Kv4Cache(_dev(pages), _ints(full), _ints(lens))
+    q = _dev(rng.standard_normal((S, q_len, 2, dim)), _dt(dtype))
+    assert _splits(cache, q) == 1
+    (out, lse), launches = _launches(lambda: cache.attend(q))
+    assert launches == 1
+    with pytest.raises(pk.PkvError) as e:
+        cache.check()
+    assert (e.value.status, e.value.vector_index) == (L.VEC_BAD_SEQUENCE, 0)
+    pos = np.arange(n, dtype=np.int64)[None, None].copy()
+    pos[0, 0, 30 * 64:31 * 64] = 1 << 30  # beyond every query: not seen
+    for s in (0, 1, S - 1):
+        w = kv4ref.attend(q[s:s + 1].double().cpu().numpy(), values, [lens[s]], [lens[s]], pos, 2, dim ** -0.5, 0, 0, [q_len])
+        _close(out[s:s + 1], lse[s:s + 1], w[0], w[1], *w[3:])
+
+
+@pytest.mark.parametrize("page,n,q_len", [(16, 300, 60), (48, 1300, 30), (64, 1300, 70)])
+def test_pages_missing_from_chunks(page, n, q_len):
+    """More than 48 rows; a page missing at the start, inside and at the end of a unit, alone and across splits."""
+    import torch
+    rng = np.random.default_rng(75 + n)
+    pages, table, values = kv4ref.fill(rng, 2, 1, 128, page, [n, 40])
+    missing = [0, 2, 3, (n - 1) // page]
+    for i, p in enumerate(missing):
+        table[0, p] = (-1, pages.shape[0], -(1 << 31), (1 << 31) - 1)[i]
+    cache = kv4.Kv4Cache(_dev(pages), _ints(table), _ints([n, 40]), mass=torch.zeros((2, 1, table.shape[1] * page), device="cuda"))
+    q = _dev(rng.standard_normal((2, q_len, 2, 128)), torch.float16)
+    out, lse = cache.attend(q, accumulate=True)
+    with pytest.raises(pk.PkvError) as e:
+        cache.check()
+    assert (e.value.status, e.value.vector_index) == (L.VEC_BAD_SEQUENCE, 0)
+    pos = np.tile(np.arange(n, dtype=np.int64), (2, 1, 1))
+    for p in missing:
+        pos[0, 0, p * page:(p + 1) * page] = 1 << 30
+    w = kv4ref.attend(q.double().cpu().numpy(), values, [n, 40], [n, 40], pos, 2, 128 ** -0.5, 0, 0, [q_len] * 2)
+    _close(out, lse, w[0], w[1], *w[3:])
+    mass = cache.mass[:, :, :n].double().cpu().numpy()
+    assert (mass[0][pos[0] == 1 << 30] == 0).all() and (mass[0, 0, page:2 * page] > 0).all()
+    eps = 2.0 ** -18 * w[4].max() + 2.0 ** -22 * np.abs(w[1][np.isfinite(w[1])]).max() + 2.0 ** -19
+    _within(mass, w[2], (2 * eps + 2.0 ** -24 * q_len * 2) * w[2], "mass")
+
+
+@pytest.mark.parametrize("dtype,group", [("bfloat16", 4), ("float32", 2), ("float32", 6), ("float16", 12)])
+def test_a_row_for_every_warp_with_one_long_sequence(dtype, group):
+    """2048 row tiles: a CTA each, nothing cut.  One sequence has more units than its warps fetch page numbers for at once."""
+    import torch
+    rng = np.random.default_rng(76)
+    S, H, n = 256, 8, 3000
+    nt = 2 if group > 8 else 1
+    pages, table, values = kv4ref.fill(rng, 2, H, 64, 16, [n, 90])
+    lens = rng.integers(0, 90, S)
+    lens[[0, 3, S - 1]] = 0, n, 90
+    full = np.repeat(table[1:], S, 0)  # short ones share a sequence's pages
+    full[3] = table[0]
+    cache = kv4.Kv4Cache(_dev(pages), _ints(full), _ints(lens), mass=torch.zeros((S, H, table.shape[1] * 16), device="cuda"))
+    q = _dev(rng.standard_normal((S, 1, H * group, 64)), _dt(dtype))
+    assert S * H * -(-group // (8 * nt)) >= 2048 and _workspace(cache, q) == 0
+    (out, lse), launches = _launches(lambda: cache.attend(q))
+    assert launches == 1
+    again, lse2 = cache.attend(q, accumulate=True)
+    cache.check()
+    assert torch.equal(out, again) and torch.equal(lse, lse2)
+    for s in (0, 1, 3, 100, S - 1):
+        which = 0 if s == 3 else 1
+        w = kv4ref.attend(q[s:s + 1].double().cpu().numpy(), values[which:which + 1], lens[s:s + 1], lens[s:s + 1], None, group, 0.125, 0, 0, [1])
+        _close(out[s:s + 1], lse[s:s + 1], w[0], w[1], *w[3:])
+        if lens[s]:
+            got = cache.mass[s:s + 1, :, :lens[s]].double().cpu().numpy()
+            eps = 2.0 ** -18 * w[4].max() + 2.0 ** -22 * np.abs(w[1]).max() + 2.0 ** -19
+            _within(got, w[2][:, :, :lens[s]], (2 * eps + 2.0 ** -24 * group) * w[2][:, :, :lens[s]], "mass")
+        assert (cache.mass[s, :, lens[s]:] == 0).all()
+
+
+@pytest.mark.parametrize("dtype,group", [("bfloat16", 4), ("float32", 1)])
+def test_weights_whose_scores_would_not_fit(dtype, group):
+    """A table of more than 256 MiB of scores: a second pass over the keys instead, with the same weights."""
+    import torch
+    rng = np.random.default_rng(77)
+    n, page = 2000, 64
+    pages, table, values = kv4ref.fill(rng, 1, 2, 64, page, [n])
+    small = kv4.Kv4Cache(_dev(pages), _ints(table), _ints([n]), mass=torch.zeros((1, 2, table.shape[1] * page), device="cuda"))
+    slots = (1 << 22) + 64  # x 2 heads x 8 rows x 4 bytes
+    wide = np.full((1, slots // page), -1, np.int32)
+    wide[:, :table.shape[1]] = table
+    large = kv4.Kv4Cache(_dev(pages), _ints(wide), _ints([n]), mass=torch.zeros((1, 2, slots), device="cuda"))
+    q = _dev(rng.standard_normal((1, 1, 2 * group, 64)), _dt(dtype))
+    assert _workspace(large, q, accumulate=1) == _workspace(large, q) and _workspace(small, q, accumulate=1) > _workspace(small, q)
+    a, b = small.attend(q, accumulate=True), large.attend(q, accumulate=True)
+    small.check()
+    large.check()
+    w = kv4ref.attend(q.double().cpu().numpy(), values, [n], [n], None, group, 0.125, 0, 0, [1])
+    eps = 2.0 ** -18 * w[4].max() + 2.0 ** -22 * np.abs(w[1]).max() + 2.0 ** -19
+    for cache, (out, lse) in ((small, a), (large, b)):
+        _close(out, lse, w[0], w[1], *w[3:])
+        _within(cache.mass[:, :, :n].double().cpu().numpy(), w[2][:, :, :n], (2 * eps + 2.0 ** -24 * group) * w[2][:, :, :n], "mass")
+    assert (large.mass[:, :, n:] == 0).all()
+
+
+@pytest.mark.parametrize("dim,heads,cap,n,budget", [(128, 2, 9984, 9984, 4000), (64, 1, 16384, 16000, 15900), (128, 1, 49152, 30011, 200),
+                                                    (128, 1, 49216, 20000, 19000), (64, 2, 131072, 2112, 2048)])
+def test_evictions_from_long_tables(dim, heads, cap, n, budget):
+    """More than 8192 slots: 1024 threads, keys in shared memory up to 49152 slots and read again beyond; short lists are moved
+    by the same launch, long ones by a second."""
+    import torch
+    rng = np.random.default_rng(cap + n)
+    page = 64
+    pages = rng.integers(0, 256, (cap // page, heads, page // 16, 18 * dim)).astype(np.uint8)
+    table = rng.permutation(cap // page).reshape(1, -1).astype(np.int32)
+    end = n + 100
+    pos, mass = np.full((1, heads, cap), -1, np.int32), np.zeros((1, heads, cap), np.float32)
+    for h in range(heads):
+        pos[0, h, :n] = rng.permutation(end)[:n]
+        mass[0, h, :n] = np.where(rng.random(n) < 0.4, 0.5, np.exp(3 * rng.standard_normal(n)))  # the budget cuts equal weights
+    cache = kv4.Kv4Cache(_dev(pages), _ints(table), _ints([n]), ends=_ints([end]), positions=_ints(pos), mass=_dev(mass))
+    _, launches = _launches(lambda: cache.evict(budget, sinks=4, recent=budget // 4))
+    cache.check()
+    assert launches == (1 if min(cap - budget, budget) <= 256 else 2)
+    want_pos, want_mass, rows = pos.copy(), mass.copy(), pages[table[0]].copy()  # slot order
+    for h in range(heads):
+        moves = kv4ref.evict(pos[0, h], mass[0, h].astype(np.float64), n, end, budget, 4, budget // 4)
+        assert moves
+        for to, fro in moves:
+            for side in range(2):
+                codes, sc = kv4ref.get_row(pages[table[0, fro // page]], h, fro % page, side, dim)
+                kv4ref.put_row(rows[to // page], h, to % page, side, codes, sc, dim)
+            want_pos[0, h, to], want_mass[0, h, to] = pos[0, h, fro], mass[0, h, fro]
+    assert np.array_equal(cache.positions.cpu().numpy(), want_pos)
+    assert np.array_equal(cache.mass.cpu().numpy(), want_mass)
+    assert np.array_equal(cache.pages[cache.page_table[0].long()].cpu().numpy(), rows)
