@@ -43,9 +43,8 @@ struct Cache {
   }
   // tokens the sequence has had; where positions are kept, fewer than it holds are reported (and taken as they are)
   __device__ __forceinline__ int end(int s, int length, uint64_t* err) const {
-    if (!ends) return length;
-    const int n = ends[s];
-    if (positions && n < length) pkv_report(err, 0, s, PKV_VEC_BAD_SEQUENCE);
+    const int n = ends ? ends[s] : length;
+    if (n < length && positions) pkv_report(err, 0, s, PKV_VEC_BAD_SEQUENCE);
     return n;
   }
   // Atom `a` (tokens 16 a .. 16 a + 15) of sequence s and kv head h, or null for a bad page number (reported).

@@ -183,20 +183,19 @@ class Kv4Cache:
             raise ValueError(f"{name} must be a contiguous int32 [{self.n_seqs}] tensor on {self.device}")
         return t.data_ptr()
 
-    def _on_device(self, fn, *args) -> int:
-        """fn(cache, *args) with the cache's device current (plans go by its size)."""
+    def _on_device(self, fn, *args):
+        """fn(*args) with the cache's device current (plans go by its size)."""
         if self._current_device() == self._index:
-            return fn(self._ref, *args)
+            return fn(*args)
         with self._torch.cuda.device(self._index):
-            return fn(self._ref, *args)
+            return fn(*args)
 
-    def _status(self, fn, *args) -> int:
-        return self._on_device(fn, *args, self._err, self._current_stream(self._index))
-
-    def _call(self, fn, *args) -> None:
-        status = self._status(fn, *args)
-        if status:
-            L.check(status)
+    def _call(self, fn, *args) -> int:
+        """The status of fn(cache, *args, error word, stream) with the cache's device current."""
+        if self._current_device() == self._index:
+            return fn(self._ref, *args, self._err, self._current_stream(self._index))
+        with self._torch.cuda.device(self._index):
+            return fn(self._ref, *args, self._err, self._current_stream(self._index))
 
     def append(self, k, v, new_lens=None) -> None:
         """Writes the newest tokens of each sequence: row i of ``k`` and ``v`` [n_seqs][n][n_kv_heads][dim] goes to slot
@@ -206,7 +205,9 @@ class Kv4Cache:
             raise ValueError("k and v must have the same shape")
         if k.numel() == 0:
             return
-        self._call(self._lib.pkv_kv4_append_dev, k.data_ptr(), kr, v.data_ptr(), vr, self._per_seq(new_lens, "new_lens"))
+        status = self._call(self._lib.pkv_kv4_append_dev, k.data_ptr(), kr, v.data_ptr(), vr, self._per_seq(new_lens, "new_lens"))
+        if status:
+            L.check(status)
 
     def read(self, n: int, dtype=None, new_lens=None, out=None):
         """(k, v) [n_seqs][n][n_kv_heads][dim]: the values the newest tokens stand for, at the rows `append` would take
@@ -226,7 +227,9 @@ class Kv4Cache:
         kr = self._rows(k, "k", self.n_kv_heads, True)
         vr = kr if fresh else self._rows(v, "v", self.n_kv_heads, True)
         if k.numel():
-            self._call(self._lib.pkv_kv4_read_dev, k.data_ptr(), kr, v.data_ptr(), vr, self._per_seq(new_lens, "new_lens"), int(fresh))
+            status = self._call(self._lib.pkv_kv4_read_dev, k.data_ptr(), kr, v.data_ptr(), vr, self._per_seq(new_lens, "new_lens"), int(fresh))
+            if status:
+                L.check(status)
         return k, v
 
     def attend(self, q, *, scale: float | None = None, window: int = 0, sinks: int = 0, q_lens=None, accumulate: bool = False,
@@ -271,18 +274,18 @@ class Kv4Cache:
                                 int(accumulate), _int32("max_len", max_len))
             if len(self._attend_of) >= 256:
                 self._attend_of.clear()
-            plan = self._attend_of[key] = (C.byref(args), self._on_device(self._lib.pkv_kv4_attend_workspace_bytes, qr, C.byref(args)),
+            plan = self._attend_of[key] = (C.byref(args), self._on_device(self._lib.pkv_kv4_attend_workspace_bytes, self._ref, qr, C.byref(args)),
                                            q.numel() == 0)
         args, need, empty = plan
         if empty:
             return out, lse
         work = self._pages.new_empty(need) if need else None
-        rest = (out.data_ptr(), outr, lse.data_ptr(), self._per_seq(q_lens, "q_lens"), args, work.data_ptr() if need else None, need)
-        status = self._status(self._lib.pkv_kv4_attend_dev, q.data_ptr(), qr, *rest)
-        if status == L.ERR_INVALID_ARGUMENT and out.untyped_storage().data_ptr() == q.untyped_storage().data_ptr():
-            q = q.clone()  # out lies over queries that are still to be read
-            status = self._status(self._lib.pkv_kv4_attend_dev, q.data_ptr(), self._rows(q, "q"), *rest)
+        to = (out.data_ptr(), outr, lse.data_ptr(), self._per_seq(q_lens, "q_lens"), args, work.data_ptr() if need else None, need)
+        status = self._call(self._lib.pkv_kv4_attend_dev, q.data_ptr(), qr, *to)
         if status:
+            if status == L.ERR_INVALID_ARGUMENT and out.untyped_storage().data_ptr() == q.untyped_storage().data_ptr():
+                q = q.clone()  # out lies over queries that are still to be read
+                status = self._call(self._lib.pkv_kv4_attend_dev, q.data_ptr(), self._rows(q, "q"), *to)
             L.check(status)
         return out, lse
 
@@ -301,7 +304,9 @@ class Kv4Cache:
                 self._evict_of.clear()
             need = self._evict_of[budget] = self._lib.pkv_kv4_evict_workspace_bytes(self._ref, budget)
         work = self._pages.new_empty(need) if need else None
-        self._call(self._lib.pkv_kv4_evict_dev, budget, sinks, recent, work.data_ptr() if need else None, need)
+        status = self._call(self._lib.pkv_kv4_evict_dev, budget, sinks, recent, work.data_ptr() if need else None, need)
+        if status:
+            L.check(status)
 
     def check(self) -> None:
         """Waits for the stream, raises PkvError for the first thing a kernel reported since the last check, and clears it."""
