@@ -858,7 +858,7 @@ kv4_mass_of_scores_kernel(const __grid_constant__ AttendParams p) {
 // has one owner and one order.  The queries come as B operands from shared memory, 64 rows at a time, eight converted by each
 // warp: rows are read and converted once for 256 tokens, keys once in all.  Two exponentials, two multiply-adds and two
 // additions a score pair are left besides the products.  512 rows over 8192 tokens, 8 heads of 128: 54 us (142 with the keys dequantised
-// again for every eight rows); 4096 rows 347 us, 380 with one chain of products an atom and divisions for the rows' positions.
+// again for every eight rows); 4096 rows 353 us, 380 with one chain of products an atom and divisions for the rows' positions.
 template <int D, int T>
 __global__ void __launch_bounds__(kMassWarps * 32, T == PKV_DST_F32 && D == 128 ? 1 : 2)
 kv4_mass_kernel(const __grid_constant__ AttendParams p) {
@@ -1053,7 +1053,8 @@ Plan make_plan(const Cache& c, int dim, const pkv_kv4_rows* q, const pkv_kv4_att
   }
   const int64_t units = (longest + kUnitTokens - 1) / kUnitTokens, most_units = (most + kUnitTokens - 1) / kUnitTokens;
   // Rows of up to six units a warp are not worth a second launch (32 sequences with a window of 1024, 8 kv heads: 17.2 us
-  // against 24.4), and with a row for every warp there is nothing to cut.
+  // against 24.4), and with a row for every warp there is nothing to cut while lengths are even (one long sequence among 255 short ones
+  // waits for its four warps).
   const int64_t tiles = (int64_t)c.heads * r.row_tiles * c.n_seqs, resident = (int64_t)sm_count() * kWarps * ctas_per_sm(dim, r.nt, q->dtype == PKV_DST_F32);
   r.runs = 0;
   // (the kernel numbers the units of all rows in 32 bits, and max_len may be below the lengths)

@@ -4,7 +4,9 @@
 // magnitude needs no other thread and both loads are in flight together.  A CTA covers 128 / (D / 16) tokens of one kv head,
 // whose code and scale bytes form contiguous runs.
 // Read: a thread owns 16 bytes of the output, so that a warp's stores are contiguous.
-// Both kernels are bound by HBM: a vector is read once and written once.
+// A vector is read once and written once.  Append of f32 runs at 82 % of the copy bandwidth (2 x 4099 tokens, 32 heads of 64: 28.5 us),
+// of 16-bit vectors, twice the values a byte, it is bound by issue (73 % of the slots; 4 x 8192, 8 heads of 128: 38 us, 4.5 TB/s).  Read
+// (36 and 38 us) by issue (65 to 68 %) and the latency of page number and codes.
 #include "pkv_kv4.cuh"
 
 using namespace pkv_kv4;
